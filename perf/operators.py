@@ -1,0 +1,554 @@
+"""The selective state space core's operators as measured cases: the scan over packed rows with its short causal convolution, the norms
+around a block, and the clipping of many gradient tensors.
+
+Rows are env-steps, packed: sequence b occupies rows [seq_off[b], seq_off[b] + seq_len[b]), as everywhere in this package.  Sizes come from
+the package's own workloads: 16-step chunks of ragged rollouts (1 065 of them), 64 or 256 sequences of 256 or 512 steps, hidden sizes
+128 / 256 / 512 (the block's inner width is twice that), ten heroes that act together, the parameter list of the recurrent policy.
+"""
+import random
+
+import torch
+
+own = False
+
+DTYPES = {'f32': torch.float32, 'bf16': torch.bfloat16}
+CHUNK = 64                       # rows per block of the plain scan
+
+# ---------------------------------------------------------------------------------------------------------------- cases
+
+
+def listed():
+    return [
+        # the optimizer's default shape: 16-step chunks of ragged rollouts, each with the state its rollout had there
+        dict(name='scan_chunks16_fwd_f32', op='scan', pass_='fwd', dtype='f32', rows=17040, n_seq=1065, ragged=False, H=4, P=64, G=1, N=64,
+             views=False, carry=True),
+        # the rollout pass of 256 trajectories of 256 steps, inner width 512; x, B and C are column slices of the convolution's output
+        dict(name='scan_rollout_fwd_bf16', op='scan', pass_='fwd', dtype='bf16', rows=65536, n_seq=256, ragged=False, H=8, P=64, G=1, N=128,
+             views=True, carry=False),
+        # one very long recording: nothing to split over but time
+        dict(name='scan_long_fwd_f32', op='scan', pass_='fwd', dtype='f32', rows=32771, n_seq=1, ragged=False, H=8, P=64, G=1, N=64,
+             views=False, carry=True),
+        # the training pass of 256 trajectories of 256 steps at inner width 256
+        dict(name='scan_train_bwd_f32', op='scan', pass_='bwd', dtype='f32', rows=65536, n_seq=256, ragged=False, H=4, P=64, G=1, N=64,
+             views=False, carry=False),
+        # ragged rollouts, an empty one among them, head sizes off the tile sizes, gradients into the carried state
+        dict(name='scan_ragged_bwd_bf16', op='scan', pass_='bwd', dtype='bf16', rows=24907, n_seq=97, ragged=True, H=6, P=48, G=2, N=40,
+             views=True, carry=True),
+        # ten heroes act: one env-step each
+        dict(name='scan_step_f32', op='scan', pass_='step', dtype='f32', rows=10, n_seq=10, ragged=False, H=8, P=64, G=1, N=64, views=False,
+             carry=True),
+        # the convolution in front of the scan in the training pass: inner width 512 and two states of 64
+        dict(name='conv_train_bwd_f32', op='conv', pass_='bwd', dtype='f32', rows=65536, n_seq=256, ragged=False, width=640, K=4, silu=True,
+             carry=False),
+        # ragged rollouts with a carried history and an odd width
+        dict(name='conv_ragged_fwd_bf16', op='conv', pass_='fwd', dtype='bf16', rows=24907, n_seq=97, ragged=True, width=387, K=3, silu=True,
+             carry=True),
+        # bf16 block outputs on an f32 residual stream, hidden 512, 256 trajectories of 256 steps
+        dict(name='norm_rollout_fwd_bf16', op='norm', pass_='fwd', dtype='bf16', rows=65536, width=512, residual='f32', gate=True, scale=True,
+             pre=True),
+        # the same block's backward pass in f32, rows and width off the powers of two
+        dict(name='norm_train_bwd_f32', op='norm', pass_='bwd', dtype='f32', rows=16389, width=1000, residual='f32', gate=True, scale=True,
+             pre=True),
+        # the gradients of the recurrent policy: 34 tensors, the largest a 256 x 896 matrix
+        dict(name='clip_policy_f32', op='clip', pass_='fwd', tensors=34, largest=229376, mixed=False, clips=True),
+        # many blocks' parameters, f32 and bf16 mixed
+        dict(name='clip_blocks_mixed', op='clip', pass_='fwd', tensors=60, largest=6291456, mixed=True, clips=True),
+    ]
+
+
+def _log_uniform(rng, lo, hi):
+    return max(lo, min(hi, int(round(lo * (hi / lo) ** rng.random()))))
+
+
+def draw(rng):
+    op = rng.choice(['scan', 'scan', 'scan', 'conv', 'norm', 'clip'])
+    dtype = rng.choice(['f32', 'bf16'])
+    if op == 'clip':
+        case = dict(op='clip', pass_='fwd', tensors=_log_uniform(rng, 1, 60), largest=_log_uniform(rng, 1000, 6291456), mixed=rng.random() < 0.5,
+                    clips=rng.random() < 0.7)
+        return case
+    if op == 'norm':
+        case = dict(op='norm', pass_=rng.choice(['fwd', 'bwd']), dtype=dtype, rows=_log_uniform(rng, 1, 65536), width=_log_uniform(rng, 16, 4096),
+                    residual=rng.choice(['f32', dtype]), gate=rng.random() < 0.7, scale=rng.random() < 0.7, pre=rng.random() < 0.8)
+    else:
+        pass_ = rng.choice(['fwd', 'bwd', 'step'])
+        rows = _log_uniform(rng, 1, 512) if pass_ == 'step' else _log_uniform(rng, 1, 65536)
+        n_seq = rows if pass_ == 'step' else _log_uniform(rng, 1, min(rows, 1065))
+        case = dict(op=op, pass_=pass_, dtype=dtype, rows=rows, n_seq=n_seq, ragged=pass_ != 'step')
+        if op == 'conv':
+            case.update(width=_log_uniform(rng, 16, 2048), K=rng.choice([2, 3, 4, 4, 5]), silu=rng.random() < 0.7, carry=rng.random() < 0.5)
+        else:
+            G = rng.choice([1, 1, 2])
+            case.update(H=G * rng.randint(1, 6), P=rng.choice([16, 32, 40, 48, 64, 64, 77, 128]), G=G, N=rng.choice([16, 24, 32, 40, 64, 64, 101, 128]),
+                        views=rng.random() < 0.5, carry=rng.random() < 0.5)
+    most = {k: max(work(c)[k] for c in listed()) for k in ('bytes', 'flops')}
+    while any(work(case)[k] > most[k] for k in most):
+        case['rows'] = max(1, case['rows'] // 2)
+        if 'n_seq' in case:
+            case['n_seq'] = min(case['n_seq'], case['rows'])
+    return case
+
+
+def _lengths(case):
+    """Host list of the sequences' lengths: all alike, or a spread with an empty sequence in it."""
+    rows, n = case['rows'], case['n_seq']
+    if not case['ragged']:
+        return [rows // n] * n
+    rng = random.Random(rows * 4099 + n)
+    w = [0.05 + rng.random() for _ in range(n)]
+    lens = [int(rows * v / sum(w)) for v in w]
+    if n >= 4:
+        lens[1] = 0
+    lens[-1] += rows - sum(lens)
+    return lens
+
+
+def _clip_sizes(case):
+    """Sizes of the gradient tensors: biases, odd small ones, matrices up to `largest`."""
+    rng = random.Random(case['tensors'] * 4099 + case['largest'])
+    sizes = [case['largest']]
+    while len(sizes) < case['tensors']:
+        sizes.append(_log_uniform(rng, 1, case['largest']) if len(sizes) % 2 else _log_uniform(rng, max(1, case['largest'] // 8), case['largest']))
+    return sizes
+
+
+def work(case):
+    op, pass_ = case['op'], case['pass_']
+    if op == 'clip':
+        b = [n * (2 if case['mixed'] and i % 2 else 4) for i, n in enumerate(_clip_sizes(case))]
+        return {'bytes': sum(b) * 2, 'flops': sum(_clip_sizes(case)) * 3}
+    rows = case['rows']
+    e = 4 if case['dtype'] == 'f32' else 2
+    if op == 'norm':
+        D, r = case['width'], 4 if case['residual'] == 'f32' else 2
+        cols = 1 + case['scale'] + case['pre']
+        if pass_ == 'fwd':                                     # y, gate, r -> r', x'
+            return {'bytes': rows * D * (e * (1 + case['gate'] + case['pre']) + 2 * r) + 4 * D * cols, 'flops': rows * D * 16}
+        # y, gate, r, dr', dx' -> dy, dgate, dr
+        return {'bytes': rows * D * (e * (2 + 2 * case['gate'] + case['pre']) + 3 * r) + 8 * D * cols, 'flops': rows * D * 40}
+    n = case['n_seq']
+    if op == 'conv':
+        D, K = case['width'], case['K']
+        hist = n * (K - 1) * D * e * (2 if case['carry'] or pass_ == 'step' else 1)
+        io = rows * D * e * (3 if pass_ == 'bwd' else 2)
+        return {'bytes': io + hist + 4 * D * (K + 1) * (2 if pass_ == 'bwd' else 1), 'flops': rows * D * (2 * K + 4) * (3 if pass_ == 'bwd' else 1)}
+    H, P, G, N = case['H'], case['P'], case['G'], case['N']
+    state = 4 * n * H * P * N
+    per_row = e * (H * P + H + 2 * G * N)                      # x, dt, B, C
+    if pass_ == 'bwd':                                         # and dy; their gradients
+        return {'bytes': rows * (2 * per_row + e * H * P) + state * (3 if case['carry'] else 1), 'flops': rows * H * 14 * P * N}
+    return {'bytes': rows * (per_row + e * H * P) + state * (2 if case['carry'] or pass_ == 'step' else 1), 'flops': rows * H * 5 * P * N}
+
+
+# --------------------------------------------------------------------------------------------------------------- inputs
+
+
+def prepare(case, seed):
+    g = torch.Generator(device='cuda').manual_seed(seed * 7919 + 13)
+
+    def randn(*shape):
+        return torch.randn(shape, generator=g, device='cuda')
+
+    def rand(*shape):
+        return torch.rand(shape, generator=g, device='cuda')
+
+    s = dict(case)
+    if case['op'] == 'clip':
+        sizes = _clip_sizes(case)
+        total = float(sum(sizes)) ** 0.5
+        s['grads'] = [(1e-2 * randn(n)).to(torch.bfloat16 if case['mixed'] and i % 2 else torch.float32) for i, n in enumerate(sizes)]
+        # the bound is passed by far or not at all: a training run sees both
+        s['out'] = [torch.empty_like(t) for t in s['grads']]   # the buffers that the clipped gradients go to, kept from step to step
+        s['max_norm'] = 1e-2 * total * (0.25 if case['clips'] else 4.0)
+        return s
+    dt = DTYPES[case['dtype']]
+    rows = case['rows']
+    if case['op'] == 'norm':
+        D, rd = case['width'], DTYPES[case['residual']]
+        s['y'] = randn(rows, D).to(dt)
+        s['residual'] = (2.0 * randn(rows, D)).to(rd)
+        s['w_post'] = 1.0 + 0.1 * randn(D)
+        s['z'] = randn(rows, D).to(dt) if case['gate'] else None
+        s['s'] = 0.1 + 0.02 * randn(D) if case['scale'] else None
+        s['w_pre'] = 1.0 + 0.1 * randn(D) if case['pre'] else None
+        if case['pass_'] == 'bwd':
+            s['dr'] = randn(rows, D).to(rd)
+            s['dx'] = randn(rows, D).to(dt) if case['pre'] else None
+        return s
+    lens = _lengths(case)
+    n = len(lens)
+    s['seq_len'] = torch.tensor(lens, dtype=torch.int32, device='cuda')
+    s['seq_off'] = (torch.cumsum(s['seq_len'].to(torch.int64), 0) - s['seq_len']).contiguous()
+    s['max_len'] = max(lens)
+    if case['op'] == 'conv':
+        D, K = case['width'], case['K']
+        s['x'] = randn(rows, D).to(dt)
+        s['weight'] = randn(D, K) * K ** -0.5
+        s['bias'] = 0.1 * randn(D)
+        s['state'] = randn(n, K - 1, D).to(dt) if case['carry'] or case['pass_'] == 'step' else None
+        if case['pass_'] == 'bwd':
+            s['dy'] = randn(rows, D).to(dt)
+            s['dstate'] = randn(n, K - 1, D).to(dt) if case['carry'] else None
+        return s
+    H, P, G, N = case['H'], case['P'], case['G'], case['N']
+    if case['views']:                                          # column slices of the convolution's output
+        xbc = torch.nn.functional.silu(randn(rows, H * P + 2 * G * N)).to(dt)
+        s['x'], s['B'], s['C'] = (xbc[:, :H * P].unflatten(1, (H, P)), xbc[:, H * P:H * P + G * N].unflatten(1, (G, N)),
+                                  xbc[:, H * P + G * N:].unflatten(1, (G, N)))
+    else:
+        s['x'], s['B'], s['C'] = randn(rows, H, P).to(dt), randn(rows, G, N).to(dt), randn(rows, G, N).to(dt)
+    s['dt'] = randn(rows, H).to(dt)
+    s['A'] = -(1.0 + 15.0 * rand(H))
+    s['D'] = 1.0 + 0.1 * randn(H)
+    want = torch.exp(rand(H) * 4.6 - 6.9)                      # step sizes of 1e-3 to 1e-1
+    s['dt_bias'] = torch.log(torch.expm1(want))
+    s['h0'] = randn(n, H, P, N) if case['carry'] else None
+    if case['pass_'] == 'bwd':
+        s['dy'] = randn(rows, H, P).to(dt)
+        s['dhT'] = randn(n, H, P, N) if case['carry'] else None
+    return s
+
+
+# ---------------------------------------------------------------------------------------------------------- plain forms
+
+
+def _padded(t, s, width):
+    """Packed rows -> [n_seq, width, ...] f32 with zeros behind each sequence's end."""
+    i = torch.arange(width, device=t.device)
+    at = (s['seq_off'][:, None] + i).clamp(max=t.shape[0] - 1)
+    inside = i < s['seq_len'][:, None]
+    return torch.where(inside.reshape(inside.shape + (1,) * (t.dim() - 1)), t[at].float(), torch.zeros((), device=t.device))
+
+
+def _packed(t, s, rows):
+    """The inverse of _padded."""
+    i = torch.arange(t.shape[1], device=t.device)
+    at = s['seq_off'][:, None] + i
+    inside = i < s['seq_len'][:, None]
+    out = torch.zeros((rows,) + t.shape[2:], device=t.device, dtype=t.dtype)
+    out[at[inside]] = t[inside]
+    return out
+
+
+def _softplus(v):
+    return torch.where(v > 20.0, v, torch.log1p(torch.exp(v.clamp(max=20.0))))
+
+
+def _scan_plain(s, x, dt, A, B, C, D, bias, h0):
+    """All f32.  Blocks of CHUNK rows: inside a block by the products of the rows with each other, between blocks by the decays."""
+    rows, n = s['rows'], s['n_seq']
+    H, G, N, P = s['H'], s['G'], s['N'], s['P']
+    nc = max(1, -(-s['max_len'] // CHUNK))
+    L = nc * CHUNK
+    inside = (torch.arange(L, device=x.device) < s['seq_len'][:, None])[..., None]
+    step = torch.where(inside, _softplus(_padded(dt, s, L) + bias), torch.zeros((), device=x.device))      # [n, L, H]
+    blocks = lambda t: t.unflatten(1, (nc, CHUNK))                                                          # noqa: E731
+    heads = lambda t: t.repeat_interleave(H // G, dim=-2)                                                   # noqa: E731
+    xp, Bp, Cp = (blocks(_padded(t, s, L)) for t in (x, B, C))
+    step = blocks(step)
+    cum = torch.cumsum((step * A).double(), dim=2)                                                          # [n, nc, T, H]
+    ch = cum.permute(0, 1, 3, 2)                                                                            # [n, nc, H, T]
+    gap = ch[..., :, None] - ch[..., None, :]
+    low = torch.ones(CHUNK, CHUNK, dtype=torch.bool, device=x.device).tril()
+    decay = torch.where(low, torch.exp(torch.where(low, gap, torch.zeros((), dtype=torch.float64, device=x.device)).float()),
+                        torch.zeros((), device=x.device))
+    score = (Cp.permute(0, 1, 3, 2, 4) @ Bp.permute(0, 1, 3, 4, 2)).repeat_interleave(H // G, dim=2)        # [n, nc, H, T, T]
+    xs = (xp * step[..., None]).permute(0, 1, 3, 2, 4)                                                      # [n, nc, H, T, P]
+    y = (score * decay) @ xs
+    to_end = torch.exp((ch[..., -1:] - ch).float())                                                         # [n, nc, H, T]
+    local = (xs * to_end[..., None]).transpose(-1, -2) @ heads(Bp).permute(0, 1, 3, 2, 4)                   # [n, nc, H, P, N]
+    total = torch.cumsum(ch[..., -1], dim=1)                                                                # [n, nc, H]
+    first = torch.zeros(n, 1, H, dtype=torch.float64, device=x.device)
+    edge = torch.cat([first, total], 1).permute(0, 2, 1)                                                    # [n, H, nc + 1]
+    between = edge[..., :, None] - edge[..., None, :]
+    low = torch.ones(nc + 1, nc + 1, dtype=torch.bool, device=x.device).tril()
+    between = torch.where(low, torch.exp(torch.where(low, between, torch.zeros((), dtype=torch.float64, device=x.device)).float()),
+                          torch.zeros((), device=x.device))
+    begin = torch.zeros(n, 1, H, P, N, device=x.device) if h0 is None else h0[:, None]
+    source = torch.cat([begin, local], 1).permute(0, 2, 1, 3, 4).flatten(3)                                 # [n, H, nc + 1, P N]
+    states = (between @ source).unflatten(-1, (P, N)).permute(0, 2, 1, 3, 4)                                # [n, nc + 1, H, P, N]
+    into = heads(Cp).permute(0, 1, 3, 2, 4) @ states[:, :-1].transpose(-1, -2)                              # [n, nc, H, T, P]
+    y = y + into * torch.exp(ch.float())[..., None]
+    y = y.permute(0, 1, 3, 2, 4) + D[:, None] * xp
+    return _packed(y.flatten(1, 2), s, rows), states[:, -1]
+
+
+def _conv_plain(s, x, weight, bias, state):
+    D, K = s['width'], s['K']
+    xp = _padded(x, s, s['max_len'])
+    past = torch.zeros(s['n_seq'], K - 1, D, device=x.device) if state is None else state.float()
+    ext = torch.cat([past, xp], 1)                                                                          # [n, K - 1 + L, D]
+    y = (ext.unfold(1, K, 1) * weight).sum(-1) + bias
+    y = y * torch.sigmoid(y) if s['silu'] else y
+    at = s['seq_len'][:, None].long() + torch.arange(K - 1, device=x.device)
+    last = torch.gather(ext, 1, at[..., None].expand(-1, -1, D))
+    return _packed(y, s, s['rows']), last
+
+
+def _norm_plain(s, y, residual, w_post, z, scale, w_pre):
+    eps = 1e-5
+    g = y if z is None else y * (z * torch.sigmoid(z))
+    post = g * torch.rsqrt((g * g).mean(-1, keepdim=True) + eps) * w_post
+    r = residual + (post if scale is None else post * scale)
+    return r, None if w_pre is None else r * torch.rsqrt((r * r).mean(-1, keepdim=True) + eps) * w_pre
+
+
+def _gradients(outs, given, wrt):
+    """Gradients of sum(out * given) for the tensors in wrt; None stays None."""
+    pairs = [(o, g.float()) for o, g in zip(outs, given) if o is not None and g is not None]
+    have = [t for t in wrt if t is not None]
+    grads = iter(torch.autograd.grad([o for o, _ in pairs], have, [g for _, g in pairs]))
+    return [None if t is None else next(grads) for t in wrt]
+
+
+def _leaf(t):
+    return None if t is None else t.detach().float().requires_grad_(True)
+
+
+def _run_plain(s):
+    op, pass_ = s['op'], s['pass_']
+    if op == 'clip':
+        norms = torch.stack([(g.double() * g.double()).sum() for g in s['grads']]).sqrt()
+        total = (norms * norms).sum().sqrt()
+        coef = (s['max_norm'] / (total + 1e-6)).clamp(max=1.0)
+        return dict(total=total.float(), norms=norms.float(), grads=[(g.double() * coef).to(g.dtype) for g in s['grads']])
+    dt = DTYPES[s['dtype']]
+    if op == 'norm':
+        args = [s['y'], s['residual'], s['w_post'], s['z'], s['s'], s['w_pre']]
+        rd = s['residual'].dtype
+        if pass_ == 'fwd':
+            r, x = _norm_plain(s, *[None if t is None else t.float() for t in args])
+            return dict(r=r.to(rd), x=None if x is None else x.to(dt))
+        leaves = [_leaf(t) for t in args]
+        dy, dr, dw_post, dz, ds, dw_pre = _gradients(_norm_plain(s, *leaves), (s['dr'], s['dx']), leaves)
+        return dict(dy=dy.to(dt), dr=dr.to(rd), dw_post=dw_post, dz=None if dz is None else dz.to(dt), ds=ds, dw_pre=dw_pre)
+    if op == 'conv':
+        if pass_ == 'step':
+            ext = torch.cat([s['state'].float(), s['x'].float()[:, None]], 1)
+            y = (ext * s['weight'].t()).sum(1) + s['bias']
+            y = y * torch.sigmoid(y) if s['silu'] else y
+            return dict(y=y.to(dt), state=ext[:, 1:].to(dt))
+        if pass_ == 'fwd':
+            y, last = _conv_plain(s, s['x'], s['weight'], s['bias'], s['state'])
+            return dict(y=y.to(dt), state=last.to(dt))
+        leaves = [_leaf(t) for t in (s['x'], s['weight'], s['bias'], s['state'])]
+        dx, dw, db, dst = _gradients(_conv_plain(s, *leaves), (s['dy'], s['dstate']), leaves)
+        return dict(dx=dx.to(dt), dw=dw, db=db, dstate=None if dst is None else dst.to(dt))
+    if pass_ == 'step':
+        step = _softplus(s['dt'].float() + s['dt_bias'])                                                    # [n, H]
+        x, rep = s['x'].float(), s['H'] // s['G']
+        B, C = (t.float().repeat_interleave(rep, dim=1) for t in (s['B'], s['C']))
+        h0 = torch.zeros(s['n_seq'], s['H'], s['P'], s['N'], device='cuda') if s['h0'] is None else s['h0']
+        h = h0 * torch.exp(step * s['A'])[..., None, None] + (step[..., None] * x)[..., None] * B[:, :, None]
+        y = (h * C[:, :, None]).sum(-1) + s['D'][:, None] * x
+        return dict(y=y.to(dt), h=h)
+    if pass_ == 'fwd':
+        y, hT = _scan_plain(s, s['x'], s['dt'], s['A'], s['B'], s['C'], s['D'], s['dt_bias'], s['h0'])
+        return dict(y=y.to(dt), hT=hT)
+    leaves = [_leaf(s[k]) for k in ('x', 'dt', 'A', 'B', 'C', 'D', 'dt_bias', 'h0')]
+    dx, ddt, dA, dB, dC, dD, dbias, dh0 = _gradients(_scan_plain(s, *leaves), (s['dy'], s['dhT']), leaves)
+    return dict(dx=dx.to(dt), ddt=ddt.to(dt), dA=dA, dB=dB.to(dt), dC=dC.to(dt), dD=dD, dbias=dbias, dh0=dh0)
+
+
+# ------------------------------------------------------------------------------------------------------- the framework
+
+
+def _run_own(s):
+    from dotaclient_amd import ops
+    op, pass_ = s['op'], s['pass_']
+    if op == 'clip':
+        total, norms = ops.grad_norm_clip(s['grads'], s['max_norm'], out=s['out'])
+        return dict(total=total, norms=norms, grads=s['out'])
+    if op == 'norm':
+        if pass_ == 'fwd':
+            r, x = ops.block_norm(s['y'], s['residual'], s['w_post'], gate=s['z'], scale=s['s'], w_pre=s['w_pre'])
+            return dict(r=r, x=x)
+        dy, dr, dw_post, dz, ds, dw_pre = ops.block_norm_backward(s['dr'], s['dx'], s['y'], s['residual'], s['w_post'], gate=s['z'], scale=s['s'],
+                                                                  w_pre=s['w_pre'])
+        return dict(dy=dy, dr=dr, dw_post=dw_post, dz=dz, ds=ds, dw_pre=dw_pre)
+    seqs = (s['seq_off'], s['seq_len'], s['max_len'])
+    if op == 'conv':
+        if pass_ == 'step':
+            y, state = ops.causal_conv_step(s['x'], s['state'], s['weight'], s['bias'], silu=s['silu'])
+            return dict(y=y, state=state)
+        if pass_ == 'fwd':
+            y, last = ops.causal_conv(s['x'], s['weight'], s['bias'], *seqs, state=s['state'], silu=s['silu'])
+            return dict(y=y, state=last)
+        dx, dw, db, dst = ops.causal_conv_backward(s['dy'], s['x'], s['weight'], s['bias'], *seqs, state=s['state'], silu=s['silu'],
+                                                   dstate_out=s['dstate'])
+        return dict(dx=dx, dw=dw, db=db, dstate=dst)
+    if pass_ == 'step':
+        y, h = ops.ssm_step(s['x'], s['dt'], s['A'], s['B'], s['C'], h0=s['h0'], D=s['D'], dt_bias=s['dt_bias'], softplus=True)
+        return dict(y=y, h=h)
+    if pass_ == 'fwd':
+        y, hT = ops.ssm_scan(s['x'], s['dt'], s['A'], s['B'], s['C'], *seqs, D=s['D'], dt_bias=s['dt_bias'], h0=s['h0'], softplus=True)
+        return dict(y=y, hT=hT)
+    g = ops.ssm_scan_backward(s['dy'], s['x'], s['dt'], s['A'], s['B'], s['C'], *seqs, D=s['D'], dt_bias=s['dt_bias'], h0=s['h0'], softplus=True,
+                              dhT=s['dhT'])
+    return dict(dx=g.dx, ddt=g.ddt, dA=g.dA, dB=g.dB, dC=g.dC, dD=g.dD, dbias=g.ddt_bias, dh0=g.dh0)
+
+
+def run(state):
+    return _run_own(state) if own else _run_plain(state)
+
+
+# --------------------------------------------------------------------------------------------- the definitions in 64 bits
+
+
+def _sequences(s):
+    return [(int(o), int(o) + int(m)) for o, m in zip(s['seq_off'].tolist(), s['seq_len'].tolist())]
+
+
+def _by_time(t, seqs, width):
+    """[width, n, ...] f64: time first, zeros behind the ends."""
+    out = torch.zeros((width, len(seqs)) + t.shape[1:], dtype=torch.float64, device=t.device)
+    for b, (lo, hi) in enumerate(seqs):
+        out[:hi - lo, b] = t[lo:hi].double()
+    return out
+
+
+def _by_row(t, seqs, rows):
+    out = torch.zeros((rows,) + t.shape[2:], dtype=torch.float64, device=t.device)
+    for b, (lo, hi) in enumerate(seqs):
+        out[lo:hi] = t[:hi - lo, b]
+    return out
+
+
+def _exact_scan(s):
+    """The recurrence step by step, and its reverse."""
+    rows, n, H, P, G, N = s['rows'], s['n_seq'], s['H'], s['P'], s['G'], s['N']
+    seqs = _sequences(s)
+    T = max(hi - lo for lo, hi in seqs)
+    bwd = s['pass_'] == 'bwd'
+    if bwd and T * n * H * P * N * 8 > 60e9:
+        return None
+    x, B, C = (_by_time(s[k], seqs, T) for k in ('x', 'B', 'C'))
+    raw = _by_time(s['dt'], seqs, T) + s['dt_bias'].double()
+    live = torch.zeros(T, n, dtype=torch.bool, device='cuda')
+    for b, (lo, hi) in enumerate(seqs):
+        live[:hi - lo, b] = True
+    step = torch.logaddexp(raw, torch.zeros_like(raw)) * live[..., None]
+    A, D = s['A'].double(), s['D'].double()
+    spread = lambda t: t[:, :, None].expand(n, G, H // G, N).reshape(n, H, N)                                # noqa: E731
+    h = torch.zeros(n, H, P, N, dtype=torch.float64, device='cuda') if s['h0'] is None else s['h0'].double()
+    before, ys = [], []
+    for t in range(T):
+        if bwd:
+            before.append(h)
+        h = h * torch.exp(step[t] * A)[..., None, None] + (step[t][..., None] * x[t])[..., None] * spread(B[t])[:, :, None]
+        if not bwd:
+            ys.append(torch.einsum('bhpn,bhn->bhp', h, spread(C[t])) + D[:, None] * x[t])
+    if not bwd:
+        return dict(y=_by_row(torch.stack(ys), seqs, rows), hT=h)
+    dy = _by_time(s['dy'], seqs, T)
+    gh = torch.zeros_like(h) if s['dhT'] is None else s['dhT'].double()
+    dx, dstep, dB, dC = torch.zeros_like(x), torch.zeros_like(step), torch.zeros_like(B), torch.zeros_like(C)
+    dA = torch.zeros_like(A)
+    for t in reversed(range(T)):
+        decay = torch.exp(step[t] * A)
+        after = before[t] * decay[..., None, None] + (step[t][..., None] * x[t])[..., None] * spread(B[t])[:, :, None]
+        dC[t] = torch.einsum('bhpn,bhp->bhn', after, dy[t]).view(n, G, H // G, N).sum(2)
+        gh = gh + dy[t][..., None] * spread(C[t])[:, :, None]
+        into = torch.einsum('bhpn,bhn->bhp', gh, spread(B[t]))
+        dx[t] = step[t][..., None] * into + D[:, None] * dy[t]
+        dB[t] = (step[t][..., None] * torch.einsum('bhpn,bhp->bhn', gh, x[t])).view(n, G, H // G, N).sum(2)
+        through = (gh * before[t]).sum((-1, -2)) * decay                                                     # d / d(step A)
+        dstep[t] = (into * x[t]).sum(-1) + through * A
+        dA = dA + (through * step[t]).sum(0)
+        gh = gh * decay[..., None, None]
+    draw_ = dstep * torch.sigmoid(raw) * live[..., None]
+    back = lambda t: _by_row(t, seqs, rows)                                                                  # noqa: E731
+    return dict(dx=back(dx), ddt=back(draw_), dA=dA, dB=back(dB), dC=back(dC), dD=(dy * x).sum((0, 1, 3)), dbias=draw_.sum((0, 1)),
+                dh0=None if s['h0'] is None else gh)
+
+
+def _exact_conv(s):
+    K, D = s['K'], s['width']
+    w, bias = s['weight'].double(), s['bias'].double()
+    if s['pass_'] == 'step':
+        ext = torch.cat([s['state'].double(), s['x'].double()[:, None]], 1)
+        v = torch.einsum('nkd,dk->nd', ext, w) + bias
+        return dict(y=v * torch.sigmoid(v) if s['silu'] else v, state=ext[:, 1:])
+    y = torch.zeros(s['rows'], D, dtype=torch.float64, device='cuda')
+    state = torch.zeros(s['n_seq'], K - 1, D, dtype=torch.float64, device='cuda')
+    dx, dw, db, dstate = torch.zeros_like(y), torch.zeros_like(w), torch.zeros_like(bias), torch.zeros_like(state)
+    for b, (lo, hi) in enumerate(_sequences(s)):
+        m = hi - lo
+        past = state.new_zeros(K - 1, D) if s['state'] is None else s['state'][b].double()
+        ext = torch.cat([past, s['x'][lo:hi].double()], 0)
+        v = bias.expand(m, D).clone()
+        for k in range(K):
+            v += w[:, k] * ext[k:k + m]
+        sig = torch.sigmoid(v)
+        y[lo:hi] = v * sig if s['silu'] else v
+        state[b] = ext[m:]
+        if s['pass_'] == 'bwd':
+            dv = s['dy'][lo:hi].double()
+            dv = dv * sig * (1 + v * (1 - sig)) if s['silu'] else dv
+            dext = torch.zeros_like(ext)
+            for k in range(K):
+                dext[k:k + m] += w[:, k] * dv
+                dw[:, k] += (dv * ext[k:k + m]).sum(0)
+            if s['dstate'] is not None:
+                dext[m:] += s['dstate'][b].double()
+            db += dv.sum(0)
+            dx[lo:hi] = dext[K - 1:]
+            dstate[b] = dext[:K - 1]
+    if s['pass_'] == 'fwd':
+        return dict(y=y, state=state)
+    return dict(dx=dx, dw=dw, db=db, dstate=None if s['state'] is None else dstate)
+
+
+def _exact_norm(s):
+    eps, D = 1e-5, s['width']
+    y, r, wp = s['y'].double(), s['residual'].double(), s['w_post'].double()
+    z = None if s['z'] is None else s['z'].double()
+    sc = torch.ones_like(wp) if s['s'] is None else s['s'].double()
+    sig = None if z is None else torch.sigmoid(z)
+    g = y if z is None else y * z * sig
+    i1 = 1.0 / torch.sqrt((g * g).sum(-1, keepdim=True) / D + eps)
+    u = g * i1
+    out = r + sc * wp * u
+    i2 = 1.0 / torch.sqrt((out * out).sum(-1, keepdim=True) / D + eps)
+    v = out * i2
+    wq = None if s['w_pre'] is None else s['w_pre'].double()
+    if s['pass_'] == 'fwd':
+        return dict(r=out, x=None if wq is None else wq * v)
+    dr = s['dr'].double()
+    if wq is not None:
+        dx = s['dx'].double()
+        dv = dx * wq
+        dr = dr + i2 * (dv - v * (dv * v).sum(-1, keepdim=True) / D)
+    du = dr * sc * wp
+    dg = i1 * (du - u * (du * u).sum(-1, keepdim=True) / D)
+    dy = dg if z is None else dg * z * sig
+    dz = None if z is None else dg * y * sig * (1 + z * (1 - sig))
+    return dict(dy=dy, dr=dr, dw_post=(dr * sc * u).sum(0), dz=dz, ds=None if s['s'] is None else (dr * wp * u).sum(0),
+                dw_pre=None if wq is None else (dx * v).sum(0))
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    if case['op'] == 'clip':
+        norms = torch.stack([g.double().norm() for g in s['grads']])
+        total = norms.norm()
+        c = min(1.0, s['max_norm'] / (float(total) + 1e-6))
+        return dict(total=total, norms=norms, grads=[g.double() * c for g in s['grads']])
+    if case['op'] == 'norm':
+        return _exact_norm(s)
+    if case['op'] == 'conv':
+        return _exact_conv(s)
+    if case['pass_'] == 'step':
+        n, H, P, G, N = s['n_seq'], s['H'], s['P'], s['G'], s['N']
+        raw = s['dt'].double() + s['dt_bias'].double()
+        step = torch.logaddexp(raw, torch.zeros_like(raw))
+        h = torch.zeros(n, H, P, N, dtype=torch.float64, device='cuda') if s['h0'] is None else s['h0'].double()
+        h = h * torch.exp(step * s['A'].double())[..., None, None]
+        x, C = s['x'].double(), s['C'].double()
+        y = torch.zeros(n, H, P, dtype=torch.float64, device='cuda')
+        for k in range(H):
+            grp = k // (H // G)
+            h[:, k] += (step[:, k, None] * x[:, k])[..., None] * s['B'][:, grp, None].double()
+            y[:, k] = (h[:, k] * C[:, grp, None]).sum(-1) + s['D'][k].double() * x[:, k]
+        return dict(y=y, h=h)
+    return _exact_scan(s)
