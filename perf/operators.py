@@ -160,6 +160,9 @@ def prepare(case, seed):
         # the bound is passed by far or not at all: a training run sees both
         s['out'] = [torch.empty_like(t) for t in s['grads']]   # the buffers that the clipped gradients go to, kept from step to step
         s['max_norm'] = 1e-2 * total * (0.25 if case['clips'] else 4.0)
+        if own:                                                # the handle over the step's gradient buffers, built once
+            from dotaclient_amd import ops
+            s['clip'] = ops.GradNormClip(s['grads'], out=s['out'])
         return s
     dt = DTYPES[case['dtype']]
     rows = case['rows']
@@ -357,7 +360,7 @@ def _run_own(s):
     from dotaclient_amd import ops
     op, pass_ = s['op'], s['pass_']
     if op == 'clip':
-        total, norms = ops.grad_norm_clip(s['grads'], s['max_norm'], out=s['out'])
+        total, norms = s['clip'](s['max_norm'])
         return dict(total=total, norms=norms, grads=s['out'])
     if op == 'norm':
         if pass_ == 'fwd':
