@@ -40,6 +40,15 @@ SIGNATURES = {
     'dc_policy_backward': (c_int, [c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr]),
     'dc_gradnorm_clip_adam': (c_int, [c_ptr, c_ptr, c_ptr, c_int, c_int] + [c_ptr] * 11 +
                               [c_flt, c_flt, c_dbl, c_dbl, c_dbl, c_flt, c_ptr]),
+    'dc_causal_conv_fwd': (c_int, [c_ptr, c_i64] + [c_ptr] * 4 + [c_i64] + [c_int] * 6 + [c_ptr, c_ptr, c_i64, c_ptr, c_ptr]),
+    'dc_causal_conv_scratch': (c_i64, [c_int] * 4),
+    'dc_causal_conv_bwd': (c_int, [c_ptr, c_i64] * 2 + [c_ptr] * 4 + [c_i64] + [c_int] * 6 + [c_ptr, c_ptr, c_ptr, c_i64] + [c_ptr] * 4 + [c_i64, c_ptr]),
+    'dc_causal_conv_step': (c_int, [c_ptr, c_i64] + [c_ptr] * 3 + [c_int] * 5 + [c_ptr, c_i64, c_ptr, c_ptr]),
+    'dc_block_norm_fwd': (c_int, [c_ptr, c_i64] * 3 + [c_ptr] * 3 + [c_i64] + [c_int] * 3 + [c_flt] + [c_ptr, c_i64] * 2 + [c_ptr]),
+    'dc_block_norm_scratch': (c_i64, [c_i64, c_int]),
+    'dc_block_norm_bwd': (c_int, [c_ptr, c_i64] * 5 + [c_ptr] * 3 + [c_i64] + [c_int] * 3 + [c_flt] + [c_ptr] * 7 + [c_i64, c_ptr]),
+    'dc_grad_norm_clip_scratch': (c_i64, [c_ptr, c_int]),
+    'dc_grad_norm_clip': (c_int, [c_ptr] * 4 + [c_int, c_flt] + [c_ptr] * 3 + [c_i64, c_ptr]),
 }
 
 DC_SINGLE_SCRATCH_FLOATS = 20480      # include/dotaclient_hip.h

@@ -1,0 +1,307 @@
+// The norms after and before a block, fused with the block's gate, its residual scale and the residual stream.
+//
+//   g  = y * z * sigmoid(z)                (gate z; g = y without one)
+//   u  = g * i1,  i1 = 1 / sqrt(mean(g^2) + eps)
+//   r' = r + s * w_post * u                (scale s; 1 without one)
+//   v  = r' * i2, i2 = 1 / sqrt(mean(r'^2) + eps),    x' = w_pre * v   (the next block's input; left out without w_pre)
+// and backwards, with R = dr' + i2 * (e - v * mean(e * v)), e = dx' * w_pre:
+//   dr = R,  du = R * s * w_post,  dg = i1 * (du - u * mean(du * u)),  dy = dg * z sigmoid(z),  dz = dg * y * sigmoid(z) * (1 + z * (1 - sigmoid(z)))
+//   q = sum over rows of R * u:  dw_post = s * q,  ds = w_post * q;     dw_pre = sum over rows of dx' * v
+//
+// Bound by HBM: forward reads y, z, r and writes r', x'; backward reads y, z, r, dr', dx' (r' is recomputed in 32 bits, so both passes use
+// the same unrounded r') and writes dy, dz, dr.  A row lives in the registers of WPR waves, EPL elements per lane, read once; the means
+// are wave sums (through LDS where WPR > 1).  Backward's column sums stay in registers over a workgroup's rows and are joined in a fixed
+// order by a second kernel: no atomics.
+#include "op_util.h"
+#include <initializer_list>
+
+namespace dc {
+namespace {
+
+struct NormArgs {
+    const void* y; int64_t ldy; const void* z; int64_t ldz; const void* r; int64_t ldr;
+    const float* w_post; const float* s; const float* w_pre;
+    int64_t rows; int D; float eps;
+    void* r_out; int64_t ldro; void* x_out; int64_t ldxo;                                              // forward
+    const void* dr; int64_t lddr; const void* dx; int64_t lddx; void* dy; void* dz; void* dres;        // backward; dy, dz, dres are contiguous
+    float* part; int n_blocks;
+};
+
+// Sum of a value over the WPR waves that hold a row; every lane gets it.  `slot` alternates so that one barrier per sum is enough.
+template <int WPR>
+__device__ __forceinline__ float row_sum(float v, float (*red)[WPR], int slot) {
+    v = wave_sum(v);
+    if constexpr (WPR > 1) {
+        if ((threadIdx.x & 63) == 0) red[slot][threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = 0.f;
+#pragma unroll
+        for (int w = 0; w < WPR; ++w) v += red[slot][w];
+    }
+    return v;
+}
+
+// Element e of lane l of a row's WPR * 64 lanes: vector e / V of that lane, column ((e / V) * lanes + l) * V + e % V.
+template <typename T, int V, int LANES, int EPL>
+__device__ __forceinline__ void load_row(const T* __restrict__ p, int l, int D, float (&f)[EPL]) {
+#pragma unroll
+    for (int i = 0; i < EPL / V; ++i) {
+        const int c = (i * LANES + l) * V;
+        float t[V];
+        if (c < D) load_vec<T, V>(p + c, t);
+#pragma unroll
+        for (int e = 0; e < V; ++e) f[i * V + e] = c < D ? t[e] : 0.f;
+    }
+}
+template <typename T, int V, int LANES, int EPL>
+__device__ __forceinline__ void store_row(T* __restrict__ p, int l, int D, const float (&f)[EPL]) {
+#pragma unroll
+    for (int i = 0; i < EPL / V; ++i) {
+        const int c = (i * LANES + l) * V;
+        float t[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) t[e] = f[i * V + e];
+        if (c < D) store_vec<T, V>(p + c, t);
+    }
+}
+
+template <typename T, typename R, int V, int WPR, int EPL>
+__global__ void __launch_bounds__(WPR == 1 ? 256 : WPR * 64) norm_fwd_kernel(NormArgs a) {
+    constexpr int LANES = WPR * 64, RPB = WPR == 1 ? 4 : 1;
+    const int l = WPR == 1 ? threadIdx.x & 63 : threadIdx.x;
+    __shared__ float red[2][WPR];
+    const int64_t row = (int64_t)blockIdx.x * RPB + (WPR == 1 ? threadIdx.x >> 6 : 0);
+    if (row >= a.rows) return;                               // whole waves (WPR == 1) or the whole workgroup
+    const int D = a.D;
+    float g[EPL], r[EPL], w[EPL];
+    load_row<T, V, LANES, EPL>(static_cast<const T*>(a.y) + row * a.ldy, l, D, g);
+    if (a.z) load_row<T, V, LANES, EPL>(static_cast<const T*>(a.z) + row * a.ldz, l, D, w);
+    load_row<R, V, LANES, EPL>(static_cast<const R*>(a.r) + row * a.ldr, l, D, r);
+    if (a.z) {
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) g[e] *= w[e] * sigmoid_fast(w[e]);
+    }
+    load_row<float, V, LANES, EPL>(a.w_post, l, D, w);
+    float sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) sum = fmaf(g[e], g[e], sum);
+    const float i1 = rsqrtf(row_sum<WPR>(sum, red, 0) / D + a.eps);
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) g[e] *= i1 * w[e];
+    if (a.s) {
+        load_row<float, V, LANES, EPL>(a.s, l, D, w);
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) g[e] *= w[e];
+    }
+    sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) { r[e] += g[e]; sum = fmaf(r[e], r[e], sum); }
+    store_row<R, V, LANES, EPL>(static_cast<R*>(a.r_out) + row * a.ldro, l, D, r);
+    if (!a.w_pre) return;
+    load_row<float, V, LANES, EPL>(a.w_pre, l, D, w);
+    const float i2 = rsqrtf(row_sum<WPR>(sum, red, 1) / D + a.eps);
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) r[e] *= i2 * w[e];
+    store_row<T, V, LANES, EPL>(static_cast<T*>(a.x_out) + row * a.ldxo, l, D, r);
+}
+
+template <typename T, typename R, int V, int WPR, int EPL>
+__global__ void __launch_bounds__(WPR == 1 ? 256 : WPR * 64) norm_bwd_kernel(NormArgs a) {
+    constexpr int LANES = WPR * 64, RPB = WPR == 1 ? 4 : 1;
+    const int l = WPR == 1 ? threadIdx.x & 63 : threadIdx.x, wv = threadIdx.x >> 6;
+    __shared__ float red[4][WPR];
+    const int D = a.D;
+    float q[EPL] = {}, dwp[EPL] = {}, sw[EPL], wq[EPL];
+    load_row<float, V, LANES, EPL>(a.w_post, l, D, sw);
+    if (a.s) {
+        load_row<float, V, LANES, EPL>(a.s, l, D, wq);
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) sw[e] *= wq[e];
+    }
+    if (a.w_pre) load_row<float, V, LANES, EPL>(a.w_pre, l, D, wq);
+    for (int64_t row = (int64_t)blockIdx.x * RPB + (WPR == 1 ? wv : 0); row < a.rows; row += (int64_t)a.n_blocks * RPB) {
+        float y[EPL], z[EPL], r[EPL], d[EPL], x[EPL];
+        load_row<T, V, LANES, EPL>(static_cast<const T*>(a.y) + row * a.ldy, l, D, y);
+        if (a.z) load_row<T, V, LANES, EPL>(static_cast<const T*>(a.z) + row * a.ldz, l, D, z);
+        load_row<R, V, LANES, EPL>(static_cast<const R*>(a.r) + row * a.ldr, l, D, r);
+        load_row<R, V, LANES, EPL>(static_cast<const R*>(a.dr) + row * a.lddr, l, D, d);
+        if (a.w_pre) load_row<T, V, LANES, EPL>(static_cast<const T*>(a.dx) + row * a.lddx, l, D, x);
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) {
+            const float g = a.z ? y[e] * (z[e] * sigmoid_fast(z[e])) : y[e];
+            sum = fmaf(g, g, sum);
+        }
+        const float i1 = rsqrtf(row_sum<WPR>(sum, red, 0) / D + a.eps);
+        float u[EPL];
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) u[e] = (a.z ? y[e] * (z[e] * sigmoid_fast(z[e])) : y[e]) * i1;
+        if (a.w_pre) {
+            float s2 = 0.f, se = 0.f;
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) {
+                r[e] = fmaf(u[e], sw[e], r[e]);
+                s2 = fmaf(r[e], r[e], s2);
+                se = fmaf(x[e] * wq[e], r[e], se);
+            }
+            s2 = row_sum<WPR>(s2, red, 1);
+            se = row_sum<WPR>(se, red, 2);
+            const float i2 = rsqrtf(s2 / D + a.eps), m = se * i2 / D;            // mean(e * v)
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) {
+                const float v = r[e] * i2;
+                dwp[e] = fmaf(x[e], v, dwp[e]);
+                d[e] = fmaf(i2, x[e] * wq[e] - v * m, d[e]);
+            }
+        }
+        store_row<R, V, LANES, EPL>(static_cast<R*>(a.dres) + row * D, l, D, d);
+        float du = 0.f;
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) {
+            q[e] = fmaf(d[e], u[e], q[e]);
+            d[e] *= sw[e];
+            du = fmaf(d[e], u[e], du);
+        }
+        du = row_sum<WPR>(du, red, 3) / D;
+        if (a.z) {
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) {
+                const float dg = i1 * (d[e] - u[e] * du), s = sigmoid_fast(z[e]);
+                d[e] = dg * (z[e] * s);
+                z[e] = dg * y[e] * s * fmaf(z[e], 1.f - s, 1.f);
+            }
+            store_row<T, V, LANES, EPL>(static_cast<T*>(a.dz) + row * D, l, D, z);
+        } else {
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) d[e] = i1 * (d[e] - u[e] * du);
+        }
+        store_row<T, V, LANES, EPL>(static_cast<T*>(a.dy) + row * D, l, D, d);
+        if constexpr (WPR > 1) __syncthreads();                                  // red[0] of the next row
+    }
+    // the workgroup's column sums: its RPB rows' waves through LDS
+    float* part = a.part + (int64_t)blockIdx.x * 2 * D;
+    if constexpr (WPR == 1) {
+        __shared__ float cols[4][64 * EPL];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) cols[wv][e * 64 + l] = k ? dwp[e] : q[e];
+            __syncthreads();
+            for (int i = threadIdx.x; i < 64 * EPL; i += 256) {
+                const int c = ((i / 64 / V) * 64 + i % 64) * V + i / 64 % V;
+                if (c < D) part[k * D + c] = (cols[0][i] + cols[1][i]) + (cols[2][i] + cols[3][i]);
+            }
+        }
+    } else {
+        store_row<float, V, LANES, EPL>(part, l, D, q);
+        store_row<float, V, LANES, EPL>(part + D, l, D, dwp);
+    }
+}
+
+// part [n_blocks][2][D] -> dw_post = s * q, ds = w_post * q, dw_pre
+__global__ void __launch_bounds__(1024) norm_reduce_kernel(const float* __restrict__ part, int n_blocks, int D, const float* __restrict__ w_post,
+                                                           const float* __restrict__ s, float* __restrict__ dw_post, float* __restrict__ ds,
+                                                           float* __restrict__ dw_pre) {
+    const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5;
+    const int i = blockIdx.x * 32 + lane, n = 2 * D;
+    __shared__ float red[32][33];
+    float sum = 0.f;
+    if (i < n)
+#pragma unroll 8
+        for (int p = grp; p < n_blocks; p += 32) sum += part[(int64_t)p * n + i];
+    red[grp][lane] = sum;
+    __syncthreads();
+    if (grp == 0 && i < n) {
+        for (int g = 1; g < 32; ++g) sum += red[g][lane];
+        if (i < D) {
+            dw_post[i] = s ? s[i] * sum : sum;
+            if (ds) ds[i] = w_post[i] * sum;
+        } else if (dw_pre) {
+            dw_pre[i - D] = sum;
+        }
+    }
+}
+
+// Four neighbouring elements per access (16 bytes of f32, 8 of bf16) where every row of every tensor starts on such a boundary.
+bool aligned_to(uintptr_t bytes, std::initializer_list<const void*> t) {
+    for (const void* p : t)
+        if (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) return false;
+    return true;
+}
+bool whole_fours(std::initializer_list<int64_t> lds) {
+    for (int64_t ld : lds)
+        if (ld % 4) return false;
+    return true;
+}
+
+// Waves per row and elements per lane: the fewest that hold the row; 16 elements per lane at most, so that backward's five rows stay in registers.
+#define NORM_SHAPES(KERNEL, T, R, V, GRID)                                                                                          \
+    do {                                                                                                                            \
+        if (a.D <= 512) hipLaunchKernelGGL((KERNEL<T, R, V, 1, 8>), GRID(4), dim3(256), 0, st, a);                                  \
+        else if (a.D <= 1024) hipLaunchKernelGGL((KERNEL<T, R, V, 1, 16>), GRID(4), dim3(256), 0, st, a);                           \
+        else if (a.D <= 4096) hipLaunchKernelGGL((KERNEL<T, R, V, 4, 16>), GRID(1), dim3(256), 0, st, a);                           \
+        else hipLaunchKernelGGL((KERNEL<T, R, V, 8, 16>), GRID(1), dim3(512), 0, st, a);                                            \
+    } while (0)
+#define NORM_DISPATCH(KERNEL, GRID)                                                                                                 \
+    do {                                                                                                                            \
+        if (type == 0) { if (vec) NORM_SHAPES(KERNEL, float, float, 4, GRID); else NORM_SHAPES(KERNEL, float, float, 1, GRID); }    \
+        else if (rtype == 0) { if (vec) NORM_SHAPES(KERNEL, bf16_t, float, 4, GRID); else NORM_SHAPES(KERNEL, bf16_t, float, 1, GRID); }   \
+        else { if (vec) NORM_SHAPES(KERNEL, bf16_t, bf16_t, 4, GRID); else NORM_SHAPES(KERNEL, bf16_t, bf16_t, 1, GRID); }          \
+    } while (0)
+
+int check_common(const char* what, const NormArgs& a, int type, int rtype) {
+    if (type < 0 || type > 1 || rtype < 0 || rtype > type) { set_error(what, 1101); return 1101; }
+    if (a.D < 1 || a.D > 8192) { set_error(what, 1102); return 1102; }
+    if (a.rows < 0 || a.rows > 0x7fffffff) { set_error(what, 1103); return 1103; }
+    if (!a.w_post || (a.rows && (!a.y || !a.r))) { set_error(what, 1104); return 1104; }
+    return 0;
+}
+
+int bwd_blocks(int64_t rows, int D) {
+    const int64_t want = D <= 1024 ? (rows + 3) / 4 : rows;
+    return (int)(want < 1024 ? want : 1024);
+}
+
+}  // namespace
+
+int block_norm_fwd(const void* y, int64_t ldy, const void* z, int64_t ldz, const void* r, int64_t ldr, const float* w_post, const float* s,
+                   const float* w_pre, int64_t rows, int D, int type, int rtype, float eps, void* r_out, int64_t ldro, void* x_out, int64_t ldxo,
+                   hipStream_t st) {
+    NormArgs a = {};
+    a.y = y; a.ldy = ldy; a.z = z; a.ldz = ldz; a.r = r; a.ldr = ldr; a.w_post = w_post; a.s = s; a.w_pre = w_pre; a.rows = rows; a.D = D; a.eps = eps;
+    a.r_out = r_out; a.ldro = ldro; a.x_out = x_out; a.ldxo = ldxo;
+    if (int rc = check_common("dc_block_norm_fwd", a, type, rtype)) return rc;
+    if (rows == 0) return 0;
+    if (!r_out || (w_pre && !x_out)) { set_error("dc_block_norm_fwd", 1104); return 1104; }
+    const bool vec = aligned_to(type ? 8 : 16, {y, z, x_out}) && aligned_to(rtype ? 8 : 16, {r, r_out}) && aligned_to(16, {w_post, s, w_pre}) &&
+                     whole_fours({D, ldy, z ? ldz : 0, ldr, ldro, w_pre ? ldxo : 0});
+#define NORM_GRID(RPB) dim3((unsigned)((rows + RPB - 1) / RPB))
+    NORM_DISPATCH(norm_fwd_kernel, NORM_GRID);
+    return launch_check("dc_block_norm_fwd");
+}
+
+int64_t block_norm_scratch(int64_t rows, int D) { return (int64_t)bwd_blocks(rows, D) * 2 * D * (int64_t)sizeof(float); }
+
+int block_norm_bwd(const void* dr, int64_t lddr, const void* dx, int64_t lddx, const void* y, int64_t ldy, const void* z, int64_t ldz, const void* r,
+                   int64_t ldr, const float* w_post, const float* s, const float* w_pre, int64_t rows, int D, int type, int rtype, float eps, void* dy,
+                   void* dz, void* dres, float* dw_post, float* ds, float* dw_pre, float* scratch, int64_t scratch_bytes, hipStream_t st) {
+    NormArgs a = {};
+    a.y = y; a.ldy = ldy; a.z = z; a.ldz = ldz; a.r = r; a.ldr = ldr; a.w_post = w_post; a.s = s; a.w_pre = w_pre; a.rows = rows; a.D = D; a.eps = eps;
+    a.dr = dr; a.lddr = lddr; a.dx = dx; a.lddx = lddx; a.dy = dy; a.dz = dz; a.dres = dres; a.part = scratch; a.n_blocks = bwd_blocks(rows, D);
+    if (int rc = check_common("dc_block_norm_bwd", a, type, rtype)) return rc;
+    if (!dw_post || (rows && (!dr || !dy || !dres || (z && !dz) || (w_pre && !dx)))) { set_error("dc_block_norm_bwd", 1104); return 1104; }
+    if (scratch_bytes < block_norm_scratch(rows, D) || (rows && !scratch)) { set_error("dc_block_norm_bwd: scratch", 1105); return 1105; }
+    if (rows) {
+        const bool vec = aligned_to(type ? 8 : 16, {y, z, dx, dy, dz}) && aligned_to(rtype ? 8 : 16, {r, dr, dres}) &&
+                         aligned_to(16, {w_post, s, w_pre, scratch}) && whole_fours({D, lddr, w_pre ? lddx : 0, ldy, z ? ldz : 0, ldr});
+#define NORM_BGRID(RPB) dim3((unsigned)a.n_blocks)
+        NORM_DISPATCH(norm_bwd_kernel, NORM_BGRID);
+        if (int rc = launch_check("dc_block_norm_bwd")) return rc;
+    }
+    hipLaunchKernelGGL(norm_reduce_kernel, dim3((2 * D + 31) / 32), dim3(1024), 0, st, scratch, a.n_blocks, D, w_post, s, dw_post, s ? ds : nullptr,
+                       w_pre ? dw_pre : nullptr);
+    return launch_check("dc_block_norm_bwd");
+}
+
+}  // namespace dc

@@ -193,4 +193,54 @@ int dc_dp_average_grads(const int64_t* seg_off, const int32_t* seg_len, const in
     return dc::dp_average_grads(seg_off, seg_len, seg_gate, n_seg, max_seg_len, grads, counts, vf_coef, (hipStream_t)stream);
 }
 
+int dc_causal_conv_fwd(const void* x, int64_t ldx, const float* w, const float* bias, const int64_t* seq_off, const int32_t* seq_len, int64_t rows,
+                       int n_seq, int max_len, int D, int K, int type, int silu, const void* state, void* y, int64_t ldy, void* state_out,
+                       dc_stream_t stream) {
+    DC_ENTER();
+    return dc::causal_conv_fwd(x, ldx, w, bias, seq_off, seq_len, rows, n_seq, max_len, D, K, type, silu, state, y, ldy, state_out, (hipStream_t)stream);
+}
+
+int64_t dc_causal_conv_scratch(int n_seq, int max_len, int D, int K) { return dc::causal_conv_scratch(n_seq, max_len, D, K); }
+
+int dc_causal_conv_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const float* w, const float* bias, const int64_t* seq_off,
+                       const int32_t* seq_len, int64_t rows, int n_seq, int max_len, int D, int K, int type, int silu, const void* state,
+                       const void* dstate_out, void* dx, int64_t lddx, float* dw, float* dbias, void* dstate, float* scratch, int64_t scratch_bytes,
+                       dc_stream_t stream) {
+    DC_ENTER();
+    return dc::causal_conv_bwd(dy, lddy, x, ldx, w, bias, seq_off, seq_len, rows, n_seq, max_len, D, K, type, silu, state, dstate_out, dx, lddx, dw, dbias,
+                               dstate, scratch, scratch_bytes, (hipStream_t)stream);
+}
+
+int dc_causal_conv_step(const void* x, int64_t ldx, const void* state, const float* w, const float* bias, int n_seq, int D, int K, int type, int silu,
+                        void* y, int64_t ldy, void* state_out, dc_stream_t stream) {
+    DC_ENTER();
+    return dc::causal_conv_step(x, ldx, state, w, bias, n_seq, D, K, type, silu, y, ldy, state_out, (hipStream_t)stream);
+}
+
+int dc_block_norm_fwd(const void* y, int64_t ldy, const void* gate, int64_t ldg, const void* r, int64_t ldr, const float* w_post, const float* scale,
+                      const float* w_pre, int64_t rows, int D, int type, int rtype, float eps, void* r_out, int64_t ldro, void* x_out, int64_t ldxo,
+                      dc_stream_t stream) {
+    DC_ENTER();
+    return dc::block_norm_fwd(y, ldy, gate, ldg, r, ldr, w_post, scale, w_pre, rows, D, type, rtype, eps, r_out, ldro, x_out, ldxo, (hipStream_t)stream);
+}
+
+int64_t dc_block_norm_scratch(int64_t rows, int D) { return dc::block_norm_scratch(rows, D); }
+
+int dc_block_norm_bwd(const void* dr_out, int64_t lddr, const void* dx_out, int64_t lddx, const void* y, int64_t ldy, const void* gate, int64_t ldg,
+                      const void* r, int64_t ldr, const float* w_post, const float* scale, const float* w_pre, int64_t rows, int D, int type, int rtype,
+                      float eps, void* dy, void* dgate, void* dr, float* dw_post, float* dscale, float* dw_pre, float* scratch, int64_t scratch_bytes,
+                      dc_stream_t stream) {
+    DC_ENTER();
+    return dc::block_norm_bwd(dr_out, lddr, dx_out, lddx, y, ldy, gate, ldg, r, ldr, w_post, scale, w_pre, rows, D, type, rtype, eps, dy, dgate, dr, dw_post,
+                              dscale, dw_pre, scratch, scratch_bytes, (hipStream_t)stream);
+}
+
+int64_t dc_grad_norm_clip_scratch(const int64_t* sizes_host, int n) { return sizes_host ? dc::grad_norm_clip_scratch(sizes_host, n) : 0; }
+
+int dc_grad_norm_clip(const int64_t* grads_host, const int64_t* outs_host, const int64_t* sizes_host, const int32_t* types_host, int n, float max_norm,
+                      float* total, float* norms, double* scratch, int64_t scratch_bytes, dc_stream_t stream) {
+    DC_ENTER();
+    return dc::grad_norm_clip(grads_host, outs_host, sizes_host, types_host, n, max_norm, total, norms, scratch, scratch_bytes, (hipStream_t)stream);
+}
+
 }  // extern "C"

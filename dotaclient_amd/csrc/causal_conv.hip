@@ -1,0 +1,368 @@
+// Short causal depthwise convolution over packed sequences, with the state that carries it from chunk to chunk.
+//
+//   v[t,d] = bias[d] + sum_k w[d,k] * ext[t + k, d],   ext = (state rows | x rows) of the sequence, k = 0 .. K-1
+//   y[t,d] = v * sigmoid(v)   (silu)   or   v
+//   state_out = the last K-1 rows of ext
+// and backwards, with dv = dy * act'(v):
+//   dext[i,d] = sum_k w[d,k] * dv[i - k, d]  (+ dstate_out on the last K-1 rows);  dx, dstate = its two parts
+//   dw[d,k]   = sum_t dv[t,d] * ext[t + k, d],   dbias[d] = sum_t dv[t,d]
+//
+// Bound by HBM: every row is read and written once, 2 K flops per element.  A thread owns V neighbouring channels and CROWS
+// consecutive rows of one sequence: the K-1 rows in front of them come from the L2 (the neighbouring thread group loads them too), all
+// loads are issued before the first use.  Backward recomputes v; the weights' gradients are summed per thread over its chunks of rows,
+// in LDS over a workgroup's chunks and, in a fixed order, by a second kernel over the workgroups: no atomics.
+#include "op_util.h"
+#include <initializer_list>
+
+namespace dc {
+namespace {
+
+constexpr int CROWS = 8;       // rows per thread
+constexpr int CLANES = 32;     // channel vectors of a workgroup
+constexpr int CGROUPS = 8;     // chunks of rows of a workgroup
+
+struct ConvArgs {
+    const void* x; int64_t ldx;
+    const float* w; const float* bias;
+    const int64_t* seq_off; const int32_t* seq_len;
+    int64_t rows; int n_seq, max_len, D, K, silu;
+    int chunks_per_seq; int64_t n_chunks;
+    const void* state;                       // [n_seq][K-1][D] or null
+    void* y; int64_t ldy; void* state_out;   // forward
+    const void* dy; int64_t lddy; const void* dstate_out; void* dx; int64_t lddx; void* dstate; float* part; int n_row_blocks;   // backward
+};
+
+// Row t of a sequence's ext, t >= -(K-1): x for t >= 0, the state below, zeros where there is neither.
+template <typename T, int V>
+__device__ __forceinline__ void load_ext(const ConvArgs& a, const SeqRange& q, int b, int t, int d0, float (&f)[V]) {
+    if (t >= 0 && t < q.len) {
+        load_vec<T, V>(static_cast<const T*>(a.x) + (q.off + t) * a.ldx + d0, f);
+    } else if (t < 0 && t >= -(a.K - 1) && a.state) {
+        load_vec<T, V>(static_cast<const T*>(a.state) + ((int64_t)b * (a.K - 1) + (t + a.K - 1)) * a.D + d0, f);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) f[i] = 0.f;
+    }
+}
+
+// Taps right-aligned in KM: tap j of KM multiplies ext row t - (KM-1) + j.  KM = K for K up to 4; for 5 .. 8 KM is 8 and the first KM - K
+// taps do not exist: a uniform branch skips them (a zero tap would turn an infinity outside the window into NaN).
+template <int KM>
+__device__ __forceinline__ bool has_tap(const ConvArgs& a, int j) { return KM <= 4 || j >= KM - a.K; }
+
+template <int V, int KM>
+__device__ __forceinline__ void load_taps(const ConvArgs& a, int d0, float (&w)[KM][V], float (&bias)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        bias[i] = a.bias ? a.bias[d0 + i] : 0.f;
+#pragma unroll
+        for (int j = 0; j < KM; ++j) w[j][i] = has_tap<KM>(a, j) ? a.w[(int64_t)(d0 + i) * a.K + j - (KM - a.K)] : 0.f;
+    }
+}
+
+// bias + the taps of KM rows of ext, from row i on
+template <int V, int KM, int N>
+__device__ __forceinline__ void taps(const ConvArgs& a, const float (&w)[KM][V], const float (&bias)[V], const float (&ext)[N][V], int i, float (&v)[V]) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = bias[e];
+#pragma unroll
+    for (int j = 0; j < KM; ++j)
+        if (has_tap<KM>(a, j)) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] = fmaf(w[j][e], ext[i + j][e], v[e]);
+        }
+}
+
+template <typename T, int V, int KM>
+__global__ void __launch_bounds__(256) conv_fwd_kernel(ConvArgs a) {
+    const int d0 = (blockIdx.y * CLANES + (threadIdx.x & (CLANES - 1))) * V;
+    const int64_t chunk = (int64_t)blockIdx.x * CGROUPS + threadIdx.x / CLANES;
+    if (d0 >= a.D || chunk >= a.n_chunks) return;
+    const int b = (int)(chunk / a.chunks_per_seq), t0 = (int)(chunk % a.chunks_per_seq) * CROWS;
+    const SeqRange q = seq_range(a.seq_off, a.seq_len, b, a.rows, a.max_len);
+    if (t0 == 0 && a.state_out) {
+        for (int j = 0; j < a.K - 1; ++j) {
+            float f[V];
+            load_ext<T, V>(a, q, b, q.len - (a.K - 1) + j, d0, f);
+            store_vec<T, V>(static_cast<T*>(a.state_out) + ((int64_t)b * (a.K - 1) + j) * a.D + d0, f);
+        }
+    }
+    if (t0 >= q.len) return;
+    float ext[CROWS + KM - 1][V];
+#pragma unroll
+    for (int i = 0; i < CROWS + KM - 1; ++i) load_ext<T, V>(a, q, b, t0 - (KM - 1) + i, d0, ext[i]);
+    float w[KM][V], bias[V];
+    load_taps<V, KM>(a, d0, w, bias);
+#pragma unroll
+    for (int r = 0; r < CROWS; ++r) {
+        if (t0 + r >= q.len) break;
+        float v[V];
+        taps<V, KM>(a, w, bias, ext, r, v);
+        if (a.silu) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] *= sigmoid_fast(v[i]);
+        }
+        store_vec<T, V>(static_cast<T*>(a.y) + (q.off + t0 + r) * a.ldy + d0, v);
+    }
+}
+
+template <typename T, int V, int KM>
+__global__ void __launch_bounds__(256) conv_bwd_kernel(ConvArgs a) {
+    const int lane = threadIdx.x & (CLANES - 1), grp = threadIdx.x / CLANES;
+    const int d0 = (blockIdx.y * CLANES + lane) * V;
+    const bool live = d0 < a.D;
+    float w[KM][V], bias[V], dw[KM][V] = {}, db[V] = {};
+    if (live) load_taps<V, KM>(a, d0, w, bias);
+    for (int64_t c0 = (int64_t)blockIdx.x * CGROUPS; c0 < a.n_chunks; c0 += (int64_t)a.n_row_blocks * CGROUPS) {
+        const int64_t chunk = c0 + grp;
+        if (!live || chunk >= a.n_chunks) continue;
+        const int b = (int)(chunk / a.chunks_per_seq), t0 = (int)(chunk % a.chunks_per_seq) * CROWS;
+        const SeqRange q = seq_range(a.seq_off, a.seq_len, b, a.rows, a.max_len);
+        if (t0 > 0 && t0 >= q.len) continue;
+        // rows t0-(KM-1) .. t0+CROWS+KM-2 of ext, dv of t0 .. t0+CROWS+KM-2
+        float ext[CROWS + 2 * (KM - 1)][V], dv[CROWS + KM - 1][V];
+#pragma unroll
+        for (int i = 0; i < CROWS + 2 * (KM - 1); ++i) load_ext<T, V>(a, q, b, t0 - (KM - 1) + i, d0, ext[i]);
+#pragma unroll
+        for (int i = 0; i < CROWS + KM - 1; ++i) {
+            if (t0 + i < q.len) {
+                load_vec<T, V>(static_cast<const T*>(a.dy) + (q.off + t0 + i) * a.lddy + d0, dv[i]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; ++e) dv[i][e] = 0.f;
+            }
+        }
+        if (a.silu) {
+#pragma unroll
+            for (int i = 0; i < CROWS + KM - 1; ++i) {
+                float v[V];
+                taps<V, KM>(a, w, bias, ext, i, v);
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    const float s = sigmoid_fast(v[e]);
+                    if (t0 + i < q.len) dv[i][e] *= s * fmaf(v[e], 1.f - s, 1.f);
+                }
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < CROWS; ++r)
+            if (t0 + r < q.len) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) db[e] += dv[r][e];
+#pragma unroll
+                for (int j = 0; j < KM; ++j)
+                    if (has_tap<KM>(a, j)) {
+#pragma unroll
+                        for (int e = 0; e < V; ++e) dw[j][e] = fmaf(dv[r][e], ext[r + j][e], dw[j][e]);
+                    }
+            }
+        // dext of row t = sum_j w[j] dv[t + KM-1 - j]; the chunk at the start of a sequence also has the state's rows (t < 0)
+        auto dext = [&](int t, float (&f)[V]) {          // t relative to t0, compile-time in every call
+#pragma unroll
+            for (int e = 0; e < V; ++e) f[e] = 0.f;
+#pragma unroll
+            for (int j = 0; j < KM; ++j) {
+                const int i = t + KM - 1 - j;
+                if (i >= 0 && i < CROWS + KM - 1 && has_tap<KM>(a, j)) {
+#pragma unroll
+                    for (int e = 0; e < V; ++e) f[e] = fmaf(w[j][e], dv[i][e], f[e]);
+                }
+            }
+            const int j = t0 + t - q.len + a.K - 1;      // row of dstate_out
+            if (a.dstate_out && j >= 0 && j < a.K - 1) {
+                float g[V];
+                load_vec<T, V>(static_cast<const T*>(a.dstate_out) + ((int64_t)b * (a.K - 1) + j) * a.D + d0, g);
+#pragma unroll
+                for (int e = 0; e < V; ++e) f[e] += g[e];
+            }
+        };
+#pragma unroll
+        for (int r = 0; r < CROWS; ++r) {
+            if (t0 + r < q.len) {
+                float f[V];
+                dext(r, f);
+                store_vec<T, V>(static_cast<T*>(a.dx) + (q.off + t0 + r) * a.lddx + d0, f);
+            }
+        }
+        if (t0 == 0 && a.dstate) {
+#pragma unroll
+            for (int r = 1; r < KM; ++r) {
+                if (r < a.K) {
+                    float f[V];
+                    dext(-r, f);
+                    store_vec<T, V>(static_cast<T*>(a.dstate) + ((int64_t)b * (a.K - 1) + (a.K - 1 - r)) * a.D + d0, f);
+                }
+            }
+        }
+    }
+    __shared__ float red[CGROUPS][CLANES * V];
+    for (int j = 0; j <= KM; ++j) {                      // KM taps and the bias
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            float s = db[e];
+#pragma unroll
+            for (int jj = 0; jj < KM; ++jj) s = jj == j ? dw[jj][e] : s;
+            red[grp][e * CLANES + lane] = s;
+        }
+        __syncthreads();
+        if (j < KM - a.K) continue;
+        if ((int)threadIdx.x < CLANES * V) {
+            float s = 0.f;
+#pragma unroll
+            for (int g = 0; g < CGROUPS; ++g) s += red[g][threadIdx.x];
+            const int d = (blockIdx.y * CLANES + (threadIdx.x & (CLANES - 1))) * V + threadIdx.x / CLANES;
+            if (d < a.D) a.part[((int64_t)blockIdx.x * (a.K + 1) + (j - (KM - a.K))) * a.D + d] = s;
+        }
+    }
+}
+
+// part [n_row_blocks][K+1][D] -> dw [D][K], dbias [D]; the workgroups' sums in their order.
+__global__ void __launch_bounds__(256) conv_reduce_kernel(const float* __restrict__ part, int n_blocks, int D, int K, float* __restrict__ dw,
+                                                          float* __restrict__ dbias) {
+    const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5;
+    const int64_t i = (int64_t)blockIdx.x * 32 + lane, n = (int64_t)(K + 1) * D;
+    __shared__ float red[8][32];
+    float s = 0.f;
+    if (i < n)
+#pragma unroll 8
+        for (int p = grp; p < n_blocks; p += 8) s += part[p * n + i];
+    red[grp][lane] = s;
+    __syncthreads();
+    if (grp == 0 && i < n) {
+        for (int g = 1; g < 8; ++g) s += red[g][lane];
+        const int j = (int)(i / D), d = (int)(i % D);
+        if (j < K) dw[(int64_t)d * K + j] = s;
+        else if (dbias) dbias[d] = s;
+    }
+}
+
+// One row per sequence: state (oldest first) and x -> y, state moved up by one row.  state_out may be state.
+template <typename T, int V, int KM>
+__global__ void __launch_bounds__(256) conv_step_kernel(ConvArgs a) {
+    const int nv = a.D / V;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= (int64_t)a.n_seq * nv) return;
+    const int b = (int)(i / nv), d0 = (int)(i % nv) * V;
+    float ext[KM][V], w[KM][V], bias[V], v[V];
+    const SeqRange q = {b, 1};
+#pragma unroll
+    for (int j = 0; j < KM; ++j) load_ext<T, V>(a, q, b, j - (KM - 1), d0, ext[j]);
+    load_taps<V, KM>(a, d0, w, bias);
+    taps<V, KM>(a, w, bias, ext, 0, v);
+    if (a.silu) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] *= sigmoid_fast(v[e]);
+    }
+    store_vec<T, V>(static_cast<T*>(a.y) + b * a.ldy + d0, v);
+#pragma unroll
+    for (int j = 1; j < KM; ++j)
+        if (j >= KM - a.K + 1) store_vec<T, V>(static_cast<T*>(a.state_out) + ((int64_t)b * (a.K - 1) + (j - (KM - a.K) - 1)) * a.D + d0, ext[j]);
+}
+
+// Four channels per thread (16 bytes of f32, 8 of bf16) where every row of every tensor starts on such a boundary, else one.  (Eight bf16
+// channels would be 16 bytes too, but the backward kernel's rows then take 256 registers.)
+bool vector_rows(int type, int D, int64_t ldx, int64_t ldy, int64_t lddx, std::initializer_list<const void*> tensors) {
+    const uintptr_t mask = type ? 7 : 15;
+    for (const void* p : tensors)
+        if (reinterpret_cast<uintptr_t>(p) & mask) return false;
+    return D % 4 == 0 && ldx % 4 == 0 && ldy % 4 == 0 && lddx % 4 == 0;
+}
+
+#define CONV_LAUNCH(KERNEL, GRID, T, V)                                                                    \
+    do {                                                                                                   \
+        if (a.K == 2) hipLaunchKernelGGL((KERNEL<T, V, 2>), GRID(V), dim3(256), 0, s, a);                  \
+        else if (a.K == 3) hipLaunchKernelGGL((KERNEL<T, V, 3>), GRID(V), dim3(256), 0, s, a);             \
+        else if (a.K == 4) hipLaunchKernelGGL((KERNEL<T, V, 4>), GRID(V), dim3(256), 0, s, a);             \
+        else hipLaunchKernelGGL((KERNEL<T, V, 8>), GRID(V), dim3(256), 0, s, a);                           \
+    } while (0)
+#define CONV_DISPATCH(KERNEL, GRID)                                                                        \
+    do {                                                                                                   \
+        if (type == 0 && vec) CONV_LAUNCH(KERNEL, GRID, float, 4);                                         \
+        else if (type == 0) CONV_LAUNCH(KERNEL, GRID, float, 1);                                           \
+        else if (vec) CONV_LAUNCH(KERNEL, GRID, bf16_t, 4);                                                \
+        else CONV_LAUNCH(KERNEL, GRID, bf16_t, 1);                                                         \
+    } while (0)
+
+int check_common(const char* what, const ConvArgs& a, int type) {
+    if (type != 0 && type != 1) { set_error(what, 1101); return 1101; }
+    if (a.K < 2 || a.K > 8 || a.D < 1 || a.D > 1 << 20) { set_error(what, 1102); return 1102; }
+    if (a.rows < 0 || a.n_seq < 0 || a.max_len < 0) { set_error(what, 1103); return 1103; }
+    if (a.n_seq && (!a.x || !a.w)) { set_error(what, 1104); return 1104; }
+    return 0;
+}
+
+int row_blocks(int64_t n_chunks, int groups) {      // enough workgroups for every CU's waves, few partial sums
+    const int64_t want = (n_chunks + CGROUPS - 1) / CGROUPS;
+    const int64_t most = groups >= 16 ? 64 : 1024 / groups;
+    return (int)(want < most ? want : most);
+}
+
+}  // namespace
+
+int causal_conv_fwd(const void* x, int64_t ldx, const float* w, const float* bias, const int64_t* seq_off, const int32_t* seq_len, int64_t rows, int n_seq,
+                    int max_len, int D, int K, int type, int silu, const void* state, void* y, int64_t ldy, void* state_out, hipStream_t s) {
+    ConvArgs a = {};
+    a.x = x; a.ldx = ldx; a.w = w; a.bias = bias; a.seq_off = seq_off; a.seq_len = seq_len; a.rows = rows; a.n_seq = n_seq; a.max_len = max_len;
+    a.D = D; a.K = K; a.silu = silu; a.state = state; a.y = y; a.ldy = ldy; a.state_out = state_out;
+    if (int rc = check_common("dc_causal_conv_fwd", a, type)) return rc;
+    if (n_seq == 0) return 0;
+    a.chunks_per_seq = max_len ? (max_len + CROWS - 1) / CROWS : 1;
+    a.n_chunks = (int64_t)n_seq * a.chunks_per_seq;
+    const bool vec = vector_rows(type, D, ldx, ldy, 0, {x, y, state, state_out});
+    const int64_t gx = (a.n_chunks + CGROUPS - 1) / CGROUPS;
+    if (gx > 0x7fffffff) { set_error("dc_causal_conv_fwd", 1103); return 1103; }
+#define CONV_GRID(V) dim3((unsigned)gx, (D + CLANES * V - 1) / (CLANES * V))
+    CONV_DISPATCH(conv_fwd_kernel, CONV_GRID);
+    return launch_check("dc_causal_conv_fwd");
+}
+
+int64_t causal_conv_scratch(int n_seq, int max_len, int D, int K) {      // bytes, for either vector width
+    const int64_t n_chunks = (int64_t)n_seq * (max_len > 0 ? (max_len + CROWS - 1) / CROWS : 1);
+    return (int64_t)row_blocks(n_chunks, 1) * (K + 1) * D * (int64_t)sizeof(float);
+}
+
+int causal_conv_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const float* w, const float* bias, const int64_t* seq_off,
+                    const int32_t* seq_len, int64_t rows, int n_seq, int max_len, int D, int K, int type, int silu, const void* state,
+                    const void* dstate_out, void* dx, int64_t lddx, float* dw, float* dbias, void* dstate, float* scratch, int64_t scratch_bytes,
+                    hipStream_t s) {
+    ConvArgs a = {};
+    a.x = x; a.ldx = ldx; a.w = w; a.bias = bias; a.seq_off = seq_off; a.seq_len = seq_len; a.rows = rows; a.n_seq = n_seq; a.max_len = max_len;
+    a.D = D; a.K = K; a.silu = silu; a.state = state;
+    a.dy = dy; a.lddy = lddy; a.dstate_out = dstate_out; a.dx = dx; a.lddx = lddx; a.dstate = dstate; a.part = scratch;
+    if (int rc = check_common("dc_causal_conv_bwd", a, type)) return rc;
+    if (!dw) { set_error("dc_causal_conv_bwd", 1104); return 1104; }
+    a.chunks_per_seq = max_len ? (max_len + CROWS - 1) / CROWS : 1;
+    a.n_chunks = (int64_t)n_seq * a.chunks_per_seq;
+    const bool vec = vector_rows(type, D, ldx, lddy, lddx, {x, dy, state, dstate_out, dx, dstate});
+    const int lanes = CLANES * (vec ? 4 : 1), groups = (D + lanes - 1) / lanes;
+    a.n_row_blocks = row_blocks(a.n_chunks, groups);
+    if (scratch_bytes < (int64_t)a.n_row_blocks * (K + 1) * D * (int64_t)sizeof(float) || (!scratch && a.n_row_blocks)) {
+        set_error("dc_causal_conv_bwd: scratch", 1105);
+        return 1105;
+    }
+    if (n_seq) {
+#define CONV_BGRID(V) dim3((unsigned)a.n_row_blocks, (D + CLANES * V - 1) / (CLANES * V))
+        CONV_DISPATCH(conv_bwd_kernel, CONV_BGRID);
+        if (int rc = launch_check("dc_causal_conv_bwd")) return rc;
+    }
+    const int64_t n = (int64_t)(K + 1) * D;
+    hipLaunchKernelGGL(conv_reduce_kernel, dim3((unsigned)((n + 31) / 32)), dim3(256), 0, s, scratch, a.n_row_blocks, D, K, dw, dbias);
+    return launch_check("dc_causal_conv_bwd");
+}
+
+int causal_conv_step(const void* x, int64_t ldx, const void* state, const float* w, const float* bias, int n_seq, int D, int K, int type, int silu, void* y,
+                     int64_t ldy, void* state_out, hipStream_t s) {
+    ConvArgs a = {};
+    a.x = x; a.ldx = ldx; a.w = w; a.bias = bias; a.rows = n_seq; a.n_seq = n_seq; a.max_len = 1; a.D = D; a.K = K; a.silu = silu; a.state = state;
+    a.y = y; a.ldy = ldy; a.state_out = state_out;
+    if (int rc = check_common("dc_causal_conv_step", a, type)) return rc;
+    if (n_seq == 0) return 0;
+    if (!y || !state_out) { set_error("dc_causal_conv_step", 1104); return 1104; }
+    const bool vec = vector_rows(type, D, ldx, ldy, 0, {x, y, state, state_out});
+#define CONV_SGRID(V) dim3((unsigned)(((int64_t)n_seq * (D / V) + 255) / 256))
+    CONV_DISPATCH(conv_step_kernel, CONV_SGRID);
+    return launch_check("dc_causal_conv_step");
+}
+
+}  // namespace dc

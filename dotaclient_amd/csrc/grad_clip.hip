@@ -1,0 +1,179 @@
+// Global gradient norm over many tensors, and clipping (optimizer.py:674-675's clip_grad_norm_ for gradients that are not one flat buffer).
+//
+//   n_i = sqrt(sum g_i^2),  total = sqrt(sum n_i^2),  c = min(1, max_norm / (total + 1e-6)),  out_i = c * g_i
+// A total that is not finite clips nothing: c = 1 (dc_gradnorm_clip_adam's guard: such a step updates nothing).
+//
+// Bound by HBM: the gradients are read for the norm and, scaled, once more (from the last-level cache as far as they fit) and written.
+// The tensors' addresses travel in the kernels' arguments, TENSORS per launch: no table in device memory, so a captured graph is whole.
+// A workgroup sums one chunk in f64 and writes its sum to its own place; one workgroup joins them in order: no atomics.
+#include "op_util.h"
+
+namespace dc {
+namespace {
+
+constexpr int TENSORS = 128;              // 28 bytes of kernel arguments each, 4 KB are the limit
+constexpr int CHUNK = 16384;              // elements per workgroup
+
+struct ClipTable {
+    const void* g[TENSORS];
+    void* out[TENSORS];
+    int64_t n[TENSORS];
+    int32_t chunk0[TENSORS + 1];          // first chunk of each tensor, in this launch
+    uint32_t bf16[(TENSORS + 31) / 32];
+    int32_t count;
+};
+
+__device__ __forceinline__ int find_tensor(const ClipTable& t, int chunk) {      // last i with chunk0[i] <= chunk; empty tensors have no chunk
+    int lo = 0, hi = t.count - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (t.chunk0[mid] <= chunk) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+template <typename T, int V>
+__device__ __forceinline__ double chunk_squares(const T* g, int64_t at, int n) {
+    double s = 0.0;
+    const int nv = n / V;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < nv; i += 256) {
+        float v[V];
+        load_vec<T, V>(g + at + (int64_t)i * V, v);
+#pragma unroll
+        for (int e = 0; e < V; ++e) s = fma((double)v[e], (double)v[e], s);
+    }
+    for (int i = nv * V + threadIdx.x; i < n; i += 256) {
+        const double v = (double)(float)g[at + i];
+        s = fma(v, v, s);
+    }
+    return s;
+}
+
+__global__ void __launch_bounds__(256) clip_squares_kernel(ClipTable t, double* __restrict__ part) {
+    const int i = find_tensor(t, blockIdx.x);
+    const int64_t at = (int64_t)(blockIdx.x - t.chunk0[i]) * CHUNK;
+    const int n = (int)(t.n[i] - at < CHUNK ? t.n[i] - at : CHUNK);
+    const bool bf = (t.bf16[i / 32] >> (i % 32)) & 1, al = (reinterpret_cast<uintptr_t>(t.g[i]) & 15) == 0;
+    double s;
+    if (bf) s = al ? chunk_squares<bf16_t, 8>(static_cast<const bf16_t*>(t.g[i]), at, n) : chunk_squares<bf16_t, 1>(static_cast<const bf16_t*>(t.g[i]), at, n);
+    else s = al ? chunk_squares<float, 4>(static_cast<const float*>(t.g[i]), at, n) : chunk_squares<float, 1>(static_cast<const float*>(t.g[i]), at, n);
+    s = wave_sum(s);
+    __shared__ double red[4];
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) part[blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
+}
+
+struct NormTable { int32_t chunk0[TENSORS + 1]; int32_t count; };
+
+// One launch per table: a wave per tensor adds its chunks and writes its norm; the squares go to sq[first + i].
+__global__ void __launch_bounds__(256) clip_norms_kernel(NormTable t, const double* __restrict__ part, double* __restrict__ sq, float* __restrict__ norms) {
+    const int i = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (i >= t.count) return;
+    double s = 0.0;
+#pragma unroll 4
+    for (int c = t.chunk0[i] + lane; c < t.chunk0[i + 1]; c += 64) s += part[c];
+    s = wave_sum(s);
+    if (lane == 0) {
+        sq[i] = s;
+        norms[i] = (float)sqrt(s);
+    }
+}
+
+// c from the tensors' squares, summed by every workgroup in the same order.
+__device__ __forceinline__ double total_norm(const double* __restrict__ sq, int n) {
+    __shared__ double red[4];
+    double s = 0.0;
+    for (int i = threadIdx.x; i < n; i += 256) s += sq[i];
+    s = wave_sum(s);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    return sqrt((red[0] + red[1]) + (red[2] + red[3]));
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void chunk_scale(const T* g, T* out, int64_t at, int n, float c) {
+    const int nv = n / V;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < nv; i += 256) {
+        float v[V];
+        load_vec<T, V>(g + at + (int64_t)i * V, v);
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] *= c;
+        store_vec<T, V>(out + at + (int64_t)i * V, v);
+    }
+    for (int i = nv * V + threadIdx.x; i < n; i += 256) out[at + i] = (T)((float)g[at + i] * c);
+}
+
+__global__ void __launch_bounds__(256) clip_scale_kernel(ClipTable t, const double* __restrict__ sq, int n_all, float max_norm, float* __restrict__ total) {
+    const double norm = total_norm(sq, n_all);
+    if (total && blockIdx.x == 0 && threadIdx.x == 0) *total = (float)norm;
+    const double want = (double)max_norm / (norm + 1e-6);
+    const float c = norm <= 1.7976931348623157e308 && want < 1.0 ? (float)want : 1.f;
+    const int i = find_tensor(t, blockIdx.x);
+    if (blockIdx.x >= t.chunk0[t.count] || (c == 1.f && t.out[i] == t.g[i])) return;
+    const int64_t at = (int64_t)(blockIdx.x - t.chunk0[i]) * CHUNK;
+    const int n = (int)(t.n[i] - at < CHUNK ? t.n[i] - at : CHUNK);
+    const bool bf = (t.bf16[i / 32] >> (i % 32)) & 1, al = ((reinterpret_cast<uintptr_t>(t.g[i]) | reinterpret_cast<uintptr_t>(t.out[i])) & 15) == 0;
+    if (bf) {
+        const bf16_t* g = static_cast<const bf16_t*>(t.g[i]); bf16_t* o = static_cast<bf16_t*>(t.out[i]);
+        if (al) chunk_scale<bf16_t, 8>(g, o, at, n, c); else chunk_scale<bf16_t, 1>(g, o, at, n, c);
+    } else {
+        const float* g = static_cast<const float*>(t.g[i]); float* o = static_cast<float*>(t.out[i]);
+        if (al) chunk_scale<float, 4>(g, o, at, n, c); else chunk_scale<float, 1>(g, o, at, n, c);
+    }
+}
+
+int64_t chunks_of(int64_t n) { return (n + CHUNK - 1) / CHUNK; }
+
+}  // namespace
+
+int64_t grad_norm_clip_scratch(const int64_t* sizes, int n) {
+    int64_t chunks = 0;
+    for (int i = 0; i < n; ++i) chunks += sizes[i] > 0 ? chunks_of(sizes[i]) : 0;
+    return (chunks + n) * (int64_t)sizeof(double);
+}
+
+int grad_norm_clip(const int64_t* grads, const int64_t* outs, const int64_t* sizes, const int32_t* types, int n, float max_norm, float* total, float* norms,
+                   double* scratch, int64_t scratch_bytes, hipStream_t s) {
+    if (n < 1 || !grads || !outs || !sizes || !types || !total || !norms || !scratch) { set_error("dc_grad_norm_clip", 1104); return 1104; }
+    if (!(max_norm >= 0.f)) { set_error("dc_grad_norm_clip: max_norm", 1103); return 1103; }
+    for (int i = 0; i < n; ++i) {
+        if (sizes[i] < 0 || chunks_of(sizes[i]) > 0x3fffffff / TENSORS) { set_error("dc_grad_norm_clip: size", 1103); return 1103; }
+        if (types[i] != 0 && types[i] != 1) { set_error("dc_grad_norm_clip: type", 1101); return 1101; }
+        if (sizes[i] && (!grads[i] || !outs[i])) { set_error("dc_grad_norm_clip", 1104); return 1104; }
+    }
+    if (scratch_bytes < grad_norm_clip_scratch(sizes, n)) { set_error("dc_grad_norm_clip: scratch", 1105); return 1105; }
+    double* sq = scratch;                    // [n], then the chunks' sums
+    double* part = scratch + n;
+    for (int pass = 0; pass < 2; ++pass) {
+        int64_t chunk0 = 0;
+        for (int first = 0; first < n; first += TENSORS) {
+            ClipTable t = {};
+            NormTable nt = {};
+            t.count = n - first < TENSORS ? n - first : TENSORS;
+            for (int i = 0; i < t.count; ++i) {
+                const int j = first + i;
+                t.g[i] = reinterpret_cast<const void*>(grads[j]); t.out[i] = reinterpret_cast<void*>(outs[j]); t.n[i] = sizes[j];
+                if (types[j]) t.bf16[i / 32] |= 1u << (i % 32);
+                t.chunk0[i + 1] = t.chunk0[i] + (int32_t)chunks_of(sizes[j]);
+            }
+            const int chunks = t.chunk0[t.count];
+            for (int i = 0; i <= t.count; ++i) nt.chunk0[i] = t.chunk0[i];
+            nt.count = t.count;
+            if (pass == 0) {
+                if (chunks) hipLaunchKernelGGL(clip_squares_kernel, dim3(chunks), dim3(256), 0, s, t, part + chunk0);
+                hipLaunchKernelGGL(clip_norms_kernel, dim3((t.count + 3) / 4), dim3(256), 0, s, nt, part + chunk0, sq + first, norms + first);
+            } else if (chunks || first == 0) {
+                hipLaunchKernelGGL(clip_scale_kernel, dim3(chunks ? chunks : 1), dim3(256), 0, s, t, sq, n, max_norm, first == 0 ? total : nullptr);
+            }
+            if (int rc = launch_check("dc_grad_norm_clip")) return rc;
+            chunk0 += chunks;
+        }
+    }
+    return 0;
+}
+
+}  // namespace dc

@@ -231,4 +231,25 @@ int gradnorm_clip_adam(const int64_t* seg_off, const int32_t* seg_len, const int
 int dp_average_grads(const int64_t* seg_off, const int32_t* seg_len, const int32_t* seg_gate, int n_seg, int max_seg_len,
                      float* grad, const float* counts, float vf_coef, hipStream_t s);
 
+// causal_conv.hip, block_norm.hip, grad_clip.hip (element types: 0 = f32, 1 = bf16)
+int causal_conv_fwd(const void* x, int64_t ldx, const float* w, const float* bias, const int64_t* seq_off, const int32_t* seq_len, int64_t rows, int n_seq,
+                    int max_len, int D, int K, int type, int silu, const void* state, void* y, int64_t ldy, void* state_out, hipStream_t s);
+int64_t causal_conv_scratch(int n_seq, int max_len, int D, int K);
+int causal_conv_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const float* w, const float* bias, const int64_t* seq_off,
+                    const int32_t* seq_len, int64_t rows, int n_seq, int max_len, int D, int K, int type, int silu, const void* state,
+                    const void* dstate_out, void* dx, int64_t lddx, float* dw, float* dbias, void* dstate, float* scratch, int64_t scratch_bytes,
+                    hipStream_t s);
+int causal_conv_step(const void* x, int64_t ldx, const void* state, const float* w, const float* bias, int n_seq, int D, int K, int type, int silu, void* y,
+                     int64_t ldy, void* state_out, hipStream_t s);
+int block_norm_fwd(const void* y, int64_t ldy, const void* z, int64_t ldz, const void* r, int64_t ldr, const float* w_post, const float* s,
+                   const float* w_pre, int64_t rows, int D, int type, int rtype, float eps, void* r_out, int64_t ldro, void* x_out, int64_t ldxo,
+                   hipStream_t st);
+int64_t block_norm_scratch(int64_t rows, int D);
+int block_norm_bwd(const void* dr, int64_t lddr, const void* dx, int64_t lddx, const void* y, int64_t ldy, const void* z, int64_t ldz, const void* r,
+                   int64_t ldr, const float* w_post, const float* s, const float* w_pre, int64_t rows, int D, int type, int rtype, float eps, void* dy,
+                   void* dz, void* dres, float* dw_post, float* ds, float* dw_pre, float* scratch, int64_t scratch_bytes, hipStream_t st);
+int64_t grad_norm_clip_scratch(const int64_t* sizes, int n);
+int grad_norm_clip(const int64_t* grads, const int64_t* outs, const int64_t* sizes, const int32_t* types, int n, float max_norm, float* total, float* norms,
+                   double* scratch, int64_t scratch_bytes, hipStream_t s);
+
 }  // namespace dc

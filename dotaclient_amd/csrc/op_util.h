@@ -1,0 +1,52 @@
+// Loads, stores and reductions shared by the state space block's kernels (causal_conv.hip, ssm_*.hip, block_norm.hip, grad_clip.hip).
+#pragma once
+#include "kernels.h"
+
+namespace dc {
+
+typedef __bf16 bf16_t;
+
+// V consecutive elements of T as floats.  V > 1 needs the address aligned to V * sizeof(T) (16 bytes for the widths used here).
+template <typename T, int V>
+__device__ __forceinline__ void load_vec(const T* __restrict__ p, float (&f)[V]) {
+    if constexpr (V == 1) {
+        f[0] = (float)p[0];
+    } else {
+        typedef T vec_t __attribute__((ext_vector_type(V)));
+        const vec_t v = *reinterpret_cast<const vec_t*>(p);
+#pragma unroll
+        for (int i = 0; i < V; ++i) f[i] = (float)v[i];
+    }
+}
+
+// Rounds to nearest even where T is narrower (the one rounding of an output).
+template <typename T, int V>
+__device__ __forceinline__ void store_vec(T* __restrict__ p, const float (&f)[V]) {
+    if constexpr (V == 1) {
+        p[0] = (T)f[0];
+    } else {
+        typedef T vec_t __attribute__((ext_vector_type(V)));
+        vec_t v;
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = (T)f[i];
+        *reinterpret_cast<vec_t*>(p) = v;
+    }
+}
+
+// 1 / (1 + exp(-v)): v_exp_f32 and v_rcp_f32, both within 1 ulp; exp(-v) = inf gives 0, NaN stays NaN.
+__device__ __forceinline__ float sigmoid_fast(float v) { return __builtin_amdgcn_rcpf(1.f + __expf(-v)); }
+
+// A sequence's place in the packed rows, cut to the rows there are: an offset or a length that points outside addresses nothing.
+struct SeqRange { int64_t off; int len; };
+__device__ __forceinline__ SeqRange seq_range(const int64_t* __restrict__ seq_off, const int32_t* __restrict__ seq_len, int b, int64_t rows, int max_len) {
+    SeqRange r;
+    r.off = seq_off[b];
+    int64_t len = seq_len[b];
+    if (len > max_len) len = max_len;
+    if (r.off < 0 || r.off > rows || len < 0) { r.off = 0; len = 0; }
+    if (len > rows - r.off) len = rows - r.off;
+    r.len = (int)len;
+    return r;
+}
+
+}  // namespace dc

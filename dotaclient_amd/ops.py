@@ -2,6 +2,8 @@
 
 torch is used here for device memory and streams; all arithmetic happens in libdotaclient_hip.so.
 """
+import ctypes
+
 import torch
 
 from . import _lib
@@ -92,3 +94,268 @@ def gemm(A, B, C, M, N, K, lda, ldb, ldc, a_kmajor=False, b_kmajor=False, bias=N
                                splits, _lib.ptr(scratch), 0 if scratch is None else scratch.numel(), _lib.stream_ptr()),
                'dc_gemm_f32')
     return C
+
+
+# ---------------------------------------------------------------------------------------------------------------------------------------
+# A state space core's operators over the same packed rows (csrc/causal_conv.hip, ssm_scan.hip, block_norm.hip, grad_clip.hip).
+# Row tensors ([rows, ...], f32 or bf16) may be column slices of wider ones: the distance between rows is free, everything inside a row is
+# contiguous.  Parameters and recurrent states are f32 and contiguous, as are their gradients.  Rows that belong to no sequence are neither
+# read nor written: in an output allocated here they hold whatever was there.  A call runs on its tensors' device, on the stream that is
+# current there; its scratch is allocated per call, so calls on several streams or in several graphs share nothing.
+# ---------------------------------------------------------------------------------------------------------------------------------------
+_TYPES = {torch.float32: 0, torch.bfloat16: 1}
+
+
+def _rows(t, name, dtype, shape):
+    """Checks a row tensor; returns the distance between its rows in elements."""
+    if t.dtype != dtype:
+        raise TypeError('%s: expected %s, got %s' % (name, dtype, t.dtype))
+    if tuple(t.shape) != shape:
+        raise ValueError('%s: expected shape %s, got %s' % (name, shape, tuple(t.shape)))
+    width, st = 1, t.stride()
+    for i in range(len(shape) - 1, 0, -1):
+        if shape[i] != 1 and st[i] != width:
+            raise ValueError('%s: everything inside a row must be contiguous' % name)
+        width *= shape[i]
+    return st[0] if shape[0] > 1 else width
+
+
+def _out_rows(t, name, dtype, shape, like):
+    """A row tensor to write to (allocated where None); returns it and the distance between its rows."""
+    if t is None:
+        t = torch.empty(shape, dtype=dtype, device=like.device)
+    ld = _rows(t, name, dtype, shape)
+    width = t.numel() // shape[0] if shape[0] else 1
+    if ld < width:
+        raise ValueError('%s: the rows of an output must not overlap' % name)
+    return t, ld
+
+
+def _param(t, name, shape, dtype=torch.float32):
+    if t.dtype != dtype:
+        raise TypeError('%s: expected %s, got %s' % (name, dtype, t.dtype))
+    if tuple(t.shape) != shape:
+        raise ValueError('%s: expected shape %s, got %s' % (name, shape, tuple(t.shape)))
+    if not t.is_contiguous():
+        raise ValueError('%s must be contiguous' % name)
+    return t
+
+
+def _float_type(t, name):
+    if t.dtype not in _TYPES:
+        raise TypeError('%s: expected torch.float32 or torch.bfloat16, got %s' % (name, t.dtype))
+    return _TYPES[t.dtype]
+
+
+def _sequences(seq_off, seq_len, max_len):
+    n = seq_off.shape[0] if seq_off.dim() == 1 else -1
+    _param(seq_off, 'seq_off', (n,), torch.int64)
+    _param(seq_len, 'seq_len', (n,), torch.int32)
+    if not 0 <= max_len < 2 ** 31:
+        raise ValueError('max_len: expected 0 <= max_len < 2^31, got %d' % max_len)
+    return n
+
+
+def _distinct(outs, ins):
+    """Refuses an output that starts where an input does."""
+    at = {t.data_ptr() for t in ins if t is not None and t.numel()}
+    for name, t in outs:
+        if t is not None and t.numel() and t.data_ptr() in at:
+            raise ValueError('%s must not be one of the inputs' % name)
+
+
+def _run(name, tensors, *args):
+    """Calls the C entry point on the tensors' device and that device's current stream."""
+    lib = _lib.load()
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise _lib.DotaHipError('%s: its tensors must live on the GPU (there is no CPU path)' % name)
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise ValueError('%s: its tensors live on %s and %s' % (name, dev, t.device))
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            _lib.check(getattr(lib, name)(*args, torch.cuda.current_stream().cuda_stream), name)
+    else:
+        _lib.check(getattr(lib, name)(*args, torch.cuda.current_stream().cuda_stream), name)
+
+
+def _p(t):
+    return None if t is None else t.data_ptr()
+
+
+def _conv_params(x, weight, bias):
+    if x.dim() != 2 or weight.dim() != 2:
+        raise ValueError('x and weight: expected [rows, D] and [D, K]')
+    rows, D, K = x.shape[0], x.shape[1], weight.shape[1]
+    if D < 1 or D > 1 << 20 or not 2 <= K <= 8:
+        raise ValueError('weight: expected 1 <= D <= 2^20 and 2 <= K <= 8, got D = %d, K = %d' % (D, K))
+    _param(weight, 'weight', (D, K))
+    if bias is not None:
+        _param(bias, 'bias', (D,))
+    return rows, D, K
+
+
+def causal_conv(x, weight, bias, seq_off, seq_len, max_len, state=None, silu=True, y=None, state_out=None):
+    """Short causal depthwise convolution over packed sequences, with SiLU: x [rows, D], weight [D, K] (2 <= K <= 8, weight[:, K-1] the
+    current row's), bias [D] or None -> (y [rows, D], state_out [n_seq, K-1, D]).  state: the K-1 inputs in front of each sequence, oldest
+    first, in x's type (None: zeros); state_out: the same for what follows, also for sequences shorter than K-1 or empty."""
+    rows, D, K = _conv_params(x, weight, bias)
+    ty, n = _float_type(x, 'x'), _sequences(seq_off, seq_len, max_len)
+    ldx = _rows(x, 'x', x.dtype, (rows, D))
+    if state is not None:
+        _param(state, 'state', (n, K - 1, D), x.dtype)
+    y, ldy = _out_rows(y, 'y', x.dtype, (rows, D), x)
+    state_out = torch.empty((n, K - 1, D), dtype=x.dtype, device=x.device) if state_out is None else _param(state_out, 'state_out', (n, K - 1, D), x.dtype)
+    _distinct((('y', y), ('state_out', state_out)), (x, state))
+    _run('dc_causal_conv_fwd', (x, weight, bias, seq_off, seq_len, state, y, state_out), x.data_ptr(), ldx, weight.data_ptr(), _p(bias),
+         seq_off.data_ptr(), seq_len.data_ptr(), rows, n, max_len, D, K, ty, int(silu), _p(state), y.data_ptr(), ldy, state_out.data_ptr())
+    return y, state_out
+
+
+def causal_conv_backward(dy, x, weight, bias, seq_off, seq_len, max_len, state=None, silu=True, dstate_out=None, dx=None):
+    """Gradients of causal_conv from dy [rows, D] and dstate_out [n_seq, K-1, D] (None: zeros) -> (dx, dweight, dbias, dstate); dbias is None
+    without a bias, dstate without a state."""
+    rows, D, K = _conv_params(x, weight, bias)
+    ty, n = _float_type(x, 'x'), _sequences(seq_off, seq_len, max_len)
+    ldx, lddy = _rows(x, 'x', x.dtype, (rows, D)), _rows(dy, 'dy', x.dtype, (rows, D))
+    for t, name in ((state, 'state'), (dstate_out, 'dstate_out')):
+        if t is not None:
+            _param(t, name, (n, K - 1, D), x.dtype)
+    dx, lddx = _out_rows(dx, 'dx', x.dtype, (rows, D), x)
+    _distinct((('dx', dx),), (x, dy, state, dstate_out))
+    dw = torch.empty_like(weight)
+    db = None if bias is None else torch.empty_like(bias)
+    dstate = None if state is None else torch.empty_like(state)
+    size = _lib.load().dc_causal_conv_scratch(n, max_len, D, K)
+    scratch = torch.empty(max(size, 16), dtype=torch.uint8, device=x.device)
+    _run('dc_causal_conv_bwd', (dy, x, weight, bias, seq_off, seq_len, state, dstate_out, dx), dy.data_ptr(), lddy, x.data_ptr(), ldx, weight.data_ptr(),
+         _p(bias), seq_off.data_ptr(), seq_len.data_ptr(), rows, n, max_len, D, K, ty, int(silu), _p(state), _p(dstate_out), dx.data_ptr(), lddx,
+         dw.data_ptr(), _p(db), _p(dstate), scratch.data_ptr(), size)
+    return dx, dw, db, dstate
+
+
+def causal_conv_step(x, state, weight, bias, silu=True, y=None, state_out=None):
+    """causal_conv for one row per sequence (the actor's env-step): x [n, D], state [n, K-1, D] (None: zeros) -> (y [n, D], state_out);
+    state_out may be state itself."""
+    n, D, K = _conv_params(x, weight, bias)
+    ty = _float_type(x, 'x')
+    ldx = _rows(x, 'x', x.dtype, (n, D))
+    if state is not None:
+        _param(state, 'state', (n, K - 1, D), x.dtype)
+    y, ldy = _out_rows(y, 'y', x.dtype, (n, D), x)
+    state_out = torch.empty((n, K - 1, D), dtype=x.dtype, device=x.device) if state_out is None else _param(state_out, 'state_out', (n, K - 1, D), x.dtype)
+    _distinct((('y', y),), (x, state))
+    _distinct((('state_out', state_out),), (x,))
+    _run('dc_causal_conv_step', (x, state, weight, bias, y, state_out), x.data_ptr(), ldx, _p(state), weight.data_ptr(), _p(bias), n, D, K, ty, int(silu),
+         y.data_ptr(), ldy, state_out.data_ptr())
+    return y, state_out
+
+
+def _norm_operands(y, residual, w_post, gate, scale, w_pre):
+    if y.dim() != 2:
+        raise ValueError('y: expected [rows, D]')
+    rows, D = y.shape
+    if not 1 <= D <= 8192:
+        raise ValueError('y: expected 1 <= D <= 8192, got %d' % D)
+    ty, tr = _float_type(y, 'y'), _float_type(residual, 'residual')
+    if tr > ty:
+        raise TypeError('residual: expected torch.float32 beside a torch.float32 y')
+    for t, name in ((w_post, 'w_post'), (scale, 'scale'), (w_pre, 'w_pre')):
+        if t is not None:
+            _param(t, name, (D,))
+    return rows, D, ty, tr, _rows(y, 'y', y.dtype, (rows, D)), _rows(residual, 'residual', residual.dtype, (rows, D)), \
+        0 if gate is None else _rows(gate, 'gate', y.dtype, (rows, D))
+
+
+def block_norm(y, residual, w_post, gate=None, scale=None, w_pre=None, eps=1e-5, residual_out=None):
+    """The norms after and before a block, fused with its gate, its residual scale and the residual stream:
+        r = residual + scale * w_post * rmsnorm(y * silu(gate)),   x = w_pre * rmsnorm(r)
+    y, gate [rows, D]; residual [rows, D] in y's type or f32; w_post, scale, w_pre [D]; gate, scale, w_pre may be None.  D <= 8192.
+    -> (r in residual's type, x in y's type; None without w_pre).  residual_out may be residual itself; x is taken from r before r is rounded."""
+    rows, D, ty, tr, ldy, ldr, ldg = _norm_operands(y, residual, w_post, gate, scale, w_pre)
+    r, ldro = _out_rows(residual_out, 'residual_out', residual.dtype, (rows, D), y)
+    _distinct((('residual_out', r),), (y, gate))
+    x = None if w_pre is None else torch.empty((rows, D), dtype=y.dtype, device=y.device)
+    _run('dc_block_norm_fwd', (y, residual, w_post, gate, scale, w_pre, r), y.data_ptr(), ldy, _p(gate), ldg, residual.data_ptr(), ldr, w_post.data_ptr(),
+         _p(scale), _p(w_pre), rows, D, ty, tr, eps, r.data_ptr(), ldro, _p(x), D)
+    return r, x
+
+
+def block_norm_backward(dr, dx, y, residual, w_post, gate=None, scale=None, w_pre=None, eps=1e-5):
+    """Gradients of block_norm from dr (residual's type) and dx (y's type; None exactly where w_pre is): takes the forward's inputs ->
+    (dy, dresidual, dw_post, dgate, dscale, dw_pre), None where there was no input."""
+    rows, D, ty, tr, ldy, ldr, ldg = _norm_operands(y, residual, w_post, gate, scale, w_pre)
+    if (dx is None) != (w_pre is None):
+        raise ValueError('dx: expected exactly with w_pre')
+    lddr = _rows(dr, 'dr', residual.dtype, (rows, D))
+    lddx = 0 if dx is None else _rows(dx, 'dx', y.dtype, (rows, D))
+    new = lambda t, d: None if t is None else torch.empty((rows, D), dtype=d, device=y.device)      # noqa: E731
+    dy, dres, dgate = new(y, y.dtype), new(residual, residual.dtype), new(gate, y.dtype)
+    dw_post = torch.empty_like(w_post)
+    dscale, dw_pre = (None if t is None else torch.empty_like(t) for t in (scale, w_pre))
+    size = _lib.load().dc_block_norm_scratch(rows, D)
+    scratch = torch.empty(max(size, 16), dtype=torch.uint8, device=y.device)
+    _run('dc_block_norm_bwd', (dr, dx, y, residual, w_post, gate, scale, w_pre), dr.data_ptr(), lddr, _p(dx), lddx, y.data_ptr(), ldy, _p(gate), ldg,
+         residual.data_ptr(), ldr, w_post.data_ptr(), _p(scale), _p(w_pre), rows, D, ty, tr, eps, dy.data_ptr(), _p(dgate), dres.data_ptr(),
+         dw_post.data_ptr(), _p(dscale), _p(dw_pre), scratch.data_ptr(), size)
+    return dy, dres, dw_post, dgate, dscale, dw_pre
+
+
+class GradNormClip:
+    """The global norm of many gradients, and clipping (clip_grad_norm_ of optimizer.py:674-675 for tensors that are not one flat buffer):
+    built once over a list of contiguous f32 / bf16 tensors and, with `out`, the tensors that the clipped gradients go to (default: in
+    place); each call reads what the tensors hold then.  No two of the tensors may overlap.
+    clip(max_norm) -> (total [] f32, norms [n] f32): out_i = grads_i * min(1, max_norm / (total + 1e-6)); a total that is not finite
+    clips nothing."""
+
+    def __init__(self, grads, out=None):
+        grads = list(grads)
+        out = grads if out is None else list(out)
+        if not grads or len(out) != len(grads):
+            raise ValueError('GradNormClip: expected one or more gradients and as many outputs')
+        spans = []
+        for i, (g, o) in enumerate(zip(grads, out)):
+            _float_type(g, 'grads[%d]' % i)
+            for t, name in ((g, 'grads'), (o, 'out')):
+                if not t.is_contiguous():
+                    raise ValueError('%s[%d] must be contiguous' % (name, i))
+            if o.dtype != g.dtype or o.shape != g.shape:
+                raise ValueError('out[%d]: expected the type and shape of its gradient' % i)
+            for t in (g,) if o is g or o.data_ptr() == g.data_ptr() else (g, o):
+                if t.numel():
+                    spans.append((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()))
+        spans.sort()
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise ValueError('GradNormClip: two of the tensors overlap')
+        n = len(grads)
+        self._tensors, self._n = (grads, out), n
+        self._grads = (ctypes.c_int64 * n)(*[t.data_ptr() for t in grads])
+        self._outs = (ctypes.c_int64 * n)(*[t.data_ptr() for t in out])
+        self._sizes = (ctypes.c_int64 * n)(*[t.numel() for t in grads])
+        self._types = (ctypes.c_int32 * n)(*[_TYPES[t.dtype] for t in grads])
+        self._check = tuple({id(t): t for t in grads + out}.values())
+        if any(not t.is_cuda for t in self._check):
+            raise _lib.DotaHipError('GradNormClip: its tensors must live on the GPU (there is no CPU path)')
+        if any(t.device != grads[0].device for t in self._check):
+            raise ValueError('GradNormClip: its tensors live on different devices')
+        self._scratch_bytes = _lib.load().dc_grad_norm_clip_scratch(self._sizes, n)
+
+    def __call__(self, max_norm):
+        if not max_norm >= 0:
+            raise ValueError('max_norm: expected a number >= 0, got %r' % (max_norm,))
+        first, n = self._tensors[0][0], self._n
+        norms = torch.empty(n + 1, dtype=torch.float32, device=first.device)
+        scratch = torch.empty(self._scratch_bytes, dtype=torch.uint8, device=first.device)
+        _run('dc_grad_norm_clip', (first,), self._grads, self._outs, self._sizes, self._types, n, max_norm, norms.data_ptr() + 4 * n, norms.data_ptr(),
+             scratch.data_ptr(), self._scratch_bytes)
+        return norms[n], norms[:n]
+
+
+def grad_norm_clip(grads, max_norm, out=None):
+    """GradNormClip for one call."""
+    return GradNormClip(grads, out)(max_norm)

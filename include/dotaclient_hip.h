@@ -333,6 +333,56 @@ int dc_gradnorm_clip_adam(const int64_t* seg_off, const int32_t* seg_len, const 
 int dc_dp_average_grads(const int64_t* seg_off, const int32_t* seg_len, const int32_t* seg_gate, int n_seg,
                         int max_seg_len, float* grads, const float* counts, float vf_coef, dc_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Operators of a state space core over the same packed rows (beside the GRU / LSTM of dc_policy_forward, policy.py:66,152-156: the same
+ * seq_off / seq_len, the same state carried from chunk to chunk and, one row at a time, from env-step to env-step).  Element types:
+ * 0 = f32, 1 = bf16; parameters, states and their gradients are f32 unless noted; `ld*` = distance of two rows in elements.  A sequence that
+ * points outside [0, rows) or is longer than max_len is cut; rows of no sequence are neither read nor written.  Outputs must not overlap inputs
+ * unless noted.  All scratch is the caller's, of the size that the matching dc_*_scratch gives (bytes; host only), and carries nothing from
+ * call to call.  Errors: 1101 type, 1102 a width out of range, 1103 a size out of range, 1104 a NULL buffer, 1105 scratch too small.
+ * ------------------------------------------------------------------------------------------------ */
+
+/* Short causal depthwise convolution: v[t,d] = bias[d] + sum_k w[d,k] ext[t+k,d] with ext = (state rows | x rows) of the sequence;
+ * y = silu ? v * sigmoid(v) : v;  state_out = the last K-1 rows of ext (NULL: not wanted).
+ *   x, y [rows,D]; w [D,K], 2 <= K <= 8; bias [D] or NULL; state, state_out [n_seq,K-1,D] in x's type, oldest row first (NULL = zeros). */
+int dc_causal_conv_fwd(const void* x, int64_t ldx, const float* w, const float* bias, const int64_t* seq_off, const int32_t* seq_len, int64_t rows,
+                       int n_seq, int max_len, int D, int K, int type, int silu, const void* state, void* y, int64_t ldy, void* state_out,
+                       dc_stream_t stream);
+/* Its gradients from dy [rows,D] (and dstate_out, NULL = zeros): dx [rows,D], dw [D,K], dbias [D] (may be NULL), dstate (NULL: not wanted).
+ * v is recomputed.  Results do not depend on the order in which workgroups run. */
+int64_t dc_causal_conv_scratch(int n_seq, int max_len, int D, int K);
+int dc_causal_conv_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const float* w, const float* bias, const int64_t* seq_off,
+                       const int32_t* seq_len, int64_t rows, int n_seq, int max_len, int D, int K, int type, int silu, const void* state,
+                       const void* dstate_out, void* dx, int64_t lddx, float* dw, float* dbias, void* dstate, float* scratch, int64_t scratch_bytes,
+                       dc_stream_t stream);
+/* One row per sequence (the actor's form): x, y [n_seq,D]; state -> state_out, which may be the same buffer. */
+int dc_causal_conv_step(const void* x, int64_t ldx, const void* state, const float* w, const float* bias, int n_seq, int D, int K, int type, int silu,
+                        void* y, int64_t ldy, void* state_out, dc_stream_t stream);
+
+/* The norms after and before a block, with its gate, residual scale and the residual stream:
+ *   g = gate ? y * gate * sigmoid(gate) : y;  r_out = r + scale * w_post * g / rms(g);  x_out = w_pre * r_out / rms(r_out);
+ *   rms(a) = sqrt(mean(a^2) + eps) over the row.  r_out is not rounded between the two norms.
+ *   y, gate, x_out [rows,D] in `type`; r, r_out [rows,D] in `rtype` (f32, or bf16 with bf16); w_post, scale, w_pre [D]; gate, scale, w_pre
+ *   (and x_out with it) may be NULL; D <= 8192.  r_out may be r. */
+int dc_block_norm_fwd(const void* y, int64_t ldy, const void* gate, int64_t ldg, const void* r, int64_t ldr, const float* w_post, const float* scale,
+                      const float* w_pre, int64_t rows, int D, int type, int rtype, float eps, void* r_out, int64_t ldro, void* x_out, int64_t ldxo,
+                      dc_stream_t stream);
+/* Its gradients from dr_out and dx_out; takes the forward's inputs (r, not r_out).  dy, dgate [rows,D] in `type` and dr in `rtype` are
+ * contiguous; dw_post, dscale, dw_pre [D]. */
+int64_t dc_block_norm_scratch(int64_t rows, int D);
+int dc_block_norm_bwd(const void* dr_out, int64_t lddr, const void* dx_out, int64_t lddx, const void* y, int64_t ldy, const void* gate, int64_t ldg,
+                      const void* r, int64_t ldr, const float* w_post, const float* scale, const float* w_pre, int64_t rows, int D, int type, int rtype,
+                      float eps, void* dy, void* dgate, void* dr, float* dw_post, float* dscale, float* dw_pre, float* scratch, int64_t scratch_bytes,
+                      dc_stream_t stream);
+
+/* optimizer.py:674-675 for gradients that are not one flat buffer: norms[i] = |g_i|, total = sqrt(sum norms^2), out_i = g_i * min(1, max_norm /
+ * (total + 1e-6)).  A total that is not finite clips nothing (the guard of dc_gradnorm_clip_adam).
+ *   grads_host, outs_host, sizes_host i64[n], types_host i32[n]: HOST arrays of device addresses, element counts (0 allowed) and types, read
+ *   before the call returns; outs_host[i] may be grads_host[i]; no two buffers may overlap otherwise.  total f32[1], norms f32[n] (device). */
+int64_t dc_grad_norm_clip_scratch(const int64_t* sizes_host, int n);
+int dc_grad_norm_clip(const int64_t* grads_host, const int64_t* outs_host, const int64_t* sizes_host, const int32_t* types_host, int n, float max_norm,
+                      float* total, float* norms, double* scratch, int64_t scratch_bytes, dc_stream_t stream);
+
 /* Host-side ingest (no device work): a list of 2-D copies src[i] (rows[i] x row_bytes[i], contiguous; 0 = write
  * zeros) -> dst[i] (row stride dst_stride[i] bytes), executed by up to n_threads host threads.  Fills the page-locked
  * staging buffers of a batch from the wire-format arrays of its rollouts in one call - replaces the per-key slicing

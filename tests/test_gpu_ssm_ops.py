@@ -1,0 +1,292 @@
+"""GPU: the state space block's operators (ops.causal_conv, ssm_scan, block_norm, GradNormClip and their gradients) against plain 64-bit
+implementations.  Tolerances: `u` is half a step of the output's type (2^-24 f32, 2^-9 relative to the binade's top, i.e. 2^-8 of the value, bf16);
+a result that is the sum of m terms computed in f32 is off by at most m * u32 * (the sum of the terms' absolute values) plus one rounding of
+the output, and each v_exp_f32 / v_rcp_f32 / v_rsq_f32 adds a few u32 of the term that it is in."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U32 = 2.0 ** -24
+HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8}
+
+
+def _dev():
+    assert torch.cuda.is_available(), 'these tests need the MI355X'
+    return torch.device('cuda:0')
+
+
+def _rand(g, *shape):
+    return torch.randn(shape, generator=g, dtype=torch.float64)
+
+
+def _close(got, want, size, terms, what):
+    """|got - want| <= half a step of got's type at `want` + terms * 2^-24 * size, elementwise; size = the sum of the terms' magnitudes."""
+    got64, want = got.detach().cpu().double(), want.double()
+    assert got64.shape == want.shape, (what, got64.shape, want.shape)
+    tol = HALF[got.dtype] * want.abs() + terms * U32 * size + 1e-37
+    bad = ~((got64 - want).abs() <= tol)
+    assert not bad.any(), '%s: %d of %d off, worst %.3e against %.3e' % (
+        what, int(bad.sum()), bad.numel(), float(((got64 - want).abs() - tol).max()), float(tol[bad].min()))
+
+
+def _packed(lens, gap=0):
+    """seq_off, seq_len (device) and the number of rows; `gap` rows of no sequence in front of each sequence and behind the last."""
+    off, at = [], gap
+    for m in lens:
+        off.append(at)
+        at += m + gap
+    dev = _dev()
+    return torch.tensor(off, dtype=torch.int64, device=dev), torch.tensor(lens, dtype=torch.int32, device=dev), at, off
+
+
+# ------------------------------------------------------------------------------------------------------------- causal convolution
+
+
+def _conv64(x, w, b, off, lens, state, silu, dy=None, dstate_out=None):
+    """The definition per sequence, with autograd in f64; also the same with every term's magnitude (for the tolerances)."""
+    K, D = w.shape[1], w.shape[0]
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b if b is not None else torch.zeros(D, dtype=torch.float64), state)]
+    x, w, b, state = leaves
+    y = torch.zeros_like(x)
+    ys, last, obj = [], [], 0.0
+    for s, (o, m) in enumerate(zip(off, lens)):
+        ext = torch.cat([state[s], x[o:o + m]])
+        v = sum(w[:, k] * ext[k:k + m] for k in range(K)) + b
+        v = v * torch.sigmoid(v) if silu else v
+        ys.append(v)
+        last.append(ext[m:])
+        if dy is not None:
+            obj = obj + (v * dy[o:o + m]).sum() + ((ext[m:] * dstate_out[s]).sum() if dstate_out is not None else 0.0)
+    grads = None if dy is None else torch.autograd.grad(obj, leaves)
+    return [v.detach() for v in ys], torch.stack(last).detach(), grads
+
+
+CONV = [  # lens, D, K, gap, pad (extra columns of the row tensors)
+    ([1], 8, 2, 0, 0), ([0, 3, 1], 5, 4, 1, 3), ([16] * 7, 64, 4, 0, 0), ([257, 0, 2, 40], 132, 3, 2, 4), ([9, 8, 7, 33], 33, 8, 1, 0), ([65], 640, 4, 0, 8),
+    ([5, 64, 31], 12, 6, 0, 4)]
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('silu', [True, False])
+@pytest.mark.parametrize('lens,D,K,gap,pad', CONV)
+def test_causal_conv_forward_and_backward(lens, D, K, gap, pad, silu, dtype):
+    from dotaclient_amd import ops
+    dev = _dev()
+    g = torch.Generator().manual_seed(D * 100 + K)
+    off_d, len_d, rows, off = _packed(lens, gap)
+    n = len(lens)
+    x, dy = _rand(g, rows, D + pad).to(dtype).to(dev), _rand(g, rows, D + pad).to(dtype).to(dev)
+    w, b = (_rand(g, D, K) * K ** -0.5).float().to(dev), _rand(g, D).float().to(dev)
+    state, dso = _rand(g, n, K - 1, D).to(dtype).to(dev), _rand(g, n, K - 1, D).to(dtype).to(dev)
+    xv, dyv = x[:, pad:], dy[:, pad:]
+    keep = torch.full((rows, D + pad), 7.0, dtype=dtype, device=dev)
+    y, so = ops.causal_conv(xv, w, b, off_d, len_d, max(lens), state=state, silu=silu, y=keep[:, pad:])
+    c = lambda t: t.cpu().double()                                                     # noqa: E731
+    want, last, grads = _conv64(c(xv), c(w), c(b), off, lens, c(state), silu, c(dyv), c(dso))
+    size, _, gsize = _conv64(c(xv).abs(), c(w).abs(), c(b).abs(), off, lens, c(state).abs(), False, c(dyv).abs(), c(dso).abs())
+    inside = torch.zeros(rows, dtype=torch.bool)
+    for s, (o, m) in enumerate(zip(off, lens)):
+        inside[o:o + m] = True
+        _close(y[o:o + m], want[s], 2 * size[s], 2 * K + 8, 'y of sequence %d' % s)
+    assert torch.equal(keep[~inside.to(dev)], torch.full_like(keep[~inside.to(dev)], 7.0)) and (pad == 0 or torch.all(keep[:, :pad] == 7.0))
+    assert torch.equal(c(so), last)
+    dx, dw, db, dst = ops.causal_conv_backward(dyv, xv, w, b, off_d, len_d, max(lens), state=state, silu=silu, dstate_out=dso)
+    # |silu'| <= 1.1, its own error a few steps of 1 + |v| (times the term): the magnitudes of the plain gradient, with the pre-activation's on top
+    mag = 2.0 * (1.0 + max(float(s.max()) if s.numel() else 0.0 for s in size))
+    terms = 3 * K + 16
+    _close(dx[inside.to(dev)], grads[0][inside], mag * gsize[0][inside], terms, 'dx')
+    # a gradient of the parameters adds up to `rows` terms: 8 rows in a thread, 8 chunks, partial sums in order
+    _close(dw, grads[1], mag * gsize[1], terms + 64 + rows // 64, 'dweight')
+    _close(db, grads[2], mag * gsize[2], terms + 64 + rows // 64, 'dbias')
+    _close(dst, grads[3], mag * gsize[3], terms, 'dstate')
+    # the same without a state and a bias
+    y0, so0 = ops.causal_conv(xv, w, None, off_d, len_d, max(lens), silu=silu)
+    want0, last0, _ = _conv64(c(xv), c(w), None, off, lens, torch.zeros(n, K - 1, D, dtype=torch.float64), silu)
+    for s, (o, m) in enumerate(zip(off, lens)):
+        _close(y0[o:o + m], want0[s], 2 * size[s], 2 * K + 8, 'y without state, sequence %d' % s)
+    assert torch.equal(c(so0), last0)
+    _, _, db0, dst0 = ops.causal_conv_backward(dyv, xv, w, None, off_d, len_d, max(lens), silu=silu)
+    assert db0 is None and dst0 is None
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_causal_conv_steps_equal_the_sequence_and_chunks_carry_the_state(dtype):
+    from dotaclient_amd import ops
+    dev = _dev()
+    g = torch.Generator().manual_seed(5)
+    n, T, D, K = 10, 21, 48, 4
+    x = _rand(g, n * T, D).to(dtype).to(dev)
+    w, b = _rand(g, D, K).float().to(dev), _rand(g, D).float().to(dev)
+    off = torch.arange(n, device=dev) * T
+    ln = torch.full((n,), T, dtype=torch.int32, device=dev)
+    y, last = ops.causal_conv(x, w, b, off, ln, T)
+    state = torch.zeros(n, K - 1, D, dtype=dtype, device=dev)
+    for t in range(T):
+        yt, state = ops.causal_conv_step(x.view(n, T, D)[:, t], state, w, b, state_out=state if t % 2 else None)
+        assert torch.equal(yt, y.view(n, T, D)[:, t]), t
+    assert torch.equal(state, last)
+    # two chunks of one sequence, the second one starting from the first one's state
+    cut = 9
+    y1, s1 = ops.causal_conv(x, w, b, off, torch.full_like(ln, cut), cut)
+    y2, s2 = ops.causal_conv(x, w, b, off + cut, ln - cut, T - cut, state=s1)
+    assert torch.equal(y1.view(n, T, D)[:, :cut], y.view(n, T, D)[:, :cut]) and torch.equal(y2.view(n, T, D)[:, cut:], y.view(n, T, D)[:, cut:])
+    assert torch.equal(s2, last)
+
+
+def test_causal_conv_reads_nothing_outside_its_window():
+    # an infinity or NaN touches the K rows that its taps reach and no other row, sequence or channel (also for the widths without own kernels)
+    from dotaclient_amd import ops
+    dev = _dev()
+    for K in (2, 3, 4, 5, 7, 8):
+        off_d, len_d, rows, off = _packed([30, 30], 0)
+        x = torch.ones(rows, 8, device=dev)
+        x[10, 3] = float('inf')
+        w = torch.full((8, K), 0.1, device=dev)
+        y, _ = ops.causal_conv(x, w, None, off_d, len_d, 30, silu=False)
+        bad = ~torch.isfinite(y)
+        want = torch.zeros_like(bad)
+        want[10:10 + K, 3] = True
+        assert torch.equal(bad, want), K
+        dx, dw, _, _ = ops.causal_conv_backward(x, torch.ones_like(x), w, None, off_d, len_d, 30, silu=False)
+        want = torch.zeros_like(bad)
+        want[10 - K + 1:11, 3] = True
+        assert torch.equal(~torch.isfinite(dx), want), K
+
+
+def test_causal_conv_sequences_that_point_outside_are_cut():
+    from dotaclient_amd import ops
+    dev = _dev()
+    x = torch.randn(40, 16, device=dev)
+    w = torch.randn(16, 3, device=dev)
+    off = torch.tensor([0, 30, 41, -5, 1 << 40], dtype=torch.int64, device=dev)
+    ln = torch.tensor([20, 4000, 7, 7, 9], dtype=torch.int32, device=dev)
+    keep = torch.full_like(x, 3.0)
+    y, _ = ops.causal_conv(x, w, None, off, ln, 16, y=keep)
+    good, _ = ops.causal_conv(x, w, None, off[:2].contiguous(), torch.tensor([16, 10], dtype=torch.int32, device=dev), 16, y=torch.full_like(x, 3.0))
+    assert torch.equal(y, good) and torch.all(y[16:30] == 3.0)
+
+
+# ------------------------------------------------------------------------------------------------------------------- block norms
+
+
+def _norm64(y, r, wp, z, s, wq, eps):
+    g = y if z is None else y * z * torch.sigmoid(z)
+    u = g / torch.sqrt((g * g).mean(-1, keepdim=True) + eps)
+    r = r + (wp * u if s is None else s * wp * u)
+    return r, None if wq is None else wq * r / torch.sqrt((r * r).mean(-1, keepdim=True) + eps)
+
+
+@pytest.mark.parametrize('types', [(torch.float32, torch.float32), (torch.bfloat16, torch.float32), (torch.bfloat16, torch.bfloat16)])
+@pytest.mark.parametrize('rows,D,parts,pad', [(1, 1, 'zsw', 0), (5, 16, 'zsw', 0), (130, 512, 'zsw', 4), (67, 513, '', 0), (33, 1000, 'zw', 0), (9, 1028, 'sw', 4),
+                                              (7, 4096, 'zsw', 0), (3, 8191, 'z', 1), (4500, 24, 'zsw', 0)])
+def test_block_norm_forward_and_backward(rows, D, parts, pad, types):
+    from dotaclient_amd import ops
+    dev = _dev()
+    ty, tr = types
+    eps = 1e-5
+    g = torch.Generator().manual_seed(rows * 10000 + D)
+    c = lambda t: None if t is None else t.cpu().double()                              # noqa: E731
+    row = lambda d: _rand(g, rows, D + pad).to(d).to(dev)[:, pad:]                     # noqa: E731
+    y, r, dr = row(ty), row(tr), row(tr)
+    z = row(ty) if 'z' in parts else None
+    s = _rand(g, D).float().to(dev) if 's' in parts else None
+    wp = (1 + 0.1 * _rand(g, D)).float().to(dev)
+    wq = (1 + 0.1 * _rand(g, D)).float().to(dev) if 'w' in parts else None
+    dx = row(ty) if wq is not None else None
+    ro, xo = ops.block_norm(y, r, wp, gate=z, scale=s, w_pre=wq, eps=eps)
+    leaves = [None if t is None else t.requires_grad_(True) for t in (c(y), c(r), c(wp), c(z), c(s), c(wq))]
+    rw, xw = _norm64(*leaves, eps)
+    # u is off by the gate's few steps, the mean's (log-depth sums: 16 terms in a lane, 6 levels, 8 waves) and rsqrt's: 40 steps of its size
+    post = (rw - leaves[1]).detach().abs()
+    _close(ro, rw.detach(), post + rw.detach().abs(), 48, 'r')
+    if wq is not None:
+        inv = xw.detach().abs() / (rw.detach().abs() + 1e-300)
+        _close(xo, xw.detach(), xw.detach().abs() + inv * (post + rw.detach().abs()), 96, 'x')
+    else:
+        assert xo is None
+    have = [t for t in leaves if t is not None]
+    obj = (rw * c(dr)).sum() + (0.0 if dx is None else (xw * c(dx)).sum())
+    grads = iter(torch.autograd.grad(obj, have))
+    want = [None if t is None else next(grads) for t in leaves]
+    dy, dres, dwp, dz, ds, dwq = ops.block_norm_backward(dr, dx, y, r, wp, gate=z, scale=s, w_pre=wq, eps=eps)
+    # magnitudes of the terms behind each gradient, from the formulas with absolute values
+    f = lambda t, o: o if t is None else c(t)                                          # noqa: E731
+    zz = f(z, None)
+    sg = 1.0 if zz is None else (zz * torch.sigmoid(zz)).abs()
+    gg = c(y) if zz is None else c(y) * zz * torch.sigmoid(zz)
+    i1 = 1 / torch.sqrt((gg * gg).mean(-1, keepdim=True) + eps)
+    u = (gg * i1).abs()
+    R = c(dr).abs()
+    if wq is not None:
+        i2 = 1 / torch.sqrt((rw.detach() ** 2).mean(-1, keepdim=True) + eps)
+        v = (c(r).abs() + post) * i2
+        e = (c(dx) * c(wq)).abs()
+        R = R + i2 * (e + v * (e * v).mean(-1, keepdim=True))
+    du = R * f(s, torch.ones(())).abs() * c(wp).abs()
+    dg = i1 * (du + u * (du * u).mean(-1, keepdim=True))
+    col = 200 + rows // 8
+    _close(dres, want[1], R, 160, 'dresidual')
+    _close(dy, want[0], dg * sg, 240, 'dy')
+    _close(dwp, want[2], (R * f(s, torch.ones(())).abs() * u).sum(0), col, 'dw_post')
+    if z is not None:
+        _close(dz, want[3], dg * c(y).abs() * torch.sigmoid(zz) * (1 + zz.abs()), 240, 'dgate')
+    if s is not None:
+        _close(ds, want[4], (R * c(wp).abs() * u).sum(0), col, 'dscale')
+    if wq is not None:
+        _close(dwq, want[5], (c(dx).abs() * v).sum(0), col, 'dw_pre')
+    assert (dz is None) == (z is None) and (ds is None) == (s is None) and (dwq is None) == (wq is None)
+    # in place on the residual stream
+    if pad == 0:
+        r2 = r.clone()
+        ro2, xo2 = ops.block_norm(y, r2, wp, gate=z, scale=s, w_pre=wq, eps=eps, residual_out=r2)
+        assert ro2.data_ptr() == r2.data_ptr() and torch.equal(ro2, ro) and (xo is None or torch.equal(xo2, xo))
+
+
+# -------------------------------------------------------------------------------------------------------------- gradient clipping
+
+
+@pytest.mark.parametrize('sizes', [[1], [0, 7, 0, 16384, 16385, 3, 0], [229376, 896, 256, 154], [5] * 300, [100003, 1, 65536]])
+@pytest.mark.parametrize('mixed', [False, True])
+def test_grad_norm_clip(sizes, mixed):
+    from dotaclient_amd import ops
+    dev = _dev()
+    g = torch.Generator().manual_seed(len(sizes) + sizes[-1])
+    base = [_rand(g, n + 1).to(torch.bfloat16 if mixed and i % 2 else torch.float32).to(dev) for i, n in enumerate(sizes)]
+    grads = [t[1:] if i % 3 == 2 else t[:-1] for i, t in enumerate(base)]              # some start off a 16-byte boundary
+    before = [t.clone() for t in grads]
+    norms64 = torch.stack([t.cpu().double().norm() for t in grads])
+    total64 = norms64.norm()
+    # sums in f64, one rounding of the norm; c rounds twice more, its product once
+    for factor, inplace in ((0.25, False), (4.0, False), (0.25, True), (4.0, True)):
+        out = None if inplace else [torch.full_like(t, 9.0) for t in grads]
+        clip = ops.GradNormClip(grads, out)
+        total, norms = clip(factor * float(total64))
+        _close(total[None], total64[None], total64[None], 1, 'total')
+        _close(norms, norms64, norms64, 1, 'norms')
+        c = min(1.0, factor * float(total64) / (float(total64) + 1e-6))
+        for i, (a, b) in enumerate(zip(grads if inplace else out, before)):
+            _close(a, b.cpu().double() * c, b.cpu().double().abs(), 4, 'tensor %d' % i)
+            if c == 1.0:
+                assert torch.equal(a, b)
+        for a, b in zip(grads, before):
+            a.copy_(b)
+    edge = [t[:1] if i % 3 == 2 else t[-1:] for i, t in enumerate(base)]
+    assert all(torch.isfinite(t).all() for t in edge)
+
+
+@pytest.mark.parametrize('bad', [float('nan'), float('inf')])
+def test_grad_norm_clip_of_a_norm_that_is_not_finite_changes_nothing(bad):
+    from dotaclient_amd import ops
+    dev = _dev()
+    grads = [torch.randn(1000, device=dev), torch.randn(50, device=dev).bfloat16()]
+    grads[1][3] = bad
+    before = [t.clone() for t in grads]
+    total, norms = ops.grad_norm_clip(grads, 0.5)
+    assert not torch.isfinite(total) and torch.isfinite(norms[0]) and not torch.isfinite(norms[1])
+    assert all(torch.equal(a.nan_to_num(1.5), b.nan_to_num(1.5)) for a, b in zip(grads, before))
+    # and the largest finite values do not overflow on the way: squares are summed in f64
+    big = [torch.full((1000,), 1e30, device=dev)]
+    total, _ = ops.grad_norm_clip(big, 1.0)
+    assert abs(float(total) / (1e30 * 1000 ** 0.5) - 1) < 1e-6 and torch.isfinite(big[0]).all() and float(big[0].norm()) < 1.001
