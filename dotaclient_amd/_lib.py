@@ -44,6 +44,12 @@ SIGNATURES = {
     'dc_causal_conv_scratch': (c_i64, [c_int] * 4),
     'dc_causal_conv_bwd': (c_int, [c_ptr, c_i64] * 2 + [c_ptr] * 4 + [c_i64] + [c_int] * 6 + [c_ptr, c_ptr, c_ptr, c_i64] + [c_ptr] * 4 + [c_i64, c_ptr]),
     'dc_causal_conv_step': (c_int, [c_ptr, c_i64] + [c_ptr] * 3 + [c_int] * 5 + [c_ptr, c_i64, c_ptr, c_ptr]),
+    'dc_ssm_scan_scratch': (c_i64, [c_int] * 5),
+    'dc_ssm_scan_fwd': (c_int, [c_ptr, c_i64] * 2 + [c_ptr] + [c_ptr, c_i64] * 2 + [c_ptr] * 5 + [c_i64] + [c_int] * 8 + [c_ptr, c_i64, c_ptr, c_ptr, c_i64, c_ptr]),
+    'dc_ssm_scan_bwd_scratch': (c_i64, [c_i64] + [c_int] * 6),
+    'dc_ssm_scan_bwd': (c_int, [c_ptr, c_i64] * 3 + [c_ptr] + [c_ptr, c_i64] * 2 + [c_ptr] * 6 + [c_i64] + [c_int] * 8 + [c_ptr, c_i64] * 4 + [c_ptr] * 5 +
+                        [c_i64, c_ptr]),
+    'dc_ssm_step': (c_int, [c_ptr, c_i64] * 2 + [c_ptr] + [c_ptr, c_i64] * 2 + [c_ptr] * 3 + [c_int] * 7 + [c_ptr, c_i64, c_ptr, c_ptr]),
     'dc_block_norm_fwd': (c_int, [c_ptr, c_i64] * 3 + [c_ptr] * 3 + [c_i64] + [c_int] * 3 + [c_flt] + [c_ptr, c_i64] * 2 + [c_ptr]),
     'dc_block_norm_scratch': (c_i64, [c_i64, c_int]),
     'dc_block_norm_bwd': (c_int, [c_ptr, c_i64] * 5 + [c_ptr] * 3 + [c_i64] + [c_int] * 3 + [c_flt] + [c_ptr] * 7 + [c_i64, c_ptr]),

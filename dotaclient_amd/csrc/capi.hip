@@ -1,6 +1,7 @@
 // extern "C" surface of libdotaclient_hip.so - see include/dotaclient_hip.h for the contract.
 #include "../../include/dotaclient_hip.h"
 #include "kernels.h"
+#include "ssm_util.h"
 #include <stdio.h>
 #include <string.h>
 
@@ -241,6 +242,52 @@ int dc_grad_norm_clip(const int64_t* grads_host, const int64_t* outs_host, const
                       float* total, float* norms, double* scratch, int64_t scratch_bytes, dc_stream_t stream) {
     DC_ENTER();
     return dc::grad_norm_clip(grads_host, outs_host, sizes_host, types_host, n, max_norm, total, norms, scratch, scratch_bytes, (hipStream_t)stream);
+}
+
+static dc::SsmArgs ssm_args(const void* x, int64_t ldx, const void* dt, int64_t lddt, const float* A, const void* B, int64_t ldb, const void* C, int64_t ldc,
+                            const float* D, const float* dt_bias, const float* h0, const int64_t* seq_off, const int32_t* seq_len, int64_t rows, int n_seq,
+                            int max_len, int H, int P, int G, int N, int softplus) {
+    dc::SsmArgs a = {};
+    a.x = x; a.ldx = ldx; a.dt = dt; a.lddt = lddt; a.A = A; a.B = B; a.ldb = ldb; a.C = C; a.ldc = ldc; a.D = D; a.dt_bias = dt_bias; a.h0 = h0;
+    a.seq_off = seq_off; a.seq_len = seq_len; a.rows = rows; a.n_seq = n_seq; a.max_len = max_len; a.H = H; a.P = P; a.G = G; a.N = N; a.softplus = softplus;
+    return a;
+}
+
+int64_t dc_ssm_scan_scratch(int n_seq, int max_len, int H, int P, int N) { return dc::ssm_scan_scratch(n_seq, max_len, H, P, N); }
+
+int dc_ssm_scan_fwd(const void* x, int64_t ldx, const void* dt, int64_t lddt, const float* A, const void* B, int64_t ldb, const void* C, int64_t ldc,
+                    const float* D, const float* dt_bias, const float* h0, const int64_t* seq_off, const int32_t* seq_len, int64_t rows, int n_seq,
+                    int max_len, int H, int P, int G, int N, int type, int softplus, void* y, int64_t ldy, float* hT, void* scratch, int64_t scratch_bytes,
+                    dc_stream_t stream) {
+    DC_ENTER();
+    dc::SsmArgs a = ssm_args(x, ldx, dt, lddt, A, B, ldb, C, ldc, D, dt_bias, h0, seq_off, seq_len, rows, n_seq, max_len, H, P, G, N, softplus);
+    a.y = y; a.ldy = ldy; a.hT = hT;
+    return dc::ssm_scan_fwd(a, type, scratch, scratch_bytes, (hipStream_t)stream);
+}
+
+int64_t dc_ssm_scan_bwd_scratch(int64_t rows, int n_seq, int max_len, int H, int P, int G, int N) {
+    return dc::ssm_scan_bwd_scratch(rows, n_seq, max_len, H, P, G, N);
+}
+
+int dc_ssm_scan_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* dt, int64_t lddt, const float* A, const void* B, int64_t ldb,
+                    const void* C, int64_t ldc, const float* D, const float* dt_bias, const float* h0, const float* dhT, const int64_t* seq_off,
+                    const int32_t* seq_len, int64_t rows, int n_seq, int max_len, int H, int P, int G, int N, int type, int softplus, void* dx, int64_t lddx,
+                    void* ddt, int64_t ldddt, void* dB, int64_t lddb, void* dC, int64_t lddc, float* dA, float* dD, float* ddt_bias, float* dh0,
+                    void* scratch, int64_t scratch_bytes, dc_stream_t stream) {
+    DC_ENTER();
+    dc::SsmArgs a = ssm_args(x, ldx, dt, lddt, A, B, ldb, C, ldc, D, dt_bias, h0, seq_off, seq_len, rows, n_seq, max_len, H, P, G, N, softplus);
+    a.dy = dy; a.lddy = lddy; a.dhT = dhT; a.dx = dx; a.lddx = lddx; a.ddt = ddt; a.ldddt = ldddt; a.dB = dB; a.lddb = lddb; a.dC = dC; a.lddc = lddc;
+    a.dA = dA; a.dD = dD; a.ddt_bias = ddt_bias; a.dh0 = dh0;
+    return dc::ssm_scan_bwd(a, type, scratch, scratch_bytes, (hipStream_t)stream);
+}
+
+int dc_ssm_step(const void* x, int64_t ldx, const void* dt, int64_t lddt, const float* A, const void* B, int64_t ldb, const void* C, int64_t ldc,
+                const float* D, const float* dt_bias, const float* h0, int n_seq, int H, int P, int G, int N, int type, int softplus, void* y, int64_t ldy,
+                float* hT, dc_stream_t stream) {
+    DC_ENTER();
+    dc::SsmArgs a = ssm_args(x, ldx, dt, lddt, A, B, ldb, C, ldc, D, dt_bias, h0, nullptr, nullptr, n_seq, n_seq, 1, H, P, G, N, softplus);
+    a.y = y; a.ldy = ldy; a.hT = hT;
+    return dc::ssm_step(a, type, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -284,11 +284,14 @@ bool vector_rows(int type, int D, int64_t ldx, int64_t ldy, int64_t lddx, std::i
         else CONV_LAUNCH(KERNEL, GRID, bf16_t, 1);                                                         \
     } while (0)
 
+// Chunks of rows of a sequence, one at least: it also writes the state.
+int chunks_in(int max_len) { return max_len > 0 ? max_len / CROWS + (max_len % CROWS != 0) : 1; }
+
 int check_common(const char* what, const ConvArgs& a, int type) {
     if (type != 0 && type != 1) { set_error(what, 1101); return 1101; }
     if (a.K < 2 || a.K > 8 || a.D < 1 || a.D > 1 << 20) { set_error(what, 1102); return 1102; }
     if (a.rows < 0 || a.n_seq < 0 || a.max_len < 0) { set_error(what, 1103); return 1103; }
-    if (a.n_seq && (!a.x || !a.w)) { set_error(what, 1104); return 1104; }
+    if (!a.w || (a.rows && !a.x)) { set_error(what, 1104); return 1104; }
     return 0;
 }
 
@@ -307,7 +310,7 @@ int causal_conv_fwd(const void* x, int64_t ldx, const float* w, const float* bia
     a.D = D; a.K = K; a.silu = silu; a.state = state; a.y = y; a.ldy = ldy; a.state_out = state_out;
     if (int rc = check_common("dc_causal_conv_fwd", a, type)) return rc;
     if (n_seq == 0) return 0;
-    a.chunks_per_seq = max_len ? (max_len + CROWS - 1) / CROWS : 1;
+    a.chunks_per_seq = chunks_in(max_len);
     a.n_chunks = (int64_t)n_seq * a.chunks_per_seq;
     const bool vec = vector_rows(type, D, ldx, ldy, 0, {x, y, state, state_out});
     const int64_t gx = (a.n_chunks + CGROUPS - 1) / CGROUPS;
@@ -318,7 +321,7 @@ int causal_conv_fwd(const void* x, int64_t ldx, const float* w, const float* bia
 }
 
 int64_t causal_conv_scratch(int n_seq, int max_len, int D, int K) {      // bytes, for either vector width
-    const int64_t n_chunks = (int64_t)n_seq * (max_len > 0 ? (max_len + CROWS - 1) / CROWS : 1);
+    const int64_t n_chunks = (int64_t)n_seq * chunks_in(max_len);
     return (int64_t)row_blocks(n_chunks, 1) * (K + 1) * D * (int64_t)sizeof(float);
 }
 
@@ -332,7 +335,7 @@ int causal_conv_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, co
     a.dy = dy; a.lddy = lddy; a.dstate_out = dstate_out; a.dx = dx; a.lddx = lddx; a.dstate = dstate; a.part = scratch;
     if (int rc = check_common("dc_causal_conv_bwd", a, type)) return rc;
     if (!dw) { set_error("dc_causal_conv_bwd", 1104); return 1104; }
-    a.chunks_per_seq = max_len ? (max_len + CROWS - 1) / CROWS : 1;
+    a.chunks_per_seq = chunks_in(max_len);
     a.n_chunks = (int64_t)n_seq * a.chunks_per_seq;
     const bool vec = vector_rows(type, D, ldx, lddy, lddx, {x, dy, state, dstate_out, dx, dstate});
     const int lanes = CLANES * (vec ? 4 : 1), groups = (D + lanes - 1) / lanes;

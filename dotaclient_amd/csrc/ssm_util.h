@@ -1,0 +1,228 @@
+// Shared pieces of the state space scan's kernels (ssm_scan.hip forward, ssm_scan_bwd.hip backward).
+//
+// Blocks of TB = 64 rows of one sequence.  With a_t = the running sum of dt_t A inside a block (<= t), the recurrence
+// S_t = exp(dt_t A) S_{t-1} + dt_t x_t B_t^T,  y_t = S_t C_t + D x_t  is, S being the state in front of the block,
+//   y_t   = sum_{s<=t} exp(a_t - a_s) (C_t . B_s) dt_s x_s + exp(a_t) S C_t + D x_t
+//   S_end = exp(a_T) S + sum_s exp(a_T - a_s) dt_s x_s B_s^T
+// : products of 64-row tiles, which run on the matrix cores.
+#pragma once
+#include "op_util.h"
+
+namespace dc {
+
+constexpr int TB = 64;            // rows of a block
+constexpr int PT = 64;            // head columns of a tile
+
+struct SsmArgs {
+    const void* x; int64_t ldx; const void* dt; int64_t lddt; const float* A; const void* B; int64_t ldb; const void* C; int64_t ldc;
+    const float* D; const float* dt_bias; const float* h0;
+    const int64_t* seq_off; const int32_t* seq_len;
+    int64_t rows; int n_seq, max_len, H, P, G, N, softplus;
+    int ptiles, nseg, seg_blocks;               // segments of a sequence, blocks of a segment
+    float* seg_state; float* seg_a;             // [n_seq][nseg][H][P][N], [n_seq][nseg][H]
+    void* y; int64_t ldy; float* hT;            // forward
+    // backward
+    const void* dy; int64_t lddy; const float* dhT;
+    void* dx; int64_t lddx; void* ddt; int64_t ldddt; void* dB; int64_t lddb; void* dC; int64_t lddc;
+    float* dA; float* dD; float* ddt_bias; float* dh0;
+    int32_t* base; int32_t* map; int cap;       // first block slot of each sequence [n_seq + 1], sequence of each slot [cap]
+    void* S; void* dS; int NS;                  // per slot and head: the state in front of the block, the gradient of the state behind it
+    float* seg_dstate;
+    float* part;                                // [cap][H][3]: sums for dA, dD, ddt_bias
+    int hsplit; float* part_bc;                 // [hsplit][rows][G][2][N] where the heads of a group are shared out
+};
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+// Matrix core fragments for D[16][16] += A[16][KS] B[KS][16]; lane l = 16 g + i.  row(): the tile holds the operand's rows (A) or columns (B)
+// with k contiguous; col(): k runs down the tile's rows.  D: element r of lane l is row 4 g + r, column i.
+template <typename T> struct Mat;
+template <> struct Mat<float> {           // v_mfma_f32_16x16x4_f32, four of them: k = 4 g + e in the e-th, the same for both operands
+    static constexpr int KS = 16, V = 4;
+    typedef f32x4 frag;
+    static __device__ __forceinline__ frag row(const float* p, int ld, int i, int g) { return *reinterpret_cast<const f32x4*>(p + i * ld + 4 * g); }
+    static __device__ __forceinline__ frag col(const float* p, int ld, int i, int g) {
+        const float* q = p + 4 * g * ld + i;
+        return frag{q[0], q[ld], q[2 * ld], q[3 * ld]};
+    }
+    static __device__ __forceinline__ f32x4 mma(frag a, frag b, f32x4 c) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
+        return c;
+    }
+};
+template <> struct Mat<bf16_t> {          // v_mfma_f32_16x16x32_bf16: k = 8 g + e
+    static constexpr int KS = 32, V = 8;
+    typedef bf16x8 frag;
+    static __device__ __forceinline__ frag row(const bf16_t* p, int ld, int i, int g) { return *reinterpret_cast<const bf16x8*>(p + i * ld + 8 * g); }
+    // ds_read_b64_tr_b16: sixteen lanes hand in the 4 x 16 block's 8-byte pieces (lane i: row i / 4, columns 4 (i % 4) ..) and get a column each
+    static __device__ __forceinline__ frag col(const bf16_t* p, int ld, int i, int g) {
+        const bf16_t* q = p + (8 * g + (i >> 2)) * ld + (i & 3) * 4;
+        union { s16x4 h[2]; bf16x8 f; } u;
+        u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(void*)q);
+        u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(void*)(q + 4 * ld));
+        return u.f;
+    }
+    static __device__ __forceinline__ f32x4 mma(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+
+// A 64-row tile of W columns on its way from global memory to LDS: 256 threads, V elements per access.  Rows and columns outside are zero.
+template <typename T, int W, int V>
+struct Tile {
+    typedef T vec_t __attribute__((ext_vector_type(V)));
+    static constexpr int PER_ROW = W / V, N = TB * PER_ROW / 256;
+    vec_t v[N];
+    __device__ __forceinline__ void load(const T* __restrict__ p, int64_t ld, int rows, int cols) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const int idx = k * 256 + threadIdx.x, r = idx / PER_ROW, c = idx % PER_ROW * V;
+            vec_t z = {};
+            if (r < rows && c < cols) z = *reinterpret_cast<const vec_t*>(p + r * ld + c);
+            v[k] = z;
+        }
+    }
+    __device__ __forceinline__ void store(T* lds, int ld) const {
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const int idx = k * 256 + threadIdx.x, r = idx / PER_ROW, c = idx % PER_ROW * V;
+            *reinterpret_cast<vec_t*>(lds + r * ld + c) = v[k];
+        }
+    }
+};
+
+// Row pitch of an LDS tile of W columns: 16 bytes more than the row, so that the 16-byte fragment reads of 8 neighbouring rows and the column
+// reads of 4 rows fall into different banks.
+template <typename T> constexpr int pitch(int W) { return W + 16 / (int)sizeof(T); }
+
+// Sum over the sixteen lanes that share a row of D, in each of them.
+__device__ __forceinline__ float sum16(float v) {
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xf, 0xf, false));    // row_ror:8, 4, 2, 1
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x124, 0xf, 0xf, false));
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x122, 0xf, 0xf, false));
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x121, 0xf, 0xf, false));
+    return v;
+}
+
+__device__ __forceinline__ float softplus_f(float v) { return v > 20.f ? v : log1pf(expf(v)); }
+
+// Inclusive sum over the lanes in f64.
+__device__ __forceinline__ double wave_prefix(double v, int lane) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const double u = __shfl_up(v, o, 64);
+        if (lane >= o) v += u;
+    }
+    return v;
+}
+
+// The block's step sizes and running sums (one wave, lane = row).  a is kept as hi + lo, so that exp(a_t - a_s) of neighbouring rows does not lose
+// what a long sum costs: a is summed in f64, the difference is taken of both halves.
+struct Steps {
+    float dt[TB], hi[TB], lo[TB], w[TB];
+    float total;                                  // a of the last row
+};
+__device__ __forceinline__ float gap(const Steps& s, int t, float hi_s, float lo_s) { return (s.hi[t] - hi_s) + (s.lo[t] - lo_s); }
+
+// w[t] = dt_t exp(a_T - a_t): the weights of the block's rows in the state behind it; REV: exp(a_t), those of the gradients in the one in front.
+template <bool REV>
+__device__ __forceinline__ void make_steps(Steps& s, const SsmArgs& a, float raw, bool live, float A, float bias, int lane) {
+    float d = raw + bias;
+    if (a.softplus) d = softplus_f(d);
+    if (!live) d = 0.f;
+    const double sum = wave_prefix((double)d * (double)A, lane);
+    const double last = __shfl(sum, 63, 64);
+    s.dt[lane] = d;
+    s.hi[lane] = (float)sum;
+    s.lo[lane] = (float)(sum - (double)(float)sum);
+    s.w[lane] = REV ? __expf((float)sum) : d * __expf((float)(last - sum));
+    if (lane == 63) s.total = (float)last;
+}
+
+__device__ __forceinline__ void split_bf16(float v, bf16_t& hi, bf16_t& lo) {
+    hi = (bf16_t)v;
+    lo = (bf16_t)(v - (float)hi);
+}
+
+// acc[p][n] (16 rows p of this wave, NP columns) += sum_t w_t X[t][p] Y[t][n], from the tiles X [64][PT] and Y [64][NP].
+// The weights are f32: bf16 operands are scaled in f32 and used as two bf16 pieces (2^-17 of the product is lost), because the states they end
+// in are f32.
+template <typename T, int NP>
+__device__ __forceinline__ void state_update(f32x4 (&acc)[NP / 16], const T* X, int ldx, const T* Y, int ldy, const float* w, int p0, int i, int g) {
+    typedef Mat<T> M;
+#pragma unroll
+    for (int k = 0; k < TB; k += M::KS) {
+        typename M::frag a = M::col(X + k * ldx + p0, ldx, i, g);
+        if constexpr (sizeof(T) == 4) {
+            const f32x4 wk = *reinterpret_cast<const f32x4*>(w + k + 4 * g);
+            a *= wk;
+#pragma unroll
+            for (int c = 0; c < NP / 16; ++c) acc[c] = M::mma(a, M::col(Y + k * ldy + 16 * c, ldy, i, g), acc[c]);
+        } else {
+            typename M::frag lo;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                bf16_t h, l;
+                split_bf16((float)a[e] * w[k + 8 * g + e], h, l);
+                a[e] = h;
+                lo[e] = l;
+            }
+#pragma unroll
+            for (int c = 0; c < NP / 16; ++c) {
+                const typename M::frag b = M::col(Y + k * ldy + 16 * c, ldy, i, g);
+                acc[c] = M::mma(a, b, acc[c]);
+                acc[c] = M::mma(lo, b, acc[c]);
+            }
+        }
+    }
+}
+
+// A user's state [P][N] f32 (or null: zeros) in the accumulators of a wave that owns rows p0 .. p0 + 15 of a tile.
+template <int NP>
+__device__ __forceinline__ void load_state(f32x4 (&acc)[NP / 16], const float* __restrict__ h, int p0, int P, int N, int i, int g) {
+#pragma unroll
+    for (int c = 0; c < NP / 16; ++c)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int p = p0 + 4 * g + r, n = 16 * c + i;
+            acc[c][r] = h && p < P && n < N ? h[(int64_t)p * N + n] : 0.f;
+        }
+}
+template <int NP>
+__device__ __forceinline__ void store_state(const f32x4 (&acc)[NP / 16], float* __restrict__ h, int p0, int P, int N, int i, int g) {
+#pragma unroll
+    for (int c = 0; c < NP / 16; ++c)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int p = p0 + 4 * g + r, n = 16 * c + i;
+            if (p < P && n < N) h[(int64_t)p * N + n] = acc[c][r];
+        }
+}
+
+__host__ __device__ __forceinline__ int blocks_of(int len) { return len / TB + (len % TB != 0); }
+
+// Workgroup -> (sequence and segment, head and column tile).  Workgroups go round the eight XCDs: the heads of one segment, which share B and C, are
+// given numbers of one XCD, so that its L2 holds what they share.
+__device__ __forceinline__ bool work_item(const SsmArgs& a, int& unit, int& h, int& p0) {
+    const int hp = a.H * a.ptiles, x = blockIdx.x & 7, j = blockIdx.x >> 3;
+    unit = j / hp * 8 + x;
+    h = j % hp / a.ptiles;
+    p0 = j % hp % a.ptiles * PT;
+    return unit < a.n_seq * a.nseg;
+}
+inline int64_t work_items(const SsmArgs& a) { return ((int64_t)a.n_seq * a.nseg + 7) / 8 * 8 * a.H * a.ptiles; }
+
+// ssm_scan.hip
+int ssm_states(const SsmArgs& a, int type, bool vec, bool both, bool final_only, hipStream_t s);
+int ssm_join_segments(const SsmArgs& a, bool both, hipStream_t s);
+int ssm_check(const char* what, const SsmArgs& a, int type);
+int64_t ssm_scan_scratch(int n_seq, int max_len, int H, int P, int N);
+int ssm_scan_fwd(SsmArgs a, int type, void* scratch, int64_t scratch_bytes, hipStream_t s);
+int ssm_step(SsmArgs a, int type, hipStream_t s);
+void ssm_segments(SsmArgs& a, int64_t workgroups);
+// ssm_scan_bwd.hip
+int64_t ssm_scan_bwd_scratch(int64_t rows, int n_seq, int max_len, int H, int P, int G, int N);
+int ssm_scan_bwd(SsmArgs a, int type, void* scratch, int64_t scratch_bytes, hipStream_t s);
+
+}  // namespace dc

@@ -3,6 +3,7 @@
 torch is used here for device memory and streams; all arithmetic happens in libdotaclient_hip.so.
 """
 import ctypes
+import typing
 
 import torch
 
@@ -254,6 +255,95 @@ def causal_conv_step(x, state, weight, bias, silu=True, y=None, state_out=None):
     _run('dc_causal_conv_step', (x, state, weight, bias, y, state_out), x.data_ptr(), ldx, _p(state), weight.data_ptr(), _p(bias), n, D, K, ty, int(silu),
          y.data_ptr(), ldy, state_out.data_ptr())
     return y, state_out
+
+
+def _scan_operands(x, dt, A, B, C, D, dt_bias):
+    if x.dim() != 3 or B.dim() != 3:
+        raise ValueError('x and B: expected [rows, H, P] and [rows, G, N]')
+    (rows, H, P), (G, N) = x.shape, B.shape[1:]
+    if H < 1 or G < 1 or H % G or not 1 <= P <= 256 or not 1 <= N <= 128 or H > 4096:
+        raise ValueError('expected G groups that divide H <= 4096 heads, 1 <= P <= 256 and 1 <= N <= 128, got H = %d, P = %d, G = %d, N = %d' % (H, P, G, N))
+    ty = _float_type(x, 'x')
+    lds = (_rows(x, 'x', x.dtype, (rows, H, P)), _rows(dt, 'dt', x.dtype, (rows, H)), _rows(B, 'B', x.dtype, (rows, G, N)),
+           _rows(C, 'C', x.dtype, (rows, G, N)))
+    _param(A, 'A', (H,))
+    for t, name in ((D, 'D'), (dt_bias, 'dt_bias')):
+        if t is not None:
+            _param(t, name, (H,))
+    return rows, H, P, G, N, ty, lds
+
+
+def ssm_scan(x, dt, A, B, C, seq_off, seq_len, max_len, D=None, dt_bias=None, h0=None, softplus=False, y=None, hT=None):
+    """Selective state space scan over packed sequences: per sequence and head, with d = dt + dt_bias (softplus of it with `softplus`),
+        S_t = exp(d_t A) S_{t-1} + d_t x_t B_t^T,   y_t = S_t C_t + D x_t
+    x [rows, H, P], dt [rows, H], B, C [rows, G, N] (head h uses group h // (H // G)) of one type; A, D, dt_bias [H] f32; P <= 256, N <= 128.
+    -> (y [rows, H, P], hT [n_seq, H, P, N] f32).  h0 (None: zeros) / hT: the state in front of / behind each sequence - what a rollout carries
+    from chunk to chunk.  Computed in blocks of 64 rows: a value that is not finite also reaches the outputs of its block's earlier rows."""
+    rows, H, P, G, N, ty, (ldx, lddt, ldb, ldc) = _scan_operands(x, dt, A, B, C, D, dt_bias)
+    n = _sequences(seq_off, seq_len, max_len)
+    if h0 is not None:
+        _param(h0, 'h0', (n, H, P, N))
+    y, ldy = _out_rows(y, 'y', x.dtype, (rows, H, P), x)
+    hT = torch.empty((n, H, P, N), dtype=torch.float32, device=x.device) if hT is None else _param(hT, 'hT', (n, H, P, N))
+    _distinct((('y', y), ('hT', hT)), (x, dt, B, C, h0))
+    size = _lib.load().dc_ssm_scan_scratch(n, max_len, H, P, N)
+    scratch = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+    _run('dc_ssm_scan_fwd', (x, dt, A, B, C, D, dt_bias, h0, seq_off, seq_len, y, hT), x.data_ptr(), ldx, dt.data_ptr(), lddt, A.data_ptr(), B.data_ptr(),
+         ldb, C.data_ptr(), ldc, _p(D), _p(dt_bias), _p(h0), seq_off.data_ptr(), seq_len.data_ptr(), rows, n, max_len, H, P, G, N, ty, int(softplus),
+         y.data_ptr(), ldy, hT.data_ptr(), _p(scratch), size)
+    return y, hT
+
+
+class ScanGrads(typing.NamedTuple):
+    """What ssm_scan_backward returns; None where there was no such input."""
+    dx: torch.Tensor
+    ddt: torch.Tensor
+    dA: torch.Tensor
+    dB: torch.Tensor
+    dC: torch.Tensor
+    dD: typing.Optional[torch.Tensor]
+    ddt_bias: typing.Optional[torch.Tensor]
+    dh0: typing.Optional[torch.Tensor]
+
+
+def ssm_scan_backward(dy, x, dt, A, B, C, seq_off, seq_len, max_len, D=None, dt_bias=None, h0=None, softplus=False, dhT=None, dx=None, ddt=None, dB=None,
+                      dC=None):
+    """Gradients of ssm_scan from dy [rows, H, P] and dhT [n_seq, H, P, N] (None: zeros) -> ScanGrads.  dx, ddt, dB, dC: tensors to write to, which
+    may be column slices of one wider gradient.  The states are computed again: the forward pass saves nothing."""
+    rows, H, P, G, N, ty, (ldx, lddt, ldb, ldc) = _scan_operands(x, dt, A, B, C, D, dt_bias)
+    n = _sequences(seq_off, seq_len, max_len)
+    lddy = _rows(dy, 'dy', x.dtype, (rows, H, P))
+    for t, name in ((h0, 'h0'), (dhT, 'dhT')):
+        if t is not None:
+            _param(t, name, (n, H, P, N))
+    dx, lddx = _out_rows(dx, 'dx', x.dtype, (rows, H, P), x)
+    ddt, ldddt = _out_rows(ddt, 'ddt', x.dtype, (rows, H), x)
+    dB, lddb = _out_rows(dB, 'dB', x.dtype, (rows, G, N), x)
+    dC, lddc = _out_rows(dC, 'dC', x.dtype, (rows, G, N), x)
+    _distinct((('dx', dx), ('ddt', ddt), ('dB', dB), ('dC', dC)), (dy, x, dt, B, C))
+    dA = torch.empty_like(A)
+    dD, dbias, dh0 = (None if t is None else torch.empty_like(t) for t in (D, dt_bias, h0))
+    size = _lib.load().dc_ssm_scan_bwd_scratch(rows, n, max_len, H, P, G, N)
+    scratch = torch.empty(size, dtype=torch.uint8, device=x.device)
+    _run('dc_ssm_scan_bwd', (dy, x, dt, A, B, C, D, dt_bias, h0, dhT, seq_off, seq_len, dx, ddt, dB, dC), dy.data_ptr(), lddy, x.data_ptr(), ldx,
+         dt.data_ptr(), lddt, A.data_ptr(), B.data_ptr(), ldb, C.data_ptr(), ldc, _p(D), _p(dt_bias), _p(h0), _p(dhT), seq_off.data_ptr(),
+         seq_len.data_ptr(), rows, n, max_len, H, P, G, N, ty, int(softplus), dx.data_ptr(), lddx, ddt.data_ptr(), ldddt, dB.data_ptr(), lddb, dC.data_ptr(),
+         lddc, dA.data_ptr(), _p(dD), _p(dbias), _p(dh0), scratch.data_ptr(), size)
+    return ScanGrads(dx, ddt, dA, dB, dC, dD, dbias, dh0)
+
+
+def ssm_step(x, dt, A, B, C, h0=None, D=None, dt_bias=None, softplus=False, y=None, hT=None):
+    """ssm_scan for one row per sequence (the actor's env-step): x [n, H, P], h0 [n, H, P, N] f32 (None: zeros) -> (y, hT); hT may be h0 itself."""
+    n, H, P, G, N, ty, (ldx, lddt, ldb, ldc) = _scan_operands(x, dt, A, B, C, D, dt_bias)
+    if h0 is not None:
+        _param(h0, 'h0', (n, H, P, N))
+    y, ldy = _out_rows(y, 'y', x.dtype, (n, H, P), x)
+    hT = torch.empty((n, H, P, N), dtype=torch.float32, device=x.device) if hT is None else _param(hT, 'hT', (n, H, P, N))
+    _distinct((('y', y),), (x, dt, B, C, h0))
+    _distinct((('hT', hT),), (x, dt, B, C))
+    _run('dc_ssm_step', (x, dt, A, B, C, D, dt_bias, h0, y, hT), x.data_ptr(), ldx, dt.data_ptr(), lddt, A.data_ptr(), B.data_ptr(), ldb, C.data_ptr(), ldc,
+         _p(D), _p(dt_bias), _p(h0), n, H, P, G, N, ty, int(softplus), y.data_ptr(), ldy, hT.data_ptr())
+    return y, hT
 
 
 def _norm_operands(y, residual, w_post, gate, scale, w_pre):

@@ -359,6 +359,29 @@ int dc_causal_conv_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx,
 int dc_causal_conv_step(const void* x, int64_t ldx, const void* state, const float* w, const float* bias, int n_seq, int D, int K, int type, int silu,
                         void* y, int64_t ldy, void* state_out, dc_stream_t stream);
 
+/* Selective state space scan, per sequence and head h (its group's B and C: group h / (H / G)):
+ *   d_t = dt_t + dt_bias (softplus of it where `softplus`);  S_t = exp(d_t A) S_{t-1} + d_t x_t B_t^T;  y_t = S_t C_t + D x_t
+ *   x, y [rows,H,P]; dt [rows,H]; B, C [rows,G,N] in `type`; A, D, dt_bias [H] (D, dt_bias may be NULL); h0, hT [n_seq,H,P,N] (h0 NULL = zeros, hT
+ *   NULL: not wanted).  P <= 256, N <= 128.  Computed in blocks of 64 rows: a value that is not finite also reaches the outputs of the rows
+ *   of its block in front of it. */
+int64_t dc_ssm_scan_scratch(int n_seq, int max_len, int H, int P, int N);
+int dc_ssm_scan_fwd(const void* x, int64_t ldx, const void* dt, int64_t lddt, const float* A, const void* B, int64_t ldb, const void* C, int64_t ldc,
+                    const float* D, const float* dt_bias, const float* h0, const int64_t* seq_off, const int32_t* seq_len, int64_t rows, int n_seq,
+                    int max_len, int H, int P, int G, int N, int type, int softplus, void* y, int64_t ldy, float* hT, void* scratch, int64_t scratch_bytes,
+                    dc_stream_t stream);
+/* Its gradients from dy [rows,H,P] and dhT [n_seq,H,P,N] (NULL = zeros): dx, ddt, dB, dC in `type`; dA, dD, ddt_bias [H] (dD, ddt_bias may be
+ * NULL); dh0 [n_seq,H,P,N] (NULL: not wanted).  The states are computed again.  Results do not depend on the order in which workgroups run. */
+int64_t dc_ssm_scan_bwd_scratch(int64_t rows, int n_seq, int max_len, int H, int P, int G, int N);
+int dc_ssm_scan_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* dt, int64_t lddt, const float* A, const void* B, int64_t ldb,
+                    const void* C, int64_t ldc, const float* D, const float* dt_bias, const float* h0, const float* dhT, const int64_t* seq_off,
+                    const int32_t* seq_len, int64_t rows, int n_seq, int max_len, int H, int P, int G, int N, int type, int softplus, void* dx, int64_t lddx,
+                    void* ddt, int64_t ldddt, void* dB, int64_t lddb, void* dC, int64_t lddc, float* dA, float* dD, float* ddt_bias, float* dh0,
+                    void* scratch, int64_t scratch_bytes, dc_stream_t stream);
+/* One row per sequence (the actor's form): x, y [n_seq,H,P]; hT may be h0. */
+int dc_ssm_step(const void* x, int64_t ldx, const void* dt, int64_t lddt, const float* A, const void* B, int64_t ldb, const void* C, int64_t ldc,
+                const float* D, const float* dt_bias, const float* h0, int n_seq, int H, int P, int G, int N, int type, int softplus, void* y, int64_t ldy,
+                float* hT, dc_stream_t stream);
+
 /* The norms after and before a block, with its gate, residual scale and the residual stream:
  *   g = gate ? y * gate * sigmoid(gate) : y;  r_out = r + scale * w_post * g / rms(g);  x_out = w_pre * r_out / rms(r_out);
  *   rms(a) = sqrt(mean(a^2) + eps) over the row.  r_out is not rounded between the two norms.

@@ -290,3 +290,137 @@ def test_grad_norm_clip_of_a_norm_that_is_not_finite_changes_nothing(bad):
     big = [torch.full((1000,), 1e30, device=dev)]
     total, _ = ops.grad_norm_clip(big, 1.0)
     assert abs(float(total) / (1e30 * 1000 ** 0.5) - 1) < 1e-6 and torch.isfinite(big[0]).all() and float(big[0].norm()) < 1.001
+
+
+# ----------------------------------------------------------------------------------------------------------- state space scan
+
+
+def _scan64(x, dt, la, B, C, D, h0, off, lens):
+    """The recurrence in f64, row by row; la = log decays [rows, H], dt the step sizes (both after bias and softplus)."""
+    rep = x.shape[1] // B.shape[1]
+    ys, hs = [], []
+    for s, (o, m) in enumerate(zip(off, lens)):
+        h = h0[s]
+        for t in range(o, o + m):
+            Bt, Ct = B[t].repeat_interleave(rep, 0), C[t].repeat_interleave(rep, 0)
+            h = h * torch.exp(la[t])[:, None, None] + (dt[t][:, None] * x[t])[:, :, None] * Bt[:, None]
+            ys.append((h * Ct[:, None]).sum(-1) + D[:, None] * x[t])
+        hs.append(h)
+    return (torch.stack(ys) if ys else x[:0]), torch.stack(hs)
+
+
+def _scan_reference(i, off, lens, softplus):
+    """Values, gradients and the magnitudes of the sums behind them, all f64 on the CPU.  i: the inputs as f64 tensors."""
+    raw = (i['dt'] + i['bias']).requires_grad_(True)
+    leaves = {k: i[k].clone().requires_grad_(True) for k in ('x', 'A', 'B', 'C', 'D', 'h0')}
+    d = torch.nn.functional.softplus(raw) if softplus else raw
+    y, hT = _scan64(leaves['x'], d, d * leaves['A'], leaves['B'], leaves['C'], leaves['D'], leaves['h0'], off, lens)
+    rows_in = torch.cat([torch.arange(o, o + m) for o, m in zip(off, lens)]) if sum(lens) else torch.zeros(0, dtype=torch.long)
+    obj = (y * i['dy'][rows_in]).sum() + (hT * i['dhT']).sum()
+    keys = ['raw'] + list(leaves)
+    got = dict(zip(keys, torch.autograd.grad(obj, [raw] + list(leaves.values()))))
+    # magnitudes: everything non-negative, the decays as they are
+    ab = {k: i[k].abs().requires_grad_(True) for k in ('x', 'B', 'C', 'D', 'h0')}
+    dm, la = d.detach().abs().requires_grad_(True), (d * i['A']).detach().requires_grad_(True)
+    ya, ha = _scan64(ab['x'], dm, la, ab['B'], ab['C'], ab['D'], ab['h0'], off, lens)
+    obja = (ya * i['dy'][rows_in].abs()).sum() + (ha * i['dhT'].abs()).sum()
+    keys = ['d', 'la'] + list(ab)
+    size = dict(zip(keys, torch.autograd.grad(obja, [dm, la] + list(ab.values()))))
+    # the kernel's way to d(la): differences of sums over the rows behind, inside a block of 64
+    flow = torch.zeros_like(size['la'])
+    ydy = torch.zeros_like(flow)
+    ydy[rows_in] = (ya.detach() * i['dy'][rows_in].abs()).sum(-1)
+    xdx = (ab['x'].detach() * size['x']).sum(-1)
+    for o, m in zip(off, lens):
+        for t0 in range(0, m, 64):
+            sl = slice(o + t0, o + min(m, t0 + 64))
+            flow[sl] = (ydy[sl] + xdx[sl]).flip(0).cumsum(0).flip(0)
+    size['la'] = size['la'] + flow
+    slope = torch.sigmoid(raw.detach()) if softplus else torch.ones_like(raw.detach())
+    inside = torch.zeros(raw.shape[0], 1, dtype=torch.float64)
+    inside[rows_in] = 1.0
+    size['raw'] = (size['d'] + size['la'] * i['A'].abs()) * slope
+    size['A'] = (size['la'] * d.detach() * inside).sum(0)
+    size['bias'] = size['raw'].sum(0)
+    got['bias'] = got['raw'].sum(0)
+    return dict(y=y.detach(), hT=hT.detach(), rows=rows_in, grads=got, size=size, ya=ya.detach(), ha=ha.detach())
+
+
+def _scan_inputs(seed, lens, gap, H, P, G, N, dtype, pad):
+    off_d, len_d, rows, off = _packed(lens, gap)
+    g = torch.Generator().manual_seed(seed)
+    dev, n = _dev(), len(lens)
+    wide = _rand(g, rows, pad + H * P + 2 * G * N).to(dtype).to(dev)
+    dev_in = dict(x=wide[:, pad:pad + H * P].unflatten(1, (H, P)), B=wide[:, pad + H * P:pad + H * P + G * N].unflatten(1, (G, N)),
+                  C=wide[:, pad + H * P + G * N:].unflatten(1, (G, N)), dt=_rand(g, rows, H).to(dtype).to(dev),
+                  A=-(1 + 15 * torch.rand(H, generator=g)).to(dev), D=_rand(g, H).float().to(dev),
+                  bias=(torch.rand(H, generator=g) * 4 - 6).to(dev), h0=_rand(g, n, H, P, N).float().to(dev),
+                  dy=_rand(g, rows, H, P).to(dtype).to(dev), dhT=_rand(g, n, H, P, N).float().to(dev))
+    return off_d, len_d, rows, off, dev_in
+
+
+SCAN = [  # lens, gap, H, P, G, N, pad
+    ([1], 0, 1, 1, 1, 1, 0), ([2, 0, 3], 1, 2, 8, 1, 8, 0), ([64], 0, 1, 64, 1, 64, 0), ([65, 63, 0, 128], 2, 2, 64, 1, 32, 8), ([16] * 9, 0, 4, 32, 2, 16, 0),
+    ([130, 7], 0, 3, 48, 3, 40, 8), ([71], 3, 2, 77, 1, 101, 1), ([200], 0, 2, 128, 1, 128, 0), ([33, 90], 0, 6, 40, 2, 24, 0), ([300], 0, 1, 64, 1, 128, 0),
+    ([513], 0, 1, 17, 1, 33, 0)]
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('softplus', [True, False])
+@pytest.mark.parametrize('lens,gap,H,P,G,N,pad', SCAN)
+def test_ssm_scan_forward_and_backward(lens, gap, H, P, G, N, pad, softplus, dtype):
+    from dotaclient_amd import ops
+    dev = _dev()
+    off_d, len_d, rows, off, d = _scan_inputs(sum(lens) * 31 + P * N, lens, gap, H, P, G, N, dtype, pad)
+    if not softplus:                                       # step sizes as they are: small and positive
+        d['dt'] = (d['dt'].float().abs() * 0.05).to(dtype)
+        d['bias'] = d['bias'].abs() * 1e-3
+    i64 = {k: v.cpu().double() for k, v in d.items()}
+    ref = _scan_reference(i64, off, lens, softplus)
+    keep = torch.full((rows, H, P), 7.0, dtype=dtype, device=dev)
+    seqs = (off_d, len_d, max(lens))
+    kw = dict(D=d['D'], dt_bias=d['bias'], h0=d['h0'], softplus=softplus)
+    y, hT = ops.ssm_scan(d['x'], d['dt'], d['A'], d['B'], d['C'], *seqs, y=keep, **kw)
+    inside = ref['rows'].to(dev)
+    # f32: sums of up to 64 + N + P terms, a few steps per factor (exp of differences up to ~100: 100 of them), 16 per block and segment on the
+    # way.  bf16: the factors G1 L dt and S are rounded once (half a step of the term); what ends in f32 is made of two pieces, 2^-16 = 256 u32
+    # lost per operand, four operands in a row at most.
+    bf = dtype == torch.bfloat16
+    terms = 64 + N + P + 160 + 32 * (1 + max(lens) // 64)
+    f32_terms = terms + (1024 if bf else 0)
+    out_terms = terms + (2 ** 16 if bf else 0)             # 2^-8 of the sum of the terms' magnitudes
+    _close(y[inside], ref['y'], ref['ya'], out_terms, 'y')
+    rest = torch.ones(rows, dtype=torch.bool)
+    rest[ref['rows']] = False
+    assert torch.all(y[rest.to(dev)] == 7.0)
+    _close(hT, ref['hT'], ref['ha'], f32_terms, 'hT')
+    g = ops.ssm_scan_backward(d['dy'], d['x'], d['dt'], d['A'], d['B'], d['C'], *seqs, dhT=d['dhT'], **kw)
+    G_, S_ = ref['grads'], ref['size']
+    _close(g.dx[inside], G_['x'][ref['rows']], S_['x'][ref['rows']], out_terms, 'dx')
+    _close(g.dB[inside], G_['B'][ref['rows']], S_['B'][ref['rows']], 2 * out_terms, 'dB')
+    _close(g.dC[inside], G_['C'][ref['rows']], S_['C'][ref['rows']], 2 * out_terms, 'dC')
+    _close(g.ddt[inside], G_['raw'][ref['rows']], S_['raw'][ref['rows']], 2 * f32_terms, 'ddt')
+    _close(g.dA, G_['A'], S_['A'], 2 * f32_terms, 'dA')
+    _close(g.dD, G_['D'], S_['D'], f32_terms, 'dD')
+    _close(g.ddt_bias, G_['bias'], S_['bias'], 2 * f32_terms, 'ddt_bias')
+    _close(g.dh0, G_['h0'], S_['h0'], f32_terms, 'dh0')
+
+
+def test_ssm_scan_without_its_optional_inputs():
+    from dotaclient_amd import ops
+    dev = _dev()
+    lens = [70, 5]
+    off_d, len_d, rows, off, d = _scan_inputs(3, lens, 0, 2, 64, 1, 64, torch.float32, 0)
+    d['dt'] = d['dt'].abs() * 0.05
+    i64 = {k: v.cpu().double() for k, v in d.items()}
+    for k in ('bias', 'D', 'h0', 'dhT'):
+        i64[k] = torch.zeros_like(i64[k])
+    ref = _scan_reference(i64, off, lens, False)
+    y, hT = ops.ssm_scan(d['x'], d['dt'], d['A'], d['B'], d['C'], off_d, len_d, 70)
+    _close(y, ref['y'], ref['ya'], 500, 'y')
+    _close(hT, ref['hT'], ref['ha'], 500, 'hT')
+    g = ops.ssm_scan_backward(d['dy'], d['x'], d['dt'], d['A'], d['B'], d['C'], off_d, len_d, 70)
+    assert g.dD is None and g.ddt_bias is None and g.dh0 is None
+    _close(g.dx, ref['grads']['x'], ref['size']['x'], 1000, 'dx')
+    _close(g.ddt, ref['grads']['raw'], ref['size']['raw'], 1000, 'ddt')
+    _close(g.dA, ref['grads']['A'], ref['size']['A'], 1000, 'dA')
