@@ -138,7 +138,7 @@ struct StateLds {
 
 // The states alone.  Forward (blockIdx.y = 0): x, B from h0; reverse (1): dy, C from dhT, the blocks from the last to the first.
 // FINAL: the segments' own sums from zero and the sum of their dt A, for ssm_join_segments.  Else: from the segment's start, the state in front of
-// (reverse: the gradient of the state behind) every block to its slot, for the backward kernel; f32, or two bf16 planes hi | lo.
+// (reverse: the gradient of the state behind) every block to its slot, for the backward kernel.
 template <typename T, int NP, int V, bool REV, bool FINAL>
 __device__ __forceinline__ void states(const SsmArgs& a, StateLds<T, NP>& L) {
     constexpr int LX = pitch<T>(PT), LN = pitch<T>(NP);
@@ -193,18 +193,7 @@ __device__ __forceinline__ void states(const SsmArgs& a, StateLds<T, NP>& L) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int p = 16 * wave + 4 * g + r, n = 16 * c + i;
-                    if (p < P && n < a.NS) {
-                        if constexpr (sizeof(T) == 4) {
-                            static_cast<float*>(REV ? a.dS : a.S)[at + (int64_t)p * a.NS + n] = S[c][r];
-                        } else {
-                            bf16_t hi, lo;
-                            split_bf16(S[c][r], hi, lo);
-                            bf16_t* d = static_cast<bf16_t*>(REV ? a.dS : a.S) + (int64_t)(slot + blk) * a.H * a.P * a.NS * 2;
-                            const int64_t o = ((int64_t)h * a.P + p0 + p) * a.NS + n;
-                            d[o] = hi;
-                            d[o + (int64_t)a.H * a.P * a.NS] = lo;
-                        }
-                    }
+                    if (p < P && n < a.NS) (REV ? a.dS : a.S)[at + (int64_t)p * a.NS + n] = S[c][r];
                 }
         }
         const float et = __expf(L.st.total);

@@ -11,8 +11,8 @@
 //
 // A workgroup owns one block and the heads of one group (or a share of them, where blocks and groups alone are too few): G1 stays in its registers,
 // the T x T sums W and the gradients of B and C are added up over the heads there, so dB and dC cost two products per block instead of two per
-// head, and no partial sums in memory.  Operands that are f32 by nature are used as two bf16 pieces where an f32 result depends on them (S and dS:
-// R, K -> dA, ddt_bias); W and G1 L, which only end in bf16 outputs, are rounded once.
+// head, and no partial sums in memory.  Operands that are f32 by nature are used as three bf16 pieces where an f32 result depends on them (S and dS:
+// R, K -> dA, ddt_bias); W and G1 L, which only end in bf16 outputs, are rounded once, and dS in dx takes its first piece.
 #include "ssm_util.h"
 
 namespace dc {
@@ -20,37 +20,46 @@ namespace {
 
 template <typename T, int NP>
 struct BwdLds {
-    static constexpr int PIECES = sizeof(T) == 4 ? 1 : 2;
+    static constexpr int PIECES = sizeof(T) == 4 ? 1 : PIECES_F32;
     T b[TB * pitch<T>(NP)], c[TB * pitch<T>(NP)], x[TB * pitch<T>(PT)], y[TB * pitch<T>(PT)], s[PIECES][PT * pitch<T>(NP)], m[TB * pitch<T>(TB)];
     Steps st;
     float R[TB], diag[TB], KI[TB], col[16][TB], dot[4], trace[4];
 };
 
-// One plane (or both pieces) of a head's S or dS tile: columns in vectors of 16 bytes (the slots' rows are padded to whole ones).
+// A head's S or dS tile on its way to LDS, as f32 or as three bf16 pieces (the slots' rows are padded to whole vectors).
 template <typename T, int NP>
 struct StateTile {
-    static constexpr int PIECES = sizeof(T) == 4 ? 1 : 2;
-    Tile<T, NP, Mat<T>::V> v[PIECES];
-    __device__ __forceinline__ void load(const SsmArgs& a, const void* buf, int64_t slot, int h, int p0, int P) {
-        const int64_t plane = (int64_t)a.H * a.P * a.NS;
-        const T* p = static_cast<const T*>(buf) + slot * plane * PIECES + ((int64_t)h * a.P + p0) * a.NS;
-#pragma unroll
-        for (int k = 0; k < PIECES; ++k) v[k].load(p + k * plane, a.NS, P, a.NS);
+    Tile<float, NP, 4> v;
+    __device__ __forceinline__ void load(const SsmArgs& a, const float* buf, int64_t slot, int h, int p0, int P) {
+        v.load(buf + ((slot * a.H + h) * a.P + p0) * a.NS, a.NS, P, a.NS);
     }
     __device__ __forceinline__ void store(T (*lds)[PT * pitch<T>(NP)]) const {
+        if constexpr (sizeof(T) == 4) {
+            v.store(lds[0], pitch<T>(NP));
+        } else {
+            typedef bf16_t four __attribute__((ext_vector_type(4)));
 #pragma unroll
-        for (int k = 0; k < PIECES; ++k) v[k].store(lds[k], pitch<T>(NP));
+            for (int k = 0; k < v.N; ++k) {
+                const int idx = k * 256 + threadIdx.x, at = idx / v.PER_ROW * pitch<T>(NP) + idx % v.PER_ROW * 4;
+                four out[PIECES_F32];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    bf16_t p[PIECES_F32];
+                    split_bf16(v.v[k][e], p);
+#pragma unroll
+                    for (int pc = 0; pc < PIECES_F32; ++pc) out[pc][e] = p[pc];
+                }
+#pragma unroll
+                for (int pc = 0; pc < PIECES_F32; ++pc) *reinterpret_cast<four*>(lds[pc] + at) = out[pc];
+            }
+        }
     }
     __device__ __forceinline__ float dot(const StateTile& o) const {
         float s = 0.f;
 #pragma unroll
-        for (int k = 0; k < Tile<T, NP, Mat<T>::V>::N; ++k)
+        for (int k = 0; k < v.N; ++k)
 #pragma unroll
-            for (int e = 0; e < Mat<T>::V; ++e) {
-                float p = (float)v[0].v[k][e], q = (float)o.v[0].v[k][e];
-                if constexpr (PIECES == 2) { p += (float)v[1].v[k][e]; q += (float)o.v[1].v[k][e]; }
-                s = fmaf(p, q, s);
-            }
+            for (int e = 0; e < 4; ++e) s = fmaf(v.v[k][e], o.v.v[k][e], s);
         return s;
     }
 };
@@ -159,7 +168,7 @@ __global__ void __launch_bounds__(256) ssm_bwd_kernel(SsmArgs a) {
 #pragma unroll
                     for (int c = 0; c < NC; ++c)
 #pragma unroll
-                        for (int pc = 0; pc < PIECES; ++pc) acc[c] = M::mma(f, M::col(L.s[pc] + k * M::KS * LN + 16 * c, LN, i, g), acc[c]);
+                        for (int pc = PIECES - 1; pc >= 0; --pc) acc[c] = M::mma(f, M::col(L.s[pc] + k * M::KS * LN + 16 * c, LN, i, g), acc[c]);
                 }
 #pragma unroll
                 for (int r = 0; r < 4; ++r) e[r] = __expf(L.st.hi[r0 + 4 * g + r]);
@@ -193,7 +202,7 @@ __global__ void __launch_bounds__(256) ssm_bwd_kernel(SsmArgs a) {
 #pragma unroll
                     for (int c = 0; c < NC; ++c)
 #pragma unroll
-                        for (int pc = 0; pc < PIECES; ++pc) acc[c] = M::mma(f, M::col(L.s[pc] + k * M::KS * LN + 16 * c, LN, i, g), acc[c]);
+                        for (int pc = PIECES - 1; pc >= 0; --pc) acc[c] = M::mma(f, M::col(L.s[pc] + k * M::KS * LN + 16 * c, LN, i, g), acc[c]);
                 }
 #pragma unroll
                 for (int c = 0; c < NC; ++c)
@@ -448,8 +457,8 @@ int64_t bwd_plan(SsmArgs& a, char* scratch) {
     a.base = reinterpret_cast<int32_t*>(take(4 * ((int64_t)a.n_seq + 1)));
     a.map = reinterpret_cast<int32_t*>(take(4 * cap));
     a.part = reinterpret_cast<float*>(take(12 * cap * a.H));
-    a.S = take(4 * cap * a.H * a.P * a.NS);
-    a.dS = take(4 * cap * a.H * a.P * a.NS);
+    a.S = reinterpret_cast<float*>(take(4 * cap * a.H * a.P * a.NS));
+    a.dS = reinterpret_cast<float*>(take(4 * cap * a.H * a.P * a.NS));
     if (a.nseg > 1) {
         const int64_t n = (int64_t)a.n_seq * a.nseg * a.H;
         a.seg_state = reinterpret_cast<float*>(take(4 * n * a.P * a.N));

@@ -26,7 +26,7 @@ struct SsmArgs {
     void* dx; int64_t lddx; void* ddt; int64_t ldddt; void* dB; int64_t lddb; void* dC; int64_t lddc;
     float* dA; float* dD; float* ddt_bias; float* dh0;
     int32_t* base; int32_t* map; int cap;       // first block slot of each sequence [n_seq + 1], sequence of each slot [cap]
-    void* S; void* dS; int NS;                  // per slot and head: the state in front of the block, the gradient of the state behind it
+    float* S; float* dS; int NS;                // per slot and head [P][NS]: the state in front of the block, the gradient of the state behind it
     float* seg_dstate;
     float* part;                                // [cap][H][3]: sums for dA, dD, ddt_bias
     int hsplit; float* part_bc;                 // [hsplit][rows][G][2][N] where the heads of a group are shared out
@@ -140,14 +140,19 @@ __device__ __forceinline__ void make_steps(Steps& s, const SsmArgs& a, float raw
     if (lane == 63) s.total = (float)last;
 }
 
-__device__ __forceinline__ void split_bf16(float v, bf16_t& hi, bf16_t& lo) {
-    hi = (bf16_t)v;
-    lo = (bf16_t)(v - (float)hi);
+// v as three bf16 pieces: 24 bits, all of an f32's.
+constexpr int PIECES_F32 = 3;
+__device__ __forceinline__ void split_bf16(float v, bf16_t (&p)[PIECES_F32]) {
+#pragma unroll
+    for (int k = 0; k < PIECES_F32; ++k) {
+        p[k] = (bf16_t)v;
+        v -= (float)p[k];
+    }
 }
 
 // acc[p][n] (16 rows p of this wave, NP columns) += sum_t w_t X[t][p] Y[t][n], from the tiles X [64][PT] and Y [64][NP].
-// The weights are f32: bf16 operands are scaled in f32 and used as two bf16 pieces (2^-17 of the product is lost), because the states they end
-// in are f32.
+// The weights are f32: bf16 operands are scaled in f32 and used as three bf16 pieces, because the states they end in are f32 (with two pieces, 16 bits,
+// the gradients of A and dt_bias were off by 4e-6 .. 8e-6 of their norm, with three by what f32 sums are off by).
 template <typename T, int NP>
 __device__ __forceinline__ void state_update(f32x4 (&acc)[NP / 16], const T* X, int ldx, const T* Y, int ldy, const float* w, int p0, int i, int g) {
     typedef Mat<T> M;
@@ -160,19 +165,19 @@ __device__ __forceinline__ void state_update(f32x4 (&acc)[NP / 16], const T* X, 
 #pragma unroll
             for (int c = 0; c < NP / 16; ++c) acc[c] = M::mma(a, M::col(Y + k * ldy + 16 * c, ldy, i, g), acc[c]);
         } else {
-            typename M::frag lo;
+            typename M::frag piece[PIECES_F32];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                bf16_t h, l;
-                split_bf16((float)a[e] * w[k + 8 * g + e], h, l);
-                a[e] = h;
-                lo[e] = l;
+                bf16_t v[PIECES_F32];
+                split_bf16((float)a[e] * w[k + 8 * g + e], v);
+#pragma unroll
+                for (int pc = 0; pc < PIECES_F32; ++pc) piece[pc][e] = v[pc];
             }
 #pragma unroll
             for (int c = 0; c < NP / 16; ++c) {
                 const typename M::frag b = M::col(Y + k * ldy + 16 * c, ldy, i, g);
-                acc[c] = M::mma(a, b, acc[c]);
-                acc[c] = M::mma(lo, b, acc[c]);
+#pragma unroll
+                for (int pc = PIECES_F32 - 1; pc >= 0; --pc) acc[c] = M::mma(piece[pc], b, acc[c]);
             }
         }
     }

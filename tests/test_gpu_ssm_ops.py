@@ -383,11 +383,11 @@ def test_ssm_scan_forward_and_backward(lens, gap, H, P, G, N, pad, softplus, dty
     y, hT = ops.ssm_scan(d['x'], d['dt'], d['A'], d['B'], d['C'], *seqs, y=keep, **kw)
     inside = ref['rows'].to(dev)
     # f32: sums of up to 64 + N + P terms, a few steps per factor (exp of differences up to ~100: 100 of them), 16 per block and segment on the
-    # way.  bf16: the factors G1 L dt and S are rounded once (half a step of the term); what ends in f32 is made of two pieces, 2^-16 = 256 u32
-    # lost per operand, four operands in a row at most.
+    # way.  bf16: the factors G1 L dt and S are rounded once (half a step of the term) for y, dx, dB, dC; what ends in f32 is made of three
+    # bf16 pieces per factor, exact to 2^-24.
     bf = dtype == torch.bfloat16
     terms = 64 + N + P + 160 + 32 * (1 + max(lens) // 64)
-    f32_terms = terms + (1024 if bf else 0)
+    f32_terms = terms + (8 if bf else 0)
     out_terms = terms + (2 ** 16 if bf else 0)             # 2^-8 of the sum of the terms' magnitudes
     _close(y[inside], ref['y'], ref['ya'], out_terms, 'y')
     rest = torch.ones(rows, dtype=torch.bool)
