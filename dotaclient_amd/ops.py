@@ -109,10 +109,12 @@ _TYPES = {torch.float32: 0, torch.bfloat16: 1}
 
 def _rows(t, name, dtype, shape):
     """Checks a row tensor; returns the distance between its rows in elements."""
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise TypeError('%s: expected %s, got %s' % (name, dtype, t.dtype))
-    if tuple(t.shape) != shape:
-        raise ValueError('%s: expected shape %s, got %s' % (name, shape, tuple(t.shape)))
+    if t.shape != shape:
+        raise ValueError('%s: expected shape %s, got %s' % (name, tuple(shape), tuple(t.shape)))
+    if t.is_contiguous():
+        return t.stride(0)
     width, st = 1, t.stride()
     for i in range(len(shape) - 1, 0, -1):
         if shape[i] != 1 and st[i] != width:
@@ -124,19 +126,19 @@ def _rows(t, name, dtype, shape):
 def _out_rows(t, name, dtype, shape, like):
     """A row tensor to write to (allocated where None); returns it and the distance between its rows."""
     if t is None:
-        t = torch.empty(shape, dtype=dtype, device=like.device)
+        t = like.new_empty(shape, dtype=dtype)
+        return t, t.stride(0)
     ld = _rows(t, name, dtype, shape)
-    width = t.numel() // shape[0] if shape[0] else 1
-    if ld < width:
+    if shape[0] and ld < t.numel() // shape[0]:
         raise ValueError('%s: the rows of an output must not overlap' % name)
     return t, ld
 
 
 def _param(t, name, shape, dtype=torch.float32):
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise TypeError('%s: expected %s, got %s' % (name, dtype, t.dtype))
-    if tuple(t.shape) != shape:
-        raise ValueError('%s: expected shape %s, got %s' % (name, shape, tuple(t.shape)))
+    if t.shape != shape:
+        raise ValueError('%s: expected shape %s, got %s' % (name, tuple(shape), tuple(t.shape)))
     if not t.is_contiguous():
         raise ValueError('%s must be contiguous' % name)
     return t
@@ -158,31 +160,28 @@ def _sequences(seq_off, seq_len, max_len):
 
 
 def _distinct(outs, ins):
-    """Refuses an output that starts where an input does."""
-    at = {t.data_ptr() for t in ins if t is not None and t.numel()}
+    """Refuses an output of the caller's that starts where an input does."""
     for name, t in outs:
-        if t is not None and t.numel() and t.data_ptr() in at:
+        if t is not None and t.numel() and any(i is not None and i.data_ptr() == t.data_ptr() for i in ins):
             raise ValueError('%s must not be one of the inputs' % name)
 
 
 def _run(name, tensors, *args):
     """Calls the C entry point on the tensors' device and that device's current stream."""
-    lib = _lib.load()
-    dev = None
+    dev = tensors[0].get_device()
     for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise _lib.DotaHipError('%s: its tensors must live on the GPU (there is no CPU path)' % name)
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise ValueError('%s: its tensors live on %s and %s' % (name, dev, t.device))
-    if dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
-            _lib.check(getattr(lib, name)(*args, torch.cuda.current_stream().cuda_stream), name)
+        if t is not None and (t.get_device() != dev or dev < 0):
+            if not all(u is None or u.is_cuda for u in tensors):
+                raise _lib.DotaHipError('%s: its tensors must live on the GPU (there is no CPU path)' % name)
+            raise ValueError('%s: its tensors live on %s and %s' % (name, tensors[0].device, t.device))
+    lib = _lib.load()
+    if dev == torch.cuda.current_device():
+        rc = getattr(lib, name)(*args, torch._C._cuda_getCurrentRawStream(dev))
     else:
-        _lib.check(getattr(lib, name)(*args, torch.cuda.current_stream().cuda_stream), name)
+        with torch.cuda.device(dev):
+            rc = getattr(lib, name)(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        _lib.check(rc, name)
 
 
 def _p(t):
@@ -210,9 +209,9 @@ def causal_conv(x, weight, bias, seq_off, seq_len, max_len, state=None, silu=Tru
     ldx = _rows(x, 'x', x.dtype, (rows, D))
     if state is not None:
         _param(state, 'state', (n, K - 1, D), x.dtype)
-    y, ldy = _out_rows(y, 'y', x.dtype, (rows, D), x)
-    state_out = torch.empty((n, K - 1, D), dtype=x.dtype, device=x.device) if state_out is None else _param(state_out, 'state_out', (n, K - 1, D), x.dtype)
     _distinct((('y', y), ('state_out', state_out)), (x, state))
+    y, ldy = _out_rows(y, 'y', x.dtype, (rows, D), x)
+    state_out = x.new_empty((n, K - 1, D)) if state_out is None else _param(state_out, 'state_out', (n, K - 1, D), x.dtype)
     _run('dc_causal_conv_fwd', (x, weight, bias, seq_off, seq_len, state, y, state_out), x.data_ptr(), ldx, weight.data_ptr(), _p(bias),
          seq_off.data_ptr(), seq_len.data_ptr(), rows, n, max_len, D, K, ty, int(silu), _p(state), y.data_ptr(), ldy, state_out.data_ptr())
     return y, state_out
@@ -227,13 +226,13 @@ def causal_conv_backward(dy, x, weight, bias, seq_off, seq_len, max_len, state=N
     for t, name in ((state, 'state'), (dstate_out, 'dstate_out')):
         if t is not None:
             _param(t, name, (n, K - 1, D), x.dtype)
-    dx, lddx = _out_rows(dx, 'dx', x.dtype, (rows, D), x)
     _distinct((('dx', dx),), (x, dy, state, dstate_out))
+    dx, lddx = _out_rows(dx, 'dx', x.dtype, (rows, D), x)
     dw = torch.empty_like(weight)
     db = None if bias is None else torch.empty_like(bias)
     dstate = None if state is None else torch.empty_like(state)
     size = _lib.load().dc_causal_conv_scratch(n, max_len, D, K)
-    scratch = torch.empty(max(size, 16), dtype=torch.uint8, device=x.device)
+    scratch = x.new_empty(max(size, 16), dtype=torch.uint8)
     _run('dc_causal_conv_bwd', (dy, x, weight, bias, seq_off, seq_len, state, dstate_out, dx), dy.data_ptr(), lddy, x.data_ptr(), ldx, weight.data_ptr(),
          _p(bias), seq_off.data_ptr(), seq_len.data_ptr(), rows, n, max_len, D, K, ty, int(silu), _p(state), _p(dstate_out), dx.data_ptr(), lddx,
          dw.data_ptr(), _p(db), _p(dstate), scratch.data_ptr(), size)
@@ -248,10 +247,10 @@ def causal_conv_step(x, state, weight, bias, silu=True, y=None, state_out=None):
     ldx = _rows(x, 'x', x.dtype, (n, D))
     if state is not None:
         _param(state, 'state', (n, K - 1, D), x.dtype)
-    y, ldy = _out_rows(y, 'y', x.dtype, (n, D), x)
-    state_out = torch.empty((n, K - 1, D), dtype=x.dtype, device=x.device) if state_out is None else _param(state_out, 'state_out', (n, K - 1, D), x.dtype)
     _distinct((('y', y),), (x, state))
     _distinct((('state_out', state_out),), (x,))
+    y, ldy = _out_rows(y, 'y', x.dtype, (n, D), x)
+    state_out = x.new_empty((n, K - 1, D)) if state_out is None else _param(state_out, 'state_out', (n, K - 1, D), x.dtype)
     _run('dc_causal_conv_step', (x, state, weight, bias, y, state_out), x.data_ptr(), ldx, _p(state), weight.data_ptr(), _p(bias), n, D, K, ty, int(silu),
          y.data_ptr(), ldy, state_out.data_ptr())
     return y, state_out
@@ -283,11 +282,11 @@ def ssm_scan(x, dt, A, B, C, seq_off, seq_len, max_len, D=None, dt_bias=None, h0
     n = _sequences(seq_off, seq_len, max_len)
     if h0 is not None:
         _param(h0, 'h0', (n, H, P, N))
-    y, ldy = _out_rows(y, 'y', x.dtype, (rows, H, P), x)
-    hT = torch.empty((n, H, P, N), dtype=torch.float32, device=x.device) if hT is None else _param(hT, 'hT', (n, H, P, N))
     _distinct((('y', y), ('hT', hT)), (x, dt, B, C, h0))
+    y, ldy = _out_rows(y, 'y', x.dtype, (rows, H, P), x)
+    hT = x.new_empty((n, H, P, N), dtype=torch.float32) if hT is None else _param(hT, 'hT', (n, H, P, N))
     size = _lib.load().dc_ssm_scan_scratch(n, max_len, H, P, N)
-    scratch = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+    scratch = x.new_empty(size, dtype=torch.uint8) if size else None
     _run('dc_ssm_scan_fwd', (x, dt, A, B, C, D, dt_bias, h0, seq_off, seq_len, y, hT), x.data_ptr(), ldx, dt.data_ptr(), lddt, A.data_ptr(), B.data_ptr(),
          ldb, C.data_ptr(), ldc, _p(D), _p(dt_bias), _p(h0), seq_off.data_ptr(), seq_len.data_ptr(), rows, n, max_len, H, P, G, N, ty, int(softplus),
          y.data_ptr(), ldy, hT.data_ptr(), _p(scratch), size)
@@ -316,15 +315,15 @@ def ssm_scan_backward(dy, x, dt, A, B, C, seq_off, seq_len, max_len, D=None, dt_
     for t, name in ((h0, 'h0'), (dhT, 'dhT')):
         if t is not None:
             _param(t, name, (n, H, P, N))
+    _distinct((('dx', dx), ('ddt', ddt), ('dB', dB), ('dC', dC)), (dy, x, dt, B, C))
     dx, lddx = _out_rows(dx, 'dx', x.dtype, (rows, H, P), x)
     ddt, ldddt = _out_rows(ddt, 'ddt', x.dtype, (rows, H), x)
     dB, lddb = _out_rows(dB, 'dB', x.dtype, (rows, G, N), x)
     dC, lddc = _out_rows(dC, 'dC', x.dtype, (rows, G, N), x)
-    _distinct((('dx', dx), ('ddt', ddt), ('dB', dB), ('dC', dC)), (dy, x, dt, B, C))
     dA = torch.empty_like(A)
     dD, dbias, dh0 = (None if t is None else torch.empty_like(t) for t in (D, dt_bias, h0))
     size = _lib.load().dc_ssm_scan_bwd_scratch(rows, n, max_len, H, P, G, N)
-    scratch = torch.empty(size, dtype=torch.uint8, device=x.device)
+    scratch = x.new_empty(size, dtype=torch.uint8)
     _run('dc_ssm_scan_bwd', (dy, x, dt, A, B, C, D, dt_bias, h0, dhT, seq_off, seq_len, dx, ddt, dB, dC), dy.data_ptr(), lddy, x.data_ptr(), ldx,
          dt.data_ptr(), lddt, A.data_ptr(), B.data_ptr(), ldb, C.data_ptr(), ldc, _p(D), _p(dt_bias), _p(h0), _p(dhT), seq_off.data_ptr(),
          seq_len.data_ptr(), rows, n, max_len, H, P, G, N, ty, int(softplus), dx.data_ptr(), lddx, ddt.data_ptr(), ldddt, dB.data_ptr(), lddb, dC.data_ptr(),
@@ -337,10 +336,10 @@ def ssm_step(x, dt, A, B, C, h0=None, D=None, dt_bias=None, softplus=False, y=No
     n, H, P, G, N, ty, (ldx, lddt, ldb, ldc) = _scan_operands(x, dt, A, B, C, D, dt_bias)
     if h0 is not None:
         _param(h0, 'h0', (n, H, P, N))
-    y, ldy = _out_rows(y, 'y', x.dtype, (n, H, P), x)
-    hT = torch.empty((n, H, P, N), dtype=torch.float32, device=x.device) if hT is None else _param(hT, 'hT', (n, H, P, N))
     _distinct((('y', y),), (x, dt, B, C, h0))
     _distinct((('hT', hT),), (x, dt, B, C))
+    y, ldy = _out_rows(y, 'y', x.dtype, (n, H, P), x)
+    hT = x.new_empty((n, H, P, N), dtype=torch.float32) if hT is None else _param(hT, 'hT', (n, H, P, N))
     _run('dc_ssm_step', (x, dt, A, B, C, D, dt_bias, h0, y, hT), x.data_ptr(), ldx, dt.data_ptr(), lddt, A.data_ptr(), B.data_ptr(), ldb, C.data_ptr(), ldc,
          _p(D), _p(dt_bias), _p(h0), n, H, P, G, N, ty, int(softplus), y.data_ptr(), ldy, hT.data_ptr())
     return y, hT
@@ -368,9 +367,9 @@ def block_norm(y, residual, w_post, gate=None, scale=None, w_pre=None, eps=1e-5,
     y, gate [rows, D]; residual [rows, D] in y's type or f32; w_post, scale, w_pre [D]; gate, scale, w_pre may be None.  D <= 8192.
     -> (r in residual's type, x in y's type; None without w_pre).  residual_out may be residual itself; x is taken from r before r is rounded."""
     rows, D, ty, tr, ldy, ldr, ldg = _norm_operands(y, residual, w_post, gate, scale, w_pre)
+    _distinct((('residual_out', residual_out),), (y, gate))
     r, ldro = _out_rows(residual_out, 'residual_out', residual.dtype, (rows, D), y)
-    _distinct((('residual_out', r),), (y, gate))
-    x = None if w_pre is None else torch.empty((rows, D), dtype=y.dtype, device=y.device)
+    x = None if w_pre is None else y.new_empty((rows, D))
     _run('dc_block_norm_fwd', (y, residual, w_post, gate, scale, w_pre, r), y.data_ptr(), ldy, _p(gate), ldg, residual.data_ptr(), ldr, w_post.data_ptr(),
          _p(scale), _p(w_pre), rows, D, ty, tr, eps, r.data_ptr(), ldro, _p(x), D)
     return r, x
@@ -384,12 +383,12 @@ def block_norm_backward(dr, dx, y, residual, w_post, gate=None, scale=None, w_pr
         raise ValueError('dx: expected exactly with w_pre')
     lddr = _rows(dr, 'dr', residual.dtype, (rows, D))
     lddx = 0 if dx is None else _rows(dx, 'dx', y.dtype, (rows, D))
-    new = lambda t, d: None if t is None else torch.empty((rows, D), dtype=d, device=y.device)      # noqa: E731
+    new = lambda t, d: None if t is None else y.new_empty((rows, D), dtype=d)      # noqa: E731
     dy, dres, dgate = new(y, y.dtype), new(residual, residual.dtype), new(gate, y.dtype)
     dw_post = torch.empty_like(w_post)
     dscale, dw_pre = (None if t is None else torch.empty_like(t) for t in (scale, w_pre))
     size = _lib.load().dc_block_norm_scratch(rows, D)
-    scratch = torch.empty(max(size, 16), dtype=torch.uint8, device=y.device)
+    scratch = y.new_empty(max(size, 16), dtype=torch.uint8)
     _run('dc_block_norm_bwd', (dr, dx, y, residual, w_post, gate, scale, w_pre), dr.data_ptr(), lddr, _p(dx), lddx, y.data_ptr(), ldy, _p(gate), ldg,
          residual.data_ptr(), ldr, w_post.data_ptr(), _p(scale), _p(w_pre), rows, D, ty, tr, eps, dy.data_ptr(), _p(dgate), dres.data_ptr(),
          dw_post.data_ptr(), _p(dscale), _p(dw_pre), scratch.data_ptr(), size)
