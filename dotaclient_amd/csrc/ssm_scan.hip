@@ -1,9 +1,11 @@
 // Selective state space scan over packed sequences, forward, and the single step.  The mathematics: ssm_util.h.
 //
-// Prompts: a workgroup of four waves walks the blocks of one sequence (or of one segment of it), one head and up to 64 of its columns; the state
-// stays in the accumulators of its waves (wave w: rows 16 w .. of the [P][N] state, 64 x 64 floats = 16 registers per lane) from the first block to the
-// last, x, B, C are read once and y is written once.  Where that gives too few workgroups (few, long sequences) the sequences are cut into segments:
-// a first kernel computes what each segment adds to a zero state, a second one runs along the segments, and the scan starts each segment from there.
+// Prompts: a workgroup of four waves walks the blocks of one sequence (or of one segment of it), one head and up to 64 of its columns p, sixteen a wave.
+// The state stays in the accumulators from the first block to the last, x, B, C are read once and y is written once.  Per block:
+//   M[t][s] = exp(a_t - a_s) (C_t . B_s) dt_s, the ten 16 x 16 tiles with s <= t shared out evenly over the waves, through LDS;
+//   y^T = x^T M^T + exp(a_t) S C^T + D x^T and the new state for each wave's own columns, so that no wave waits for another one's part of S.
+// Where the sequences, heads and columns give too few workgroups (few, long sequences) the sequences are cut into segments: a first kernel computes what
+// each segment adds to a zero state, a second one runs along the segments, and the scan starts each segment from there.
 #include "ssm_util.h"
 
 namespace dc {
@@ -11,129 +13,148 @@ namespace {
 
 template <typename T, int NP>
 struct FwdLds {
-    T x[TB * pitch<T>(PT)], b[TB * pitch<T>(NP)], c[TB * pitch<T>(NP)], s[PT * pitch<T>(NP)], m[TB * pitch<T>(TB)];
-    Steps st;
+    T x[TB * pitch<T>(PT)], b[TB * pitch<T>(NP)], c[TB * pitch<T>(NP)], m[TB * pitch<T>(TB)];
+    Steps st[2];
 };
+
+// The twelve 16 x 16 tiles (row tile, column tile) of M that products with it read: ten with s <= t, and two zero ones that complete
+// the 32-column steps of row tiles 0 and 2.  Wave w takes w, w + 4, w + 8.
+__device__ __forceinline__ int tile_row(int u) { return (0x203323213210ull >> (4 * u)) & 15; }
+__device__ __forceinline__ int tile_col(int u) { return (0x310102103210ull >> (4 * u)) & 15; }
 
 template <typename T, int NP, int V>
 __global__ void __launch_bounds__(256) ssm_fwd_kernel(SsmArgs a) {
     typedef Mat<T> M;
-    constexpr int LX = pitch<T>(PT), LN = pitch<T>(NP), LM = pitch<T>(TB);
+    constexpr int LX = pitch<T>(PT), LN = pitch<T>(NP), LM = pitch<T>(TB), NK = NP / M::KS;
     extern __shared__ __attribute__((aligned(16))) char lds_raw[];
     FwdLds<T, NP>& L = *reinterpret_cast<FwdLds<T, NP>*>(lds_raw);
-    int unit, h, p0;
-    if (!work_item(a, unit, h, p0)) return;
+    int unit, h, pbase;
+    if (!work_item(a, unit, h, pbase)) return;
     const int b = unit / a.nseg, seg = unit % a.nseg, grp = h / (a.H / a.G);
     const SeqRange q = seq_range(a.seq_off, a.seq_len, b, a.rows, a.max_len);
     const int nb = blocks_of(q.len), first = seg * a.seg_blocks;
     if (first >= nb && seg > 0) return;
     const int last = min(nb, first + a.seg_blocks);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
-    const int P = min(a.P - p0, PT), N = a.N;
-    const int64_t state_at = ((int64_t)b * a.H + h) * a.P * N + (int64_t)p0 * N;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4, p0 = 16 * wave;
+    const int P = min(a.P - pbase, PT), N = a.N;
+    const int64_t state_at = ((int64_t)b * a.H + h) * a.P * N + (int64_t)pbase * N;
     f32x4 S[NP / 16];
-    const float* init = a.nseg > 1 ? a.seg_state + ((int64_t)unit * a.H + h) * a.P * N + (int64_t)p0 * N : a.h0 ? a.h0 + state_at : nullptr;
-    load_state<NP>(S, init, 16 * wave, P, N, i, g);
+    const float* init = a.nseg > 1 ? a.seg_state + ((int64_t)unit * a.H + h) * a.P * N + (int64_t)pbase * N : a.h0 ? a.h0 + state_at : nullptr;
+    load_state<NP, V>(S, init, N, p0, P, N, i, g);
     const float A = a.A[h], bias = a.dt_bias ? a.dt_bias[h] : 0.f, D = a.D ? a.D[h] : 0.f;
-    const T* xp = static_cast<const T*>(a.x) + q.off * a.ldx + (int64_t)h * a.P + p0;
+    const T* xp = static_cast<const T*>(a.x) + q.off * a.ldx + (int64_t)h * a.P + pbase;
     const T* bp = static_cast<const T*>(a.B) + q.off * a.ldb + (int64_t)grp * N;
     const T* cp = static_cast<const T*>(a.C) + q.off * a.ldc + (int64_t)grp * N;
     const T* dp = static_cast<const T*>(a.dt) + q.off * a.lddt + h;
-    T* yp = static_cast<T*>(a.y) + q.off * a.ldy + (int64_t)h * a.P + p0;
+    T* yp = static_cast<T*>(a.y) + q.off * a.ldy + (int64_t)h * a.P + pbase;
     Tile<T, PT, V> tx;
     Tile<T, NP, V> tb, tc;
-    float raw = 0.f;
     auto fetch = [&](int blk) {
         const int64_t t0 = (int64_t)blk * TB;
         const int rows = min(TB, q.len - (int)t0);
         tx.load(xp + t0 * a.ldx, a.ldx, rows, P);
         tb.load(bp + t0 * a.ldb, a.ldb, rows, N);
         tc.load(cp + t0 * a.ldc, a.ldc, rows, N);
-        if (wave == 0) raw = lane < rows ? (float)dp[(t0 + lane) * a.lddt] : 0.f;
     };
-    if (first < last) fetch(first);
+    auto fetch_dt = [&](int blk) {
+        const int64_t t = (int64_t)blk * TB + lane;
+        return t < q.len ? (float)dp[t * a.lddt] : 0.f;
+    };
+    if (first < last) {
+        float raw = 0.f;
+        if (wave == 3) raw = fetch_dt(first);
+        fetch(first);
+        if (wave == 3) make_steps<false>(L.st[first & 1], a, raw, first * TB + lane < q.len, A, bias, lane);
+    }
     for (int blk = first; blk < last; ++blk) {
         const int64_t t0 = (int64_t)blk * TB;
         const int rows = min(TB, q.len - (int)t0);
+        const Steps& st = L.st[blk & 1];
         tx.store(L.x, LX);
         tb.store(L.b, LN);
         tc.store(L.c, LN);
-        if (wave == 0) make_steps<false>(L.st, a, raw, lane < rows, A, bias, lane);
-#pragma unroll
-        for (int c = 0; c < NP / 16; ++c)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) L.s[(16 * wave + 4 * g + r) * LN + 16 * c + i] = (T)S[c][r];
         __syncthreads();
+        float raw = 0.f;
+        if (wave == 3 && blk + 1 < last) raw = fetch_dt(blk + 1);
         if (blk + 1 < last) fetch(blk + 1);
-        // rows t = 16 wave + 4 g + r of this wave against columns s <= t
-        typename M::frag cf[NP / M::KS];
+        // M, as (C B^T)^T: lane i owns row t, four neighbouring s of it
 #pragma unroll
-        for (int k = 0; k < NP / M::KS; ++k) cf[k] = M::row(L.c + 16 * wave * LN + k * M::KS, LN, i, g);
-        T* m = L.m + 16 * wave * LM;
-        const int kend = (16 * (wave + 1) + M::KS - 1) / M::KS * M::KS;       // columns of m that the product with x reads
-        for (int c = 0; c * 16 < kend; ++c) {
-            f32x4 acc = {};
-            if (c <= wave) {
+        for (int u = 0; u < 3; ++u) {
+            const int jt = tile_row(wave + 4 * u), js = tile_col(wave + 4 * u);
+            if (16 * jt >= rows) continue;
+            f32x4 m = {};
+            if (js <= jt) {
 #pragma unroll
-                for (int k = 0; k < NP / M::KS; ++k) acc = M::mma(cf[k], M::row(L.b + 16 * c * LN + k * M::KS, LN, i, g), acc);
-                const int s = 16 * c + i;
-                const float hs = L.st.hi[s], ls = L.st.lo[s], ds = L.st.dt[s];
+                for (int k = 0; k < NK; ++k)
+                    m = M::mma(M::row(L.b + 16 * js * LN + k * M::KS, LN, i, g), M::row(L.c + 16 * jt * LN + k * M::KS, LN, i, g), m);
+                const int t = 16 * jt + i, s = 16 * js + 4 * g;
+                const float ht = st.hi[t], lt = st.lo[t];
+                const f32x4 hs = *reinterpret_cast<const f32x4*>(st.hi + s), ls = *reinterpret_cast<const f32x4*>(st.lo + s),
+                            ds = *reinterpret_cast<const f32x4*>(st.dt + s);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int t = 16 * wave + 4 * g + r;
-                    acc[r] = s <= t ? acc[r] * (__expf(gap(L.st, t, hs, ls)) * ds) : 0.f;
+                for (int r = 0; r < 4; ++r) m[r] = s + r <= t ? m[r] * (__expf((ht - hs[r]) + (lt - ls[r])) * ds[r]) : 0.f;
+            }
+            *reinterpret_cast<typename Four<T>::vec*>(L.m + (16 * jt + i) * LM + 16 * js + 4 * g) = four<T>(m);
+        }
+        if (wave == 3 && blk + 1 < last) make_steps<false>(L.st[(blk + 1) & 1], a, raw, t0 + TB + lane < q.len, A, bias, lane);
+        __syncthreads();
+        f32x4 y[TB / 16];
+#pragma unroll
+        for (int jt = 0; jt < TB / 16; ++jt) {
+            y[jt] = f32x4{};
+            if (16 * jt >= rows) continue;
+            // S is rounded once to bf16 there, like M: both only end in y
+#pragma unroll
+            for (int k = 0; k < NK; ++k) {
+                typename M::frag sf;
+                if constexpr (sizeof(T) == 4) {
+                    sf = S[k];
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) sf[e] = (T)S[2 * k + (e >> 2)][e & 3];
                 }
+                y[jt] = M::mma(sf, M::row(L.c + 16 * jt * LN + k * M::KS, LN, i, g), y[jt]);
             }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) m[(4 * g + r) * LM + 16 * c + i] = (T)acc[r];
-        }
-        f32x4 y[PT / 16];
-        float ea[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) ea[r] = __expf(L.st.hi[16 * wave + 4 * g + r]);
-#pragma unroll
-        for (int c = 0; c < PT / 16; ++c) {
-            y[c] = f32x4{};
-#pragma unroll
-            for (int k = 0; k < NP / M::KS; ++k) y[c] = M::mma(cf[k], M::row(L.s + 16 * c * LN + k * M::KS, LN, i, g), y[c]);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) y[c][r] *= ea[r];
-        }
-        for (int k = 0; k < kend; k += M::KS) {
-            const typename M::frag mf = M::row(m + k, LM, i, g);
-#pragma unroll
-            for (int c = 0; c < PT / 16; ++c) y[c] = M::mma(mf, M::col(L.x + k * LX + 16 * c, LX, i, g), y[c]);
+            y[jt] *= __expf(st.hi[16 * jt + i]);
         }
 #pragma unroll
-        for (int c = 0; c < PT / 16; ++c)
+        for (int k = 0; k < TB; k += M::KS) {
+            if (k >= rows) continue;
+            const typename M::frag xf = M::col(L.x + k * LX + p0, LX, i, g);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int t = 16 * wave + 4 * g + r;
-                m[(4 * g + r) * LM + 16 * c + i] = (T)(y[c][r] + D * (float)L.x[t * LX + 16 * c + i]);
-            }
-        // the wave's sixteen rows of y, through its part of m, in whole 16-byte pieces
-        {
-            typedef T vec_t __attribute__((ext_vector_type(V)));
-            constexpr int PER_ROW = PT / V;
+            for (int jt = k / 16; jt < TB / 16; ++jt)
+                if (16 * jt < rows) y[jt] = M::mma(xf, M::row(L.m + 16 * jt * LM + k, LM, i, g), y[jt]);
+        }
 #pragma unroll
-            for (int k = 0; k < 16 * PER_ROW / 64; ++k) {
-                const int idx = k * 64 + lane, r = idx / PER_ROW, c = idx % PER_ROW * V, t = 16 * wave + r;
-                if (t < rows && c < P) *reinterpret_cast<vec_t*>(yp + (t0 + t) * a.ldy + c) = *reinterpret_cast<const vec_t*>(m + r * LM + c);
+        for (int jt = 0; jt < TB / 16; ++jt) {
+            const int t = 16 * jt + i, p = p0 + 4 * g;
+            if (t >= rows || p >= P) continue;
+            const typename Four<T>::vec xv = *reinterpret_cast<const typename Four<T>::vec*>(L.x + t * LX + p);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) y[jt][r] = fmaf(D, (float)xv[r], y[jt][r]);
+            T* out = yp + (t0 + t) * a.ldy + p;
+            const typename Four<T>::vec o = four<T>(y[jt]);
+            if (V > 1) {
+                *reinterpret_cast<typename Four<T>::vec*>(out) = o;
+            } else {
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (p + r < P) out[r] = o[r];
             }
         }
-        const float et = __expf(L.st.total);
+        const float et = __expf(st.total);
 #pragma unroll
         for (int c = 0; c < NP / 16; ++c) S[c] *= et;
-        state_update<T, NP>(S, L.x, LX, L.b, LN, L.st.w, 16 * wave, i, g);
+        state_update<T, NP>(S, L.x, LX, L.b, LN, st.w, p0, rows, i, g);
         __syncthreads();
     }
-    if (last == nb && a.hT) store_state<NP>(S, a.hT + state_at, 16 * wave, P, N, i, g);
+    if (last == nb && a.hT) store_state<NP, V>(S, a.hT + state_at, N, p0, P, N, i, g);
 }
 
 template <typename T, int NP>
 struct StateLds {
     T x[TB * pitch<T>(PT)], b[TB * pitch<T>(NP)];
-    Steps st;
+    Steps st[2];
 };
 
 // The states alone.  Forward (blockIdx.y = 0): x, B from h0; reverse (1): dy, C from dhT, the blocks from the last to the first.
@@ -142,8 +163,8 @@ struct StateLds {
 template <typename T, int NP, int V, bool REV, bool FINAL>
 __device__ __forceinline__ void states(const SsmArgs& a, StateLds<T, NP>& L) {
     constexpr int LX = pitch<T>(PT), LN = pitch<T>(NP);
-    int unit, h, p0;
-    if (!work_item(a, unit, h, p0)) return;
+    int unit, h, pbase;
+    if (!work_item(a, unit, h, pbase)) return;
     const int b = unit / a.nseg, seg = unit % a.nseg, grp = h / (a.H / a.G);
     const SeqRange q = seq_range(a.seq_off, a.seq_len, b, a.rows, a.max_len);
     int nb = blocks_of(q.len), slot = 0;
@@ -152,62 +173,65 @@ __device__ __forceinline__ void states(const SsmArgs& a, StateLds<T, NP>& L) {
         nb = min(nb, a.base[b + 1] - slot);
     }
     const int first = seg * a.seg_blocks, last = min(nb, first + a.seg_blocks);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
-    const int P = min(a.P - p0, PT), N = a.N;
-    const int64_t seg_at = ((int64_t)unit * a.H + h) * a.P * N + (int64_t)p0 * N, state_at = ((int64_t)b * a.H + h) * a.P * N + (int64_t)p0 * N;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4, p0 = 16 * wave;
+    const int P = min(a.P - pbase, PT), N = a.N;
+    const int64_t seg_at = ((int64_t)unit * a.H + h) * a.P * N + (int64_t)pbase * N, state_at = ((int64_t)b * a.H + h) * a.P * N + (int64_t)pbase * N;
     float* const seg_state = REV ? a.seg_dstate : a.seg_state;
     const float* const user = REV ? a.dhT : a.h0;
     f32x4 S[NP / 16];
-    load_state<NP>(S, FINAL ? nullptr : a.nseg > 1 ? seg_state + seg_at : user ? user + state_at : nullptr, 16 * wave, P, N, i, g);
+    load_state<NP, V>(S, FINAL ? nullptr : a.nseg > 1 ? seg_state + seg_at : user ? user + state_at : nullptr, N, p0, P, N, i, g);
     const float A = a.A[h], bias = a.dt_bias ? a.dt_bias[h] : 0.f;
     const T* xp = static_cast<const T*>(REV ? a.dy : a.x);
     const T* bp = static_cast<const T*>(REV ? a.C : a.B);
     const int64_t ldx = REV ? a.lddy : a.ldx, ldb = REV ? a.ldc : a.ldb;
-    xp += q.off * ldx + (int64_t)h * a.P + p0;
+    xp += q.off * ldx + (int64_t)h * a.P + pbase;
     bp += q.off * ldb + (int64_t)grp * N;
     const T* dp = static_cast<const T*>(a.dt) + q.off * a.lddt + h;
     Tile<T, PT, V> tx;
     Tile<T, NP, V> tb;
-    float raw = 0.f;
     double sum = 0.0;
     auto fetch = [&](int blk) {
         const int64_t t0 = (int64_t)blk * TB;
         const int rows = min(TB, q.len - (int)t0);
         tx.load(xp + t0 * ldx, ldx, rows, P);
         tb.load(bp + t0 * ldb, ldb, rows, N);
-        if (wave == 0) raw = lane < rows ? (float)dp[(t0 + lane) * a.lddt] : 0.f;
     };
-    if (first < last) fetch(REV ? last - 1 : first);
+    auto fetch_dt = [&](int blk) {
+        const int64_t t = (int64_t)blk * TB + lane;
+        return t < q.len ? (float)dp[t * a.lddt] : 0.f;
+    };
+    auto block = [&](int j) { return REV ? last - 1 - j : first + j; };
+    if (first < last) {
+        float raw = 0.f;
+        if (wave == 3) raw = fetch_dt(block(0));
+        fetch(block(0));
+        if (wave == 3) make_steps<REV>(L.st[0], a, raw, block(0) * TB + lane < q.len, A, bias, lane);
+    }
     for (int j = 0; j < last - first; ++j) {
-        const int blk = REV ? last - 1 - j : first + j;
+        const int blk = block(j);
         const int rows = min(TB, q.len - blk * TB);
+        const Steps& st = L.st[j & 1];
+        const bool more = j + 1 < last - first;
         tx.store(L.x, LX);
         tb.store(L.b, LN);
-        if (wave == 0) make_steps<REV>(L.st, a, raw, lane < rows, A, bias, lane);
         __syncthreads();
-        if (j + 1 < last - first) fetch(REV ? blk - 1 : blk + 1);
-        if constexpr (!FINAL) {
-            const int64_t at = (((int64_t)(slot + blk) * a.H + h) * a.P + p0) * a.NS;
-#pragma unroll
-            for (int c = 0; c < NP / 16; ++c)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int p = 16 * wave + 4 * g + r, n = 16 * c + i;
-                    if (p < P && n < a.NS) (REV ? a.dS : a.S)[at + (int64_t)p * a.NS + n] = S[c][r];
-                }
-        }
-        const float et = __expf(L.st.total);
-        sum += (double)L.st.total;
+        float raw = 0.f;
+        if (wave == 3 && more) raw = fetch_dt(block(j + 1));
+        if (more) fetch(block(j + 1));
+        if constexpr (!FINAL) store_state<NP, 4>(S, (REV ? a.dS : a.S) + (((int64_t)(slot + blk) * a.H + h) * a.P + pbase) * a.NS, a.NS, p0, P, a.NS, i, g);
+        const float et = __expf(st.total);
+        sum += (double)st.total;
 #pragma unroll
         for (int c = 0; c < NP / 16; ++c) S[c] *= et;
-        state_update<T, NP>(S, L.x, LX, L.b, LN, L.st.w, 16 * wave, i, g);
+        state_update<T, NP>(S, L.x, LX, L.b, LN, st.w, p0, rows, i, g);
+        if (wave == 3 && more) make_steps<REV>(L.st[(j + 1) & 1], a, raw, block(j + 1) * TB + lane < q.len, A, bias, lane);
         __syncthreads();
     }
     if constexpr (FINAL) {
-        store_state<NP>(S, seg_state + seg_at, 16 * wave, P, N, i, g);
-        if (!REV && p0 == 0 && threadIdx.x == 0) a.seg_a[(int64_t)unit * a.H + h] = (float)sum;
+        store_state<NP, V>(S, seg_state + seg_at, N, p0, P, N, i, g);
+        if (!REV && pbase == 0 && threadIdx.x == 0) a.seg_a[(int64_t)unit * a.H + h] = (float)sum;
     } else if (REV) {
-        if (first == 0 && a.dh0) store_state<NP>(S, a.dh0 + state_at, 16 * wave, P, N, i, g);
+        if (first == 0 && a.dh0) store_state<NP, V>(S, a.dh0 + state_at, N, p0, P, N, i, g);
     }
 }
 
@@ -333,7 +357,8 @@ void ssm_segments(SsmArgs& a, int64_t workgroups) {
 
 static bool scan_vec(const SsmArgs& a, int type) {
     const int V = type ? 8 : 4;
-    const uintptr_t p = reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.B) | reinterpret_cast<uintptr_t>(a.C) | reinterpret_cast<uintptr_t>(a.y);
+    const uintptr_t p = reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.B) | reinterpret_cast<uintptr_t>(a.C) | reinterpret_cast<uintptr_t>(a.y) |
+                        reinterpret_cast<uintptr_t>(a.h0) | reinterpret_cast<uintptr_t>(a.hT);
     return a.P % V == 0 && a.N % V == 0 && a.ldx % V == 0 && a.ldb % V == 0 && a.ldc % V == 0 && a.ldy % V == 0 && (p & 15) == 0;
 }
 

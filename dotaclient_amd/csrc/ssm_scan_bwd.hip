@@ -431,7 +431,7 @@ int launch_bwd_n(const SsmArgs& a, hipStream_t s) {
 bool bwd_vec(const SsmArgs& a, int type) {
     const int V = type ? 8 : 4;
     uintptr_t p = 0;
-    for (const void* t : {a.x, a.B, a.C, a.dy, (const void*)a.dx, (const void*)a.dB, (const void*)a.dC}) p |= reinterpret_cast<uintptr_t>(t);
+    for (const void* t : {a.x, a.B, a.C, a.dy, (const void*)a.dx, (const void*)a.dB, (const void*)a.dC, (const void*)a.h0, (const void*)a.dhT, (const void*)a.dh0}) p |= reinterpret_cast<uintptr_t>(t);
     return a.P % V == 0 && a.N % V == 0 && a.ldx % V == 0 && a.ldb % V == 0 && a.ldc % V == 0 && a.lddy % V == 0 && a.lddx % V == 0 && a.lddb % V == 0 &&
            a.lddc % V == 0 && (p & 15) == 0;
 }

@@ -33,13 +33,16 @@ struct SsmArgs {
 };
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
-// Matrix core fragments for D[16][16] += A[16][KS] B[KS][16]; lane l = 16 g + i.  row(): the tile holds the operand's rows (A) or columns (B)
-// with k contiguous; col(): k runs down the tile's rows.  D: element r of lane l is row 4 g + r, column i.
+// Matrix core fragments for D[16][16] += A[16][KS] B[KS][16]; lane l = 16 g + i holds row i of A, column i of B, and of D the rows 4 g + r (r = 0 .. 3)
+// of column i.  Which k an element stands for is free as long as A and B agree: here lane group g holds k = 4 g + e (f32, K = 16) or
+// 4 g + e, 16 + 4 g + e (bf16, K = 32; e = 0 .. 3) - so the accumulators of D tiles are themselves operands whose k is D's row, with no
+// exchange between lanes.  row(): the operand's rows (A) or columns (B) are rows of the tile, k contiguous; col(): k runs down the tile's rows.
 template <typename T> struct Mat;
-template <> struct Mat<float> {           // v_mfma_f32_16x16x4_f32, four of them: k = 4 g + e in the e-th, the same for both operands
+template <> struct Mat<float> {           // v_mfma_f32_16x16x4_f32, four of them: the e-th takes k = 4 g + e
     static constexpr int KS = 16, V = 4;
     typedef f32x4 frag;
     static __device__ __forceinline__ frag row(const float* p, int ld, int i, int g) { return *reinterpret_cast<const f32x4*>(p + i * ld + 4 * g); }
@@ -53,20 +56,35 @@ template <> struct Mat<float> {           // v_mfma_f32_16x16x4_f32, four of the
         return c;
     }
 };
-template <> struct Mat<bf16_t> {          // v_mfma_f32_16x16x32_bf16: k = 8 g + e
+template <> struct Mat<bf16_t> {          // v_mfma_f32_16x16x32_bf16
     static constexpr int KS = 32, V = 8;
     typedef bf16x8 frag;
-    static __device__ __forceinline__ frag row(const bf16_t* p, int ld, int i, int g) { return *reinterpret_cast<const bf16x8*>(p + i * ld + 8 * g); }
-    // ds_read_b64_tr_b16: sixteen lanes hand in the 4 x 16 block's 8-byte pieces (lane i: row i / 4, columns 4 (i % 4) ..) and get a column each
+    static __device__ __forceinline__ frag row(const bf16_t* p, int ld, int i, int g) {
+        const bf16_t* q = p + i * ld + 4 * g;
+        union { bf16x4 h[2]; bf16x8 f; } u;
+        u.h[0] = *reinterpret_cast<const bf16x4*>(q);
+        u.h[1] = *reinterpret_cast<const bf16x4*>(q + 16);
+        return u.f;
+    }
+    // ds_read_b64_tr_b16: sixteen lanes hand in a 4 x 16 block's 8-byte pieces (lane i: row i / 4, columns 4 (i % 4) ..) and get a column each
     static __device__ __forceinline__ frag col(const bf16_t* p, int ld, int i, int g) {
-        const bf16_t* q = p + (8 * g + (i >> 2)) * ld + (i & 3) * 4;
+        const bf16_t* q = p + (4 * g + (i >> 2)) * ld + (i & 3) * 4;
         union { s16x4 h[2]; bf16x8 f; } u;
         u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(void*)q);
-        u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(void*)(q + 4 * ld));
+        u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(void*)(q + 16 * ld));
         return u.f;
     }
     static __device__ __forceinline__ f32x4 mma(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
+
+// Four consecutive elements.
+template <typename T> struct Four { typedef T vec __attribute__((ext_vector_type(4))); };
+template <typename T> __device__ __forceinline__ typename Four<T>::vec four(f32x4 v) {
+    typename Four<T>::vec o;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) o[r] = (T)v[r];
+    return o;
+}
 
 // A 64-row tile of W columns on its way from global memory to LDS: 256 threads, V elements per access.  Rows and columns outside are zero.
 template <typename T, int W, int V>
@@ -150,59 +168,76 @@ __device__ __forceinline__ void split_bf16(float v, bf16_t (&p)[PIECES_F32]) {
     }
 }
 
-// acc[p][n] (16 rows p of this wave, NP columns) += sum_t w_t X[t][p] Y[t][n], from the tiles X [64][PT] and Y [64][NP].
+// The state of a wave: S^T, its 16 head columns p (lane i: p = p0 + i) by NP rows n (tile c, element r: n = 16 c + 4 g + r).  As accumulators of
+//   S^T[n][p] += sum_t Y[t][n] w_t X[t][p]     (tiles X [64][PT], Y [64][NP]; rows t < rows)
+// they are at once the operand of the products over n, and a lane's four neighbouring n leave in one access.
 // The weights are f32: bf16 operands are scaled in f32 and used as three bf16 pieces, because the states they end in are f32 (with two pieces, 16 bits,
 // the gradients of A and dt_bias were off by 4e-6 .. 8e-6 of their norm, with three by what f32 sums are off by).
 template <typename T, int NP>
-__device__ __forceinline__ void state_update(f32x4 (&acc)[NP / 16], const T* X, int ldx, const T* Y, int ldy, const float* w, int p0, int i, int g) {
+__device__ __forceinline__ void state_update(f32x4 (&acc)[NP / 16], const T* X, int ldx, const T* Y, int ldy, const float* w, int p0, int rows, int i, int g) {
     typedef Mat<T> M;
-#pragma unroll
-    for (int k = 0; k < TB; k += M::KS) {
-        typename M::frag a = M::col(X + k * ldx + p0, ldx, i, g);
+    for (int k = 0; k < rows; k += M::KS) {
+        typename M::frag x = M::col(X + k * ldx + p0, ldx, i, g);
         if constexpr (sizeof(T) == 4) {
-            const f32x4 wk = *reinterpret_cast<const f32x4*>(w + k + 4 * g);
-            a *= wk;
+            x *= *reinterpret_cast<const f32x4*>(w + k + 4 * g);
 #pragma unroll
-            for (int c = 0; c < NP / 16; ++c) acc[c] = M::mma(a, M::col(Y + k * ldy + 16 * c, ldy, i, g), acc[c]);
+            for (int c = 0; c < NP / 16; ++c) acc[c] = M::mma(M::col(Y + k * ldy + 16 * c, ldy, i, g), x, acc[c]);
         } else {
+            const f32x4 w0 = *reinterpret_cast<const f32x4*>(w + k + 4 * g), w1 = *reinterpret_cast<const f32x4*>(w + k + 16 + 4 * g);
             typename M::frag piece[PIECES_F32];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 bf16_t v[PIECES_F32];
-                split_bf16((float)a[e] * w[k + 8 * g + e], v);
+                split_bf16((float)x[e] * (e < 4 ? w0[e & 3] : w1[e & 3]), v);
 #pragma unroll
                 for (int pc = 0; pc < PIECES_F32; ++pc) piece[pc][e] = v[pc];
             }
 #pragma unroll
             for (int c = 0; c < NP / 16; ++c) {
-                const typename M::frag b = M::col(Y + k * ldy + 16 * c, ldy, i, g);
+                const typename M::frag y = M::col(Y + k * ldy + 16 * c, ldy, i, g);
 #pragma unroll
-                for (int pc = PIECES_F32 - 1; pc >= 0; --pc) acc[c] = M::mma(piece[pc], b, acc[c]);
+                for (int pc = PIECES_F32 - 1; pc >= 0; --pc) acc[c] = M::mma(y, piece[pc], acc[c]);
             }
         }
     }
 }
 
-// A user's state [P][N] f32 (or null: zeros) in the accumulators of a wave that owns rows p0 .. p0 + 15 of a tile.
-template <int NP>
-__device__ __forceinline__ void load_state(f32x4 (&acc)[NP / 16], const float* __restrict__ h, int p0, int P, int N, int i, int g) {
+// A state [P][ld] f32 (or null: zeros) of N columns in and out of a wave's accumulators; h points at the tile's first p.
+template <int NP, int V>
+__device__ __forceinline__ void load_state(f32x4 (&acc)[NP / 16], const float* __restrict__ h, int ld, int p0, int P, int N, int i, int g) {
+    const int p = p0 + i;
 #pragma unroll
-    for (int c = 0; c < NP / 16; ++c)
+    for (int c = 0; c < NP / 16; ++c) {
+        const int n = 16 * c + 4 * g;
+        acc[c] = f32x4{};
+        if (h && p < P) {
+            const float* q = h + (int64_t)p * ld + n;
+            if (V > 1) {
+                if (n < N) acc[c] = *reinterpret_cast<const f32x4*>(q);
+            } else {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int p = p0 + 4 * g + r, n = 16 * c + i;
-            acc[c][r] = h && p < P && n < N ? h[(int64_t)p * N + n] : 0.f;
+                for (int r = 0; r < 4; ++r)
+                    if (n + r < N) acc[c][r] = q[r];
+            }
         }
+    }
 }
-template <int NP>
-__device__ __forceinline__ void store_state(const f32x4 (&acc)[NP / 16], float* __restrict__ h, int p0, int P, int N, int i, int g) {
+template <int NP, int V>
+__device__ __forceinline__ void store_state(const f32x4 (&acc)[NP / 16], float* __restrict__ h, int ld, int p0, int P, int N, int i, int g) {
+    const int p = p0 + i;
+    if (p >= P) return;
 #pragma unroll
-    for (int c = 0; c < NP / 16; ++c)
+    for (int c = 0; c < NP / 16; ++c) {
+        const int n = 16 * c + 4 * g;
+        float* q = h + (int64_t)p * ld + n;
+        if (V > 1) {
+            if (n < N) *reinterpret_cast<f32x4*>(q) = acc[c];
+        } else {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int p = p0 + 4 * g + r, n = 16 * c + i;
-            if (p < P && n < N) h[(int64_t)p * N + n] = acc[c][r];
+            for (int r = 0; r < 4; ++r)
+                if (n + r < N) q[r] = acc[c][r];
         }
+    }
 }
 
 __host__ __device__ __forceinline__ int blocks_of(int len) { return len / TB + (len % TB != 0); }
