@@ -56,26 +56,25 @@ __global__ void __launch_bounds__(256) ssm_fwd_kernel(SsmArgs a) {
         tb.load(bp + t0 * a.ldb, a.ldb, rows, N);
         tc.load(cp + t0 * a.ldc, a.ldc, rows, N);
     };
-    auto fetch_dt = [&](int blk) {
-        const int64_t t = (int64_t)blk * TB + lane;
-        return t < q.len ? (float)dp[t * a.lddt] : 0.f;
-    };
+    // step sizes: wave 3 makes those of the next block from what it loaded one block before
+    auto fetch_dt = [&](int blk) { return dp[min((int64_t)blk * TB + lane, (int64_t)q.len - 1) * a.lddt]; };
+    T raw = (T)0.f;
     if (first < last) {
-        float raw = 0.f;
         if (wave == 3) raw = fetch_dt(first);
         fetch(first);
-        if (wave == 3) make_steps<false>(L.st[first & 1], a, raw, first * TB + lane < q.len, A, bias, lane);
+        if (wave == 3) {
+            make_steps<false>(L.st[first & 1], a, (float)raw, first * TB + lane < q.len, A, bias, lane);
+            raw = fetch_dt(first + 1);
+        }
     }
     for (int blk = first; blk < last; ++blk) {
         const int64_t t0 = (int64_t)blk * TB;
         const int rows = min(TB, q.len - (int)t0);
         const Steps& st = L.st[blk & 1];
-        tx.store(L.x, LX);
-        tb.store(L.b, LN);
-        tc.store(L.c, LN);
+        tx.store(L.x, LX, rows, P);
+        tb.store(L.b, LN, rows, N);
+        tc.store(L.c, LN, rows, N);
         __syncthreads();
-        float raw = 0.f;
-        if (wave == 3 && blk + 1 < last) raw = fetch_dt(blk + 1);
         if (blk + 1 < last) fetch(blk + 1);
         // M, as (C B^T)^T: lane i owns row t, four neighbouring s of it
 #pragma unroll
@@ -96,7 +95,10 @@ __global__ void __launch_bounds__(256) ssm_fwd_kernel(SsmArgs a) {
             }
             *reinterpret_cast<typename Four<T>::vec*>(L.m + (16 * jt + i) * LM + 16 * js + 4 * g) = four<T>(m);
         }
-        if (wave == 3 && blk + 1 < last) make_steps<false>(L.st[(blk + 1) & 1], a, raw, t0 + TB + lane < q.len, A, bias, lane);
+        if (wave == 3 && blk + 1 < last) {
+            make_steps<false>(L.st[(blk + 1) & 1], a, (float)raw, t0 + TB + lane < q.len, A, bias, lane);
+            raw = fetch_dt(blk + 2);
+        }
         __syncthreads();
         f32x4 y[TB / 16];
 #pragma unroll
@@ -196,27 +198,25 @@ __device__ __forceinline__ void states(const SsmArgs& a, StateLds<T, NP>& L) {
         tx.load(xp + t0 * ldx, ldx, rows, P);
         tb.load(bp + t0 * ldb, ldb, rows, N);
     };
-    auto fetch_dt = [&](int blk) {
-        const int64_t t = (int64_t)blk * TB + lane;
-        return t < q.len ? (float)dp[t * a.lddt] : 0.f;
-    };
+    auto fetch_dt = [&](int blk) { return dp[max((int64_t)0, min((int64_t)blk * TB + lane, (int64_t)q.len - 1)) * a.lddt]; };
     auto block = [&](int j) { return REV ? last - 1 - j : first + j; };
+    T raw = (T)0.f;
     if (first < last) {
-        float raw = 0.f;
         if (wave == 3) raw = fetch_dt(block(0));
         fetch(block(0));
-        if (wave == 3) make_steps<REV>(L.st[0], a, raw, block(0) * TB + lane < q.len, A, bias, lane);
+        if (wave == 3) {
+            make_steps<REV>(L.st[0], a, (float)raw, block(0) * TB + lane < q.len, A, bias, lane);
+            raw = fetch_dt(block(1));
+        }
     }
     for (int j = 0; j < last - first; ++j) {
         const int blk = block(j);
         const int rows = min(TB, q.len - blk * TB);
         const Steps& st = L.st[j & 1];
         const bool more = j + 1 < last - first;
-        tx.store(L.x, LX);
-        tb.store(L.b, LN);
+        tx.store(L.x, LX, rows, P);
+        tb.store(L.b, LN, rows, N);
         __syncthreads();
-        float raw = 0.f;
-        if (wave == 3 && more) raw = fetch_dt(block(j + 1));
         if (more) fetch(block(j + 1));
         if constexpr (!FINAL) store_state<NP, 4>(S, (REV ? a.dS : a.S) + (((int64_t)(slot + blk) * a.H + h) * a.P + pbase) * a.NS, a.NS, p0, P, a.NS, i, g);
         const float et = __expf(st.total);
@@ -224,7 +224,10 @@ __device__ __forceinline__ void states(const SsmArgs& a, StateLds<T, NP>& L) {
 #pragma unroll
         for (int c = 0; c < NP / 16; ++c) S[c] *= et;
         state_update<T, NP>(S, L.x, LX, L.b, LN, st.w, p0, rows, i, g);
-        if (wave == 3 && more) make_steps<REV>(L.st[(j + 1) & 1], a, raw, block(j + 1) * TB + lane < q.len, A, bias, lane);
+        if (wave == 3 && more) {
+            make_steps<REV>(L.st[(j + 1) & 1], a, (float)raw, block(j + 1) * TB + lane < q.len, A, bias, lane);
+            raw = fetch_dt(block(j + 2));
+        }
         __syncthreads();
     }
     if constexpr (FINAL) {

@@ -33,9 +33,9 @@ struct StateTile {
     __device__ __forceinline__ void load(const SsmArgs& a, const float* buf, int64_t slot, int h, int p0, int P) {
         v.load(buf + ((slot * a.H + h) * a.P + p0) * a.NS, a.NS, P, a.NS);
     }
-    __device__ __forceinline__ void store(T (*lds)[PT * pitch<T>(NP)]) const {
+    __device__ __forceinline__ void store(T (*lds)[PT * pitch<T>(NP)], int P, int NS) const {
         if constexpr (sizeof(T) == 4) {
-            v.store(lds[0], pitch<T>(NP));
+            v.store(lds[0], pitch<T>(NP), P, NS);
         } else {
             typedef bf16_t four __attribute__((ext_vector_type(4)));
 #pragma unroll
@@ -45,7 +45,7 @@ struct StateTile {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     bf16_t p[PIECES_F32];
-                    split_bf16(v.v[k][e], p);
+                    split_bf16(idx / v.PER_ROW < P && idx % v.PER_ROW * 4 < NS ? v.v[k][e] : 0.f, p);
 #pragma unroll
                     for (int pc = 0; pc < PIECES_F32; ++pc) out[pc][e] = p[pc];
                 }
@@ -54,12 +54,15 @@ struct StateTile {
             }
         }
     }
-    __device__ __forceinline__ float dot(const StateTile& o) const {
+    __device__ __forceinline__ float dot(const StateTile& o, int P, int NS) const {
         float s = 0.f;
 #pragma unroll
-        for (int k = 0; k < v.N; ++k)
+        for (int k = 0; k < v.N; ++k) {
+            const int idx = k * 256 + threadIdx.x;
+            if (idx / v.PER_ROW < P && idx % v.PER_ROW * 4 < NS)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s = fmaf(v.v[k][e], o.v.v[k][e], s);
+                for (int e = 0; e < 4; ++e) s = fmaf(v.v[k][e], o.v.v[k][e], s);
+        }
         return s;
     }
 };
@@ -82,8 +85,8 @@ __global__ void __launch_bounds__(256) ssm_bwd_kernel(SsmArgs a) {
         Tile<T, NP, V> tb, tc;
         tb.load(static_cast<const T*>(a.B) + row0 * a.ldb + (int64_t)grp * N, a.ldb, rows, N);
         tc.load(static_cast<const T*>(a.C) + row0 * a.ldc + (int64_t)grp * N, a.ldc, rows, N);
-        tb.store(L.b, LN);
-        tc.store(L.c, LN);
+        tb.store(L.b, LN, rows, N);
+        tc.store(L.c, LN, rows, N);
     }
     __syncthreads();
     // this wave's rows: r0 + 4 g + r, of t as of s
@@ -119,10 +122,10 @@ __global__ void __launch_bounds__(256) ssm_bwd_kernel(SsmArgs a) {
             ty.load(static_cast<const T*>(a.dy) + row0 * a.lddy + (int64_t)h * a.P + p0, a.lddy, rows, P);
             ts.load(a, a.S, slot, h, p0, P);
             td.load(a, a.dS, slot, h, p0, P);
-            tx.store(L.x, LX);
-            ty.store(L.y, LX);
-            ts.store(L.s);
-            dot += ts.dot(td);
+            tx.store(L.x, LX, rows, P);
+            ty.store(L.y, LX, rows, P);
+            ts.store(L.s, P, a.NS);
+            dot += ts.dot(td, P, a.NS);
             __syncthreads();
             // the rows with each other
 #pragma unroll
@@ -182,7 +185,7 @@ __global__ void __launch_bounds__(256) ssm_bwd_kernel(SsmArgs a) {
                     }
             }
             __syncthreads();
-            td.store(L.s);
+            td.store(L.s, P, a.NS);
             __syncthreads();
             // dB_s += dt_s e_s dS^T x_s
             float ds[4];

@@ -86,26 +86,27 @@ template <typename T> __device__ __forceinline__ typename Four<T>::vec four(f32x
     return o;
 }
 
-// A 64-row tile of W columns on its way from global memory to LDS: 256 threads, V elements per access.  Rows and columns outside are zero.
-template <typename T, int W, int V>
+// A 64-row tile of W columns on its way from global memory to LDS: 256 threads, V elements per access.  Rows and columns outside become zeros on the
+// way to LDS; their loads go to the last row and the first column instead of being left out, so that no branch stands between the loads of a tile and
+// nothing waits for them before store().  rows, cols >= 1.
+template <typename T, int W, int V, int THREADS = 256>
 struct Tile {
     typedef T vec_t __attribute__((ext_vector_type(V)));
-    static constexpr int PER_ROW = W / V, N = TB * PER_ROW / 256;
+    static constexpr int PER_ROW = W / V, N = TB * PER_ROW / THREADS;
     vec_t v[N];
     __device__ __forceinline__ void load(const T* __restrict__ p, int64_t ld, int rows, int cols) {
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-            const int idx = k * 256 + threadIdx.x, r = idx / PER_ROW, c = idx % PER_ROW * V;
-            vec_t z = {};
-            if (r < rows && c < cols) z = *reinterpret_cast<const vec_t*>(p + r * ld + c);
-            v[k] = z;
+            const int idx = k * THREADS + threadIdx.x, r = idx / PER_ROW, c = idx % PER_ROW * V;
+            v[k] = *reinterpret_cast<const vec_t*>(p + min(r, rows - 1) * ld + (c < cols ? c : 0));
         }
     }
-    __device__ __forceinline__ void store(T* lds, int ld) const {
+    __device__ __forceinline__ void store(T* lds, int ld, int rows, int cols) const {
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-            const int idx = k * 256 + threadIdx.x, r = idx / PER_ROW, c = idx % PER_ROW * V;
-            *reinterpret_cast<vec_t*>(lds + r * ld + c) = v[k];
+            const int idx = k * THREADS + threadIdx.x, r = idx / PER_ROW, c = idx % PER_ROW * V;
+            vec_t z = {};
+            *reinterpret_cast<vec_t*>(lds + r * ld + c) = r < rows && c < cols ? v[k] : z;
         }
     }
 };
@@ -205,22 +206,26 @@ __device__ __forceinline__ void state_update(f32x4 (&acc)[NP / 16], const T* X, 
 // A state [P][ld] f32 (or null: zeros) of N columns in and out of a wave's accumulators; h points at the tile's first p.
 template <int NP, int V>
 __device__ __forceinline__ void load_state(f32x4 (&acc)[NP / 16], const float* __restrict__ h, int ld, int p0, int P, int N, int i, int g) {
+#pragma unroll
+    for (int c = 0; c < NP / 16; ++c) acc[c] = f32x4{};
+    if (!h) return;
     const int p = p0 + i;
+    const float* row = h + (int64_t)min(p, P - 1) * ld;
 #pragma unroll
-    for (int c = 0; c < NP / 16; ++c) {
+    for (int c = 0; c < NP / 16; ++c) {                    // what lies outside is loaded from inside: no branch between the loads
         const int n = 16 * c + 4 * g;
-        acc[c] = f32x4{};
-        if (h && p < P) {
-            const float* q = h + (int64_t)p * ld + n;
-            if (V > 1) {
-                if (n < N) acc[c] = *reinterpret_cast<const f32x4*>(q);
-            } else {
+        if (V > 1) {
+            acc[c] = *reinterpret_cast<const f32x4*>(row + (n < N ? n : 0));
+        } else {
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (n + r < N) acc[c][r] = q[r];
-            }
+            for (int r = 0; r < 4; ++r) acc[c][r] = row[min(n + r, N - 1)];
         }
     }
+#pragma unroll
+    for (int c = 0; c < NP / 16; ++c)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (p >= P || 16 * c + 4 * g + r >= N) acc[c][r] = 0.f;
 }
 template <int NP, int V>
 __device__ __forceinline__ void store_state(const f32x4 (&acc)[NP / 16], float* __restrict__ h, int ld, int p0, int P, int N, int i, int g) {
