@@ -7,137 +7,158 @@
 // Where the sequences, heads and columns give too few workgroups (few, long sequences) the sequences are cut into segments: a first kernel computes what
 // each segment adds to a zero state, a second one runs along the segments, and the scan starts each segment from there.
 #include "ssm_util.h"
+#include <type_traits>
 
 namespace dc {
 namespace {
 
-template <typename T, int NP>
+template <typename T, int NP, int ROWS>
 struct FwdLds {
-    T x[TB * pitch<T>(PT)], b[TB * pitch<T>(NP)], c[TB * pitch<T>(NP)], m[TB * pitch<T>(TB)];
+    T x[ROWS * pitch<T>(PT)], b[ROWS * pitch<T>(NP)], c[ROWS * pitch<T>(NP)], m[ROWS * pitch<T>(ROWS)];
     Steps st[2];
 };
 
-// The twelve 16 x 16 tiles (row tile, column tile) of M that products with it read: ten with s <= t, and two zero ones that complete
-// the 32-column steps of row tiles 0 and 2.  Wave w takes w, w + 4, w + 8.
-__device__ __forceinline__ int tile_row(int u) { return (0x203323213210ull >> (4 * u)) & 15; }
-__device__ __forceinline__ int tile_col(int u) { return (0x310102103210ull >> (4 * u)) & 15; }
-
-template <typename T, int NP, int V>
-__global__ void __launch_bounds__(256) ssm_fwd_kernel(SsmArgs a) {
+// ROWS: rows of a block.
+template <typename T, int NP, int V, int ROWS>
+__global__ void __launch_bounds__(256, V > 1 && NP <= 64 ? (ROWS == 32 ? 4 : sizeof(T) == 2 ? 3 : 2) : 1) ssm_fwd_kernel(SsmArgs a) {
     typedef Mat<T> M;
-    constexpr int LX = pitch<T>(PT), LN = pitch<T>(NP), LM = pitch<T>(TB), NK = NP / M::KS;
+    typedef typename Four<T>::vec four_t;
+    constexpr int LX = pitch<T>(PT), LN = pitch<T>(NP), LM = pitch<T>(ROWS), NK = NP / M::KS, NT = ROWS / 16;
     extern __shared__ __attribute__((aligned(16))) char lds_raw[];
-    FwdLds<T, NP>& L = *reinterpret_cast<FwdLds<T, NP>*>(lds_raw);
+    FwdLds<T, NP, ROWS>& L = *reinterpret_cast<FwdLds<T, NP, ROWS>*>(lds_raw);
     int unit, h, pbase;
     if (!work_item(a, unit, h, pbase)) return;
     const int b = unit / a.nseg, seg = unit % a.nseg, grp = h / (a.H / a.G);
-    const SeqRange q = seq_range(a.seq_off, a.seq_len, b, a.rows, a.max_len);
-    const int nb = blocks_of(q.len), first = seg * a.seg_blocks;
+    const SeqRange q = uniform_range(a, b);
+    const int nb = q.len / ROWS + (q.len % ROWS != 0), first = seg * a.seg_blocks;
     if (first >= nb && seg > 0) return;
     const int last = min(nb, first + a.seg_blocks);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4, p0 = 16 * wave;
+    const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), i = lane & 15, g = lane >> 4, p0 = 16 * wave;
     const int P = min(a.P - pbase, PT), N = a.N;
     const int64_t state_at = ((int64_t)b * a.H + h) * a.P * N + (int64_t)pbase * N;
     f32x4 S[NP / 16];
     const float* init = a.nseg > 1 ? a.seg_state + ((int64_t)unit * a.H + h) * a.P * N + (int64_t)pbase * N : a.h0 ? a.h0 + state_at : nullptr;
-    load_state<NP, V>(S, init, N, p0, P, N, i, g);
     const float A = a.A[h], bias = a.dt_bias ? a.dt_bias[h] : 0.f, D = a.D ? a.D[h] : 0.f;
     const T* xp = static_cast<const T*>(a.x) + q.off * a.ldx + (int64_t)h * a.P + pbase;
     const T* bp = static_cast<const T*>(a.B) + q.off * a.ldb + (int64_t)grp * N;
     const T* cp = static_cast<const T*>(a.C) + q.off * a.ldc + (int64_t)grp * N;
     const T* dp = static_cast<const T*>(a.dt) + q.off * a.lddt + h;
     T* yp = static_cast<T*>(a.y) + q.off * a.ldy + (int64_t)h * a.P + pbase;
-    Tile<T, PT, V> tx;
-    Tile<T, NP, V> tb, tc;
+    const uint32_t yoff = (uint32_t)i * (uint32_t)a.ldy + p0 + 4 * g;
+    const bool all_p = P == PT, all_n = N == NP;
+    Tile<T, PT, V, ROWS> tx(a.ldx, P);
+    Tile<T, NP, V, ROWS> tb(a.ldb, N), tc(a.ldc, N);
     auto fetch = [&](int blk) {
-        const int64_t t0 = (int64_t)blk * TB;
-        const int rows = min(TB, q.len - (int)t0);
-        tx.load(xp + t0 * a.ldx, a.ldx, rows, P);
-        tb.load(bp + t0 * a.ldb, a.ldb, rows, N);
-        tc.load(cp + t0 * a.ldc, a.ldc, rows, N);
+        const int64_t t0 = (int64_t)blk * ROWS;
+        const int rows = min(ROWS, q.len - (int)t0);
+        if (rows == ROWS) {
+            tx.template load<true>(xp + t0 * a.ldx, a.ldx, ROWS);
+            tb.template load<true>(bp + t0 * a.ldb, a.ldb, ROWS);
+            tc.template load<true>(cp + t0 * a.ldc, a.ldc, ROWS);
+        } else {
+            tx.template load<false>(xp + t0 * a.ldx, a.ldx, rows);
+            tb.template load<false>(bp + t0 * a.ldb, a.ldb, rows);
+            tc.template load<false>(cp + t0 * a.ldc, a.ldc, rows);
+        }
     };
     // step sizes: wave 3 makes those of the next block from what it loaded one block before
-    auto fetch_dt = [&](int blk) { return dp[min((int64_t)blk * TB + lane, (int64_t)q.len - 1) * a.lddt]; };
+    auto fetch_dt = [&](int blk) { return dp[min((int64_t)blk * ROWS + lane, (int64_t)q.len - 1) * a.lddt]; };
+    auto steps = [&](int blk, T raw) {
+        make_steps<false, true>(L.st[blk & 1], a, (float)raw, lane < ROWS && (int64_t)blk * ROWS + lane < q.len, A, bias, lane);
+    };
     T raw = (T)0.f;
     if (first < last) {
         if (wave == 3) raw = fetch_dt(first);
         fetch(first);
-        if (wave == 3) {
-            make_steps<false>(L.st[first & 1], a, (float)raw, first * TB + lane < q.len, A, bias, lane);
-            raw = fetch_dt(first + 1);
-        }
     }
-    for (int blk = first; blk < last; ++blk) {
-        const int64_t t0 = (int64_t)blk * TB;
-        const int rows = min(TB, q.len - (int)t0);
+    load_state<NP, V>(S, init, N, p0, P, N, i, g);
+    if (first < last && wave == 3) {
+        steps(first, raw);
+        raw = fetch_dt(first + 1);
+    }
+    auto block = [&](int blk, auto full_t) {
+        constexpr bool FULL = decltype(full_t)::value;
+        const int64_t t0 = (int64_t)blk * ROWS;
+        const int rows = FULL ? ROWS : q.len - (int)t0;
         const Steps& st = L.st[blk & 1];
-        tx.store(L.x, LX, rows, P);
-        tb.store(L.b, LN, rows, N);
-        tc.store(L.c, LN, rows, N);
+        tx.template store<FULL>(L.x, LX, rows, all_p);
+        tb.template store<FULL>(L.b, LN, rows, all_n);
+        tc.template store<FULL>(L.c, LN, rows, all_n);
         __syncthreads();
         if (blk + 1 < last) fetch(blk + 1);
         // M, as (C B^T)^T: lane i owns row t, four neighbouring s of it
 #pragma unroll
-        for (int u = 0; u < 3; ++u) {
-            const int jt = tile_row(wave + 4 * u), js = tile_col(wave + 4 * u);
-            if (16 * jt >= rows) continue;
+        for (int u = 0; u < (ROWS == 64 ? 3 : 1); ++u) {
+            // 64 rows: three tiles of the list a wave; 32 rows: 00, 11, 10 and the zero 01
+            const int jt = ROWS == 64 ? tile_row(wave + 4 * u) : (0x0110 >> (4 * wave)) & 15, js = ROWS == 64 ? tile_col(wave + 4 * u) : (0x1010 >> (4 * wave)) & 15;
+            if (!FULL && 16 * jt >= rows) continue;
             f32x4 m = {};
             if (js <= jt) {
 #pragma unroll
                 for (int k = 0; k < NK; ++k)
                     m = M::mma(M::row(L.b + 16 * js * LN + k * M::KS, LN, i, g), M::row(L.c + 16 * jt * LN + k * M::KS, LN, i, g), m);
                 const int t = 16 * jt + i, s = 16 * js + 4 * g;
-                const float ht = st.hi[t], lt = st.lo[t];
-                const f32x4 hs = *reinterpret_cast<const f32x4*>(st.hi + s), ls = *reinterpret_cast<const f32x4*>(st.lo + s),
-                            ds = *reinterpret_cast<const f32x4*>(st.dt + s);
+                if (js < jt) {
+                    const float f = st.rf[t] * between(st, jt, js);
+                    const f32x4 cd = *reinterpret_cast<const f32x4*>(st.cd + s);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) m[r] = s + r <= t ? m[r] * (__expf((ht - hs[r]) + (lt - ls[r])) * ds[r]) : 0.f;
+                    for (int r = 0; r < 4; ++r) m[r] *= f * cd[r];
+                } else {
+                    const float ht = st.hi[t], lt = st.lo[t];
+                    const f32x4 hs = *reinterpret_cast<const f32x4*>(st.hi + s), ls = *reinterpret_cast<const f32x4*>(st.lo + s),
+                                ds = *reinterpret_cast<const f32x4*>(st.dt + s);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) m[r] = s + r <= t ? m[r] * (__expf((ht - hs[r]) + (lt - ls[r])) * ds[r]) : 0.f;
+                }
             }
-            *reinterpret_cast<typename Four<T>::vec*>(L.m + (16 * jt + i) * LM + 16 * js + 4 * g) = four<T>(m);
+            *reinterpret_cast<four_t*>(L.m + (16 * jt + i) * LM + 16 * js + 4 * g) = four<T>(m);
         }
         if (wave == 3 && blk + 1 < last) {
-            make_steps<false>(L.st[(blk + 1) & 1], a, (float)raw, t0 + TB + lane < q.len, A, bias, lane);
+            steps(blk + 1, raw);
             raw = fetch_dt(blk + 2);
         }
         __syncthreads();
-        f32x4 y[TB / 16];
-#pragma unroll
-        for (int jt = 0; jt < TB / 16; ++jt) {
-            y[jt] = f32x4{};
-            if (16 * jt >= rows) continue;
-            // S is rounded once to bf16 there, like M: both only end in y
+        f32x4 y[NT];
+        {
+            // S is rounded once to bf16 here, like M: both only end in y
+            typename M::frag sf[NK];
 #pragma unroll
             for (int k = 0; k < NK; ++k) {
-                typename M::frag sf;
                 if constexpr (sizeof(T) == 4) {
-                    sf = S[k];
+                    sf[k] = S[k];
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) sf[e] = (T)S[2 * k + (e >> 2)][e & 3];
+                    for (int e = 0; e < 8; ++e) sf[k][e] = (T)S[2 * k + (e >> 2)][e & 3];
                 }
-                y[jt] = M::mma(sf, M::row(L.c + 16 * jt * LN + k * M::KS, LN, i, g), y[jt]);
             }
-            y[jt] *= __expf(st.hi[16 * jt + i]);
+#pragma unroll
+            for (int jt = 0; jt < NT; ++jt) {
+                y[jt] = f32x4{};
+                if (!FULL && 16 * jt >= rows) continue;
+#pragma unroll
+                for (int k = 0; k < NK; ++k) y[jt] = M::mma(sf[k], M::row(L.c + 16 * jt * LN + k * M::KS, LN, i, g), y[jt]);
+                y[jt] *= st.ea[16 * jt + i];
+            }
         }
 #pragma unroll
-        for (int k = 0; k < TB; k += M::KS) {
-            if (k >= rows) continue;
+        for (int k = 0; k < ROWS; k += M::KS) {
+            if (!FULL && k >= rows) continue;
             const typename M::frag xf = M::col(L.x + k * LX + p0, LX, i, g);
 #pragma unroll
-            for (int jt = k / 16; jt < TB / 16; ++jt)
-                if (16 * jt < rows) y[jt] = M::mma(xf, M::row(L.m + 16 * jt * LM + k, LM, i, g), y[jt]);
+            for (int jt = k / 16; jt < NT; ++jt)
+                if (FULL || 16 * jt < rows) y[jt] = M::mma(xf, M::row(L.m + 16 * jt * LM + k, LM, i, g), y[jt]);
         }
 #pragma unroll
-        for (int jt = 0; jt < TB / 16; ++jt) {
+        for (int jt = 0; jt < NT; ++jt) {
             const int t = 16 * jt + i, p = p0 + 4 * g;
-            if (t >= rows || p >= P) continue;
-            const typename Four<T>::vec xv = *reinterpret_cast<const typename Four<T>::vec*>(L.x + t * LX + p);
+            if ((!FULL && t >= rows) || (!all_p && p >= P)) continue;
+            const four_t xv = *reinterpret_cast<const four_t*>(L.x + t * LX + p);
 #pragma unroll
             for (int r = 0; r < 4; ++r) y[jt][r] = fmaf(D, (float)xv[r], y[jt][r]);
-            T* out = yp + (t0 + t) * a.ldy + p;
-            const typename Four<T>::vec o = four<T>(y[jt]);
+            T* out = yp + (t0 + 16 * jt) * a.ldy + yoff;
+            const four_t o = four<T>(y[jt]);
             if (V > 1) {
-                *reinterpret_cast<typename Four<T>::vec*>(out) = o;
+                *reinterpret_cast<four_t*>(out) = o;
             } else {
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
@@ -147,9 +168,12 @@ __global__ void __launch_bounds__(256) ssm_fwd_kernel(SsmArgs a) {
         const float et = __expf(st.total);
 #pragma unroll
         for (int c = 0; c < NP / 16; ++c) S[c] *= et;
-        state_update<T, NP>(S, L.x, LX, L.b, LN, st.w, p0, rows, i, g);
+        state_update<T, NP, ROWS>(S, L.x, LX, L.b, LN, st.w, p0, rows, i, g);
         __syncthreads();
-    }
+    };
+    const int whole = min(last, q.len / ROWS);
+    for (int blk = first; blk < whole; ++blk) block(blk, std::true_type{});
+    if (whole < last && whole >= first) block(whole, std::false_type{});
     if (last == nb && a.hT) store_state<NP, V>(S, a.hT + state_at, N, p0, P, N, i, g);
 }
 
@@ -168,14 +192,14 @@ __device__ __forceinline__ void states(const SsmArgs& a, StateLds<T, NP>& L) {
     int unit, h, pbase;
     if (!work_item(a, unit, h, pbase)) return;
     const int b = unit / a.nseg, seg = unit % a.nseg, grp = h / (a.H / a.G);
-    const SeqRange q = seq_range(a.seq_off, a.seq_len, b, a.rows, a.max_len);
+    const SeqRange q = uniform_range(a, b);
     int nb = blocks_of(q.len), slot = 0;
     if constexpr (!FINAL) {
-        slot = a.base[b];
-        nb = min(nb, a.base[b + 1] - slot);
+        slot = uniform(a.base[b]);
+        nb = min(nb, uniform(a.base[b + 1]) - slot);
     }
     const int first = seg * a.seg_blocks, last = min(nb, first + a.seg_blocks);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4, p0 = 16 * wave;
+    const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), i = lane & 15, g = lane >> 4, p0 = 16 * wave;
     const int P = min(a.P - pbase, PT), N = a.N;
     const int64_t seg_at = ((int64_t)unit * a.H + h) * a.P * N + (int64_t)pbase * N, state_at = ((int64_t)b * a.H + h) * a.P * N + (int64_t)pbase * N;
     float* const seg_state = REV ? a.seg_dstate : a.seg_state;
@@ -189,14 +213,20 @@ __device__ __forceinline__ void states(const SsmArgs& a, StateLds<T, NP>& L) {
     xp += q.off * ldx + (int64_t)h * a.P + pbase;
     bp += q.off * ldb + (int64_t)grp * N;
     const T* dp = static_cast<const T*>(a.dt) + q.off * a.lddt + h;
-    Tile<T, PT, V> tx;
-    Tile<T, NP, V> tb;
+    const bool all_p = P == PT, all_n = N == NP;
+    Tile<T, PT, V> tx(ldx, P);
+    Tile<T, NP, V> tb(ldb, N);
     double sum = 0.0;
     auto fetch = [&](int blk) {
         const int64_t t0 = (int64_t)blk * TB;
         const int rows = min(TB, q.len - (int)t0);
-        tx.load(xp + t0 * ldx, ldx, rows, P);
-        tb.load(bp + t0 * ldb, ldb, rows, N);
+        if (rows == TB) {
+            tx.template load<true>(xp + t0 * ldx, ldx, TB);
+            tb.template load<true>(bp + t0 * ldb, ldb, TB);
+        } else {
+            tx.template load<false>(xp + t0 * ldx, ldx, rows);
+            tb.template load<false>(bp + t0 * ldb, ldb, rows);
+        }
     };
     auto fetch_dt = [&](int blk) { return dp[max((int64_t)0, min((int64_t)blk * TB + lane, (int64_t)q.len - 1)) * a.lddt]; };
     auto block = [&](int j) { return REV ? last - 1 - j : first + j; };
@@ -205,7 +235,7 @@ __device__ __forceinline__ void states(const SsmArgs& a, StateLds<T, NP>& L) {
         if (wave == 3) raw = fetch_dt(block(0));
         fetch(block(0));
         if (wave == 3) {
-            make_steps<REV>(L.st[0], a, (float)raw, block(0) * TB + lane < q.len, A, bias, lane);
+            make_steps<REV, false>(L.st[0], a, (float)raw, block(0) * TB + lane < q.len, A, bias, lane);
             raw = fetch_dt(block(1));
         }
     }
@@ -214,8 +244,13 @@ __device__ __forceinline__ void states(const SsmArgs& a, StateLds<T, NP>& L) {
         const int rows = min(TB, q.len - blk * TB);
         const Steps& st = L.st[j & 1];
         const bool more = j + 1 < last - first;
-        tx.store(L.x, LX, rows, P);
-        tb.store(L.b, LN, rows, N);
+        if (rows == TB) {
+            tx.template store<true>(L.x, LX, TB, all_p);
+            tb.template store<true>(L.b, LN, TB, all_n);
+        } else {
+            tx.template store<false>(L.x, LX, rows, all_p);
+            tb.template store<false>(L.b, LN, rows, all_n);
+        }
         __syncthreads();
         if (more) fetch(block(j + 1));
         if constexpr (!FINAL) store_state<NP, 4>(S, (REV ? a.dS : a.S) + (((int64_t)(slot + blk) * a.H + h) * a.P + pbase) * a.NS, a.NS, p0, P, a.NS, i, g);
@@ -223,9 +258,9 @@ __device__ __forceinline__ void states(const SsmArgs& a, StateLds<T, NP>& L) {
         sum += (double)st.total;
 #pragma unroll
         for (int c = 0; c < NP / 16; ++c) S[c] *= et;
-        state_update<T, NP>(S, L.x, LX, L.b, LN, st.w, p0, rows, i, g);
+        state_update<T, NP, TB>(S, L.x, LX, L.b, LN, st.w, p0, rows, i, g);
         if (wave == 3 && more) {
-            make_steps<REV>(L.st[(j + 1) & 1], a, (float)raw, block(j + 1) * TB + lane < q.len, A, bias, lane);
+            make_steps<REV, false>(L.st[(j + 1) & 1], a, (float)raw, block(j + 1) * TB + lane < q.len, A, bias, lane);
             raw = fetch_dt(block(j + 2));
         }
         __syncthreads();
@@ -296,16 +331,21 @@ __global__ void __launch_bounds__(256) ssm_step_kernel(SsmArgs a) {
     if (i == 0) static_cast<T*>(a.y)[b * a.ldy + (int64_t)h * a.P + p] = (T)(y + (a.D ? a.D[h] : 0.f) * x);
 }
 
-template <typename T, int NP, int V>
-int launch_fwd(const SsmArgs& a, hipStream_t s) {
-    constexpr size_t bytes = sizeof(FwdLds<T, NP>);
+template <typename T, int NP, int V, int ROWS>
+int launch_fwd_rows(const SsmArgs& a, hipStream_t s) {
+    constexpr size_t bytes = sizeof(FwdLds<T, NP, ROWS>);
     static_assert(bytes <= 160 * 1024, "LDS of a workgroup");
     if (bytes > 64 * 1024) {
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(ssm_fwd_kernel<T, NP, V>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(ssm_fwd_kernel<T, NP, V, ROWS>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
         if (e != hipSuccess) { set_error("dc_ssm_scan_fwd: LDS", (int)e); return (int)e; }
     }
-    hipLaunchKernelGGL((ssm_fwd_kernel<T, NP, V>), dim3((unsigned)work_items(a)), dim3(256), bytes, s, a);
+    hipLaunchKernelGGL((ssm_fwd_kernel<T, NP, V, ROWS>), dim3((unsigned)work_items(a)), dim3(256), bytes, s, a);
     return launch_check("dc_ssm_scan_fwd");
+}
+// Sequences that fit 32 rows (chunks of 16 steps) in blocks of 32: half the LDS and registers, so twice the workgroups on a CU.
+template <typename T, int NP, int V>
+int launch_fwd(const SsmArgs& a, hipStream_t s) {
+    return a.max_len <= 32 ? launch_fwd_rows<T, NP, V, 32>(a, s) : launch_fwd_rows<T, NP, V, 64>(a, s);
 }
 template <typename T, int V>
 int launch_fwd_n(const SsmArgs& a, hipStream_t s) {
@@ -342,6 +382,8 @@ int ssm_check(const char* what, const SsmArgs& a, int type) {
     if (type != 0 && type != 1) { set_error(what, 1101); return 1101; }
     if (a.H < 1 || a.G < 1 || a.H % a.G || a.H > 4096 || a.P < 1 || a.P > 256 || a.N < 1 || a.N > 128) { set_error(what, 1102); return 1102; }
     if (a.rows < 0 || a.n_seq < 0 || a.max_len < 0 || (int64_t)a.n_seq * a.H * ((a.P + 15) / 16) > 0x3fffffff) { set_error(what, 1103); return 1103; }
+    for (int64_t ld : {a.ldx, a.lddt, a.ldb, a.ldc, a.ldy, a.lddy, a.lddx, a.lddb, a.lddc})
+        if (ld < 0 || ld > 1 << 22) { set_error(what, 1103); return 1103; }
     if (!a.A || (a.rows && (!a.x || !a.dt || !a.B || !a.C))) { set_error(what, 1104); return 1104; }
     return 0;
 }

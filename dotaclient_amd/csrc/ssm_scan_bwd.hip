@@ -9,333 +9,407 @@
 //   d(dt')_t = A d(a step)_t + K_t,   dA = sum_t dt_t d(a step)_t,   dD = sum_t G2[t,t]
 // (the diagonal cancels in R - dt K and is left out of both, so that strong decays do not lose the gradient of A in it).
 //
-// A workgroup owns one block and the heads of one group (or a share of them, where blocks and groups alone are too few): G1 stays in its registers,
-// the T x T sums W and the gradients of B and C are added up over the heads there, so dB and dC cost two products per block instead of two per
-// head, and no partial sums in memory.  Operands that are f32 by nature are used as three bf16 pieces where an f32 result depends on them (S and dS:
-// R, K -> dA, ddt_bias); W and G1 L, which only end in bf16 outputs, are rounded once, and dS in dx takes its first piece.
+// A workgroup of eight waves owns one block and the heads of one group (or a share of them, where blocks and groups alone are too few): G1 stays in its
+// registers, W and the gradients of B and C are added up over the heads there, so dB and dC cost two products per block instead of two per head, and
+// no partial sums in memory.  Per head two phases with a barrier between them:
+//   1. the ten 16 x 16 tiles of G2 with s <= t, shared out over the waves: W, Q's row and column sums, G1 L to LDS; S^T dy and dS^T x for the columns n
+//      that a wave owns, whose part of S and dS it alone reads - straight from memory into operands;
+//   2. dx for the columns p that a wave owns; one wave runs along the rows for d(a step), ddt and the sums for dA, dD, ddt_bias.
+// The next head's x, dy, S, dS are loaded as soon as this one's are used.  Operands that are f32 by nature are used as three bf16 pieces where an f32
+// result depends on them (S and dS: R, K -> dA, ddt_bias); W and G1 L, which only end in bf16 outputs, are rounded once, and dS in dx takes its
+// first piece.
 #include "ssm_util.h"
 
 namespace dc {
 namespace {
 
+constexpr int WAVES = 8, THREADS = 64 * WAVES;
+
 template <typename T, int NP>
 struct BwdLds {
-    static constexpr int PIECES = sizeof(T) == 4 ? 1 : PIECES_F32;
-    T b[TB * pitch<T>(NP)], c[TB * pitch<T>(NP)], x[TB * pitch<T>(PT)], y[TB * pitch<T>(PT)], s[PIECES][PT * pitch<T>(NP)], m[TB * pitch<T>(TB)];
-    Steps st;
-    float R[TB], diag[TB], KI[TB], col[16][TB], dot[4], trace[4];
+    // how the waves share out the 16-column tiles of N and the four row tiles: WN x WT waves, JT row tiles each
+    static constexpr int WN = NP / 16, WT = WAVES / WN, JT = 4 / WT;
+    T b[TB * pitch<T>(NP)], c[TB * pitch<T>(NP)], x[TB * pitch<T>(PT)], y[TB * pitch<T>(PT)], m[TB * pitch<T>(TB)];
+    Steps st[2];
+    float R[4][TB], K[16][TB], RI[4 * WN][TB], KI[4 * WN][TB], diag[TB], dot[4 * WAVES], trace[4 * WAVES];
 };
 
-// A head's S or dS tile on its way to LDS, as f32 or as three bf16 pieces (the slots' rows are padded to whole vectors).
-template <typename T, int NP>
-struct StateTile {
-    Tile<float, NP, 4> v;
-    __device__ __forceinline__ void load(const SsmArgs& a, const float* buf, int64_t slot, int h, int p0, int P) {
-        v.load(buf + ((slot * a.H + h) * a.P + p0) * a.NS, a.NS, P, a.NS);
+// 64 x 16 of S or dS as an operand whose rows are its columns n and whose k is p: element 4 kk + e of lane (i, g) is [16 kk + 4 g + e][n0 + i].
+struct StateCols {
+    float v[PT / 4];
+    __device__ __forceinline__ void load(const float* __restrict__ p, int NS, int P, int n0, int i, int g) {
+        const int n = min(n0 + i, NS - 1);
+#pragma unroll
+        for (int kk = 0; kk < PT / 16; ++kk)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[4 * kk + e] = p[(uint32_t)(min(16 * kk + 4 * g + e, P - 1) * NS + n)];
     }
-    __device__ __forceinline__ void store(T (*lds)[PT * pitch<T>(NP)], int P, int NS) const {
-        if constexpr (sizeof(T) == 4) {
-            v.store(lds[0], pitch<T>(NP), P, NS);
-        } else {
-            typedef bf16_t four __attribute__((ext_vector_type(4)));
+};
+template <typename T> struct Pieces;
+template <> struct Pieces<float> {
+    static constexpr int N = 1;
+    f32x4 f[1][PT / 16];
+    __device__ __forceinline__ Pieces(const float* v) {
 #pragma unroll
-            for (int k = 0; k < v.N; ++k) {
-                const int idx = k * 256 + threadIdx.x, at = idx / v.PER_ROW * pitch<T>(NP) + idx % v.PER_ROW * 4;
-                four out[PIECES_F32];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    bf16_t p[PIECES_F32];
-                    split_bf16(idx / v.PER_ROW < P && idx % v.PER_ROW * 4 < NS ? v.v[k][e] : 0.f, p);
-#pragma unroll
-                    for (int pc = 0; pc < PIECES_F32; ++pc) out[pc][e] = p[pc];
-                }
-#pragma unroll
-                for (int pc = 0; pc < PIECES_F32; ++pc) *reinterpret_cast<four*>(lds[pc] + at) = out[pc];
-            }
-        }
+        for (int k = 0; k < PT; ++k) if (k < PT / 4) f[0][k / 4][k % 4] = v[k];
     }
-    __device__ __forceinline__ float dot(const StateTile& o, int P, int NS) const {
-        float s = 0.f;
+};
+template <> struct Pieces<bf16_t> {
+    static constexpr int N = PIECES_F32;
+    bf16x8 f[PIECES_F32][PT / 32];
+    __device__ __forceinline__ Pieces(const float* v) {
 #pragma unroll
-        for (int k = 0; k < v.N; ++k) {
-            const int idx = k * 256 + threadIdx.x;
-            if (idx / v.PER_ROW < P && idx % v.PER_ROW * 4 < NS)
+        for (int k = 0; k < PT / 4; ++k) {
+            bf16_t p[PIECES_F32];
+            split_bf16(v[k], p);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s = fmaf(v.v[k][e], o.v.v[k][e], s);
+            for (int pc = 0; pc < PIECES_F32; ++pc) f[pc][k / 8][k % 8] = p[pc];
         }
-        return s;
     }
 };
 
 template <typename T, int NP, int V>
-__global__ void __launch_bounds__(256) ssm_bwd_kernel(SsmArgs a) {
+__global__ void __launch_bounds__(THREADS) ssm_bwd_kernel(SsmArgs a) {
     typedef Mat<T> M;
-    constexpr int LX = pitch<T>(PT), LN = pitch<T>(NP), LM = pitch<T>(TB), NK = NP / M::KS, NC = NP / 16;
-    constexpr int PIECES = BwdLds<T, NP>::PIECES;
+    typedef typename Four<T>::vec four_t;
+    typedef BwdLds<T, NP> Lds;
+    constexpr int LX = pitch<T>(PT), LN = pitch<T>(NP), LM = pitch<T>(TB), NK = NP / M::KS, PK = PT / M::KS, WN = Lds::WN, WT = Lds::WT, JT = Lds::JT;
+    constexpr int GT = (12 + WAVES - 1) / WAVES;
     extern __shared__ __attribute__((aligned(16))) char lds_raw[];
-    BwdLds<T, NP>& L = *reinterpret_cast<BwdLds<T, NP>*>(lds_raw);
+    Lds& L = *reinterpret_cast<Lds*>(lds_raw);
     const int slot = blockIdx.x, grp = blockIdx.y, share = blockIdx.z, Hg = a.H / a.G;
-    if (slot >= a.base[a.n_seq]) return;
-    const int b = a.map[slot], blk = slot - a.base[b];
-    const SeqRange q = seq_range(a.seq_off, a.seq_len, b, a.rows, a.max_len);
+    if (slot >= uniform(a.base[a.n_seq])) return;
+    const int b = uniform(a.map[slot]), blk = slot - uniform(a.base[b]);
+    const SeqRange q = uniform_range(a, b);
     const int64_t row0 = q.off + (int64_t)blk * TB;
     const int rows = min(TB, q.len - blk * TB);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, i = lane & 15, g = lane >> 4, N = a.N;
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), i = lane & 15, g = lane >> 4, N = a.N;
+    const int n0 = 16 * (wave % WN), jt0 = wave / WN;                     // this wave's columns n; its row tiles jt0 + WT j
+    const int pw = 16 * (wave & 3), js0 = wave >> 2;                      // its columns p and row tiles js0 + 2 j of dx
+    const int h_first = grp * Hg + share * Hg / a.hsplit, h_last = grp * Hg + (share + 1) * Hg / a.hsplit;
+    const int ldx = (int)a.ldx, lddy = (int)a.lddy, lddx = (int)a.lddx, NS = a.NS;
+    const T* const xp = static_cast<const T*>(a.x) + row0 * ldx;
+    const T* const yp = static_cast<const T*>(a.dy) + row0 * lddy;
+    const T* const dtp = static_cast<const T*>(a.dt) + row0 * a.lddt;
+    const uint32_t dt_off = (uint32_t)min(lane, rows - 1) * (uint32_t)a.lddt;
+    T* const dxp = static_cast<T*>(a.dx) + row0 * lddx;
+    const float* const Sp = a.S + (int64_t)slot * a.H * a.P * NS;
+    const float* const dSp = a.dS + (int64_t)slot * a.H * a.P * NS;
+
+    BlockTile<T, PT, V, THREADS> tx(ldx, rows), ty(lddy, rows);
+    StateCols S, dS;
+    f32x4 dSr[NP / 16];                                                   // rows p of dS, k = n
+    auto fetch_xy = [&](int h, int pt) {
+        const int col = h * a.P + pt * PT, P = min(a.P - pt * PT, PT);
+        tx.load(xp + col, P);
+        ty.load(yp + col, P);
+    };
+    auto fetch_cols = [&](int h, int pt) {
+        const int64_t at = (int64_t)(h * a.P + pt * PT) * NS;
+        const int P = min(a.P - pt * PT, PT);
+        S.load(Sp + at, NS, P, n0, i, g);
+        dS.load(dSp + at, NS, P, n0, i, g);
+    };
+    auto fetch_rows = [&](int h, int pt) {
+        const int64_t at = (int64_t)(h * a.P + pt * PT) * NS;
+        const int P = min(a.P - pt * PT, PT);
+        const uint32_t row = min(pw + i, P - 1) * NS;
+#pragma unroll
+        for (int k = 0; k < NP / 16; ++k) dSr[k] = *reinterpret_cast<const f32x4*>(dSp + at + (row + (16 * k + 4 * g < NS ? 16 * k + 4 * g : 0)));
+    };
+    auto steps = [&](int h, T raw) {
+        make_steps<false, true>(L.st[h & 1], a, (float)raw, lane < rows, a.A[h], a.dt_bias ? a.dt_bias[h] : 0.f, lane);
+    };
+    T raw = dtp[dt_off + h_first];
     {
-        Tile<T, NP, V> tb, tc;
-        tb.load(static_cast<const T*>(a.B) + row0 * a.ldb + (int64_t)grp * N, a.ldb, rows, N);
-        tc.load(static_cast<const T*>(a.C) + row0 * a.ldc + (int64_t)grp * N, a.ldc, rows, N);
+        BlockTile<T, NP, V, THREADS> tb((int)a.ldb, rows), tc((int)a.ldc, rows);
+        tb.load(static_cast<const T*>(a.B) + row0 * a.ldb + (int64_t)grp * N, N);
+        tc.load(static_cast<const T*>(a.C) + row0 * a.ldc + (int64_t)grp * N, N);
+        fetch_xy(h_first, 0);
+        fetch_cols(h_first, 0);
+        fetch_rows(h_first, 0);
+        if (wave == WAVES - 1) {
+            steps(h_first, raw);
+            raw = dtp[dt_off + min(h_first + 1, h_last - 1)];
+        }
+        // sums that no tile writes
+        for (int k = tid; k < 4 * TB; k += THREADS) (&L.R[0][0])[k] = 0.f;
+        for (int k = tid; k < 16 * TB; k += THREADS) (&L.K[0][0])[k] = 0.f;
         tb.store(L.b, LN, rows, N);
         tc.store(L.c, LN, rows, N);
     }
     __syncthreads();
-    // this wave's rows: r0 + 4 g + r, of t as of s
-    const int r0 = 16 * wave;
-    f32x4 G1[TB / 16], W[TB / 16], dB[NC], dC[NC];
+    f32x4 G1[GT], W[GT], dB[JT], dC[JT];
 #pragma unroll
-    for (int c = 0; c < TB / 16; ++c) {
-        G1[c] = f32x4{};
-        W[c] = f32x4{};
-        if (c <= wave) {
+    for (int u = 0; u < GT; ++u) {
+        G1[u] = f32x4{};
+        W[u] = f32x4{};
+        const int w = wave + WAVES * u;
+        if (w < 10) {
 #pragma unroll
             for (int k = 0; k < NK; ++k)
-                G1[c] = M::mma(M::row(L.c + r0 * LN + k * M::KS, LN, i, g), M::row(L.b + 16 * c * LN + k * M::KS, LN, i, g), G1[c]);
+                G1[u] = M::mma(M::row(L.c + 16 * tile_row(w) * LN + k * M::KS, LN, i, g), M::row(L.b + 16 * tile_col(w) * LN + k * M::KS, LN, i, g), G1[u]);
         }
     }
 #pragma unroll
-    for (int c = 0; c < NC; ++c) { dB[c] = f32x4{}; dC[c] = f32x4{}; }
-    const int kbegin = r0 / M::KS * M::KS, kend = (r0 + 16 + M::KS - 1) / M::KS * M::KS;      // rows t >= s, columns s <= t, in whole steps
-    const int h_first = grp * Hg + share * Hg / a.hsplit, h_last = grp * Hg + (share + 1) * Hg / a.hsplit;
-    for (int h = h_first; h < h_last; ++h) {
-        const float A = a.A[h], bias = a.dt_bias ? a.dt_bias[h] : 0.f, D = a.D ? a.D[h] : 0.f;
-        float raw = 0.f;
-        if (wave == 0) {
-            raw = lane < rows ? (float)static_cast<const T*>(a.dt)[(row0 + lane) * a.lddt + h] : 0.f;
-            make_steps<false>(L.st, a, raw, lane < rows, A, bias, lane);
-        }
-        float dot = 0.f, trace = 0.f, R[4] = {}, KI[4] = {}, diag[4] = {}, col[TB / 16] = {};   // sums over this lane's columns
-        for (int pt = 0; pt < a.ptiles; ++pt) {
-            const int p0 = pt * PT, P = min(a.P - p0, PT);
-            Tile<T, PT, V> tx, ty;
-            StateTile<T, NP> ts, td;
-            tx.load(static_cast<const T*>(a.x) + row0 * a.ldx + (int64_t)h * a.P + p0, a.ldx, rows, P);
-            ty.load(static_cast<const T*>(a.dy) + row0 * a.lddy + (int64_t)h * a.P + p0, a.lddy, rows, P);
-            ts.load(a, a.S, slot, h, p0, P);
-            td.load(a, a.dS, slot, h, p0, P);
-            tx.store(L.x, LX, rows, P);
-            ty.store(L.y, LX, rows, P);
-            ts.store(L.s, P, a.NS);
-            dot += ts.dot(td, P, a.NS);
-            __syncthreads();
-            // the rows with each other
+    for (int j = 0; j < JT; ++j) { dB[j] = f32x4{}; dC[j] = f32x4{}; }
+
+    for (int h = h_first, pt = 0; h < h_last;) {
+        // what comes next is loaded without asking whether there is more: the last one is loaded again, and nothing waits for it
+        const bool tiles_left = pt + 1 < a.ptiles;
+        const int hn = tiles_left ? h : min(h + 1, h_last - 1), ptn = tiles_left ? pt + 1 : h + 1 < h_last ? 0 : pt;
+        const int p0 = pt * PT, P = min(a.P - p0, PT);
+        const Steps& st = L.st[h & 1];
+        tx.store(L.x, LX, rows, P);
+        ty.store(L.y, LX, rows, P);
+        __syncthreads();
+        fetch_xy(hn, ptn);
+        // the rows with each other: lane i owns column s, four neighbouring rows t of it
+        float trace = 0.f;
 #pragma unroll
-            for (int c = 0; c < TB / 16; ++c) {
-                f32x4 m = {};
-                if (c <= wave) {
-                    f32x4 G2 = {};
+        for (int u = 0; u < GT; ++u) {
+            const int w = wave + WAVES * u;
+            if (w >= 12) break;
+            const int jt = tile_row(w), js = tile_col(w), s = 16 * js + i, t = 16 * jt + 4 * g;
+            f32x4 m = {};
+            if (w < 10) {
+                f32x4 G2 = {}, l;
 #pragma unroll
-                    for (int k = 0; k < PT / M::KS; ++k)
-                        G2 = M::mma(M::row(L.y + r0 * LX + k * M::KS, LX, i, g), M::row(L.x + 16 * c * LX + k * M::KS, LX, i, g), G2);
-                    const int s = 16 * c + i;
-                    const float hs = L.st.hi[s], ls = L.st.lo[s], ds = L.st.dt[s];
+                for (int k = 0; k < PK; ++k) G2 = M::mma(M::row(L.y + 16 * jt * LX + k * M::KS, LX, i, g), M::row(L.x + 16 * js * LX + k * M::KS, LX, i, g), G2);
+                const float ds = st.dt[s];
+                if (js < jt) {
+                    const float f = between(st, jt, js) * st.cf[s];
+                    l = *reinterpret_cast<const f32x4*>(st.rf + t) * f;
+                } else {
+                    const float hs = st.hi[s], ls = st.lo[s];
+                    const f32x4 ht = *reinterpret_cast<const f32x4*>(st.hi + t), lt = *reinterpret_cast<const f32x4*>(st.lo + t);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int t = r0 + 4 * g + r;
-                        const float l = s <= t ? __expf(gap(L.st, t, hs, ls)) : 0.f, gl = s <= t ? G2[r] * l : 0.f;
-                        m[r] = s <= t ? G1[c][r] * l : 0.f;
-                        const float qv = s <= t ? G1[c][r] * gl : 0.f;
-                        W[c][r] = fmaf(gl, ds, W[c][r]);
-                        if (s < t) {
-                            col[c] += qv;
-                            R[r] = fmaf(qv, ds, R[r]);
-                        } else if (s == t) {
-                            diag[r] += qv;
-                            trace += G2[r];
-                        }
-                    }
+                    for (int r = 0; r < 4; ++r) l[r] = s <= t + r ? __expf((ht[r] - hs) + (lt[r] - ls)) : 0.f;
                 }
-                if (pt == 0) {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) L.m[(r0 + 4 * g + r) * LM + 16 * c + i] = (T)m[r];
-                }
-            }
-            // dC_t += exp(a_t) S^T dy_t
-            float e[4];
-            {
-                f32x4 acc[NC];
-#pragma unroll
-                for (int c = 0; c < NC; ++c) acc[c] = f32x4{};
-#pragma unroll
-                for (int k = 0; k < PT / M::KS; ++k) {
-                    const typename M::frag f = M::row(L.y + r0 * LX + k * M::KS, LX, i, g);
-#pragma unroll
-                    for (int c = 0; c < NC; ++c)
-#pragma unroll
-                        for (int pc = PIECES - 1; pc >= 0; --pc) acc[c] = M::mma(f, M::col(L.s[pc] + k * M::KS * LN + 16 * c, LN, i, g), acc[c]);
-                }
-#pragma unroll
-                for (int r = 0; r < 4; ++r) e[r] = __expf(L.st.hi[r0 + 4 * g + r]);
-#pragma unroll
-                for (int c = 0; c < NC; ++c)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float v = e[r] * acc[c][r];
-                        dC[c][r] += v;
-                        R[r] = fmaf(v, (float)L.c[(r0 + 4 * g + r) * LN + 16 * c + i], R[r]);
-                    }
-            }
-            __syncthreads();
-            td.store(L.s, P, a.NS);
-            __syncthreads();
-            // dB_s += dt_s e_s dS^T x_s
-            float ds[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int s = r0 + 4 * g + r;
-                ds[r] = L.st.dt[s];
-                e[r] = __expf(gap(L.st, TB - 1, L.st.hi[s], L.st.lo[s]));
-            }
-            {
-                f32x4 acc[NC];
-#pragma unroll
-                for (int c = 0; c < NC; ++c) acc[c] = f32x4{};
-#pragma unroll
-                for (int k = 0; k < PT / M::KS; ++k) {
-                    const typename M::frag f = M::row(L.x + r0 * LX + k * M::KS, LX, i, g);
-#pragma unroll
-                    for (int c = 0; c < NC; ++c)
-#pragma unroll
-                        for (int pc = PIECES - 1; pc >= 0; --pc) acc[c] = M::mma(f, M::col(L.s[pc] + k * M::KS * LN + 16 * c, LN, i, g), acc[c]);
-                }
-#pragma unroll
-                for (int c = 0; c < NC; ++c)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float v = e[r] * acc[c][r];
-                        dB[c][r] = fmaf(ds[r], v, dB[c][r]);
-                        KI[r] = fmaf(v, (float)L.b[(r0 + 4 * g + r) * LN + 16 * c + i], KI[r]);
-                    }
-            }
-            // dx_s = dt_s (e_s dS B_s + sum_t G1 L dy_t) + D dy_s
-            {
-                f32x4 acc[PT / 16];
-#pragma unroll
-                for (int c = 0; c < PT / 16; ++c) acc[c] = f32x4{};
-#pragma unroll
-                for (int k = 0; k < NK; ++k) {
-                    const typename M::frag f = M::row(L.b + r0 * LN + k * M::KS, LN, i, g);
-#pragma unroll
-                    for (int c = 0; c < PT / 16; ++c) acc[c] = M::mma(f, M::row(L.s[0] + 16 * c * LN + k * M::KS, LN, i, g), acc[c]);
-                }
-#pragma unroll
-                for (int c = 0; c < PT / 16; ++c)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) acc[c][r] *= e[r];
-                for (int k = kbegin; k < TB; k += M::KS) {
-                    const typename M::frag f = M::col(L.m + k * LM + r0, LM, i, g);
-#pragma unroll
-                    for (int c = 0; c < PT / 16; ++c) acc[c] = M::mma(f, M::col(L.y + k * LX + 16 * c, LX, i, g), acc[c]);
-                }
-                // out through this wave's rows of x, which nobody else reads any more
-                T* out = L.x + r0 * LX;
-#pragma unroll
-                for (int c = 0; c < PT / 16; ++c)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        out[(4 * g + r) * LX + 16 * c + i] = (T)fmaf(ds[r], acc[c][r], D * (float)L.y[(r0 + 4 * g + r) * LX + 16 * c + i]);
-                typedef T vec_t __attribute__((ext_vector_type(V)));
-                constexpr int PER_ROW = PT / V;
-                T* dx = static_cast<T*>(a.dx) + (row0 + r0) * a.lddx + (int64_t)h * a.P + p0;
-#pragma unroll
-                for (int k = 0; k < 16 * PER_ROW / 64; ++k) {
-                    const int idx = k * 64 + lane, r = idx / PER_ROW, c = idx % PER_ROW * V;
-                    if (r0 + r < rows && c < P) *reinterpret_cast<vec_t*>(dx + r * a.lddx + c) = *reinterpret_cast<const vec_t*>(out + r * LX + c);
-                }
-            }
-            if (pt + 1 == a.ptiles) {
+                float col = 0.f, rq[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const float sR = sum16(R[r]), sK = sum16(KI[r]), sd = sum16(diag[r]);
-                    if (i == 0) { L.R[r0 + 4 * g + r] = sR; L.KI[r0 + 4 * g + r] = sK; L.diag[r0 + 4 * g + r] = sd; }
+                    const bool in = js < jt || s <= t + r;               // a product that is not finite stays out of what it does not belong to
+                    const float gl = in ? G2[r] * l[r] : 0.f, qv = in ? G1[u][r] * gl : 0.f;
+                    m[r] = in ? G1[u][r] * l[r] : 0.f;
+                    W[u][r] = fmaf(gl, ds, W[u][r]);
+                    const bool strict = js < jt || s < t + r;
+                    col += strict ? qv : 0.f;
+                    rq[r] = strict ? qv * ds : 0.f;
+                    if (js == jt && s == t + r) {
+                        L.diag[s] = pt ? L.diag[s] + qv : qv;
+                        trace += G2[r];
+                    }
                 }
+                float* K = &L.K[4 * jt + g][s];
+                *K = pt ? *K + col : col;
 #pragma unroll
-                for (int c = 0; c < TB / 16; ++c) L.col[4 * wave + g][16 * c + i] = col[c];
-                dot = wave_sum(dot);
-                trace = wave_sum(trace);
-                if (lane == 0) { L.dot[wave] = dot; L.trace[wave] = trace; }
+                for (int r = 0; r < 4; ++r) rq[r] = sum16(rq[r]);
+                if (i == 0) {
+                    f32x4* R = reinterpret_cast<f32x4*>(&L.R[js][t]);
+                    const f32x4 v = {rq[0], rq[1], rq[2], rq[3]};
+                    *R = pt ? *R + v : v;
+                }
             }
-            __syncthreads();
+            *reinterpret_cast<four_t*>(L.m + s * LM + t) = four<T>(m);
         }
-        if (wave == 0) {                                     // lane = row
-            float K = L.KI[lane];
+        __builtin_amdgcn_sched_barrier(0);
+        // dC_t += exp(a_t) S^T dy_t, dB_s += dt_s exp(a_T - a_s) dS^T x_s: lane i owns the row, four neighbouring columns n of it
+        float dot = 0.f;
 #pragma unroll
-            for (int k = 0; k < 16; ++k) K += L.col[k][lane];
-            const float d = L.st.dt[lane];
+        for (int k = 0; k < PT / 4; ++k) dot += n0 + i < N && 16 * (k / 4) + 4 * g + k % 4 < P ? S.v[k] * dS.v[k] : 0.f;
+        {
+            const Pieces<T> f(S.v);
+#pragma unroll
+            for (int j = 0; j < JT; ++j) {
+                const int t = 16 * (jt0 + WT * j);
+                f32x4 acc = {};
+#pragma unroll
+                for (int k = 0; k < PK; ++k) {
+                    const typename M::frag y = M::row(L.y + t * LX + k * M::KS, LX, i, g);
+#pragma unroll
+                    for (int pc = Pieces<T>::N - 1; pc >= 0; --pc) acc = M::mma(f.f[pc][k], y, acc);
+                }
+                acc *= st.ea[t + i];
+                dC[j] += acc;
+                const four_t c = *reinterpret_cast<const four_t*>(L.c + (t + i) * LN + n0 + 4 * g);
+                float v = 0.f;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) v = fmaf(acc[r], (float)c[r], v);
+                float* RI = &L.RI[wave % WN * 4 + g][t + i];
+                *RI = pt ? *RI + v : v;
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        {
+            const Pieces<T> f(dS.v);
+#pragma unroll
+            for (int j = 0; j < JT; ++j) {
+                const int s = 16 * (jt0 + WT * j);
+                f32x4 acc = {};
+#pragma unroll
+                for (int k = 0; k < PK; ++k) {
+                    const typename M::frag x = M::row(L.x + s * LX + k * M::KS, LX, i, g);
+#pragma unroll
+                    for (int pc = Pieces<T>::N - 1; pc >= 0; --pc) acc = M::mma(f.f[pc][k], x, acc);
+                }
+                acc *= st.es[s + i];
+                const float ds = st.dt[s + i];
+                const four_t bv = *reinterpret_cast<const four_t*>(L.b + (s + i) * LN + n0 + 4 * g);
+                float v = 0.f;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    dB[j][r] = fmaf(ds, acc[r], dB[j][r]);
+                    v = fmaf(acc[r], (float)bv[r], v);
+                }
+                float* KI = &L.KI[wave % WN * 4 + g][s + i];
+                *KI = pt ? *KI + v : v;
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        fetch_cols(hn, ptn);
+        // every row tile's columns n are counted once: the waves that share them hold the same S
+        dot = jt0 == 0 ? sum16(dot) : 0.f;
+        trace = sum16(trace);
+        if (i == 0) {
+            const int k = 4 * wave + g;
+            L.dot[k] = pt ? L.dot[k] + dot : dot;
+            L.trace[k] = pt ? L.trace[k] + trace : trace;
+        }
+        if (wave == WAVES - 1 && !tiles_left && h + 1 < h_last) {
+            steps(h + 1, raw);
+            raw = dtp[dt_off + min(h + 2, h_last - 1)];
+        }
+        __syncthreads();
+        // dx_s = dt_s (exp(a_T - a_s) dS B_s + sum_t G1 L dy_t) + D dy_s: lane i owns the row, four neighbouring columns p of it
+        {
+            const float D = a.D ? a.D[h] : 0.f;
+            typename M::frag sf[NK];
+#pragma unroll
+            for (int k = 0; k < NK; ++k) {
+                if constexpr (sizeof(T) == 4) {
+                    sf[k] = dSr[k];
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) sf[k][e] = (T)dSr[2 * k + (e >> 2)][e & 3];
+                }
+            }
+            f32x4 acc[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int s = 16 * (js0 + 2 * j);
+                acc[j] = f32x4{};
+#pragma unroll
+                for (int k = 0; k < NK; ++k) acc[j] = M::mma(sf[k], M::row(L.b + s * LN + k * M::KS, LN, i, g), acc[j]);
+                acc[j] *= st.es[s + i];
+            }
+            fetch_rows(hn, ptn);
+#pragma unroll
+            for (int k = 0; k < TB; k += M::KS) {
+                if (k >= rows || k + M::KS <= 16 * js0) continue;
+                const typename M::frag yf = M::col(L.y + k * LX + pw, LX, i, g);
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                    if (k + M::KS > 16 * (js0 + 2 * j)) acc[j] = M::mma(yf, M::row(L.m + 16 * (js0 + 2 * j) * LM + k, LM, i, g), acc[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int s = 16 * (js0 + 2 * j) + i, p = pw + 4 * g;
+                if (s >= rows || p >= P) continue;
+                const float ds = st.dt[s];
+                const four_t yv = *reinterpret_cast<const four_t*>(L.y + s * LX + p);
+                four_t o;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[r] = (T)fmaf(ds, acc[j][r], D * (float)yv[r]);
+                T* out = dxp + (h * a.P + p0) + (uint32_t)(s * lddx + p);
+                if (V > 1) {
+                    *reinterpret_cast<four_t*>(out) = o;
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (p + r < P) out[r] = o[r];
+                }
+            }
+        }
+        if (wave == 0 && !tiles_left) {                                   // lane = row
+            float R = 0.f, K = 0.f, KI = 0.f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) R += L.R[k][lane];
+#pragma unroll
+            for (int k = 0; k < 16; ++k) K += L.K[k][lane];
+#pragma unroll
+            for (int k = 0; k < 4 * WN; ++k) { R += L.RI[k][lane]; KI += L.KI[k][lane]; }
+            K += KI;
+            const float d = st.dt[lane], A = a.A[h];
             // exp(a_T) <S, dS> + sum_s dt_s KI_s reach every row of the block: they stand behind its last one
-            const double behind = (double)__expf(L.st.total) * (double)((L.dot[0] + L.dot[1]) + (L.dot[2] + L.dot[3])) + wave_sum((double)(d * L.KI[lane]));
-            const double da = (double)L.R[lane] - (double)(d * K);
+            const int k = lane & (4 * WAVES - 1);
+            const float dot_k = lane == k ? L.dot[k] : 0.f, trace_k = lane == k ? L.trace[k] : 0.f;
+            const double behind = wave_sum(fma((double)__expf(st.total), (double)dot_k, (double)(d * KI)));
+            const double da = (double)R - (double)(d * K);
             const double pre = wave_prefix(da, lane), all = __shfl(pre, 63, 64);
             const float suffix = (float)(all - pre + da + behind);
             float ddt = fmaf(A, suffix, K + L.diag[lane]);
-            if (a.softplus) ddt *= 1.f / (1.f + expf(-(raw + bias)));
+            if (a.softplus) ddt *= -expm1f(-d);                           // sigmoid(v) = 1 - exp(-softplus(v))
             if (lane >= rows) ddt = 0.f;
             if (lane < rows) static_cast<T*>(a.ddt)[(row0 + lane) * a.ldddt + h] = (T)ddt;
-            const float sA = wave_sum(d * suffix), sb = wave_sum(ddt);
+            const float sA = wave_sum(d * suffix), sb = wave_sum(ddt), sD = wave_sum(trace_k);
             if (lane == 0) {
                 float* p = a.part + ((int64_t)slot * a.H + h) * 3;
                 p[0] = sA;
-                p[1] = (L.trace[0] + L.trace[1]) + (L.trace[2] + L.trace[3]);
+                p[1] = sD;
                 p[2] = sb;
             }
         }
+        __syncthreads();
+        pt = tiles_left ? pt + 1 : 0;
+        h = tiles_left ? h : h + 1;
     }
     // dC_t += sum_s W[t,s] B_s, dB_s += sum_t W[t,s] C_t
-    // (no wave reads m between here and the barrier; wave 0's last rows of R, K, .. are not touched any more)
 #pragma unroll
-    for (int c = 0; c < TB / 16; ++c)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) L.m[(r0 + 4 * g + r) * LM + 16 * c + i] = (T)W[c][r];
+    for (int u = 0; u < GT; ++u) {
+        const int w = wave + WAVES * u;
+        if (w >= 12) break;
+        *reinterpret_cast<four_t*>(L.m + (16 * tile_col(w) + i) * LM + 16 * tile_row(w) + 4 * g) = four<T>(W[u]);
+    }
     __syncthreads();
-    for (int k = 0; k < kend; k += M::KS) {
-        const typename M::frag f = M::row(L.m + r0 * LM + k, LM, i, g);
 #pragma unroll
-        for (int c = 0; c < NC; ++c) dC[c] = M::mma(f, M::col(L.b + k * LN + 16 * c, LN, i, g), dC[c]);
+    for (int k = 0; k < TB; k += M::KS) {
+        if (k >= rows) continue;
+        const typename M::frag bf = M::col(L.b + k * LN + n0, LN, i, g), cf = M::col(L.c + k * LN + n0, LN, i, g);
+#pragma unroll
+        for (int j = 0; j < JT; ++j) {
+            const int t = 16 * (jt0 + WT * j);
+            if (k <= t) dC[j] = M::mma(bf, M::col(L.m + k * LM + t, LM, i, g), dC[j]);
+            if (k + M::KS > t) dB[j] = M::mma(cf, M::row(L.m + t * LM + k, LM, i, g), dB[j]);
+        }
     }
-    for (int k = kbegin; k < TB; k += M::KS) {
-        const typename M::frag f = M::col(L.m + k * LM + r0, LM, i, g);
 #pragma unroll
-        for (int c = 0; c < NC; ++c) dB[c] = M::mma(f, M::col(L.c + k * LN + 16 * c, LN, i, g), dB[c]);
-    }
-    if (a.hsplit > 1) {
-        float* p = a.part_bc + (((int64_t)share * a.rows + row0) * a.G + grp) * 2 * N;
+    for (int j = 0; j < JT; ++j) {
+        const int t = 16 * (jt0 + WT * j) + i, n = n0 + 4 * g;
+        if (t >= rows || n >= N) continue;
+        if (a.hsplit > 1) {
+            float* o = a.part_bc + (((int64_t)share * a.rows + row0 + t) * a.G + grp) * 2 * N + n;
 #pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int t = r0 + 4 * g + r, n = 16 * c + i;
-                if (t < rows && n < N) {
-                    float* o = p + (int64_t)t * a.G * 2 * N + n;
-                    o[0] = dB[c][r];
-                    o[N] = dC[c][r];
+            for (int r = 0; r < 4; ++r)
+                if (n + r < N) {
+                    o[r] = dB[j][r];
+                    o[N + r] = dC[j][r];
                 }
+        } else {
+            T* pb = static_cast<T*>(a.dB) + (row0 + t) * a.lddb + (int64_t)grp * N + n;
+            T* pc = static_cast<T*>(a.dC) + (row0 + t) * a.lddc + (int64_t)grp * N + n;
+            const four_t ob = four<T>(dB[j]), oc = four<T>(dC[j]);
+            if (V > 1) {
+                *reinterpret_cast<four_t*>(pb) = ob;
+                *reinterpret_cast<four_t*>(pc) = oc;
+            } else {
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (n + r < N) {
+                        pb[r] = ob[r];
+                        pc[r] = oc[r];
+                    }
             }
-        return;
-    }
-    typedef T vec_t __attribute__((ext_vector_type(V)));
-    constexpr int PER_ROW = NP / V;
-    T* const out = L.s[0] + r0 * LN;                          // this wave's rows; S and dS are used up
-#pragma unroll
-    for (int w = 0; w < 2; ++w) {
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) out[(4 * g + r) * LN + 16 * c + i] = (T)(w ? dC[c][r] : dB[c][r]);
-        const int64_t ld = w ? a.lddc : a.lddb;
-        T* const p = static_cast<T*>(w ? a.dC : a.dB) + (row0 + r0) * ld + (int64_t)grp * N;
-#pragma unroll
-        for (int k = 0; k < 16 * PER_ROW / 64; ++k) {
-            const int idx = k * 64 + lane, r = idx / PER_ROW, c = idx % PER_ROW * V;
-            if (r0 + r < rows && c < N) *reinterpret_cast<vec_t*>(p + r * ld + c) = *reinterpret_cast<const vec_t*>(out + r * LN + c);
         }
     }
 }
@@ -423,7 +497,7 @@ int launch_bwd(const SsmArgs& a, hipStream_t s) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(ssm_bwd_kernel<T, NP, V>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
         if (e != hipSuccess) { set_error("dc_ssm_scan_bwd: LDS", (int)e); return (int)e; }
     }
-    hipLaunchKernelGGL((ssm_bwd_kernel<T, NP, V>), dim3(a.cap, a.G, a.hsplit), dim3(256), bytes, s, a);
+    hipLaunchKernelGGL((ssm_bwd_kernel<T, NP, V>), dim3(a.cap, a.G, a.hsplit), dim3(THREADS), bytes, s, a);
     return launch_check("dc_ssm_scan_bwd");
 }
 template <typename T, int V>

@@ -86,27 +86,89 @@ template <typename T> __device__ __forceinline__ typename Four<T>::vec four(f32x
     return o;
 }
 
-// A 64-row tile of W columns on its way from global memory to LDS: 256 threads, V elements per access.  Rows and columns outside become zeros on the
-// way to LDS; their loads go to the last row and the first column instead of being left out, so that no branch stands between the loads of a tile and
-// nothing waits for them before store().  rows, cols >= 1.
-template <typename T, int W, int V, int THREADS = 256>
+// A value that all lanes share, for scalar registers: what a load returns does not look like one to the compiler.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+    return (int64_t)(((uint64_t)(uint32_t)uniform((int)(v >> 32)) << 32) | (uint32_t)uniform((int)v));
+}
+__device__ __forceinline__ SeqRange uniform_range(const SsmArgs& a, int b) {
+    SeqRange q = seq_range(a.seq_off, a.seq_len, b, a.rows, a.max_len);
+    q.off = uniform(q.off);
+    q.len = uniform(q.len);
+    return q;
+}
+
+// ROWS rows of W columns on their way from global memory to LDS: 256 threads, V elements per access, a scalar base and one 32-bit offset per thread
+// (the host refuses row distances beyond 2^22 elements).  Rows and columns outside become zeros on the way to LDS; their loads go to the last row and the
+// first column instead of being left out, so that no branch stands between the loads of a tile and nothing waits for them before store().
+// FULL: all ROWS rows are there.  rows, cols >= 1.
+template <typename T, int W, int V, int ROWS = TB, int THREADS = 256>
 struct Tile {
     typedef T vec_t __attribute__((ext_vector_type(V)));
-    static constexpr int PER_ROW = W / V, N = TB * PER_ROW / THREADS;
+    static constexpr int PER_ROW = W / V, STEP = THREADS / PER_ROW, N = (ROWS + STEP - 1) / STEP;
     vec_t v[N];
-    __device__ __forceinline__ void load(const T* __restrict__ p, int64_t ld, int rows, int cols) {
+    uint32_t off;            // of this thread's first row and column, in bytes
+    int r, c;
+    bool inside;
+    __device__ __forceinline__ Tile(int64_t ld, int cols) {
+        r = threadIdx.x / PER_ROW;
+        c = threadIdx.x % PER_ROW * V;
+        inside = c < cols;
+        off = ((uint32_t)r * (uint32_t)ld + (inside ? c : 0)) * sizeof(T);
+    }
+    template <bool FULL>
+    __device__ __forceinline__ void load(const T* __restrict__ p, int64_t ld, int rows) {
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-            const int idx = k * THREADS + threadIdx.x, r = idx / PER_ROW, c = idx % PER_ROW * V;
-            v[k] = *reinterpret_cast<const vec_t*>(p + min(r, rows - 1) * ld + (c < cols ? c : 0));
+            if (FULL && STEP <= ROWS) {
+                v[k] = *reinterpret_cast<const vec_t*>(reinterpret_cast<const char*>(p + k * STEP * ld) + off);
+            } else {
+                const int back = max(0, r + k * STEP - (rows - 1));
+                v[k] = *reinterpret_cast<const vec_t*>(reinterpret_cast<const char*>(p) + (int64_t)off + (int64_t)(k * STEP - back) * ld * (int64_t)sizeof(T));
+            }
         }
     }
-    __device__ __forceinline__ void store(T* lds, int ld, int rows, int cols) const {
+    template <bool FULL>
+    __device__ __forceinline__ void store(T* lds, int ld, int rows, bool all_cols) const {
+        T* q = lds + r * ld + c;
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-            const int idx = k * THREADS + threadIdx.x, r = idx / PER_ROW, c = idx % PER_ROW * V;
-            vec_t z = {};
-            *reinterpret_cast<vec_t*>(lds + r * ld + c) = r < rows && c < cols ? v[k] : z;
+            if (ROWS % STEP && r + k * STEP >= ROWS) continue;
+            vec_t o = v[k];
+            if (!FULL || !all_cols) {
+                vec_t z = {};
+                if (!(inside && (FULL || r + k * STEP < rows))) o = z;
+            }
+            *reinterpret_cast<vec_t*>(q + k * STEP * ld) = o;
+        }
+    }
+};
+
+// The same for a block whose rows stay while its columns move (the heads of one block): the rows' offsets are made once.
+template <typename T, int W, int V, int THREADS>
+struct BlockTile {
+    typedef T vec_t __attribute__((ext_vector_type(V)));
+    static constexpr int PER_ROW = W / V, STEP = THREADS / PER_ROW, N = (TB + STEP - 1) / STEP;
+    vec_t v[N];
+    uint32_t off[N];
+    __device__ __forceinline__ BlockTile(int ld, int rows) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) off[k] = (uint32_t)(min((int)threadIdx.x / PER_ROW + k * STEP, rows - 1) * ld) * (uint32_t)sizeof(T);
+    }
+    __device__ __forceinline__ void load(const T* __restrict__ p, int cols) {
+        const int c = threadIdx.x % PER_ROW * V;
+        const uint32_t co = (c < cols ? c : 0) * sizeof(T);
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[k] = *reinterpret_cast<const vec_t*>(reinterpret_cast<const char*>(p) + (off[k] + co));
+    }
+    __device__ __forceinline__ void store(T* lds, int ld, int rows, int cols) const {
+        const int r = threadIdx.x / PER_ROW, c = threadIdx.x % PER_ROW * V;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            if (TB % STEP && r + k * STEP >= TB) continue;
+            vec_t o = v[k], z = {};
+            if (r + k * STEP >= rows || c >= cols) o = z;
+            *reinterpret_cast<vec_t*>(lds + (r + k * STEP) * ld + c) = o;
         }
     }
 };
@@ -140,12 +202,19 @@ __device__ __forceinline__ double wave_prefix(double v, int lane) {
 // what a long sum costs: a is summed in f64, the difference is taken of both halves.
 struct Steps {
     float dt[TB], hi[TB], lo[TB], w[TB];
+    float ea[TB], es[TB];                         // exp(a_t), exp(a_T - a_t)
+    float rf[TB], cf[TB], cd[TB];                 // exp(a_t - a of its tile of 16's first row), exp(a of its tile's last row - a_t), the same times dt_t
     float total;                                  // a of the last row
 };
-__device__ __forceinline__ float gap(const Steps& s, int t, float hi_s, float lo_s) { return (s.hi[t] - hi_s) + (s.lo[t] - lo_s); }
+// exp(a of row tile jt's first row - a of row tile js's last one), js < jt: with rf and cf the decay from s to t in three factors, none above 1 where
+// the decays are not.
+__device__ __forceinline__ float between(const Steps& s, int jt, int js) {
+    return __expf((s.hi[16 * jt] - s.hi[16 * js + 15]) + (s.lo[16 * jt] - s.lo[16 * js + 15]));
+}
 
 // w[t] = dt_t exp(a_T - a_t): the weights of the block's rows in the state behind it; REV: exp(a_t), those of the gradients in the one in front.
-template <bool REV>
+// FACTORS: ea, es, rf, cf, cd too.
+template <bool REV, bool FACTORS>
 __device__ __forceinline__ void make_steps(Steps& s, const SsmArgs& a, float raw, bool live, float A, float bias, int lane) {
     float d = raw + bias;
     if (a.softplus) d = softplus_f(d);
@@ -155,7 +224,16 @@ __device__ __forceinline__ void make_steps(Steps& s, const SsmArgs& a, float raw
     s.dt[lane] = d;
     s.hi[lane] = (float)sum;
     s.lo[lane] = (float)(sum - (double)(float)sum);
-    s.w[lane] = REV ? __expf((float)sum) : d * __expf((float)(last - sum));
+    const float es = __expf((float)(last - sum));
+    s.w[lane] = REV ? __expf((float)sum) : d * es;
+    if (FACTORS) {
+        const float cf = __expf((float)(__shfl(sum, lane | 15, 64) - sum));
+        s.ea[lane] = __expf((float)sum);
+        s.es[lane] = es;
+        s.rf[lane] = __expf((float)(sum - __shfl(sum, lane & 48, 64)));
+        s.cf[lane] = cf;
+        s.cd[lane] = d * cf;
+    }
     if (lane == 63) s.total = (float)last;
 }
 
@@ -174,10 +252,12 @@ __device__ __forceinline__ void split_bf16(float v, bf16_t (&p)[PIECES_F32]) {
 // they are at once the operand of the products over n, and a lane's four neighbouring n leave in one access.
 // The weights are f32: bf16 operands are scaled in f32 and used as three bf16 pieces, because the states they end in are f32 (with two pieces, 16 bits,
 // the gradients of A and dt_bias were off by 4e-6 .. 8e-6 of their norm, with three by what f32 sums are off by).
-template <typename T, int NP>
+template <typename T, int NP, int ROWS>
 __device__ __forceinline__ void state_update(f32x4 (&acc)[NP / 16], const T* X, int ldx, const T* Y, int ldy, const float* w, int p0, int rows, int i, int g) {
     typedef Mat<T> M;
-    for (int k = 0; k < rows; k += M::KS) {
+#pragma unroll
+    for (int k = 0; k < ROWS; k += M::KS) {
+        if (k >= rows) break;
         typename M::frag x = M::col(X + k * ldx + p0, ldx, i, g);
         if constexpr (sizeof(T) == 4) {
             x *= *reinterpret_cast<const f32x4*>(w + k + 4 * g);
@@ -244,6 +324,11 @@ __device__ __forceinline__ void store_state(const f32x4 (&acc)[NP / 16], float* 
         }
     }
 }
+
+// The 16 x 16 tiles (row tile, column tile) of a 64 x 64 triangle s <= t that products with it read: ten with s <= t, and two zero ones that complete the
+// 32-wide steps beside row tiles 0 and 2.
+__device__ __forceinline__ int tile_row(int u) { return (int)(0x203323213210ull >> (4 * u)) & 15; }
+__device__ __forceinline__ int tile_col(int u) { return (int)(0x310102103210ull >> (4 * u)) & 15; }
 
 __host__ __device__ __forceinline__ int blocks_of(int len) { return len / TB + (len % TB != 0); }
 
