@@ -253,7 +253,7 @@ __device__ __forceinline__ void states(const SsmArgs& a, StateLds<T, NP>& L) {
         }
         __syncthreads();
         if (more) fetch(block(j + 1));
-        if constexpr (!FINAL) store_state<NP, 4>(S, (REV ? a.dS : a.S) + (((int64_t)(slot + blk) * a.H + h) * a.P + pbase) * a.NS, a.NS, p0, P, a.NS, i, g);
+        if constexpr (!FINAL) store_state<NP, 4>(S, (REV ? a.dS : a.S) + (((int64_t)(slot + blk) * a.H + h) * a.PS + pbase) * a.NS, a.NS, p0, a.PS - pbase, a.NS, i, g);
         const float et = __expf(st.total);
         sum += (double)st.total;
 #pragma unroll

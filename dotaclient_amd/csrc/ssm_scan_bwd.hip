@@ -9,13 +9,13 @@
 //   d(dt')_t = A d(a step)_t + K_t,   dA = sum_t dt_t d(a step)_t,   dD = sum_t G2[t,t]
 // (the diagonal cancels in R - dt K and is left out of both, so that strong decays do not lose the gradient of A in it).
 //
-// A workgroup of eight waves owns one block and the heads of one group (or a share of them, where blocks and groups alone are too few): G1 stays in its
+// A workgroup of four or eight waves owns one block and the heads of one group (or a share of them, where blocks and groups alone are too few): G1 stays in its
 // registers, W and the gradients of B and C are added up over the heads there, so dB and dC cost two products per block instead of two per head, and
 // no partial sums in memory.  Per head two phases with a barrier between them:
 //   1. the ten 16 x 16 tiles of G2 with s <= t, shared out over the waves: W, Q's row and column sums, G1 L to LDS; S^T dy and dS^T x for the columns n
 //      that a wave owns, whose part of S and dS it alone reads - straight from memory into operands;
-//   2. dx for the columns p that a wave owns; one wave runs along the rows for d(a step), ddt and the sums for dA, dD, ddt_bias.
-// The next head's x, dy, S, dS are loaded as soon as this one's are used.  Operands that are f32 by nature are used as three bf16 pieces where an f32
+//   2. dx for the columns p that a wave owns.
+// In the next head's phase 1 the last wave runs along the rows for d(a step), ddt and the sums for dA, dD, ddt_bias.  The next head's x, dy, S, dS are loaded as soon as this one's are used.  Operands that are f32 by nature are used as three bf16 pieces where an f32
 // result depends on them (S and dS: R, K -> dA, ddt_bias); W and G1 L, which only end in bf16 outputs, are rounded once, and dS in dx takes its
 // first piece.
 #include "ssm_util.h"
@@ -23,26 +23,25 @@
 namespace dc {
 namespace {
 
-constexpr int WAVES = 8, THREADS = 64 * WAVES;
-
-template <typename T, int NP>
+template <typename T, int NP, int WAVES>
 struct BwdLds {
     // how the waves share out the 16-column tiles of N and the four row tiles: WN x WT waves, JT row tiles each
-    static constexpr int WN = NP / 16, WT = WAVES / WN, JT = 4 / WT;
+    static constexpr int WN = NP / 16 < WAVES ? NP / 16 : WAVES, WT = WAVES / WN, JT = 4 / WT;
+    static_assert(NP / 16 <= WAVES, "a column tile of N for every wave at most");
     T b[TB * pitch<T>(NP)], c[TB * pitch<T>(NP)], x[TB * pitch<T>(PT)], y[TB * pitch<T>(PT)], m[TB * pitch<T>(TB)];
     Steps st[2];
-    float R[4][TB], K[16][TB], RI[4 * WN][TB], KI[4 * WN][TB], diag[TB], dot[4 * WAVES], trace[4 * WAVES];
+    struct Sums { float R[4][TB], K[4][TB], RI[WN][TB], KI[WN][TB], diag[TB], dot[4 * WAVES], trace[4 * WAVES]; } sums[2];      // of one head
 };
 
 // 64 x 16 of S or dS as an operand whose rows are its columns n and whose k is p: element 4 kk + e of lane (i, g) is [16 kk + 4 g + e][n0 + i].
+// P16 = P in whole row tiles: what is behind P was written as zeros, whole tiles behind it are not there.
 struct StateCols {
     float v[PT / 4];
-    __device__ __forceinline__ void load(const float* __restrict__ p, int NS, int P, int n0, int i, int g) {
-        const int n = min(n0 + i, NS - 1);
+    __device__ __forceinline__ void load(const float* __restrict__ p, int NS, int P16, uint32_t off) {      // off: (4 g) NS + n
 #pragma unroll
         for (int kk = 0; kk < PT / 16; ++kk)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[4 * kk + e] = p[(uint32_t)(min(16 * kk + 4 * g + e, P - 1) * NS + n)];
+            for (int e = 0; e < 4; ++e) v[4 * kk + e] = 16 * kk < P16 ? (p + (16 * kk + e) * NS)[off] : 0.f;
     }
 };
 template <typename T> struct Pieces;
@@ -68,13 +67,14 @@ template <> struct Pieces<bf16_t> {
     }
 };
 
-template <typename T, int NP, int V>
-__global__ void __launch_bounds__(THREADS) ssm_bwd_kernel(SsmArgs a) {
+template <typename T, int NP, int V, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, 2) ssm_bwd_kernel(SsmArgs a) {
     typedef Mat<T> M;
     typedef typename Four<T>::vec four_t;
-    typedef BwdLds<T, NP> Lds;
+    typedef BwdLds<T, NP, WAVES> Lds;
+    constexpr int THREADS = 64 * WAVES;
     constexpr int LX = pitch<T>(PT), LN = pitch<T>(NP), LM = pitch<T>(TB), NK = NP / M::KS, PK = PT / M::KS, WN = Lds::WN, WT = Lds::WT, JT = Lds::JT;
-    constexpr int GT = (12 + WAVES - 1) / WAVES;
+    constexpr int GT = (12 + WAVES - 1) / WAVES, JS = 16 / WAVES, SS = WAVES / 4;
     extern __shared__ __attribute__((aligned(16))) char lds_raw[];
     Lds& L = *reinterpret_cast<Lds*>(lds_raw);
     const int slot = blockIdx.x, grp = blockIdx.y, share = blockIdx.z, Hg = a.H / a.G;
@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(THREADS) ssm_bwd_kernel(SsmArgs a) {
     const int rows = min(TB, q.len - blk * TB);
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), i = lane & 15, g = lane >> 4, N = a.N;
     const int n0 = 16 * (wave % WN), jt0 = wave / WN;                     // this wave's columns n; its row tiles jt0 + WT j
-    const int pw = 16 * (wave & 3), js0 = wave >> 2;                      // its columns p and row tiles js0 + 2 j of dx
+    const int pw = 16 * (wave & 3), js0 = wave >> 2;                      // its columns p and row tiles js0 + SS j of dx
     const int h_first = grp * Hg + share * Hg / a.hsplit, h_last = grp * Hg + (share + 1) * Hg / a.hsplit;
     const int ldx = (int)a.ldx, lddy = (int)a.lddy, lddx = (int)a.lddx, NS = a.NS;
     const T* const xp = static_cast<const T*>(a.x) + row0 * ldx;
@@ -93,8 +93,9 @@ __global__ void __launch_bounds__(THREADS) ssm_bwd_kernel(SsmArgs a) {
     const T* const dtp = static_cast<const T*>(a.dt) + row0 * a.lddt;
     const uint32_t dt_off = (uint32_t)min(lane, rows - 1) * (uint32_t)a.lddt;
     T* const dxp = static_cast<T*>(a.dx) + row0 * lddx;
-    const float* const Sp = a.S + (int64_t)slot * a.H * a.P * NS;
-    const float* const dSp = a.dS + (int64_t)slot * a.H * a.P * NS;
+    const float* const Sp = a.S + (int64_t)slot * a.H * a.PS * NS;
+    const float* const dSp = a.dS + (int64_t)slot * a.H * a.PS * NS;
+    const uint32_t col_off = 4 * g * NS + min(n0 + i, NS - 1);
 
     BlockTile<T, PT, V, THREADS> tx(ldx, rows), ty(lddy, rows);
     StateCols S, dS;
@@ -105,15 +106,13 @@ __global__ void __launch_bounds__(THREADS) ssm_bwd_kernel(SsmArgs a) {
         ty.load(yp + col, P);
     };
     auto fetch_cols = [&](int h, int pt) {
-        const int64_t at = (int64_t)(h * a.P + pt * PT) * NS;
-        const int P = min(a.P - pt * PT, PT);
-        S.load(Sp + at, NS, P, n0, i, g);
-        dS.load(dSp + at, NS, P, n0, i, g);
+        const int64_t at = (int64_t)(h * a.PS + pt * PT) * NS;
+        S.load(Sp + at, NS, a.PS - pt * PT, col_off);
+        dS.load(dSp + at, NS, a.PS - pt * PT, col_off);
     };
     auto fetch_rows = [&](int h, int pt) {
-        const int64_t at = (int64_t)(h * a.P + pt * PT) * NS;
-        const int P = min(a.P - pt * PT, PT);
-        const uint32_t row = min(pw + i, P - 1) * NS;
+        const int64_t at = (int64_t)(h * a.PS + pt * PT) * NS;
+        const uint32_t row = min(pw + i, a.PS - pt * PT - 1) * NS;
 #pragma unroll
         for (int k = 0; k < NP / 16; ++k) dSr[k] = *reinterpret_cast<const f32x4*>(dSp + at + (row + (16 * k + 4 * g < NS ? 16 * k + 4 * g : 0)));
     };
@@ -133,8 +132,9 @@ __global__ void __launch_bounds__(THREADS) ssm_bwd_kernel(SsmArgs a) {
             raw = dtp[dt_off + min(h_first + 1, h_last - 1)];
         }
         // sums that no tile writes
-        for (int k = tid; k < 4 * TB; k += THREADS) (&L.R[0][0])[k] = 0.f;
-        for (int k = tid; k < 16 * TB; k += THREADS) (&L.K[0][0])[k] = 0.f;
+        for (int k = tid; k < 4 * TB; k += THREADS)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) { (&L.sums[s].R[0][0])[k] = 0.f; (&L.sums[s].K[0][0])[k] = 0.f; }
         tb.store(L.b, LN, rows, N);
         tc.store(L.c, LN, rows, N);
     }
@@ -154,12 +154,40 @@ __global__ void __launch_bounds__(THREADS) ssm_bwd_kernel(SsmArgs a) {
 #pragma unroll
     for (int j = 0; j < JT; ++j) { dB[j] = f32x4{}; dC[j] = f32x4{}; }
 
+    // The gradients of a head's step sizes from its row sums.  One wave, lane = row.
+    auto finish = [&](int h) {
+        const Steps& st = L.st[h & 1];
+        const typename Lds::Sums& s = L.sums[h & 1];
+        float R = (s.R[0][lane] + s.R[1][lane]) + (s.R[2][lane] + s.R[3][lane]), K = (s.K[0][lane] + s.K[1][lane]) + (s.K[2][lane] + s.K[3][lane]), KI = 0.f;
+#pragma unroll
+        for (int k = 0; k < WN; ++k) { R += s.RI[k][lane]; KI += s.KI[k][lane]; }
+        K += KI;
+        const int k = lane & (4 * WAVES - 1);
+        const float d = st.dt[lane], A = a.A[h], dot = lane == k ? s.dot[k] : 0.f, trace = lane == k ? s.trace[k] : 0.f;
+        // exp(a_T) <S, dS> + sum_s dt_s KI_s reach every row of the block: they stand behind its last one
+        const double behind = lane_sum(fma((double)__expf(st.total), (double)dot, (double)(d * KI)));
+        const double da = (double)R - (double)(d * K);
+        const double pre = lane_prefix(da);
+        const float suffix = (float)(last_lane(pre) - pre + da + behind);
+        float ddt = fmaf(A, suffix, K + s.diag[lane]);
+        if (a.softplus) ddt *= -expm1f(-d);                               // sigmoid(v) = 1 - exp(-softplus(v))
+        if (lane >= rows) ddt = 0.f;
+        if (lane < rows) static_cast<T*>(a.ddt)[(row0 + lane) * a.ldddt + h] = (T)ddt;
+        const float sA = lane_sum(d * suffix), sD = lane_sum(trace), sb = lane_sum(ddt);
+        if (lane == 0) {
+            float* p = a.part + ((int64_t)slot * a.H + h) * 3;
+            p[0] = sA;
+            p[1] = sD;
+            p[2] = sb;
+        }
+    };
     for (int h = h_first, pt = 0; h < h_last;) {
         // what comes next is loaded without asking whether there is more: the last one is loaded again, and nothing waits for it
         const bool tiles_left = pt + 1 < a.ptiles;
         const int hn = tiles_left ? h : min(h + 1, h_last - 1), ptn = tiles_left ? pt + 1 : h + 1 < h_last ? 0 : pt;
         const int p0 = pt * PT, P = min(a.P - p0, PT);
         const Steps& st = L.st[h & 1];
+        typename Lds::Sums& sums = L.sums[h & 1];
         tx.store(L.x, LX, rows, P);
         ty.store(L.y, LX, rows, P);
         __syncthreads();
@@ -197,16 +225,16 @@ __global__ void __launch_bounds__(THREADS) ssm_bwd_kernel(SsmArgs a) {
                     col += strict ? qv : 0.f;
                     rq[r] = strict ? qv * ds : 0.f;
                     if (js == jt && s == t + r) {
-                        L.diag[s] = pt ? L.diag[s] + qv : qv;
+                        sums.diag[s] = pt ? sums.diag[s] + qv : qv;
                         trace += G2[r];
                     }
                 }
-                float* K = &L.K[4 * jt + g][s];
-                *K = pt ? *K + col : col;
+                col = sum_g(col);
+                if (g == 0) sums.K[jt][s] = pt ? sums.K[jt][s] + col : col;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) rq[r] = sum16(rq[r]);
                 if (i == 0) {
-                    f32x4* R = reinterpret_cast<f32x4*>(&L.R[js][t]);
+                    f32x4* R = reinterpret_cast<f32x4*>(&sums.R[js][t]);
                     const f32x4 v = {rq[0], rq[1], rq[2], rq[3]};
                     *R = pt ? *R + v : v;
                 }
@@ -217,7 +245,8 @@ __global__ void __launch_bounds__(THREADS) ssm_bwd_kernel(SsmArgs a) {
         // dC_t += exp(a_t) S^T dy_t, dB_s += dt_s exp(a_T - a_s) dS^T x_s: lane i owns the row, four neighbouring columns n of it
         float dot = 0.f;
 #pragma unroll
-        for (int k = 0; k < PT / 4; ++k) dot += n0 + i < N && 16 * (k / 4) + 4 * g + k % 4 < P ? S.v[k] * dS.v[k] : 0.f;
+        for (int k = 0; k < PT / 4; ++k) dot = fmaf(S.v[k], dS.v[k], dot);
+        if (n0 + i >= N) dot = 0.f;
         {
             const Pieces<T> f(S.v);
 #pragma unroll
@@ -236,8 +265,9 @@ __global__ void __launch_bounds__(THREADS) ssm_bwd_kernel(SsmArgs a) {
                 float v = 0.f;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) v = fmaf(acc[r], (float)c[r], v);
-                float* RI = &L.RI[wave % WN * 4 + g][t + i];
-                *RI = pt ? *RI + v : v;
+                v = sum_g(v);
+                float* RI = &sums.RI[wave % WN][t + i];
+                if (g == 0) *RI = pt ? *RI + v : v;
             }
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -262,8 +292,9 @@ __global__ void __launch_bounds__(THREADS) ssm_bwd_kernel(SsmArgs a) {
                     dB[j][r] = fmaf(ds, acc[r], dB[j][r]);
                     v = fmaf(acc[r], (float)bv[r], v);
                 }
-                float* KI = &L.KI[wave % WN * 4 + g][s + i];
-                *KI = pt ? *KI + v : v;
+                v = sum_g(v);
+                float* KI = &sums.KI[wave % WN][s + i];
+                if (g == 0) *KI = pt ? *KI + v : v;
             }
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -273,12 +304,15 @@ __global__ void __launch_bounds__(THREADS) ssm_bwd_kernel(SsmArgs a) {
         trace = sum16(trace);
         if (i == 0) {
             const int k = 4 * wave + g;
-            L.dot[k] = pt ? L.dot[k] + dot : dot;
-            L.trace[k] = pt ? L.trace[k] + trace : trace;
+            sums.dot[k] = pt ? sums.dot[k] + dot : dot;
+            sums.trace[k] = pt ? sums.trace[k] + trace : trace;
         }
-        if (wave == WAVES - 1 && !tiles_left && h + 1 < h_last) {
-            steps(h + 1, raw);
-            raw = dtp[dt_off + min(h + 2, h_last - 1)];
+        if (wave == WAVES - 1 && pt == 0) {
+            if (h > h_first) finish(h - 1);                               // then its steps make room for the next head's
+            if (h + 1 < h_last) {
+                steps(h + 1, raw);
+                raw = dtp[dt_off + min(h + 2, h_last - 1)];
+            }
         }
         __syncthreads();
         // dx_s = dt_s (exp(a_T - a_s) dS B_s + sum_t G1 L dy_t) + D dy_s: lane i owns the row, four neighbouring columns p of it
@@ -294,10 +328,10 @@ __global__ void __launch_bounds__(THREADS) ssm_bwd_kernel(SsmArgs a) {
                     for (int e = 0; e < 8; ++e) sf[k][e] = (T)dSr[2 * k + (e >> 2)][e & 3];
                 }
             }
-            f32x4 acc[2];
+            f32x4 acc[JS];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int s = 16 * (js0 + 2 * j);
+            for (int j = 0; j < JS; ++j) {
+                const int s = 16 * (js0 + SS * j);
                 acc[j] = f32x4{};
 #pragma unroll
                 for (int k = 0; k < NK; ++k) acc[j] = M::mma(sf[k], M::row(L.b + s * LN + k * M::KS, LN, i, g), acc[j]);
@@ -309,12 +343,12 @@ __global__ void __launch_bounds__(THREADS) ssm_bwd_kernel(SsmArgs a) {
                 if (k >= rows || k + M::KS <= 16 * js0) continue;
                 const typename M::frag yf = M::col(L.y + k * LX + pw, LX, i, g);
 #pragma unroll
-                for (int j = 0; j < 2; ++j)
-                    if (k + M::KS > 16 * (js0 + 2 * j)) acc[j] = M::mma(yf, M::row(L.m + 16 * (js0 + 2 * j) * LM + k, LM, i, g), acc[j]);
+                for (int j = 0; j < JS; ++j)
+                    if (k + M::KS > 16 * (js0 + SS * j)) acc[j] = M::mma(yf, M::row(L.m + 16 * (js0 + SS * j) * LM + k, LM, i, g), acc[j]);
             }
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int s = 16 * (js0 + 2 * j) + i, p = pw + 4 * g;
+            for (int j = 0; j < JS; ++j) {
+                const int s = 16 * (js0 + SS * j) + i, p = pw + 4 * g;
                 if (s >= rows || p >= P) continue;
                 const float ds = st.dt[s];
                 const four_t yv = *reinterpret_cast<const four_t*>(L.y + s * LX + p);
@@ -331,39 +365,11 @@ __global__ void __launch_bounds__(THREADS) ssm_bwd_kernel(SsmArgs a) {
                 }
             }
         }
-        if (wave == 0 && !tiles_left) {                                   // lane = row
-            float R = 0.f, K = 0.f, KI = 0.f;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) R += L.R[k][lane];
-#pragma unroll
-            for (int k = 0; k < 16; ++k) K += L.K[k][lane];
-#pragma unroll
-            for (int k = 0; k < 4 * WN; ++k) { R += L.RI[k][lane]; KI += L.KI[k][lane]; }
-            K += KI;
-            const float d = st.dt[lane], A = a.A[h];
-            // exp(a_T) <S, dS> + sum_s dt_s KI_s reach every row of the block: they stand behind its last one
-            const int k = lane & (4 * WAVES - 1);
-            const float dot_k = lane == k ? L.dot[k] : 0.f, trace_k = lane == k ? L.trace[k] : 0.f;
-            const double behind = wave_sum(fma((double)__expf(st.total), (double)dot_k, (double)(d * KI)));
-            const double da = (double)R - (double)(d * K);
-            const double pre = wave_prefix(da, lane), all = __shfl(pre, 63, 64);
-            const float suffix = (float)(all - pre + da + behind);
-            float ddt = fmaf(A, suffix, K + L.diag[lane]);
-            if (a.softplus) ddt *= -expm1f(-d);                           // sigmoid(v) = 1 - exp(-softplus(v))
-            if (lane >= rows) ddt = 0.f;
-            if (lane < rows) static_cast<T*>(a.ddt)[(row0 + lane) * a.ldddt + h] = (T)ddt;
-            const float sA = wave_sum(d * suffix), sb = wave_sum(ddt), sD = wave_sum(trace_k);
-            if (lane == 0) {
-                float* p = a.part + ((int64_t)slot * a.H + h) * 3;
-                p[0] = sA;
-                p[1] = sD;
-                p[2] = sb;
-            }
-        }
         __syncthreads();
         pt = tiles_left ? pt + 1 : 0;
         h = tiles_left ? h : h + 1;
     }
+    if (wave == WAVES - 1) finish(h_last - 1);
     // dC_t += sum_s W[t,s] B_s, dB_s += sum_t W[t,s] C_t
 #pragma unroll
     for (int u = 0; u < GT; ++u) {
@@ -489,20 +495,22 @@ __global__ void __launch_bounds__(256) ssm_params_kernel(SsmArgs a) {
     }
 }
 
-template <typename T, int NP, int V>
+template <typename T, int NP, int V, int WAVES>
 int launch_bwd(const SsmArgs& a, hipStream_t s) {
-    constexpr size_t bytes = sizeof(BwdLds<T, NP>);
+    constexpr size_t bytes = sizeof(BwdLds<T, NP, WAVES>);
     static_assert(bytes <= 160 * 1024, "LDS of a workgroup");
     if (bytes > 64 * 1024) {
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(ssm_bwd_kernel<T, NP, V>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(ssm_bwd_kernel<T, NP, V, WAVES>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
         if (e != hipSuccess) { set_error("dc_ssm_scan_bwd: LDS", (int)e); return (int)e; }
     }
-    hipLaunchKernelGGL((ssm_bwd_kernel<T, NP, V>), dim3(a.cap, a.G, a.hsplit), dim3(THREADS), bytes, s, a);
+    hipLaunchKernelGGL((ssm_bwd_kernel<T, NP, V, WAVES>), dim3(a.cap, a.G, a.hsplit), dim3(64 * WAVES), bytes, s, a);
     return launch_check("dc_ssm_scan_bwd");
 }
+// Four waves where two workgroups fit a CU's LDS - they fill each other's waits -, else eight.
 template <typename T, int V>
 int launch_bwd_n(const SsmArgs& a, hipStream_t s) {
-    return a.N <= 32 ? launch_bwd<T, 32, V>(a, s) : a.N <= 64 ? launch_bwd<T, 64, V>(a, s) : launch_bwd<T, 128, V>(a, s);
+    constexpr int W64 = sizeof(T) == 4 ? 8 : 4;
+    return a.N <= 32 ? launch_bwd<T, 32, V, 4>(a, s) : a.N <= 64 ? launch_bwd<T, 64, V, W64>(a, s) : launch_bwd<T, 128, V, 8>(a, s);
 }
 
 bool bwd_vec(const SsmArgs& a, int type) {
@@ -521,6 +529,7 @@ int64_t bwd_plan(SsmArgs& a, char* scratch) {
     const int64_t cap = a.rows / TB + a.n_seq, blocks = (int64_t)a.n_seq * blocks_of(a.max_len);
     a.cap = (int)cap;
     a.NS = (a.N + 7) / 8 * 8;
+    a.PS = (a.P + 15) / 16 * 16;
     const int64_t have = (blocks < cap ? blocks : cap) * a.G;
     int64_t split = have > 0 ? BWD_WORKGROUPS / have : 1;
     if (split > a.H / a.G) split = a.H / a.G;
@@ -534,8 +543,8 @@ int64_t bwd_plan(SsmArgs& a, char* scratch) {
     a.base = reinterpret_cast<int32_t*>(take(4 * ((int64_t)a.n_seq + 1)));
     a.map = reinterpret_cast<int32_t*>(take(4 * cap));
     a.part = reinterpret_cast<float*>(take(12 * cap * a.H));
-    a.S = reinterpret_cast<float*>(take(4 * cap * a.H * a.P * a.NS));
-    a.dS = reinterpret_cast<float*>(take(4 * cap * a.H * a.P * a.NS));
+    a.S = reinterpret_cast<float*>(take(4 * cap * a.H * a.PS * a.NS));
+    a.dS = reinterpret_cast<float*>(take(4 * cap * a.H * a.PS * a.NS));
     if (a.nseg > 1) {
         const int64_t n = (int64_t)a.n_seq * a.nseg * a.H;
         a.seg_state = reinterpret_cast<float*>(take(4 * n * a.P * a.N));

@@ -26,7 +26,7 @@ struct SsmArgs {
     void* dx; int64_t lddx; void* ddt; int64_t ldddt; void* dB; int64_t lddb; void* dC; int64_t lddc;
     float* dA; float* dD; float* ddt_bias; float* dh0;
     int32_t* base; int32_t* map; int cap;       // first block slot of each sequence [n_seq + 1], sequence of each slot [cap]
-    float* S; float* dS; int NS;                // per slot and head [P][NS]: the state in front of the block, the gradient of the state behind it
+    float* S; float* dS; int NS, PS;            // per slot and head [PS][NS]: the state in front of the block, the gradient of the state behind it
     float* seg_dstate;
     float* part;                                // [cap][H][3]: sums for dA, dD, ddt_bias
     int hsplit; float* part_bc;                 // [hsplit][rows][G][2][N] where the heads of a group are shared out
@@ -177,26 +177,49 @@ struct BlockTile {
 // reads of 4 rows fall into different banks.
 template <typename T> constexpr int pitch(int W) { return W + 16 / (int)sizeof(T); }
 
+// Lane exchanges by DPP: rows are the sixteen lanes with the same g.
+template <int CTRL, int ROWS = 0xf> __device__ __forceinline__ float dpp(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, ROWS, 0xf, false));
+}
+template <int CTRL, int ROWS = 0xf> __device__ __forceinline__ double dpp(double v) {
+    const int hi = __builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, ROWS, 0xf, false), lo = __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, ROWS, 0xf, false);
+    return __hiloint2double(hi, lo);
+}
+constexpr int ROW_SHR = 0x110, ROW_ROR = 0x120, ROW_BCAST15 = 0x142, ROW_BCAST31 = 0x143, ROW_NEWBCAST = 0x150;
+
 // Sum over the sixteen lanes that share a row of D, in each of them.
 __device__ __forceinline__ float sum16(float v) {
-    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xf, 0xf, false));    // row_ror:8, 4, 2, 1
-    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x124, 0xf, 0xf, false));
-    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x122, 0xf, 0xf, false));
-    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x121, 0xf, 0xf, false));
+    v += dpp<ROW_ROR + 8>(v);
+    v += dpp<ROW_ROR + 4>(v);
+    v += dpp<ROW_ROR + 2>(v);
+    v += dpp<ROW_ROR + 1>(v);
     return v;
 }
+// Sum over g, the four lanes that share a column of D, in each of them.
+__device__ __forceinline__ float sum_g(float v) {
+    typedef unsigned pair __attribute__((ext_vector_type(2)));
+    pair p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+    p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(p[0]) + __uint_as_float(p[1]);
+}
+// Inclusive sum over the lanes, and what the last lane holds.
+template <typename F> __device__ __forceinline__ F lane_prefix(F v) {
+    v += dpp<ROW_SHR + 1>(v);
+    v += dpp<ROW_SHR + 2>(v);
+    v += dpp<ROW_SHR + 4>(v);
+    v += dpp<ROW_SHR + 8>(v);
+    v += dpp<ROW_BCAST15, 0xa>(v);
+    v += dpp<ROW_BCAST31, 0xc>(v);
+    return v;
+}
+__device__ __forceinline__ float last_lane(float v) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63)); }
+__device__ __forceinline__ double last_lane(double v) {
+    return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), 63), __builtin_amdgcn_readlane(__double2loint(v), 63));
+}
+template <typename F> __device__ __forceinline__ F lane_sum(F v) { return last_lane(lane_prefix(v)); }
 
 __device__ __forceinline__ float softplus_f(float v) { return v > 20.f ? v : log1pf(expf(v)); }
-
-// Inclusive sum over the lanes in f64.
-__device__ __forceinline__ double wave_prefix(double v, int lane) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const double u = __shfl_up(v, o, 64);
-        if (lane >= o) v += u;
-    }
-    return v;
-}
 
 // The block's step sizes and running sums (one wave, lane = row).  a is kept as hi + lo, so that exp(a_t - a_s) of neighbouring rows does not lose
 // what a long sum costs: a is summed in f64, the difference is taken of both halves.
@@ -219,18 +242,17 @@ __device__ __forceinline__ void make_steps(Steps& s, const SsmArgs& a, float raw
     float d = raw + bias;
     if (a.softplus) d = softplus_f(d);
     if (!live) d = 0.f;
-    const double sum = wave_prefix((double)d * (double)A, lane);
-    const double last = __shfl(sum, 63, 64);
+    const double sum = lane_prefix((double)d * (double)A), last = last_lane(sum);
     s.dt[lane] = d;
     s.hi[lane] = (float)sum;
     s.lo[lane] = (float)(sum - (double)(float)sum);
     const float es = __expf((float)(last - sum));
     s.w[lane] = REV ? __expf((float)sum) : d * es;
     if (FACTORS) {
-        const float cf = __expf((float)(__shfl(sum, lane | 15, 64) - sum));
+        const float cf = __expf((float)(dpp<ROW_NEWBCAST + 15>(sum) - sum));
         s.ea[lane] = __expf((float)sum);
         s.es[lane] = es;
-        s.rf[lane] = __expf((float)(sum - __shfl(sum, lane & 48, 64)));
+        s.rf[lane] = __expf((float)(sum - dpp<ROW_NEWBCAST>(sum)));
         s.cf[lane] = cf;
         s.cd[lane] = d * cf;
     }
