@@ -86,32 +86,40 @@ __global__ void __launch_bounds__(256, V > 1 && NP <= 64 ? (ROWS == 32 ? 4 : siz
         tc.template store<FULL>(L.c, LN, rows, all_n);
         __syncthreads();
         if (blk + 1 < last) fetch(blk + 1);
-        // M, as (C B^T)^T: lane i owns row t, four neighbouring s of it
+        // M, as (C B^T)^T: lane i owns row t, four neighbouring s of it.  64 rows: a wave takes a diagonal tile, one below, and one below or a zero
+        // one; 32 rows: 00, 11, 10 and the zero 01.
+        constexpr int TILES = ROWS == 64 ? 3 : 1;
+        int jt[TILES], js[TILES];
+        f32x4 m[TILES];
 #pragma unroll
-        for (int u = 0; u < (ROWS == 64 ? 3 : 1); ++u) {
-            // 64 rows: three tiles of the list a wave; 32 rows: 00, 11, 10 and the zero 01
-            const int jt = ROWS == 64 ? tile_row(wave + 4 * u) : (0x0110 >> (4 * wave)) & 15, js = ROWS == 64 ? tile_col(wave + 4 * u) : (0x1010 >> (4 * wave)) & 15;
-            if (!FULL && 16 * jt >= rows) continue;
-            f32x4 m = {};
-            if (js <= jt) {
+        for (int u = 0; u < TILES; ++u) {
+            jt[u] = ROWS == 64 ? tile_row(wave + 4 * u) : (0x0110 >> (4 * wave)) & 15;
+            js[u] = ROWS == 64 ? tile_col(wave + 4 * u) : (0x1010 >> (4 * wave)) & 15;
+            m[u] = f32x4{};
+        }
+        // (the zero tile's products are left out where they cost: f32)
+        const int real = sizeof(T) == 4 && TILES == 3 && wave >= 2 ? 2 : TILES;
 #pragma unroll
-                for (int k = 0; k < NK; ++k)
-                    m = M::mma(M::row(L.b + 16 * js * LN + k * M::KS, LN, i, g), M::row(L.c + 16 * jt * LN + k * M::KS, LN, i, g), m);
-                const int t = 16 * jt + i, s = 16 * js + 4 * g;
-                if (js < jt) {
-                    const float f = st.rf[t] * between(st, jt, js);
-                    const f32x4 cd = *reinterpret_cast<const f32x4*>(st.cd + s);
+        for (int k = 0; k < NK; ++k)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) m[r] *= f * cd[r];
-                } else {
-                    const float ht = st.hi[t], lt = st.lo[t];
-                    const f32x4 hs = *reinterpret_cast<const f32x4*>(st.hi + s), ls = *reinterpret_cast<const f32x4*>(st.lo + s),
-                                ds = *reinterpret_cast<const f32x4*>(st.dt + s);
+            for (int u = 0; u < TILES; ++u)
+                if (u < 2 || real == 3) m[u] = M::mma(M::row(L.b + 16 * js[u] * LN + k * M::KS, LN, i, g), M::row(L.c + 16 * jt[u] * LN + k * M::KS, LN, i, g), m[u]);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) m[r] = s + r <= t ? m[r] * (__expf((ht - hs[r]) + (lt - ls[r])) * ds[r]) : 0.f;
-                }
+        for (int u = 0; u < TILES; ++u) {
+            const int t = 16 * jt[u] + i, s = 16 * js[u] + 4 * g;
+            if (ROWS == 64 ? u == 0 : wave < 2) {
+                const float ht = st.hi[t], lt = st.lo[t];
+                const f32x4 hs = *reinterpret_cast<const f32x4*>(st.hi + s), ls = *reinterpret_cast<const f32x4*>(st.lo + s),
+                            ds = *reinterpret_cast<const f32x4*>(st.dt + s);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) m[u][r] = s + r <= t ? m[u][r] * (__expf((ht - hs[r]) + (lt - ls[r])) * ds[r]) : 0.f;
+            } else {
+                const float f = st.rf[t] * between(st, jt[u], js[u]);
+                const f32x4 cd = *reinterpret_cast<const f32x4*>(st.cd + s);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) m[u][r] = js[u] < jt[u] ? m[u][r] * (f * cd[r]) : 0.f;
             }
-            *reinterpret_cast<four_t*>(L.m + (16 * jt + i) * LM + 16 * js + 4 * g) = four<T>(m);
+            *reinterpret_cast<four_t*>(L.m + t * LM + s) = four<T>(m[u]);
         }
         if (wave == 3 && blk + 1 < last) {
             steps(blk + 1, raw);

@@ -140,16 +140,17 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ssm_bwd_kernel(SsmArgs a) {
     }
     __syncthreads();
     f32x4 G1[GT], W[GT], dB[JT], dC[JT];
+    int jt_of[GT], js_of[GT];                                             // its tiles of the triangle; where there is none, any
 #pragma unroll
     for (int u = 0; u < GT; ++u) {
+        const int w = min(wave + WAVES * u, 11);
+        jt_of[u] = tile_row(w);
+        js_of[u] = tile_col(w);
         G1[u] = f32x4{};
         W[u] = f32x4{};
-        const int w = wave + WAVES * u;
-        if (w < 10) {
 #pragma unroll
-            for (int k = 0; k < NK; ++k)
-                G1[u] = M::mma(M::row(L.c + 16 * tile_row(w) * LN + k * M::KS, LN, i, g), M::row(L.b + 16 * tile_col(w) * LN + k * M::KS, LN, i, g), G1[u]);
-        }
+        for (int k = 0; k < NK; ++k)
+            G1[u] = M::mma(M::row(L.c + 16 * jt_of[u] * LN + k * M::KS, LN, i, g), M::row(L.b + 16 * js_of[u] * LN + k * M::KS, LN, i, g), G1[u]);
     }
 #pragma unroll
     for (int j = 0; j < JT; ++j) { dB[j] = f32x4{}; dC[j] = f32x4{}; }
@@ -194,40 +195,52 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ssm_bwd_kernel(SsmArgs a) {
         fetch_xy(hn, ptn);
         // the rows with each other: lane i owns column s, four neighbouring rows t of it
         float trace = 0.f;
+        f32x4 G2[GT];
+#pragma unroll
+        for (int u = 0; u < GT; ++u) G2[u] = f32x4{};
+        // (the products of a tile that is not there are left out where they cost: f32)
+        const bool all_real = sizeof(T) == 2 || wave + WAVES * (GT - 1) < 10;
+#pragma unroll
+        for (int k = 0; k < PK; ++k)
+#pragma unroll
+            for (int u = 0; u < GT; ++u)
+                if (u + 1 < GT || all_real) G2[u] = M::mma(M::row(L.y + 16 * jt_of[u] * LX + k * M::KS, LX, i, g), M::row(L.x + 16 * js_of[u] * LX + k * M::KS, LX, i, g), G2[u]);
 #pragma unroll
         for (int u = 0; u < GT; ++u) {
-            const int w = wave + WAVES * u;
-            if (w >= 12) break;
-            const int jt = tile_row(w), js = tile_col(w), s = 16 * js + i, t = 16 * jt + 4 * g;
+            const int w = wave + WAVES * u, jt = jt_of[u], js = js_of[u], s = 16 * js + i, t = 16 * jt + 4 * g;
+            if (WAVES * (u + 1) > 12 && w >= 12) break;
             f32x4 m = {};
-            if (w < 10) {
-                f32x4 G2 = {}, l;
-#pragma unroll
-                for (int k = 0; k < PK; ++k) G2 = M::mma(M::row(L.y + 16 * jt * LX + k * M::KS, LX, i, g), M::row(L.x + 16 * js * LX + k * M::KS, LX, i, g), G2);
+            if (WAVES * (u + 1) <= 10 || w < 10) {
+                f32x4 l;
                 const float ds = st.dt[s];
-                if (js < jt) {
-                    const float f = between(st, jt, js) * st.cf[s];
-                    l = *reinterpret_cast<const f32x4*>(st.rf + t) * f;
-                } else {
+                float col = 0.f;
+                f32x4 rq;
+                if (u == 0 && (WAVES == 4 || w < 4)) {
                     const float hs = st.hi[s], ls = st.lo[s];
                     const f32x4 ht = *reinterpret_cast<const f32x4*>(st.hi + t), lt = *reinterpret_cast<const f32x4*>(st.lo + t);
+                    float diag = 0.f;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) l[r] = s <= t + r ? __expf((ht[r] - hs) + (lt[r] - ls)) : 0.f;
-                }
-                float col = 0.f, rq[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const bool in = js < jt || s <= t + r;               // a product that is not finite stays out of what it does not belong to
-                    const float gl = in ? G2[r] * l[r] : 0.f, qv = in ? G1[u][r] * gl : 0.f;
-                    m[r] = in ? G1[u][r] * l[r] : 0.f;
-                    W[u][r] = fmaf(gl, ds, W[u][r]);
-                    const bool strict = js < jt || s < t + r;
-                    col += strict ? qv : 0.f;
-                    rq[r] = strict ? qv * ds : 0.f;
-                    if (js == jt && s == t + r) {
-                        sums.diag[s] = pt ? sums.diag[s] + qv : qv;
-                        trace += G2[r];
+                    for (int r = 0; r < 4; ++r) {
+                        // a product that is not finite stays out of what it does not belong to
+                        const bool in = s <= t + r, strict = s < t + r;
+                        l[r] = in ? __expf((ht[r] - hs) + (lt[r] - ls)) : 0.f;
+                        const float gl = in ? G2[u][r] * l[r] : 0.f, qv = in ? G1[u][r] * gl : 0.f;
+                        m[r] = in ? G1[u][r] * l[r] : 0.f;
+                        W[u][r] = fmaf(gl, ds, W[u][r]);
+                        col += strict ? qv : 0.f;
+                        rq[r] = strict ? qv * ds : 0.f;
+                        diag += in && !strict ? qv : 0.f;
+                        trace += in && !strict ? G2[u][r] : 0.f;
                     }
+                    if ((i >> 2) == g) sums.diag[s] = pt ? sums.diag[s] + diag : diag;       // the lane whose rows hold s
+                } else {
+                    const float f = between(st, jt, js) * st.cf[s];
+                    l = *reinterpret_cast<const f32x4*>(st.rf + t) * f;
+                    m = G1[u] * l;
+                    const f32x4 gl = G2[u] * l, qv = G1[u] * gl;
+                    W[u] += gl * ds;
+                    col = (qv[0] + qv[1]) + (qv[2] + qv[3]);
+                    rq = qv * ds;
                 }
                 col = sum_g(col);
                 if (g == 0) sums.K[jt][s] = pt ? sums.K[jt][s] + col : col;
@@ -235,8 +248,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ssm_bwd_kernel(SsmArgs a) {
                 for (int r = 0; r < 4; ++r) rq[r] = sum16(rq[r]);
                 if (i == 0) {
                     f32x4* R = reinterpret_cast<f32x4*>(&sums.R[js][t]);
-                    const f32x4 v = {rq[0], rq[1], rq[2], rq[3]};
-                    *R = pt ? *R + v : v;
+                    *R = pt ? *R + rq : rq;
                 }
             }
             *reinterpret_cast<four_t*>(L.m + s * LM + t) = four<T>(m);

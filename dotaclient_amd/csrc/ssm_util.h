@@ -347,8 +347,8 @@ __device__ __forceinline__ void store_state(const f32x4 (&acc)[NP / 16], float* 
     }
 }
 
-// The 16 x 16 tiles (row tile, column tile) of a 64 x 64 triangle s <= t that products with it read: ten with s <= t, and two zero ones that complete the
-// 32-wide steps beside row tiles 0 and 2.
+// The 16 x 16 tiles (row tile, column tile) of a 64 x 64 triangle s <= t that products with it read: the four diagonal ones (0 .. 3), the six below them
+// (4 .. 9), and two zero ones (10, 11) that complete the 32-wide steps beside row tiles 0 and 2.
 __device__ __forceinline__ int tile_row(int u) { return (int)(0x203323213210ull >> (4 * u)) & 15; }
 __device__ __forceinline__ int tile_col(int u) { return (int)(0x310102103210ull >> (4 * u)) & 15; }
 
