@@ -67,7 +67,8 @@ template <> struct Pieces<bf16_t> {
     }
 };
 
-template <typename T, int NP, int V, int WAVES>
+// WIDE: a head of more than 64 columns takes several tiles of them; its sums then stay spread over the lanes until the last one.
+template <typename T, int NP, int V, int WAVES, bool WIDE>
 __global__ void __launch_bounds__(64 * WAVES, 2) ssm_bwd_kernel(SsmArgs a) {
     typedef Mat<T> M;
     typedef typename Four<T>::vec four_t;
@@ -155,6 +156,9 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ssm_bwd_kernel(SsmArgs a) {
 #pragma unroll
     for (int j = 0; j < JT; ++j) { dB[j] = f32x4{}; dC[j] = f32x4{}; }
 
+    // sums of a head over its column tiles, still spread over the lanes
+    f32x4 R[GT];
+    float K[GT], RI[JT], KI[JT], diag = 0.f, trace = 0.f, dot = 0.f;
     // The gradients of a head's step sizes from its row sums.  One wave, lane = row.
     auto finish = [&](int h) {
         const Steps& st = L.st[h & 1];
@@ -184,17 +188,30 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ssm_bwd_kernel(SsmArgs a) {
     };
     for (int h = h_first, pt = 0; h < h_last;) {
         // what comes next is loaded without asking whether there is more: the last one is loaded again, and nothing waits for it
-        const bool tiles_left = pt + 1 < a.ptiles;
+        const bool tiles_left = WIDE && pt + 1 < a.ptiles;
         const int hn = tiles_left ? h : min(h + 1, h_last - 1), ptn = tiles_left ? pt + 1 : h + 1 < h_last ? 0 : pt;
         const int p0 = pt * PT, P = min(a.P - p0, PT);
         const Steps& st = L.st[h & 1];
         typename Lds::Sums& sums = L.sums[h & 1];
+        // a head's row and column sums, over the lanes that share them
+        auto put_tile = [&](int u) {
+            if (wave + WAVES * u >= 10) return;
+            const float k = sum_g(K[u]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) R[u][r] = sum16(R[u][r]);
+            if (g == 0) sums.K[jt_of[u]][16 * js_of[u] + i] = k;
+            if (i == 0) *reinterpret_cast<f32x4*>(&sums.R[js_of[u]][16 * jt_of[u] + 4 * g]) = R[u];
+            if (u == 0 && wave < 4 && (i >> 2) == g) sums.diag[16 * js_of[0] + i] = diag;    // the lane whose rows hold s
+        };
+        auto put = [&](float (*to)[TB], float v, int j) {
+            v = sum_g(v);
+            if (g == 0) to[wave % WN][16 * (jt0 + WT * j) + i] = v;
+        };
         tx.store(L.x, LX, rows, P);
         ty.store(L.y, LX, rows, P);
         __syncthreads();
         fetch_xy(hn, ptn);
         // the rows with each other: lane i owns column s, four neighbouring rows t of it
-        float trace = 0.f;
         f32x4 G2[GT];
 #pragma unroll
         for (int u = 0; u < GT; ++u) G2[u] = f32x4{};
@@ -205,60 +222,53 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ssm_bwd_kernel(SsmArgs a) {
 #pragma unroll
             for (int u = 0; u < GT; ++u)
                 if (u + 1 < GT || all_real) G2[u] = M::mma(M::row(L.y + 16 * jt_of[u] * LX + k * M::KS, LX, i, g), M::row(L.x + 16 * js_of[u] * LX + k * M::KS, LX, i, g), G2[u]);
+        if (!WIDE || pt == 0) {
+#pragma unroll
+            for (int u = 0; u < GT; ++u) { R[u] = f32x4{}; K[u] = 0.f; }
+#pragma unroll
+            for (int k = 0; k < JT; ++k) { RI[k] = 0.f; KI[k] = 0.f; }
+            diag = trace = dot = 0.f;
+        }
 #pragma unroll
         for (int u = 0; u < GT; ++u) {
-            const int w = wave + WAVES * u, jt = jt_of[u], js = js_of[u], s = 16 * js + i, t = 16 * jt + 4 * g;
+            const int w = wave + WAVES * u, s = 16 * js_of[u] + i, t = 16 * jt_of[u] + 4 * g;
             if (WAVES * (u + 1) > 12 && w >= 12) break;
             f32x4 m = {};
             if (WAVES * (u + 1) <= 10 || w < 10) {
-                f32x4 l;
                 const float ds = st.dt[s];
-                float col = 0.f;
-                f32x4 rq;
                 if (u == 0 && (WAVES == 4 || w < 4)) {
                     const float hs = st.hi[s], ls = st.lo[s];
                     const f32x4 ht = *reinterpret_cast<const f32x4*>(st.hi + t), lt = *reinterpret_cast<const f32x4*>(st.lo + t);
-                    float diag = 0.f;
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         // a product that is not finite stays out of what it does not belong to
                         const bool in = s <= t + r, strict = s < t + r;
-                        l[r] = in ? __expf((ht[r] - hs) + (lt[r] - ls)) : 0.f;
-                        const float gl = in ? G2[u][r] * l[r] : 0.f, qv = in ? G1[u][r] * gl : 0.f;
-                        m[r] = in ? G1[u][r] * l[r] : 0.f;
+                        const float l = in ? __expf((ht[r] - hs) + (lt[r] - ls)) : 0.f, gl = in ? G2[u][r] * l : 0.f, qv = in ? G1[u][r] * gl : 0.f;
+                        m[r] = in ? G1[u][r] * l : 0.f;
                         W[u][r] = fmaf(gl, ds, W[u][r]);
-                        col += strict ? qv : 0.f;
-                        rq[r] = strict ? qv * ds : 0.f;
+                        K[u] += strict ? qv : 0.f;
+                        R[u][r] = fmaf(strict ? qv : 0.f, ds, R[u][r]);
                         diag += in && !strict ? qv : 0.f;
                         trace += in && !strict ? G2[u][r] : 0.f;
                     }
-                    if ((i >> 2) == g) sums.diag[s] = pt ? sums.diag[s] + diag : diag;       // the lane whose rows hold s
                 } else {
-                    const float f = between(st, jt, js) * st.cf[s];
-                    l = *reinterpret_cast<const f32x4*>(st.rf + t) * f;
+                    const f32x4 l = *reinterpret_cast<const f32x4*>(st.rf + t) * (between(st, jt_of[u], js_of[u]) * st.cf[s]);
                     m = G1[u] * l;
                     const f32x4 gl = G2[u] * l, qv = G1[u] * gl;
                     W[u] += gl * ds;
-                    col = (qv[0] + qv[1]) + (qv[2] + qv[3]);
-                    rq = qv * ds;
-                }
-                col = sum_g(col);
-                if (g == 0) sums.K[jt][s] = pt ? sums.K[jt][s] + col : col;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) rq[r] = sum16(rq[r]);
-                if (i == 0) {
-                    f32x4* R = reinterpret_cast<f32x4*>(&sums.R[js][t]);
-                    *R = pt ? *R + rq : rq;
+                    K[u] += (qv[0] + qv[1]) + (qv[2] + qv[3]);
+                    R[u] += qv * ds;
                 }
             }
             *reinterpret_cast<four_t*>(L.m + s * LM + t) = four<T>(m);
+            if (!WIDE) put_tile(u);
         }
         __builtin_amdgcn_sched_barrier(0);
         // dC_t += exp(a_t) S^T dy_t, dB_s += dt_s exp(a_T - a_s) dS^T x_s: lane i owns the row, four neighbouring columns n of it
-        float dot = 0.f;
+        if (jt0 == 0 && n0 + i < N) {                                     // the waves that share columns n hold the same S: one counts
 #pragma unroll
-        for (int k = 0; k < PT / 4; ++k) dot = fmaf(S.v[k], dS.v[k], dot);
-        if (n0 + i >= N) dot = 0.f;
+            for (int k = 0; k < PT / 4; ++k) dot = fmaf(S.v[k], dS.v[k], dot);
+        }
         {
             const Pieces<T> f(S.v);
 #pragma unroll
@@ -274,12 +284,9 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ssm_bwd_kernel(SsmArgs a) {
                 acc *= st.ea[t + i];
                 dC[j] += acc;
                 const four_t c = *reinterpret_cast<const four_t*>(L.c + (t + i) * LN + n0 + 4 * g);
-                float v = 0.f;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) v = fmaf(acc[r], (float)c[r], v);
-                v = sum_g(v);
-                float* RI = &sums.RI[wave % WN][t + i];
-                if (g == 0) *RI = pt ? *RI + v : v;
+                for (int r = 0; r < 4; ++r) RI[j] = fmaf(acc[r], (float)c[r], RI[j]);
+                if (!WIDE) put(sums.RI, RI[j], j);
             }
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -298,26 +305,31 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ssm_bwd_kernel(SsmArgs a) {
                 acc *= st.es[s + i];
                 const float ds = st.dt[s + i];
                 const four_t bv = *reinterpret_cast<const four_t*>(L.b + (s + i) * LN + n0 + 4 * g);
-                float v = 0.f;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     dB[j][r] = fmaf(ds, acc[r], dB[j][r]);
-                    v = fmaf(acc[r], (float)bv[r], v);
+                    KI[j] = fmaf(acc[r], (float)bv[r], KI[j]);
                 }
-                v = sum_g(v);
-                float* KI = &sums.KI[wave % WN][s + i];
-                if (g == 0) *KI = pt ? *KI + v : v;
+                if (!WIDE) put(sums.KI, KI[j], j);
             }
         }
         __builtin_amdgcn_sched_barrier(0);
         fetch_cols(hn, ptn);
-        // every row tile's columns n are counted once: the waves that share them hold the same S
-        dot = jt0 == 0 ? sum16(dot) : 0.f;
-        trace = sum16(trace);
-        if (i == 0) {
-            const int k = 4 * wave + g;
-            sums.dot[k] = pt ? sums.dot[k] + dot : dot;
-            sums.trace[k] = pt ? sums.trace[k] + trace : trace;
+        if (!tiles_left) {
+            if (WIDE) {
+#pragma unroll
+                for (int u = 0; u < GT; ++u) put_tile(u);
+#pragma unroll
+                for (int k = 0; k < JT; ++k) {
+                    put(sums.RI, RI[k], k);
+                    put(sums.KI, KI[k], k);
+                }
+            }
+            const float sdot = sum16(dot), strace = sum16(trace);
+            if (i == 0) {
+                sums.dot[4 * wave + g] = sdot;
+                sums.trace[4 * wave + g] = strace;
+            }
         }
         if (wave == WAVES - 1 && pt == 0) {
             if (h > h_first) finish(h - 1);                               // then its steps make room for the next head's
@@ -507,16 +519,22 @@ __global__ void __launch_bounds__(256) ssm_params_kernel(SsmArgs a) {
     }
 }
 
-template <typename T, int NP, int V, int WAVES>
-int launch_bwd(const SsmArgs& a, hipStream_t s) {
+template <typename T, int NP, int V, int WAVES, bool WIDE>
+int launch_bwd_wide(const SsmArgs& a, hipStream_t s) {
     constexpr size_t bytes = sizeof(BwdLds<T, NP, WAVES>);
     static_assert(bytes <= 160 * 1024, "LDS of a workgroup");
     if (bytes > 64 * 1024) {
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(ssm_bwd_kernel<T, NP, V, WAVES>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(ssm_bwd_kernel<T, NP, V, WAVES, WIDE>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
         if (e != hipSuccess) { set_error("dc_ssm_scan_bwd: LDS", (int)e); return (int)e; }
     }
-    hipLaunchKernelGGL((ssm_bwd_kernel<T, NP, V, WAVES>), dim3(a.cap, a.G, a.hsplit), dim3(64 * WAVES), bytes, s, a);
+    hipLaunchKernelGGL((ssm_bwd_kernel<T, NP, V, WAVES, WIDE>), dim3(a.cap, a.G, a.hsplit), dim3(64 * WAVES), bytes, s, a);
     return launch_check("dc_ssm_scan_bwd");
+}
+template <typename T, int NP, int V, int WAVES>
+int launch_bwd(const SsmArgs& a, hipStream_t s) {
+    if constexpr (V > 1)
+        if (a.ptiles == 1) return launch_bwd_wide<T, NP, V, WAVES, false>(a, s);
+    return launch_bwd_wide<T, NP, V, WAVES, true>(a, s);
 }
 // Four waves where two workgroups fit a CU's LDS - they fill each other's waits -, else eight.
 template <typename T, int V>
