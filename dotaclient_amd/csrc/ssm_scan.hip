@@ -243,7 +243,7 @@ __device__ __forceinline__ void states(const SsmArgs& a, StateLds<T, NP>& L) {
         if (wave == 3) raw = fetch_dt(block(0));
         fetch(block(0));
         if (wave == 3) {
-            make_steps<REV, false>(L.st[0], a, (float)raw, block(0) * TB + lane < q.len, A, bias, lane);
+            make_steps<REV, !REV && !FINAL>(L.st[0], a, (float)raw, block(0) * TB + lane < q.len, A, bias, lane);
             raw = fetch_dt(block(1));
         }
     }
@@ -261,6 +261,14 @@ __device__ __forceinline__ void states(const SsmArgs& a, StateLds<T, NP>& L) {
         }
         __syncthreads();
         if (more) fetch(block(j + 1));
+        if constexpr (!FINAL && !REV) {
+            // the step sizes and what is made of them: the backward kernel needs the same
+            if (wave == 2 && pbase == 0) {
+                float* to = a.steps + ((int64_t)(slot + blk) * a.H + h) * STEPS_KEPT + lane;
+#pragma unroll
+                for (int k = 0; k < STEPS_KEPT / TB; ++k) to[k * TB] = (&st.dt[0])[k * TB + lane];
+            }
+        }
         if constexpr (!FINAL) store_state<NP, 4>(S, (REV ? a.dS : a.S) + (((int64_t)(slot + blk) * a.H + h) * a.PS + pbase) * a.NS, a.NS, p0, a.PS - pbase, a.NS, i, g);
         const float et = __expf(st.total);
         sum += (double)st.total;
@@ -268,7 +276,7 @@ __device__ __forceinline__ void states(const SsmArgs& a, StateLds<T, NP>& L) {
         for (int c = 0; c < NP / 16; ++c) S[c] *= et;
         state_update<T, NP, TB>(S, L.x, LX, L.b, LN, st.w, p0, rows, i, g);
         if (wave == 3 && more) {
-            make_steps<REV, false>(L.st[(j + 1) & 1], a, (float)raw, block(j + 1) * TB + lane < q.len, A, bias, lane);
+            make_steps<REV, !REV && !FINAL>(L.st[(j + 1) & 1], a, (float)raw, block(j + 1) * TB + lane < q.len, A, bias, lane);
             raw = fetch_dt(block(j + 2));
         }
         __syncthreads();

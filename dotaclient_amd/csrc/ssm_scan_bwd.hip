@@ -15,7 +15,8 @@
 //   1. the ten 16 x 16 tiles of G2 with s <= t, shared out over the waves: W, Q's row and column sums, G1 L to LDS; S^T dy and dS^T x for the columns n
 //      that a wave owns, whose part of S and dS it alone reads - straight from memory into operands;
 //   2. dx for the columns p that a wave owns.
-// In the next head's phase 1 the last wave runs along the rows for d(a step), ddt and the sums for dA, dD, ddt_bias.  The next head's x, dy, S, dS are loaded as soon as this one's are used.  Operands that are f32 by nature are used as three bf16 pieces where an f32
+// In the next head's phase 1 a wave that has fewer tiles of G2 runs along the rows for d(a step), ddt and the sums for dA, dD, ddt_bias.  What is made of
+// the step sizes comes from the forward states' pass, which needs it too.  The next head's x, dy, S, dS are loaded as soon as this one's are used.  Operands that are f32 by nature are used as three bf16 pieces where an f32
 // result depends on them (S and dS: R, K -> dA, ddt_bias); W and G1 L, which only end in bf16 outputs, are rounded once, and dS in dx takes its
 // first piece.
 #include "ssm_util.h"
@@ -27,8 +28,11 @@ template <typename T, int NP, int WAVES>
 struct BwdLds {
     // how the waves share out the 16-column tiles of N and the four row tiles: WN x WT waves, JT row tiles each
     static constexpr int WN = NP / 16 < WAVES ? NP / 16 : WAVES, WT = WAVES / WN, JT = 4 / WT;
+    static_assert(2 * pitch<T>(PT) >= pitch<T>(NP), "C over x and dy");
     static_assert(NP / 16 <= WAVES, "a column tile of N for every wave at most");
-    T b[TB * pitch<T>(NP)], c[TB * pitch<T>(NP)], x[TB * pitch<T>(PT)], y[TB * pitch<T>(PT)], m[TB * pitch<T>(TB)];
+    // C is there before the first head and after the last one, where x and dy are not
+    union { struct { T x[TB * pitch<T>(PT)], y[TB * pitch<T>(PT)]; }; T c[TB * pitch<T>(NP)]; };
+    T b[TB * pitch<T>(NP)], m[TB * pitch<T>(TB)];
     Steps st[2];
     struct Sums { float R[4][TB], K[4][TB], RI[WN][TB], KI[WN][TB], diag[TB], dot[4 * WAVES], trace[4 * WAVES]; } sums[2];      // of one head
 };
@@ -75,6 +79,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ssm_bwd_kernel(SsmArgs a) {
     typedef BwdLds<T, NP, WAVES> Lds;
     constexpr int THREADS = 64 * WAVES;
     constexpr int LX = pitch<T>(PT), LN = pitch<T>(NP), LM = pitch<T>(TB), NK = NP / M::KS, PK = PT / M::KS, WN = Lds::WN, WT = Lds::WT, JT = Lds::JT;
+    constexpr bool EARLY = WAVES == 8;                                    // registers for the next head's x and dy all along
     constexpr int GT = (12 + WAVES - 1) / WAVES, JS = 16 / WAVES, SS = WAVES / 4;
     extern __shared__ __attribute__((aligned(16))) char lds_raw[];
     Lds& L = *reinterpret_cast<Lds*>(lds_raw);
@@ -84,15 +89,14 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ssm_bwd_kernel(SsmArgs a) {
     const SeqRange q = uniform_range(a, b);
     const int64_t row0 = q.off + (int64_t)blk * TB;
     const int rows = min(TB, q.len - blk * TB);
-    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), i = lane & 15, g = lane >> 4, N = a.N;
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), N = a.N;
+    int i = lane & 15, g = lane >> 4;
     const int n0 = 16 * (wave % WN), jt0 = wave / WN;                     // this wave's columns n; its row tiles jt0 + WT j
     const int pw = 16 * (wave & 3), js0 = wave >> 2;                      // its columns p and row tiles js0 + SS j of dx
     const int h_first = grp * Hg + share * Hg / a.hsplit, h_last = grp * Hg + (share + 1) * Hg / a.hsplit;
     const int ldx = (int)a.ldx, lddy = (int)a.lddy, lddx = (int)a.lddx, NS = a.NS;
     const T* const xp = static_cast<const T*>(a.x) + row0 * ldx;
     const T* const yp = static_cast<const T*>(a.dy) + row0 * lddy;
-    const T* const dtp = static_cast<const T*>(a.dt) + row0 * a.lddt;
-    const uint32_t dt_off = (uint32_t)min(lane, rows - 1) * (uint32_t)a.lddt;
     T* const dxp = static_cast<T*>(a.dx) + row0 * lddx;
     const float* const Sp = a.S + (int64_t)slot * a.H * a.PS * NS;
     const float* const dSp = a.dS + (int64_t)slot * a.H * a.PS * NS;
@@ -117,27 +121,32 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ssm_bwd_kernel(SsmArgs a) {
 #pragma unroll
         for (int k = 0; k < NP / 16; ++k) dSr[k] = *reinterpret_cast<const f32x4*>(dSp + at + (row + (16 * k + 4 * g < NS ? 16 * k + 4 * g : 0)));
     };
-    auto steps = [&](int h, T raw) {
-        make_steps<false, true>(L.st[h & 1], a, (float)raw, lane < rows, a.A[h], a.dt_bias ? a.dt_bias[h] : 0.f, lane);
+    constexpr int ST = (STEPS_KEPT + THREADS - 1) / THREADS;
+    float kept[ST];
+    auto fetch_steps = [&](int h) {
+        const float* p = a.steps + ((int64_t)slot * a.H + h) * STEPS_KEPT;
+#pragma unroll
+        for (int k = 0; k < ST; ++k) kept[k] = p[min(tid + k * THREADS, STEPS_KEPT - 1)];
     };
-    T raw = dtp[dt_off + h_first];
+    auto store_steps = [&](int h) {
+#pragma unroll
+        for (int k = 0; k < ST; ++k)
+            if (tid + k * THREADS < STEPS_KEPT) L.st[h & 1].dt[tid + k * THREADS] = kept[k];
+    };
     {
         BlockTile<T, NP, V, THREADS> tb((int)a.ldb, rows), tc((int)a.ldc, rows);
         tb.load(static_cast<const T*>(a.B) + row0 * a.ldb + (int64_t)grp * N, N);
         tc.load(static_cast<const T*>(a.C) + row0 * a.ldc + (int64_t)grp * N, N);
         fetch_xy(h_first, 0);
         fetch_cols(h_first, 0);
-        fetch_rows(h_first, 0);
-        if (wave == WAVES - 1) {
-            steps(h_first, raw);
-            raw = dtp[dt_off + min(h_first + 1, h_last - 1)];
-        }
+        fetch_steps(h_first);
         // sums that no tile writes
         for (int k = tid; k < 4 * TB; k += THREADS)
 #pragma unroll
             for (int s = 0; s < 2; ++s) { (&L.sums[s].R[0][0])[k] = 0.f; (&L.sums[s].K[0][0])[k] = 0.f; }
         tb.store(L.b, LN, rows, N);
         tc.store(L.c, LN, rows, N);
+        store_steps(h_first);
     }
     __syncthreads();
     f32x4 G1[GT], W[GT], dB[JT], dC[JT];
@@ -155,11 +164,15 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ssm_bwd_kernel(SsmArgs a) {
     }
 #pragma unroll
     for (int j = 0; j < JT; ++j) { dB[j] = f32x4{}; dC[j] = f32x4{}; }
+    four_t Cv[JT];                                                        // C of this wave's rows t (lane i) and columns n
+#pragma unroll
+    for (int j = 0; j < JT; ++j) Cv[j] = *reinterpret_cast<const four_t*>(L.c + (16 * (jt0 + WT * j) + i) * LN + n0 + 4 * g);
+    __syncthreads();
 
     // sums of a head over its column tiles, still spread over the lanes
     f32x4 R[GT];
     float K[GT], RI[JT], KI[JT], diag = 0.f, trace = 0.f, dot = 0.f;
-    // The gradients of a head's step sizes from its row sums.  One wave, lane = row.
+    // The gradients of a head's step sizes from its row L.  One wave, lane = row.
     auto finish = [&](int h) {
         const Steps& st = L.st[h & 1];
         const typename Lds::Sums& s = L.sums[h & 1];
@@ -170,7 +183,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ssm_bwd_kernel(SsmArgs a) {
         const int k = lane & (4 * WAVES - 1);
         const float d = st.dt[lane], A = a.A[h], dot = lane == k ? s.dot[k] : 0.f, trace = lane == k ? s.trace[k] : 0.f;
         // exp(a_T) <S, dS> + sum_s dt_s KI_s reach every row of the block: they stand behind its last one
-        const double behind = lane_sum(fma((double)__expf(st.total), (double)dot, (double)(d * KI)));
+        const double behind = lane_sum(fma((double)st.ea[TB - 1], (double)dot, (double)(d * KI)));
         const double da = (double)R - (double)(d * K);
         const double pre = lane_prefix(da);
         const float suffix = (float)(last_lane(pre) - pre + da + behind);
@@ -190,6 +203,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ssm_bwd_kernel(SsmArgs a) {
         // what comes next is loaded without asking whether there is more: the last one is loaded again, and nothing waits for it
         const bool tiles_left = WIDE && pt + 1 < a.ptiles;
         const int hn = tiles_left ? h : min(h + 1, h_last - 1), ptn = tiles_left ? pt + 1 : h + 1 < h_last ? 0 : pt;
+        asm volatile("" : "+v"(i), "+v"(g));
         const int p0 = pt * PT, P = min(a.P - p0, PT);
         const Steps& st = L.st[h & 1];
         typename Lds::Sums& sums = L.sums[h & 1];
@@ -210,7 +224,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ssm_bwd_kernel(SsmArgs a) {
         tx.store(L.x, LX, rows, P);
         ty.store(L.y, LX, rows, P);
         __syncthreads();
-        fetch_xy(hn, ptn);
+        fetch_steps(hn);
+        if (EARLY) fetch_xy(hn, ptn);
         // the rows with each other: lane i owns column s, four neighbouring rows t of it
         f32x4 G2[GT];
 #pragma unroll
@@ -218,10 +233,11 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ssm_bwd_kernel(SsmArgs a) {
         // (the products of a tile that is not there are left out where they cost: f32)
         const bool all_real = sizeof(T) == 2 || wave + WAVES * (GT - 1) < 10;
 #pragma unroll
-        for (int k = 0; k < PK; ++k)
+        for (int k = 0; k < PK; ++k) {
 #pragma unroll
             for (int u = 0; u < GT; ++u)
                 if (u + 1 < GT || all_real) G2[u] = M::mma(M::row(L.y + 16 * jt_of[u] * LX + k * M::KS, LX, i, g), M::row(L.x + 16 * js_of[u] * LX + k * M::KS, LX, i, g), G2[u]);
+        }
         if (!WIDE || pt == 0) {
 #pragma unroll
             for (int u = 0; u < GT; ++u) { R[u] = f32x4{}; K[u] = 0.f; }
@@ -283,13 +299,13 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ssm_bwd_kernel(SsmArgs a) {
                 }
                 acc *= st.ea[t + i];
                 dC[j] += acc;
-                const four_t c = *reinterpret_cast<const four_t*>(L.c + (t + i) * LN + n0 + 4 * g);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) RI[j] = fmaf(acc[r], (float)c[r], RI[j]);
+                for (int r = 0; r < 4; ++r) RI[j] = fmaf(acc[r], (float)Cv[j][r], RI[j]);
                 if (!WIDE) put(sums.RI, RI[j], j);
-            }
+                }
         }
         __builtin_amdgcn_sched_barrier(0);
+        fetch_rows(h, pt);
         {
             const Pieces<T> f(dS.v);
 #pragma unroll
@@ -311,9 +327,10 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ssm_bwd_kernel(SsmArgs a) {
                     KI[j] = fmaf(acc[r], (float)bv[r], KI[j]);
                 }
                 if (!WIDE) put(sums.KI, KI[j], j);
-            }
+                }
         }
         __builtin_amdgcn_sched_barrier(0);
+        if (!EARLY) fetch_xy(hn, ptn);
         fetch_cols(hn, ptn);
         if (!tiles_left) {
             if (WIDE) {
@@ -331,14 +348,9 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ssm_bwd_kernel(SsmArgs a) {
                 sums.trace[4 * wave + g] = strace;
             }
         }
-        if (wave == WAVES - 1 && pt == 0) {
-            if (h > h_first) finish(h - 1);                               // then its steps make room for the next head's
-            if (h + 1 < h_last) {
-                steps(h + 1, raw);
-                raw = dtp[dt_off + min(h + 2, h_last - 1)];
-            }
-        }
+        if (wave == 3 && pt == 0 && h > h_first) finish(h - 1);
         __syncthreads();
+        if (!tiles_left) store_steps(h + 1);                              // (the previous head's are finished with)
         // dx_s = dt_s (exp(a_T - a_s) dS B_s + sum_t G1 L dy_t) + D dy_s: lane i owns the row, four neighbouring columns p of it
         {
             const float D = a.D ? a.D[h] : 0.f;
@@ -360,8 +372,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ssm_bwd_kernel(SsmArgs a) {
 #pragma unroll
                 for (int k = 0; k < NK; ++k) acc[j] = M::mma(sf[k], M::row(L.b + s * LN + k * M::KS, LN, i, g), acc[j]);
                 acc[j] *= st.es[s + i];
-            }
-            fetch_rows(hn, ptn);
+                }
 #pragma unroll
             for (int k = 0; k < TB; k += M::KS) {
                 if (k >= rows || k + M::KS <= 16 * js0) continue;
@@ -369,7 +380,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ssm_bwd_kernel(SsmArgs a) {
 #pragma unroll
                 for (int j = 0; j < JS; ++j)
                     if (k + M::KS > 16 * (js0 + SS * j)) acc[j] = M::mma(yf, M::row(L.m + 16 * (js0 + SS * j) * LM + k, LM, i, g), acc[j]);
-            }
+                }
 #pragma unroll
             for (int j = 0; j < JS; ++j) {
                 const int s = 16 * (js0 + SS * j) + i, p = pw + 4 * g;
@@ -393,13 +404,18 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ssm_bwd_kernel(SsmArgs a) {
         pt = tiles_left ? pt + 1 : 0;
         h = tiles_left ? h : h + 1;
     }
-    if (wave == WAVES - 1) finish(h_last - 1);
+    if (wave == 3) finish(h_last - 1);
     // dC_t += sum_s W[t,s] B_s, dB_s += sum_t W[t,s] C_t
 #pragma unroll
     for (int u = 0; u < GT; ++u) {
         const int w = wave + WAVES * u;
         if (w >= 12) break;
         *reinterpret_cast<four_t*>(L.m + (16 * tile_col(w) + i) * LM + 16 * tile_row(w) + 4 * g) = four<T>(W[u]);
+    }
+    {
+        BlockTile<T, NP, V, THREADS> tc((int)a.ldc, rows);
+        tc.load(static_cast<const T*>(a.C) + row0 * a.ldc + (int64_t)grp * N, N);
+        tc.store(L.c, LN, rows, N);
     }
     __syncthreads();
 #pragma unroll
@@ -539,7 +555,7 @@ int launch_bwd(const SsmArgs& a, hipStream_t s) {
 // Four waves where two workgroups fit a CU's LDS - they fill each other's waits -, else eight.
 template <typename T, int V>
 int launch_bwd_n(const SsmArgs& a, hipStream_t s) {
-    constexpr int W64 = sizeof(T) == 4 ? 8 : 4;
+    constexpr int W64 = sizeof(T) == 4 ? 8 : 4;                          // f32 with four waves: 300 registers
     return a.N <= 32 ? launch_bwd<T, 32, V, 4>(a, s) : a.N <= 64 ? launch_bwd<T, 64, V, W64>(a, s) : launch_bwd<T, 128, V, 8>(a, s);
 }
 
@@ -573,6 +589,7 @@ int64_t bwd_plan(SsmArgs& a, char* scratch) {
     a.base = reinterpret_cast<int32_t*>(take(4 * ((int64_t)a.n_seq + 1)));
     a.map = reinterpret_cast<int32_t*>(take(4 * cap));
     a.part = reinterpret_cast<float*>(take(12 * cap * a.H));
+    a.steps = reinterpret_cast<float*>(take(4 * cap * a.H * STEPS_KEPT));
     a.S = reinterpret_cast<float*>(take(4 * cap * a.H * a.PS * a.NS));
     a.dS = reinterpret_cast<float*>(take(4 * cap * a.H * a.PS * a.NS));
     if (a.nseg > 1) {

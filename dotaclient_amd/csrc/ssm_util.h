@@ -25,6 +25,7 @@ struct SsmArgs {
     const void* dy; int64_t lddy; const float* dhT;
     void* dx; int64_t lddx; void* ddt; int64_t ldddt; void* dB; int64_t lddb; void* dC; int64_t lddc;
     float* dA; float* dD; float* ddt_bias; float* dh0;
+    float* steps;                               // [cap][H][STEPS_KEPT]
     int32_t* base; int32_t* map; int cap;       // first block slot of each sequence [n_seq + 1], sequence of each slot [cap]
     float* S; float* dS; int NS, PS;            // per slot and head [PS][NS]: the state in front of the block, the gradient of the state behind it
     float* seg_dstate;
@@ -224,11 +225,13 @@ __device__ __forceinline__ float softplus_f(float v) { return v > 20.f ? v : log
 // The block's step sizes and running sums (one wave, lane = row).  a is kept as hi + lo, so that exp(a_t - a_s) of neighbouring rows does not lose
 // what a long sum costs: a is summed in f64, the difference is taken of both halves.
 struct Steps {
-    float dt[TB], hi[TB], lo[TB], w[TB];
+    float dt[TB], hi[TB], lo[TB];
     float ea[TB], es[TB];                         // exp(a_t), exp(a_T - a_t)
-    float rf[TB], cf[TB], cd[TB];                 // exp(a_t - a of its tile of 16's first row), exp(a of its tile's last row - a_t), the same times dt_t
+    float rf[TB], cf[TB];                         // exp(a_t - a of its tile of 16's first row), exp(a of its tile's last row - a_t)
+    float w[TB], cd[TB];                          // see make_steps; dt_t cf_t
     float total;                                  // a of the last row
 };
+constexpr int STEPS_KEPT = 7 * TB;                // what the backward kernel takes over from the forward states' pass: dt .. cf
 // exp(a of row tile jt's first row - a of row tile js's last one), js < jt: with rf and cf the decay from s to t in three factors, none above 1 where
 // the decays are not.
 __device__ __forceinline__ float between(const Steps& s, int jt, int js) {
