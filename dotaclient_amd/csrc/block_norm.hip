@@ -13,7 +13,6 @@
 // are wave sums (through LDS where WPR > 1).  Backward's column sums stay in registers over a workgroup's rows and are joined in a fixed
 // order by a second kernel: no atomics.
 #include "op_util.h"
-#include <initializer_list>
 
 namespace dc {
 namespace {
@@ -41,16 +40,26 @@ __device__ __forceinline__ float row_sum(float v, float (*red)[WPR], int slot) {
     return v;
 }
 
-// Element e of lane l of a row's WPR * 64 lanes: vector e / V of that lane, column ((e / V) * lanes + l) * V + e % V.
+// Element e of lane l of a row's WPR * 64 lanes: vector e / V of that lane, column ((e / V) * lanes + l) * V + e % V.  Rows of any width and alignment:
+// what lies behind the row's end is 0, its last vector may be a part of one.
 template <typename T, int V, int LANES, int EPL>
 __device__ __forceinline__ void load_row(const T* __restrict__ p, int l, int D, float (&f)[EPL]) {
+    typename Loose<T, V>::vec v[EPL / V];
+#pragma unroll
+    for (int i = 0; i < EPL / V; ++i) {                    // whole vectors: those that are not are loaded from the row's start, and again below
+        const int c = (i * LANES + l) * V;
+        if (D >= V) v[i] = *reinterpret_cast<const typename Loose<T, V>::vec*>(p + (c + V <= D ? c : 0));
+    }
 #pragma unroll
     for (int i = 0; i < EPL / V; ++i) {
         const int c = (i * LANES + l) * V;
-        float t[V];
-        if (c < D) load_vec<T, V>(p + c, t);
 #pragma unroll
-        for (int e = 0; e < V; ++e) f[i * V + e] = c < D ? t[e] : 0.f;
+        for (int e = 0; e < V; ++e) f[i * V + e] = c + V <= D ? (float)v[i][e] : 0.f;
+        if (c < D && c + V > D) {
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                if (c + e < D) f[i * V + e] = (float)p[c + e];
+        }
     }
 }
 template <typename T, int V, int LANES, int EPL>
@@ -61,7 +70,7 @@ __device__ __forceinline__ void store_row(T* __restrict__ p, int l, int D, const
         float t[V];
 #pragma unroll
         for (int e = 0; e < V; ++e) t[e] = f[i * V + e];
-        if (c < D) store_vec<T, V>(p + c, t);
+        if (c < D) store_vec<T, V>(p + c, t, D - c);
     }
 }
 
@@ -223,18 +232,6 @@ __global__ void __launch_bounds__(1024) norm_reduce_kernel(const float* __restri
     }
 }
 
-// Four neighbouring elements per access (16 bytes of f32, 8 of bf16) where every row of every tensor starts on such a boundary.
-bool aligned_to(uintptr_t bytes, std::initializer_list<const void*> t) {
-    for (const void* p : t)
-        if (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) return false;
-    return true;
-}
-bool whole_fours(std::initializer_list<int64_t> lds) {
-    for (int64_t ld : lds)
-        if (ld % 4) return false;
-    return true;
-}
-
 // Waves per row and elements per lane: the fewest that hold the row; 16 elements per lane at most, so that backward's five rows stay in registers.
 #define NORM_SHAPES(KERNEL, T, R, V, GRID)                                                                                          \
     do {                                                                                                                            \
@@ -245,9 +242,9 @@ bool whole_fours(std::initializer_list<int64_t> lds) {
     } while (0)
 #define NORM_DISPATCH(KERNEL, GRID)                                                                                                 \
     do {                                                                                                                            \
-        if (type == 0) { if (vec) NORM_SHAPES(KERNEL, float, float, 4, GRID); else NORM_SHAPES(KERNEL, float, float, 1, GRID); }    \
-        else if (rtype == 0) { if (vec) NORM_SHAPES(KERNEL, bf16_t, float, 4, GRID); else NORM_SHAPES(KERNEL, bf16_t, float, 1, GRID); }   \
-        else { if (vec) NORM_SHAPES(KERNEL, bf16_t, bf16_t, 4, GRID); else NORM_SHAPES(KERNEL, bf16_t, bf16_t, 1, GRID); }          \
+        if (type == 0) NORM_SHAPES(KERNEL, float, float, 4, GRID);                                                                  \
+        else if (rtype == 0) NORM_SHAPES(KERNEL, bf16_t, float, 4, GRID);                                                           \
+        else NORM_SHAPES(KERNEL, bf16_t, bf16_t, 4, GRID);                                                                          \
     } while (0)
 
 int check_common(const char* what, const NormArgs& a, int type, int rtype) {
@@ -274,8 +271,6 @@ int block_norm_fwd(const void* y, int64_t ldy, const void* z, int64_t ldz, const
     if (int rc = check_common("dc_block_norm_fwd", a, type, rtype)) return rc;
     if (rows == 0) return 0;
     if (!r_out || (w_pre && !x_out)) { set_error("dc_block_norm_fwd", 1104); return 1104; }
-    const bool vec = aligned_to(type ? 8 : 16, {y, z, x_out}) && aligned_to(rtype ? 8 : 16, {r, r_out}) && aligned_to(16, {w_post, s, w_pre}) &&
-                     whole_fours({D, ldy, z ? ldz : 0, ldr, ldro, w_pre ? ldxo : 0});
 #define NORM_GRID(RPB) dim3((unsigned)((rows + RPB - 1) / RPB))
     NORM_DISPATCH(norm_fwd_kernel, NORM_GRID);
     return launch_check("dc_block_norm_fwd");
@@ -293,9 +288,7 @@ int block_norm_bwd(const void* dr, int64_t lddr, const void* dx, int64_t lddx, c
     if (!dw_post || (rows && (!dr || !dy || !dres || (z && !dz) || (w_pre && !dx)))) { set_error("dc_block_norm_bwd", 1104); return 1104; }
     if (scratch_bytes < block_norm_scratch(rows, D) || (rows && !scratch)) { set_error("dc_block_norm_bwd: scratch", 1105); return 1105; }
     if (rows) {
-        const bool vec = aligned_to(type ? 8 : 16, {y, z, dx, dy, dz}) && aligned_to(rtype ? 8 : 16, {r, dr, dres}) &&
-                         aligned_to(16, {w_post, s, w_pre, scratch}) && whole_fours({D, lddr, w_pre ? lddx : 0, ldy, z ? ldz : 0, ldr});
-#define NORM_BGRID(RPB) dim3((unsigned)a.n_blocks)
+    #define NORM_BGRID(RPB) dim3((unsigned)a.n_blocks)
         NORM_DISPATCH(norm_bwd_kernel, NORM_BGRID);
         if (int rc = launch_check("dc_block_norm_bwd")) return rc;
     }

@@ -12,7 +12,7 @@
 // loads are issued before the first use.  Backward recomputes v; the weights' gradients are summed per thread over its chunks of rows,
 // in LDS over a workgroup's chunks and, in a fixed order, by a second kernel over the workgroups: no atomics.
 #include "op_util.h"
-#include <initializer_list>
+#include <type_traits>
 
 namespace dc {
 namespace {
@@ -36,9 +36,9 @@ struct ConvArgs {
 template <typename T, int V>
 __device__ __forceinline__ void load_ext(const ConvArgs& a, const SeqRange& q, int b, int t, int d0, float (&f)[V]) {
     if (t >= 0 && t < q.len) {
-        load_vec<T, V>(static_cast<const T*>(a.x) + (q.off + t) * a.ldx + d0, f);
+        load_vec<T, V>(static_cast<const T*>(a.x) + (q.off + t) * a.ldx + d0, f, a.D - d0);
     } else if (t < 0 && t >= -(a.K - 1) && a.state) {
-        load_vec<T, V>(static_cast<const T*>(a.state) + ((int64_t)b * (a.K - 1) + (t + a.K - 1)) * a.D + d0, f);
+        load_vec<T, V>(static_cast<const T*>(a.state) + ((int64_t)b * (a.K - 1) + (t + a.K - 1)) * a.D + d0, f, a.D - d0);
     } else {
 #pragma unroll
         for (int i = 0; i < V; ++i) f[i] = 0.f;
@@ -54,9 +54,10 @@ template <int V, int KM>
 __device__ __forceinline__ void load_taps(const ConvArgs& a, int d0, float (&w)[KM][V], float (&bias)[V]) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        bias[i] = a.bias ? a.bias[d0 + i] : 0.f;
+        const int d = min(d0 + i, a.D - 1);
+        bias[i] = a.bias ? a.bias[d] : 0.f;
 #pragma unroll
-        for (int j = 0; j < KM; ++j) w[j][i] = has_tap<KM>(a, j) ? a.w[(int64_t)(d0 + i) * a.K + j - (KM - a.K)] : 0.f;
+        for (int j = 0; j < KM; ++j) w[j][i] = has_tap<KM>(a, j) ? a.w[(int64_t)d * a.K + j - (KM - a.K)] : 0.f;
     }
 }
 
@@ -73,6 +74,30 @@ __device__ __forceinline__ void taps(const ConvArgs& a, const float (&w)[KM][V],
         }
 }
 
+// Rows t0 - (KM-1) .. of ext, N of them, all loads on their way before the first is used: what is not there is loaded from a row that is and
+// becomes zero afterwards.  The sequence has a row at least.
+template <typename T, int V, int KM, int N, bool TAIL>
+__device__ __forceinline__ void load_rows(const ConvArgs& a, const SeqRange& q, int b, int t0, int d0, float (&f)[N][V]) {
+    const T* x = static_cast<const T*>(a.x) + q.off * a.ldx + d0;
+    typename Loose<T, V>::vec v[N];
+    bool ok[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int t = t0 - (KM - 1) + i;
+        const T* p = x + (int64_t)max(0, min(t, q.len - 1)) * a.ldx;
+        ok[i] = t < q.len;
+        if (i < KM - 1) {                                  // the rows in front of the chunk may be the state's
+            if (t < 0 && a.state) p = static_cast<const T*>(a.state) + ((int64_t)b * (a.K - 1) + max(t + a.K - 1, 0)) * a.D + d0;
+            ok[i] = ok[i] && (t >= 0 || (a.state && t >= -(a.K - 1)));
+        }
+        v[i] = load_raw<T, V, TAIL>(p, a.D - d0);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int e = 0; e < V; ++e) f[i][e] = ok[i] ? (float)v[i][e] : 0.f;
+}
+
 template <typename T, int V, int KM>
 __global__ void __launch_bounds__(256) conv_fwd_kernel(ConvArgs a) {
     const int d0 = (blockIdx.y * CLANES + (threadIdx.x & (CLANES - 1))) * V;
@@ -84,26 +109,29 @@ __global__ void __launch_bounds__(256) conv_fwd_kernel(ConvArgs a) {
         for (int j = 0; j < a.K - 1; ++j) {
             float f[V];
             load_ext<T, V>(a, q, b, q.len - (a.K - 1) + j, d0, f);
-            store_vec<T, V>(static_cast<T*>(a.state_out) + ((int64_t)b * (a.K - 1) + j) * a.D + d0, f);
+            store_vec<T, V>(static_cast<T*>(a.state_out) + ((int64_t)b * (a.K - 1) + j) * a.D + d0, f, a.D - d0);
         }
     }
     if (t0 >= q.len) return;
-    float ext[CROWS + KM - 1][V];
+    auto rows = [&](auto tail) {
+        constexpr bool TAIL = decltype(tail)::value;
+        float ext[CROWS + KM - 1][V], w[KM][V], bias[V];
+        load_rows<T, V, KM, CROWS + KM - 1, TAIL>(a, q, b, t0, d0, ext);
+        load_taps<V, KM>(a, d0, w, bias);
 #pragma unroll
-    for (int i = 0; i < CROWS + KM - 1; ++i) load_ext<T, V>(a, q, b, t0 - (KM - 1) + i, d0, ext[i]);
-    float w[KM][V], bias[V];
-    load_taps<V, KM>(a, d0, w, bias);
+        for (int r = 0; r < CROWS; ++r) {
+            if (t0 + r >= q.len) break;
+            float v[V];
+            taps<V, KM>(a, w, bias, ext, r, v);
+            if (a.silu) {
 #pragma unroll
-    for (int r = 0; r < CROWS; ++r) {
-        if (t0 + r >= q.len) break;
-        float v[V];
-        taps<V, KM>(a, w, bias, ext, r, v);
-        if (a.silu) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) v[i] *= sigmoid_fast(v[i]);
+                for (int i = 0; i < V; ++i) v[i] *= sigmoid_fast(v[i]);
+            }
+            store_vec<T, V>(static_cast<T*>(a.y) + (q.off + t0 + r) * a.ldy + d0, v, TAIL ? a.D - d0 : V);
         }
-        store_vec<T, V>(static_cast<T*>(a.y) + (q.off + t0 + r) * a.ldy + d0, v);
-    }
+    };
+    if (d0 + V <= a.D) rows(std::false_type{});
+    else rows(std::true_type{});
 }
 
 template <typename T, int V, int KM>
@@ -113,25 +141,30 @@ __global__ void __launch_bounds__(256) conv_bwd_kernel(ConvArgs a) {
     const bool live = d0 < a.D;
     float w[KM][V], bias[V], dw[KM][V] = {}, db[V] = {};
     if (live) load_taps<V, KM>(a, d0, w, bias);
-    for (int64_t c0 = (int64_t)blockIdx.x * CGROUPS; c0 < a.n_chunks; c0 += (int64_t)a.n_row_blocks * CGROUPS) {
-        const int64_t chunk = c0 + grp;
-        if (!live || chunk >= a.n_chunks) continue;
+    auto chunk_rows = [&](int64_t chunk, auto tail) {
+        constexpr bool TAIL = decltype(tail)::value;
+        const int valid = TAIL ? a.D - d0 : V;
         const int b = (int)(chunk / a.chunks_per_seq), t0 = (int)(chunk % a.chunks_per_seq) * CROWS;
         const SeqRange q = seq_range(a.seq_off, a.seq_len, b, a.rows, a.max_len);
-        if (t0 > 0 && t0 >= q.len) continue;
-        // rows t0-(KM-1) .. t0+CROWS+KM-2 of ext, dv of t0 .. t0+CROWS+KM-2
-        float ext[CROWS + 2 * (KM - 1)][V], dv[CROWS + KM - 1][V];
-#pragma unroll
-        for (int i = 0; i < CROWS + 2 * (KM - 1); ++i) load_ext<T, V>(a, q, b, t0 - (KM - 1) + i, d0, ext[i]);
-#pragma unroll
-        for (int i = 0; i < CROWS + KM - 1; ++i) {
-            if (t0 + i < q.len) {
-                load_vec<T, V>(static_cast<const T*>(a.dy) + (q.off + t0 + i) * a.lddy + d0, dv[i]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < V; ++e) dv[i][e] = 0.f;
+        if (q.len == 0 && t0 == 0 && a.dstate) {             // nothing between the state and what it became
+            for (int j = 0; j < a.K - 1; ++j) {
+                float g[V] = {};
+                if (a.dstate_out) load_vec<T, V>(static_cast<const T*>(a.dstate_out) + ((int64_t)b * (a.K - 1) + j) * a.D + d0, g, valid);
+                store_vec<T, V>(static_cast<T*>(a.dstate) + ((int64_t)b * (a.K - 1) + j) * a.D + d0, g, valid);
             }
         }
+        if (t0 >= q.len) return;
+        // rows t0-(KM-1) .. t0+CROWS+KM-2 of ext, dv of t0 .. t0+CROWS+KM-2
+        float ext[CROWS + 2 * (KM - 1)][V], dv[CROWS + KM - 1][V];
+        typename Loose<T, V>::vec raw[CROWS + KM - 1];
+        const T* dy = static_cast<const T*>(a.dy) + q.off * a.lddy + d0;
+#pragma unroll
+        for (int i = 0; i < CROWS + KM - 1; ++i) raw[i] = load_raw<T, V, TAIL>(dy + (int64_t)min(t0 + i, q.len - 1) * a.lddy, valid);
+        load_rows<T, V, KM, CROWS + 2 * (KM - 1), TAIL>(a, q, b, t0, d0, ext);
+#pragma unroll
+        for (int i = 0; i < CROWS + KM - 1; ++i)
+#pragma unroll
+            for (int e = 0; e < V; ++e) dv[i][e] = t0 + i < q.len ? (float)raw[i][e] : 0.f;
         if (a.silu) {
 #pragma unroll
             for (int i = 0; i < CROWS + KM - 1; ++i) {
@@ -171,7 +204,7 @@ __global__ void __launch_bounds__(256) conv_bwd_kernel(ConvArgs a) {
             const int j = t0 + t - q.len + a.K - 1;      // row of dstate_out
             if (a.dstate_out && j >= 0 && j < a.K - 1) {
                 float g[V];
-                load_vec<T, V>(static_cast<const T*>(a.dstate_out) + ((int64_t)b * (a.K - 1) + j) * a.D + d0, g);
+                load_vec<T, V>(static_cast<const T*>(a.dstate_out) + ((int64_t)b * (a.K - 1) + j) * a.D + d0, g, valid);
 #pragma unroll
                 for (int e = 0; e < V; ++e) f[e] += g[e];
             }
@@ -181,7 +214,7 @@ __global__ void __launch_bounds__(256) conv_bwd_kernel(ConvArgs a) {
             if (t0 + r < q.len) {
                 float f[V];
                 dext(r, f);
-                store_vec<T, V>(static_cast<T*>(a.dx) + (q.off + t0 + r) * a.lddx + d0, f);
+                store_vec<T, V>(static_cast<T*>(a.dx) + (q.off + t0 + r) * a.lddx + d0, f, valid);
             }
         }
         if (t0 == 0 && a.dstate) {
@@ -190,10 +223,16 @@ __global__ void __launch_bounds__(256) conv_bwd_kernel(ConvArgs a) {
                 if (r < a.K) {
                     float f[V];
                     dext(-r, f);
-                    store_vec<T, V>(static_cast<T*>(a.dstate) + ((int64_t)b * (a.K - 1) + (a.K - 1 - r)) * a.D + d0, f);
+                    store_vec<T, V>(static_cast<T*>(a.dstate) + ((int64_t)b * (a.K - 1) + (a.K - 1 - r)) * a.D + d0, f, valid);
                 }
             }
         }
+    };
+    for (int64_t c0 = (int64_t)blockIdx.x * CGROUPS; c0 < a.n_chunks; c0 += (int64_t)a.n_row_blocks * CGROUPS) {
+        const int64_t chunk = c0 + grp;
+        if (!live || chunk >= a.n_chunks) continue;
+        if (d0 + V <= a.D) chunk_rows(chunk, std::false_type{});
+        else chunk_rows(chunk, std::true_type{});
     }
     __shared__ float red[CGROUPS][CLANES * V];
     for (int j = 0; j <= KM; ++j) {                      // KM taps and the bias
@@ -240,7 +279,7 @@ __global__ void __launch_bounds__(256) conv_reduce_kernel(const float* __restric
 // One row per sequence: state (oldest first) and x -> y, state moved up by one row.  state_out may be state.
 template <typename T, int V, int KM>
 __global__ void __launch_bounds__(256) conv_step_kernel(ConvArgs a) {
-    const int nv = a.D / V;
+    const int nv = (a.D + V - 1) / V;
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= (int64_t)a.n_seq * nv) return;
     const int b = (int)(i / nv), d0 = (int)(i % nv) * V;
@@ -254,20 +293,14 @@ __global__ void __launch_bounds__(256) conv_step_kernel(ConvArgs a) {
 #pragma unroll
         for (int e = 0; e < V; ++e) v[e] *= sigmoid_fast(v[e]);
     }
-    store_vec<T, V>(static_cast<T*>(a.y) + b * a.ldy + d0, v);
+    store_vec<T, V>(static_cast<T*>(a.y) + b * a.ldy + d0, v, a.D - d0);
 #pragma unroll
     for (int j = 1; j < KM; ++j)
-        if (j >= KM - a.K + 1) store_vec<T, V>(static_cast<T*>(a.state_out) + ((int64_t)b * (a.K - 1) + (j - (KM - a.K) - 1)) * a.D + d0, ext[j]);
+        if (j >= KM - a.K + 1) store_vec<T, V>(static_cast<T*>(a.state_out) + ((int64_t)b * (a.K - 1) + (j - (KM - a.K) - 1)) * a.D + d0, ext[j], a.D - d0);
 }
 
-// Four channels per thread (16 bytes of f32, 8 of bf16) where every row of every tensor starts on such a boundary, else one.  (Eight bf16
-// channels would be 16 bytes too, but the backward kernel's rows then take 256 registers.)
-bool vector_rows(int type, int D, int64_t ldx, int64_t ldy, int64_t lddx, std::initializer_list<const void*> tensors) {
-    const uintptr_t mask = type ? 7 : 15;
-    for (const void* p : tensors)
-        if (reinterpret_cast<uintptr_t>(p) & mask) return false;
-    return D % 4 == 0 && ldx % 4 == 0 && ldy % 4 == 0 && lddx % 4 == 0;
-}
+// Four channels per thread: 16 bytes of f32, 8 of bf16.  (Eight bf16 channels would be 16 bytes too, but the backward kernel's rows then take 256 registers.)
+constexpr int CV = 4;
 
 #define CONV_LAUNCH(KERNEL, GRID, T, V)                                                                    \
     do {                                                                                                   \
@@ -278,10 +311,8 @@ bool vector_rows(int type, int D, int64_t ldx, int64_t ldy, int64_t lddx, std::i
     } while (0)
 #define CONV_DISPATCH(KERNEL, GRID)                                                                        \
     do {                                                                                                   \
-        if (type == 0 && vec) CONV_LAUNCH(KERNEL, GRID, float, 4);                                         \
-        else if (type == 0) CONV_LAUNCH(KERNEL, GRID, float, 1);                                           \
-        else if (vec) CONV_LAUNCH(KERNEL, GRID, bf16_t, 4);                                                \
-        else CONV_LAUNCH(KERNEL, GRID, bf16_t, 1);                                                         \
+        if (type == 0) CONV_LAUNCH(KERNEL, GRID, float, CV);                                               \
+        else CONV_LAUNCH(KERNEL, GRID, bf16_t, CV);                                                        \
     } while (0)
 
 // Chunks of rows of a sequence, one at least: it also writes the state.
@@ -312,7 +343,6 @@ int causal_conv_fwd(const void* x, int64_t ldx, const float* w, const float* bia
     if (n_seq == 0) return 0;
     a.chunks_per_seq = chunks_in(max_len);
     a.n_chunks = (int64_t)n_seq * a.chunks_per_seq;
-    const bool vec = vector_rows(type, D, ldx, ldy, 0, {x, y, state, state_out});
     const int64_t gx = (a.n_chunks + CGROUPS - 1) / CGROUPS;
     if (gx > 0x7fffffff) { set_error("dc_causal_conv_fwd", 1103); return 1103; }
 #define CONV_GRID(V) dim3((unsigned)gx, (D + CLANES * V - 1) / (CLANES * V))
@@ -337,8 +367,7 @@ int causal_conv_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, co
     if (!dw) { set_error("dc_causal_conv_bwd", 1104); return 1104; }
     a.chunks_per_seq = chunks_in(max_len);
     a.n_chunks = (int64_t)n_seq * a.chunks_per_seq;
-    const bool vec = vector_rows(type, D, ldx, lddy, lddx, {x, dy, state, dstate_out, dx, dstate});
-    const int lanes = CLANES * (vec ? 4 : 1), groups = (D + lanes - 1) / lanes;
+    const int lanes = CLANES * CV, groups = (D + lanes - 1) / lanes;
     a.n_row_blocks = row_blocks(a.n_chunks, groups);
     if (scratch_bytes < (int64_t)a.n_row_blocks * (K + 1) * D * (int64_t)sizeof(float) || (!scratch && a.n_row_blocks)) {
         set_error("dc_causal_conv_bwd: scratch", 1105);
@@ -362,8 +391,7 @@ int causal_conv_step(const void* x, int64_t ldx, const void* state, const float*
     if (int rc = check_common("dc_causal_conv_step", a, type)) return rc;
     if (n_seq == 0) return 0;
     if (!y || !state_out) { set_error("dc_causal_conv_step", 1104); return 1104; }
-    const bool vec = vector_rows(type, D, ldx, ldy, 0, {x, y, state, state_out});
-#define CONV_SGRID(V) dim3((unsigned)(((int64_t)n_seq * (D / V) + 255) / 256))
+#define CONV_SGRID(V) dim3((unsigned)(((int64_t)n_seq * ((D + V - 1) / V) + 255) / 256))
     CONV_DISPATCH(conv_step_kernel, CONV_SGRID);
     return launch_check("dc_causal_conv_step");
 }

@@ -5,7 +5,8 @@
 //
 // Bound by HBM: the gradients are read for the norm and, scaled, once more (from the last-level cache as far as they fit) and written.
 // The tensors' addresses travel in the kernels' arguments, TENSORS per launch: no table in device memory, so a captured graph is whole.
-// A workgroup sums one chunk in f64 and writes its sum to its own place; one workgroup joins them in order: no atomics.
+// A workgroup sums one chunk in f64 and writes its sum to its own place; the sums are joined in order: no atomics.  Up to FEW chunks (2 MB
+// of gradients or so) every workgroup of the second kernel adds all of them up itself: two launches instead of three, where the launches are the time.
 #include "op_util.h"
 
 namespace dc {
@@ -13,6 +14,7 @@ namespace {
 
 constexpr int TENSORS = 128;              // 28 bytes of kernel arguments each, 4 KB are the limit
 constexpr int CHUNK = 16384;              // elements per workgroup
+constexpr int FEW = 1024;                 // chunks
 
 struct ClipTable {
     const void* g[TENSORS];
@@ -35,15 +37,25 @@ __device__ __forceinline__ int find_tensor(const ClipTable& t, int chunk) {     
 
 template <typename T, int V>
 __device__ __forceinline__ double chunk_squares(const T* g, int64_t at, int n) {
-    double s = 0.0;
+    double sum[4] = {};                   // four chains of additions
     const int nv = n / V;
-#pragma unroll 4
-    for (int i = threadIdx.x; i < nv; i += 256) {
+    int i = threadIdx.x;
+    for (; i + 3 * 256 < nv; i += 4 * 256) {
+        typename Loose<T, V>::vec v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = load_raw<T, V, false>(g + at + (int64_t)(i + k * 256) * V, V);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int e = 0; e < V; ++e) sum[k] = fma((double)(float)v[k][e], (double)(float)v[k][e], sum[k]);
+    }
+    for (; i < nv; i += 256) {
         float v[V];
         load_vec<T, V>(g + at + (int64_t)i * V, v);
 #pragma unroll
-        for (int e = 0; e < V; ++e) s = fma((double)v[e], (double)v[e], s);
+        for (int e = 0; e < V; ++e) sum[e % 4] = fma((double)v[e], (double)v[e], sum[e % 4]);
     }
+    double s = (sum[0] + sum[1]) + (sum[2] + sum[3]);
     for (int i = nv * V + threadIdx.x; i < n; i += 256) {
         const double v = (double)(float)g[at + i];
         s = fma(v, v, s);
@@ -55,10 +67,8 @@ __global__ void __launch_bounds__(256) clip_squares_kernel(ClipTable t, double* 
     const int i = find_tensor(t, blockIdx.x);
     const int64_t at = (int64_t)(blockIdx.x - t.chunk0[i]) * CHUNK;
     const int n = (int)(t.n[i] - at < CHUNK ? t.n[i] - at : CHUNK);
-    const bool bf = (t.bf16[i / 32] >> (i % 32)) & 1, al = (reinterpret_cast<uintptr_t>(t.g[i]) & 15) == 0;
-    double s;
-    if (bf) s = al ? chunk_squares<bf16_t, 8>(static_cast<const bf16_t*>(t.g[i]), at, n) : chunk_squares<bf16_t, 1>(static_cast<const bf16_t*>(t.g[i]), at, n);
-    else s = al ? chunk_squares<float, 4>(static_cast<const float*>(t.g[i]), at, n) : chunk_squares<float, 1>(static_cast<const float*>(t.g[i]), at, n);
+    const bool bf = (t.bf16[i / 32] >> (i % 32)) & 1;
+    double s = bf ? chunk_squares<bf16_t, 8>(static_cast<const bf16_t*>(t.g[i]), at, n) : chunk_squares<float, 4>(static_cast<const float*>(t.g[i]), at, n);
     s = wave_sum(s);
     __shared__ double red[4];
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
@@ -107,23 +117,26 @@ __device__ __forceinline__ void chunk_scale(const T* g, T* out, int64_t at, int 
     for (int i = nv * V + threadIdx.x; i < n; i += 256) out[at + i] = (T)((float)g[at + i] * c);
 }
 
-__global__ void __launch_bounds__(256) clip_scale_kernel(ClipTable t, const double* __restrict__ sq, int n_all, float max_norm, float* __restrict__ total) {
+// FUSED: sq holds the n_all chunks' sums, of one table; workgroup i also writes the norm of tensor i.
+template <bool FUSED>
+__global__ void __launch_bounds__(256) clip_scale_kernel(ClipTable t, const double* __restrict__ sq, int n_all, float max_norm, float* __restrict__ total,
+                                                         float* __restrict__ norms) {
     const double norm = total_norm(sq, n_all);
     if (total && blockIdx.x == 0 && threadIdx.x == 0) *total = (float)norm;
+    if (FUSED && (int)blockIdx.x < t.count && threadIdx.x < 64) {
+        double s = 0.0;
+        for (int c = t.chunk0[blockIdx.x] + threadIdx.x; c < t.chunk0[blockIdx.x + 1]; c += 64) s += sq[c];
+        s = wave_sum(s);
+        if (threadIdx.x == 0) norms[blockIdx.x] = (float)sqrt(s);
+    }
     const double want = (double)max_norm / (norm + 1e-6);
     const float c = norm <= 1.7976931348623157e308 && want < 1.0 ? (float)want : 1.f;
     const int i = find_tensor(t, blockIdx.x);
-    if (blockIdx.x >= t.chunk0[t.count] || (c == 1.f && t.out[i] == t.g[i])) return;
+    if ((int)blockIdx.x >= t.chunk0[t.count] || (c == 1.f && t.out[i] == t.g[i])) return;
     const int64_t at = (int64_t)(blockIdx.x - t.chunk0[i]) * CHUNK;
     const int n = (int)(t.n[i] - at < CHUNK ? t.n[i] - at : CHUNK);
-    const bool bf = (t.bf16[i / 32] >> (i % 32)) & 1, al = ((reinterpret_cast<uintptr_t>(t.g[i]) | reinterpret_cast<uintptr_t>(t.out[i])) & 15) == 0;
-    if (bf) {
-        const bf16_t* g = static_cast<const bf16_t*>(t.g[i]); bf16_t* o = static_cast<bf16_t*>(t.out[i]);
-        if (al) chunk_scale<bf16_t, 8>(g, o, at, n, c); else chunk_scale<bf16_t, 1>(g, o, at, n, c);
-    } else {
-        const float* g = static_cast<const float*>(t.g[i]); float* o = static_cast<float*>(t.out[i]);
-        if (al) chunk_scale<float, 4>(g, o, at, n, c); else chunk_scale<float, 1>(g, o, at, n, c);
-    }
+    if ((t.bf16[i / 32] >> (i % 32)) & 1) chunk_scale<bf16_t, 8>(static_cast<const bf16_t*>(t.g[i]), static_cast<bf16_t*>(t.out[i]), at, n, c);
+    else chunk_scale<float, 4>(static_cast<const float*>(t.g[i]), static_cast<float*>(t.out[i]), at, n, c);
 }
 
 int64_t chunks_of(int64_t n) { return (n + CHUNK - 1) / CHUNK; }
@@ -148,30 +161,43 @@ int grad_norm_clip(const int64_t* grads, const int64_t* outs, const int64_t* siz
     if (scratch_bytes < grad_norm_clip_scratch(sizes, n)) { set_error("dc_grad_norm_clip: scratch", 1105); return 1105; }
     double* sq = scratch;                    // [n], then the chunks' sums
     double* part = scratch + n;
-    for (int pass = 0; pass < 2; ++pass) {
-        int64_t chunk0 = 0;
-        for (int first = 0; first < n; first += TENSORS) {
-            ClipTable t = {};
-            NormTable nt = {};
-            t.count = n - first < TENSORS ? n - first : TENSORS;
-            for (int i = 0; i < t.count; ++i) {
-                const int j = first + i;
-                t.g[i] = reinterpret_cast<const void*>(grads[j]); t.out[i] = reinterpret_cast<void*>(outs[j]); t.n[i] = sizes[j];
-                if (types[j]) t.bf16[i / 32] |= 1u << (i % 32);
-                t.chunk0[i + 1] = t.chunk0[i] + (int32_t)chunks_of(sizes[j]);
-            }
-            const int chunks = t.chunk0[t.count];
-            for (int i = 0; i <= t.count; ++i) nt.chunk0[i] = t.chunk0[i];
-            nt.count = t.count;
-            if (pass == 0) {
-                if (chunks) hipLaunchKernelGGL(clip_squares_kernel, dim3(chunks), dim3(256), 0, s, t, part + chunk0);
-                hipLaunchKernelGGL(clip_norms_kernel, dim3((t.count + 3) / 4), dim3(256), 0, s, nt, part + chunk0, sq + first, norms + first);
-            } else if (chunks || first == 0) {
-                hipLaunchKernelGGL(clip_scale_kernel, dim3(chunks ? chunks : 1), dim3(256), 0, s, t, sq, n, max_norm, first == 0 ? total : nullptr);
-            }
-            if (int rc = launch_check("dc_grad_norm_clip")) return rc;
-            chunk0 += chunks;
+    auto fill = [&](int first, ClipTable& t) {
+        t.count = n - first < TENSORS ? n - first : TENSORS;
+        t.chunk0[0] = 0;
+        for (int k = 0; k < (TENSORS + 31) / 32; ++k) t.bf16[k] = 0;
+        for (int i = 0; i < t.count; ++i) {
+            const int j = first + i;
+            t.g[i] = reinterpret_cast<const void*>(grads[j]); t.out[i] = reinterpret_cast<void*>(outs[j]); t.n[i] = sizes[j];
+            if (types[j]) t.bf16[i / 32] |= 1u << (i % 32);
+            t.chunk0[i + 1] = t.chunk0[i] + (int32_t)chunks_of(sizes[j]);
         }
+        return t.chunk0[t.count];
+    };
+    ClipTable t;
+    if (n <= TENSORS) {
+        const int chunks = fill(0, t);
+        if (chunks <= FEW) {
+            if (chunks) hipLaunchKernelGGL(clip_squares_kernel, dim3(chunks), dim3(256), 0, s, t, part);
+            hipLaunchKernelGGL(clip_scale_kernel<true>, dim3(chunks > n ? chunks : n), dim3(256), 0, s, t, part, chunks, max_norm, total, norms);
+            return launch_check("dc_grad_norm_clip");
+        }
+    }
+    int64_t chunk0 = 0;
+    for (int first = 0; first < n; first += TENSORS) {
+        const int chunks = fill(first, t);
+        NormTable nt;
+        for (int i = 0; i <= t.count; ++i) nt.chunk0[i] = t.chunk0[i];
+        nt.count = t.count;
+        if (chunks) hipLaunchKernelGGL(clip_squares_kernel, dim3(chunks), dim3(256), 0, s, t, part + chunk0);
+        hipLaunchKernelGGL(clip_norms_kernel, dim3((t.count + 3) / 4), dim3(256), 0, s, nt, part + chunk0, sq + first, norms + first);
+        if (int rc = launch_check("dc_grad_norm_clip")) return rc;
+        chunk0 += chunks;
+    }
+    for (int first = 0; first < n; first += TENSORS) {
+        const int chunks = fill(first, t);
+        if (chunks || first == 0)
+            hipLaunchKernelGGL(clip_scale_kernel<false>, dim3(chunks ? chunks : 1), dim3(256), 0, s, t, sq, n, max_norm, first == 0 ? total : nullptr, nullptr);
+        if (int rc = launch_check("dc_grad_norm_clip")) return rc;
     }
     return 0;
 }

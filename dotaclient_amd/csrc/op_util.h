@@ -6,30 +6,51 @@ namespace dc {
 
 typedef __bf16 bf16_t;
 
-// V consecutive elements of T as floats.  V > 1 needs the address aligned to V * sizeof(T) (16 bytes for the widths used here).
+// V consecutive elements of T as floats, in one access wherever they lie (global memory takes accesses off their size's boundary; a row of an odd number
+// of elements, or a column slice, starts at any element).  The last vector of a row may hold fewer than V elements of it: `valid` of them are
+// accessed then, one by one, and the others read as 0.
+template <typename T, int V> struct Loose { typedef T vec __attribute__((ext_vector_type(V), aligned(sizeof(T)))); };
 template <typename T, int V>
-__device__ __forceinline__ void load_vec(const T* __restrict__ p, float (&f)[V]) {
+__device__ __forceinline__ void load_vec(const T* __restrict__ p, float (&f)[V], int valid = V) {
     if constexpr (V == 1) {
         f[0] = (float)p[0];
-    } else {
-        typedef T vec_t __attribute__((ext_vector_type(V)));
-        const vec_t v = *reinterpret_cast<const vec_t*>(p);
+    } else if (valid >= V) {
+        const typename Loose<T, V>::vec v = *reinterpret_cast<const typename Loose<T, V>::vec*>(p);
 #pragma unroll
         for (int i = 0; i < V; ++i) f[i] = (float)v[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) f[i] = i < valid ? (float)p[i] : 0.f;
+    }
+}
+
+// The same in two steps, so that a kernel can have many loads on their way before it converts what came: raw() does not wait.  TAIL: fewer than V.
+template <typename T, int V, bool TAIL>
+__device__ __forceinline__ typename Loose<T, V>::vec load_raw(const T* __restrict__ p, int valid) {
+    if constexpr (!TAIL) {
+        return *reinterpret_cast<const typename Loose<T, V>::vec*>(p);
+    } else {
+        typename Loose<T, V>::vec v = {};
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = p[i < valid ? i : 0];
+        return v;
     }
 }
 
 // Rounds to nearest even where T is narrower (the one rounding of an output).
 template <typename T, int V>
-__device__ __forceinline__ void store_vec(T* __restrict__ p, const float (&f)[V]) {
+__device__ __forceinline__ void store_vec(T* __restrict__ p, const float (&f)[V], int valid = V) {
     if constexpr (V == 1) {
         p[0] = (T)f[0];
-    } else {
-        typedef T vec_t __attribute__((ext_vector_type(V)));
-        vec_t v;
+    } else if (valid >= V) {
+        typename Loose<T, V>::vec v;
 #pragma unroll
         for (int i = 0; i < V; ++i) v[i] = (T)f[i];
-        *reinterpret_cast<vec_t*>(p) = v;
+        *reinterpret_cast<typename Loose<T, V>::vec*>(p) = v;
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i < valid) p[i] = (T)f[i];
     }
 }
 

@@ -307,12 +307,22 @@ __global__ void __launch_bounds__(256) ssm_join_kernel(SsmArgs a) {
     float* buf = (rev ? a.seg_dstate : a.seg_state) + (int64_t)b * a.nseg * n + e % n;
     const float* dec = a.seg_a + (int64_t)b * a.nseg * a.H + h;
     float S = user ? user[e] : 0.f;
-#pragma unroll 8
-    for (int j = 0; j < a.nseg; ++j) {
-        const int seg = rev ? a.nseg - 1 - j : j;
-        const float add = buf[seg * n], d = dec[(int64_t)seg * a.H];
-        buf[seg * n] = S;
-        S = fmaf(__expf(d), S, add);
+    constexpr int AHEAD = 16;                              // segments whose sums are on their way at a time
+    for (int j0 = 0; j0 < a.nseg; j0 += AHEAD) {
+        float add[AHEAD], d[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            const int j = min(j0 + k, a.nseg - 1), seg = rev ? a.nseg - 1 - j : j;
+            add[k] = buf[seg * n];
+            d[k] = dec[(int64_t)seg * a.H];
+        }
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            if (j0 + k >= a.nseg) break;
+            const int seg = rev ? a.nseg - 1 - (j0 + k) : j0 + k;
+            buf[seg * n] = S;
+            S = fmaf(__expf(d[k]), S, add[k]);
+        }
     }
 }
 
