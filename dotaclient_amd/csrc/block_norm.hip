@@ -42,27 +42,28 @@ __device__ __forceinline__ float row_sum(float v, float (*red)[WPR], int slot) {
 
 // Element e of lane l of a row's WPR * 64 lanes: vector e / V of that lane, column ((e / V) * lanes + l) * V + e % V.  Rows of any width and alignment:
 // what lies behind the row's end is 0, its last vector may be a part of one.
-template <typename T, int V, int LANES, int EPL>
+// EVEN: D is a multiple of V, no vector is a part (the checks for parts cost 4 to 7 % of a pass).
+template <typename T, int V, int LANES, int EPL, bool EVEN>
 __device__ __forceinline__ void load_row(const T* __restrict__ p, int l, int D, float (&f)[EPL]) {
     typename Loose<T, V>::vec v[EPL / V];
 #pragma unroll
     for (int i = 0; i < EPL / V; ++i) {                    // whole vectors: those that are not are loaded from the row's start, and again below
         const int c = (i * LANES + l) * V;
-        if (D >= V) v[i] = *reinterpret_cast<const typename Loose<T, V>::vec*>(p + (c + V <= D ? c : 0));
+        if (EVEN || D >= V) v[i] = *reinterpret_cast<const typename Loose<T, V>::vec*>(p + (c + V <= D ? c : 0));
     }
 #pragma unroll
     for (int i = 0; i < EPL / V; ++i) {
         const int c = (i * LANES + l) * V;
 #pragma unroll
         for (int e = 0; e < V; ++e) f[i * V + e] = c + V <= D ? (float)v[i][e] : 0.f;
-        if (c < D && c + V > D) {
+        if (!EVEN && c < D && c + V > D) {
 #pragma unroll
             for (int e = 0; e < V; ++e)
                 if (c + e < D) f[i * V + e] = (float)p[c + e];
         }
     }
 }
-template <typename T, int V, int LANES, int EPL>
+template <typename T, int V, int LANES, int EPL, bool EVEN>
 __device__ __forceinline__ void store_row(T* __restrict__ p, int l, int D, const float (&f)[EPL]) {
 #pragma unroll
     for (int i = 0; i < EPL / V; ++i) {
@@ -70,11 +71,11 @@ __device__ __forceinline__ void store_row(T* __restrict__ p, int l, int D, const
         float t[V];
 #pragma unroll
         for (int e = 0; e < V; ++e) t[e] = f[i * V + e];
-        if (c < D) store_vec<T, V>(p + c, t, D - c);
+        if (c < D) store_vec<T, V>(p + c, t, EVEN ? V : D - c);
     }
 }
 
-template <typename T, typename R, int V, int WPR, int EPL>
+template <typename T, typename R, int V, int WPR, int EPL, bool EVEN>
 __global__ void __launch_bounds__(WPR == 1 ? 256 : WPR * 64) norm_fwd_kernel(NormArgs a) {
     constexpr int LANES = WPR * 64, RPB = WPR == 1 ? 4 : 1;
     const int l = WPR == 1 ? threadIdx.x & 63 : threadIdx.x;
@@ -83,14 +84,14 @@ __global__ void __launch_bounds__(WPR == 1 ? 256 : WPR * 64) norm_fwd_kernel(Nor
     if (row >= a.rows) return;                               // whole waves (WPR == 1) or the whole workgroup
     const int D = a.D;
     float g[EPL], r[EPL], w[EPL];
-    load_row<T, V, LANES, EPL>(static_cast<const T*>(a.y) + row * a.ldy, l, D, g);
-    if (a.z) load_row<T, V, LANES, EPL>(static_cast<const T*>(a.z) + row * a.ldz, l, D, w);
-    load_row<R, V, LANES, EPL>(static_cast<const R*>(a.r) + row * a.ldr, l, D, r);
+    load_row<T, V, LANES, EPL, EVEN>(static_cast<const T*>(a.y) + row * a.ldy, l, D, g);
+    if (a.z) load_row<T, V, LANES, EPL, EVEN>(static_cast<const T*>(a.z) + row * a.ldz, l, D, w);
+    load_row<R, V, LANES, EPL, EVEN>(static_cast<const R*>(a.r) + row * a.ldr, l, D, r);
     if (a.z) {
 #pragma unroll
         for (int e = 0; e < EPL; ++e) g[e] *= w[e] * sigmoid_fast(w[e]);
     }
-    load_row<float, V, LANES, EPL>(a.w_post, l, D, w);
+    load_row<float, V, LANES, EPL, EVEN>(a.w_post, l, D, w);
     float sum = 0.f;
 #pragma unroll
     for (int e = 0; e < EPL; ++e) sum = fmaf(g[e], g[e], sum);
@@ -98,43 +99,43 @@ __global__ void __launch_bounds__(WPR == 1 ? 256 : WPR * 64) norm_fwd_kernel(Nor
 #pragma unroll
     for (int e = 0; e < EPL; ++e) g[e] *= i1 * w[e];
     if (a.s) {
-        load_row<float, V, LANES, EPL>(a.s, l, D, w);
+        load_row<float, V, LANES, EPL, EVEN>(a.s, l, D, w);
 #pragma unroll
         for (int e = 0; e < EPL; ++e) g[e] *= w[e];
     }
     sum = 0.f;
 #pragma unroll
     for (int e = 0; e < EPL; ++e) { r[e] += g[e]; sum = fmaf(r[e], r[e], sum); }
-    store_row<R, V, LANES, EPL>(static_cast<R*>(a.r_out) + row * a.ldro, l, D, r);
+    store_row<R, V, LANES, EPL, EVEN>(static_cast<R*>(a.r_out) + row * a.ldro, l, D, r);
     if (!a.w_pre) return;
-    load_row<float, V, LANES, EPL>(a.w_pre, l, D, w);
+    load_row<float, V, LANES, EPL, EVEN>(a.w_pre, l, D, w);
     const float i2 = rsqrtf(row_sum<WPR>(sum, red, 1) / D + a.eps);
 #pragma unroll
     for (int e = 0; e < EPL; ++e) r[e] *= i2 * w[e];
-    store_row<T, V, LANES, EPL>(static_cast<T*>(a.x_out) + row * a.ldxo, l, D, r);
+    store_row<T, V, LANES, EPL, EVEN>(static_cast<T*>(a.x_out) + row * a.ldxo, l, D, r);
 }
 
-template <typename T, typename R, int V, int WPR, int EPL>
+template <typename T, typename R, int V, int WPR, int EPL, bool EVEN>
 __global__ void __launch_bounds__(WPR == 1 ? 256 : WPR * 64) norm_bwd_kernel(NormArgs a) {
     constexpr int LANES = WPR * 64, RPB = WPR == 1 ? 4 : 1;
     const int l = WPR == 1 ? threadIdx.x & 63 : threadIdx.x, wv = threadIdx.x >> 6;
     __shared__ float red[4][WPR];
     const int D = a.D;
     float q[EPL] = {}, dwp[EPL] = {}, sw[EPL], wq[EPL];
-    load_row<float, V, LANES, EPL>(a.w_post, l, D, sw);
+    load_row<float, V, LANES, EPL, EVEN>(a.w_post, l, D, sw);
     if (a.s) {
-        load_row<float, V, LANES, EPL>(a.s, l, D, wq);
+        load_row<float, V, LANES, EPL, EVEN>(a.s, l, D, wq);
 #pragma unroll
         for (int e = 0; e < EPL; ++e) sw[e] *= wq[e];
     }
-    if (a.w_pre) load_row<float, V, LANES, EPL>(a.w_pre, l, D, wq);
+    if (a.w_pre) load_row<float, V, LANES, EPL, EVEN>(a.w_pre, l, D, wq);
     for (int64_t row = (int64_t)blockIdx.x * RPB + (WPR == 1 ? wv : 0); row < a.rows; row += (int64_t)a.n_blocks * RPB) {
         float y[EPL], z[EPL], r[EPL], d[EPL], x[EPL];
-        load_row<T, V, LANES, EPL>(static_cast<const T*>(a.y) + row * a.ldy, l, D, y);
-        if (a.z) load_row<T, V, LANES, EPL>(static_cast<const T*>(a.z) + row * a.ldz, l, D, z);
-        load_row<R, V, LANES, EPL>(static_cast<const R*>(a.r) + row * a.ldr, l, D, r);
-        load_row<R, V, LANES, EPL>(static_cast<const R*>(a.dr) + row * a.lddr, l, D, d);
-        if (a.w_pre) load_row<T, V, LANES, EPL>(static_cast<const T*>(a.dx) + row * a.lddx, l, D, x);
+        load_row<T, V, LANES, EPL, EVEN>(static_cast<const T*>(a.y) + row * a.ldy, l, D, y);
+        if (a.z) load_row<T, V, LANES, EPL, EVEN>(static_cast<const T*>(a.z) + row * a.ldz, l, D, z);
+        load_row<R, V, LANES, EPL, EVEN>(static_cast<const R*>(a.r) + row * a.ldr, l, D, r);
+        load_row<R, V, LANES, EPL, EVEN>(static_cast<const R*>(a.dr) + row * a.lddr, l, D, d);
+        if (a.w_pre) load_row<T, V, LANES, EPL, EVEN>(static_cast<const T*>(a.dx) + row * a.lddx, l, D, x);
         float sum = 0.f;
 #pragma unroll
         for (int e = 0; e < EPL; ++e) {
@@ -163,7 +164,7 @@ __global__ void __launch_bounds__(WPR == 1 ? 256 : WPR * 64) norm_bwd_kernel(Nor
                 d[e] = fmaf(i2, x[e] * wq[e] - v * m, d[e]);
             }
         }
-        store_row<R, V, LANES, EPL>(static_cast<R*>(a.dres) + row * D, l, D, d);
+        store_row<R, V, LANES, EPL, EVEN>(static_cast<R*>(a.dres) + row * D, l, D, d);
         float du = 0.f;
 #pragma unroll
         for (int e = 0; e < EPL; ++e) {
@@ -179,12 +180,12 @@ __global__ void __launch_bounds__(WPR == 1 ? 256 : WPR * 64) norm_bwd_kernel(Nor
                 d[e] = dg * (z[e] * s);
                 z[e] = dg * y[e] * s * fmaf(z[e], 1.f - s, 1.f);
             }
-            store_row<T, V, LANES, EPL>(static_cast<T*>(a.dz) + row * D, l, D, z);
+            store_row<T, V, LANES, EPL, EVEN>(static_cast<T*>(a.dz) + row * D, l, D, z);
         } else {
 #pragma unroll
             for (int e = 0; e < EPL; ++e) d[e] = i1 * (d[e] - u[e] * du);
         }
-        store_row<T, V, LANES, EPL>(static_cast<T*>(a.dy) + row * D, l, D, d);
+        store_row<T, V, LANES, EPL, EVEN>(static_cast<T*>(a.dy) + row * D, l, D, d);
         if constexpr (WPR > 1) __syncthreads();                                  // red[0] of the next row
     }
     // the workgroup's column sums: its RPB rows' waves through LDS
@@ -203,8 +204,8 @@ __global__ void __launch_bounds__(WPR == 1 ? 256 : WPR * 64) norm_bwd_kernel(Nor
             }
         }
     } else {
-        store_row<float, V, LANES, EPL>(part, l, D, q);
-        store_row<float, V, LANES, EPL>(part + D, l, D, dwp);
+        store_row<float, V, LANES, EPL, EVEN>(part, l, D, q);
+        store_row<float, V, LANES, EPL, EVEN>(part + D, l, D, dwp);
     }
 }
 
@@ -233,12 +234,17 @@ __global__ void __launch_bounds__(1024) norm_reduce_kernel(const float* __restri
 }
 
 // Waves per row and elements per lane: the fewest that hold the row; 16 elements per lane at most, so that backward's five rows stay in registers.
+#define NORM_EVEN(KERNEL, T, R, V, WPR, EPL, GRID, THREADS)                                                                         \
+    do {                                                                                                                            \
+        if (a.D % V == 0) hipLaunchKernelGGL((KERNEL<T, R, V, WPR, EPL, true>), GRID, dim3(THREADS), 0, st, a);                     \
+        else hipLaunchKernelGGL((KERNEL<T, R, V, WPR, EPL, false>), GRID, dim3(THREADS), 0, st, a);                                 \
+    } while (0)
 #define NORM_SHAPES(KERNEL, T, R, V, GRID)                                                                                          \
     do {                                                                                                                            \
-        if (a.D <= 512) hipLaunchKernelGGL((KERNEL<T, R, V, 1, 8>), GRID(4), dim3(256), 0, st, a);                                  \
-        else if (a.D <= 1024) hipLaunchKernelGGL((KERNEL<T, R, V, 1, 16>), GRID(4), dim3(256), 0, st, a);                           \
-        else if (a.D <= 4096) hipLaunchKernelGGL((KERNEL<T, R, V, 4, 16>), GRID(1), dim3(256), 0, st, a);                           \
-        else hipLaunchKernelGGL((KERNEL<T, R, V, 8, 16>), GRID(1), dim3(512), 0, st, a);                                            \
+        if (a.D <= 512) NORM_EVEN(KERNEL, T, R, V, 1, 8, GRID(4), 256);                                                             \
+        else if (a.D <= 1024) NORM_EVEN(KERNEL, T, R, V, 1, 16, GRID(4), 256);                                                      \
+        else if (a.D <= 4096) NORM_EVEN(KERNEL, T, R, V, 4, 16, GRID(1), 256);                                                      \
+        else NORM_EVEN(KERNEL, T, R, V, 8, 16, GRID(1), 512);                                                                       \
     } while (0)
 #define NORM_DISPATCH(KERNEL, GRID)                                                                                                 \
     do {                                                                                                                            \

@@ -131,9 +131,12 @@ __global__ void __launch_bounds__(256) clip_scale_kernel(ClipTable t, const doub
     }
     const double want = (double)max_norm / (norm + 1e-6);
     const float c = norm <= 1.7976931348623157e308 && want < 1.0 ? (float)want : 1.f;
-    const int i = find_tensor(t, blockIdx.x);
-    if ((int)blockIdx.x >= t.chunk0[t.count] || (c == 1.f && t.out[i] == t.g[i])) return;
-    const int64_t at = (int64_t)(blockIdx.x - t.chunk0[i]) * CHUNK;
+    // from the last chunk to the first: the ones that were read last are still in the last-level cache
+    const int chunk = t.chunk0[t.count] - 1 - (int)blockIdx.x;
+    if (chunk < 0) return;
+    const int i = find_tensor(t, chunk);
+    if (c == 1.f && t.out[i] == t.g[i]) return;
+    const int64_t at = (int64_t)(chunk - t.chunk0[i]) * CHUNK;
     const int n = (int)(t.n[i] - at < CHUNK ? t.n[i] - at : CHUNK);
     if ((t.bf16[i / 32] >> (i % 32)) & 1) chunk_scale<bf16_t, 8>(static_cast<const bf16_t*>(t.g[i]), static_cast<bf16_t*>(t.out[i]), at, n, c);
     else chunk_scale<float, 4>(static_cast<const float*>(t.g[i]), static_cast<float*>(t.out[i]), at, n, c);
@@ -193,7 +196,7 @@ int grad_norm_clip(const int64_t* grads, const int64_t* outs, const int64_t* siz
         if (int rc = launch_check("dc_grad_norm_clip")) return rc;
         chunk0 += chunks;
     }
-    for (int first = 0; first < n; first += TENSORS) {
+    for (int first = (n - 1) / TENSORS * TENSORS; first >= 0; first -= TENSORS) {
         const int chunks = fill(first, t);
         if (chunks || first == 0)
             hipLaunchKernelGGL(clip_scale_kernel<false>, dim3(chunks ? chunks : 1), dim3(256), 0, s, t, sq, n, max_norm, first == 0 ? total : nullptr, nullptr);

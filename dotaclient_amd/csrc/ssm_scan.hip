@@ -127,6 +127,7 @@ __global__ void __launch_bounds__(256, V > 1 && NP <= 64 ? (ROWS == 32 ? 4 : siz
         }
         __syncthreads();
         f32x4 y[NT];
+        const bool have = state_in_front(a, blk);
         {
             // S is rounded once to bf16 here, like M: both only end in y
             typename M::frag sf[NK];
@@ -142,7 +143,7 @@ __global__ void __launch_bounds__(256, V > 1 && NP <= 64 ? (ROWS == 32 ? 4 : siz
 #pragma unroll
             for (int jt = 0; jt < NT; ++jt) {
                 y[jt] = f32x4{};
-                if (!FULL && 16 * jt >= rows) continue;
+                if ((!FULL && 16 * jt >= rows) || !have) continue;
 #pragma unroll
                 for (int k = 0; k < NK; ++k) y[jt] = M::mma(sf[k], M::row(L.c + 16 * jt * LN + k * M::KS, LN, i, g), y[jt]);
                 y[jt] *= st.ea[16 * jt + i];
@@ -207,6 +208,8 @@ __device__ __forceinline__ void states(const SsmArgs& a, StateLds<T, NP>& L) {
         nb = min(nb, uniform(a.base[b + 1]) - slot);
     }
     const int first = seg * a.seg_blocks, last = min(nb, first + a.seg_blocks);
+    // the state behind the last block, the gradient in front of the first one: nobody asks for them, but for dh0
+    const int unasked = FINAL || (REV && a.dh0) ? -1 : REV ? 0 : nb - 1;
     const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), i = lane & 15, g = lane >> 4, p0 = 16 * wave;
     const int P = min(a.P - pbase, PT), N = a.N;
     const int64_t seg_at = ((int64_t)unit * a.H + h) * a.P * N + (int64_t)pbase * N, state_at = ((int64_t)b * a.H + h) * a.P * N + (int64_t)pbase * N;
@@ -226,6 +229,7 @@ __device__ __forceinline__ void states(const SsmArgs& a, StateLds<T, NP>& L) {
     Tile<T, NP, V> tb(ldb, N);
     double sum = 0.0;
     auto fetch = [&](int blk) {
+        if (blk == unasked) return;
         const int64_t t0 = (int64_t)blk * TB;
         const int rows = min(TB, q.len - (int)t0);
         if (rows == TB) {
@@ -252,7 +256,8 @@ __device__ __forceinline__ void states(const SsmArgs& a, StateLds<T, NP>& L) {
         const int rows = min(TB, q.len - blk * TB);
         const Steps& st = L.st[j & 1];
         const bool more = j + 1 < last - first;
-        if (rows == TB) {
+        if (blk == unasked) {
+        } else if (rows == TB) {
             tx.template store<true>(L.x, LX, TB, all_p);
             tb.template store<true>(L.b, LN, TB, all_n);
         } else {
@@ -269,12 +274,15 @@ __device__ __forceinline__ void states(const SsmArgs& a, StateLds<T, NP>& L) {
                 for (int k = 0; k < STEPS_KEPT / TB; ++k) to[k * TB] = (&st.dt[0])[k * TB + lane];
             }
         }
-        if constexpr (!FINAL) store_state<NP, 4>(S, (REV ? a.dS : a.S) + (((int64_t)(slot + blk) * a.H + h) * a.PS + pbase) * a.NS, a.NS, p0, a.PS - pbase, a.NS, i, g);
-        const float et = __expf(st.total);
+        if (!FINAL && (REV ? gradient_behind(a, blk, nb) : state_in_front(a, blk)))
+            store_state<NP, 4>(S, (REV ? a.dS : a.S) + (((int64_t)(slot + blk) * a.H + h) * a.PS + pbase) * a.NS, a.NS, p0, a.PS - pbase, a.NS, i, g);
         sum += (double)st.total;
+        if (blk != unasked) {
+            const float et = __expf(st.total);
 #pragma unroll
-        for (int c = 0; c < NP / 16; ++c) S[c] *= et;
-        state_update<T, NP, TB>(S, L.x, LX, L.b, LN, st.w, p0, rows, i, g);
+            for (int c = 0; c < NP / 16; ++c) S[c] *= et;
+            state_update<T, NP, TB>(S, L.x, LX, L.b, LN, st.w, p0, rows, i, g);
+        }
         if (wave == 3 && more) {
             make_steps<REV, !REV && !FINAL>(L.st[(j + 1) & 1], a, (float)raw, block(j + 1) * TB + lane < q.len, A, bias, lane);
             raw = fetch_dt(block(j + 2));
@@ -307,7 +315,7 @@ __global__ void __launch_bounds__(256) ssm_join_kernel(SsmArgs a) {
     float* buf = (rev ? a.seg_dstate : a.seg_state) + (int64_t)b * a.nseg * n + e % n;
     const float* dec = a.seg_a + (int64_t)b * a.nseg * a.H + h;
     float S = user ? user[e] : 0.f;
-    constexpr int AHEAD = 16;                              // segments whose sums are on their way at a time
+    constexpr int AHEAD = 32;                              // segments whose sums are on their way at a time
     for (int j0 = 0; j0 < a.nseg; j0 += AHEAD) {
         float add[AHEAD], d[AHEAD];
 #pragma unroll
@@ -433,7 +441,7 @@ static bool scan_vec(const SsmArgs& a, int type) {
     return a.P % V == 0 && a.N % V == 0 && a.ldx % V == 0 && a.ldb % V == 0 && a.ldc % V == 0 && a.ldy % V == 0 && (p & 15) == 0;
 }
 
-constexpr int64_t FWD_WORKGROUPS = 1024;
+constexpr int64_t FWD_WORKGROUPS = 512;
 
 int64_t ssm_scan_scratch(int n_seq, int max_len, int H, int P, int N) {
     SsmArgs a = {};

@@ -89,6 +89,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ssm_bwd_kernel(SsmArgs a) {
     const SeqRange q = uniform_range(a, b);
     const int64_t row0 = q.off + (int64_t)blk * TB;
     const int rows = min(TB, q.len - blk * TB);
+    const bool have_S = state_in_front(a, blk), have_dS = gradient_behind(a, blk, blocks_of(q.len));
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), N = a.N;
     int i = lane & 15, g = lane >> 4;
     const int n0 = 16 * (wave % WN), jt0 = wave / WN;                     // this wave's columns n; its row tiles jt0 + WT j
@@ -112,10 +113,11 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ssm_bwd_kernel(SsmArgs a) {
     };
     auto fetch_cols = [&](int h, int pt) {
         const int64_t at = (int64_t)(h * a.PS + pt * PT) * NS;
-        S.load(Sp + at, NS, a.PS - pt * PT, col_off);
-        dS.load(dSp + at, NS, a.PS - pt * PT, col_off);
+        if (have_S) S.load(Sp + at, NS, a.PS - pt * PT, col_off);
+        if (have_dS) dS.load(dSp + at, NS, a.PS - pt * PT, col_off);
     };
     auto fetch_rows = [&](int h, int pt) {
+        if (!have_dS) return;
         const int64_t at = (int64_t)(h * a.PS + pt * PT) * NS;
         const uint32_t row = min(pw + i, a.PS - pt * PT - 1) * NS;
 #pragma unroll
@@ -144,6 +146,9 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ssm_bwd_kernel(SsmArgs a) {
         for (int k = tid; k < 4 * TB; k += THREADS)
 #pragma unroll
             for (int s = 0; s < 2; ++s) { (&L.sums[s].R[0][0])[k] = 0.f; (&L.sums[s].K[0][0])[k] = 0.f; }
+        for (int k = tid; k < WN * TB; k += THREADS)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) { (&L.sums[s].RI[0][0])[k] = 0.f; (&L.sums[s].KI[0][0])[k] = 0.f; }
         tb.store(L.b, LN, rows, N);
         tc.store(L.c, LN, rows, N);
         store_steps(h_first);
@@ -281,11 +286,11 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ssm_bwd_kernel(SsmArgs a) {
         }
         __builtin_amdgcn_sched_barrier(0);
         // dC_t += exp(a_t) S^T dy_t, dB_s += dt_s exp(a_T - a_s) dS^T x_s: lane i owns the row, four neighbouring columns n of it
-        if (jt0 == 0 && n0 + i < N) {                                     // the waves that share columns n hold the same S: one counts
+        if (have_S && have_dS && jt0 == 0 && n0 + i < N) {                                     // the waves that share columns n hold the same S: one counts
 #pragma unroll
             for (int k = 0; k < PT / 4; ++k) dot = fmaf(S.v[k], dS.v[k], dot);
         }
-        {
+        if (have_S) {
             const Pieces<T> f(S.v);
 #pragma unroll
             for (int j = 0; j < JT; ++j) {
@@ -306,7 +311,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ssm_bwd_kernel(SsmArgs a) {
         }
         __builtin_amdgcn_sched_barrier(0);
         fetch_rows(h, pt);
-        {
+        if (have_dS) {
             const Pieces<T> f(dS.v);
 #pragma unroll
             for (int j = 0; j < JT; ++j) {
@@ -369,6 +374,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ssm_bwd_kernel(SsmArgs a) {
             for (int j = 0; j < JS; ++j) {
                 const int s = 16 * (js0 + SS * j);
                 acc[j] = f32x4{};
+                if (!have_dS) continue;
 #pragma unroll
                 for (int k = 0; k < NK; ++k) acc[j] = M::mma(sf[k], M::row(L.b + s * LN + k * M::KS, LN, i, g), acc[j]);
                 acc[j] *= st.es[s + i];

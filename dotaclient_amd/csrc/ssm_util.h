@@ -357,6 +357,10 @@ __device__ __forceinline__ int tile_col(int u) { return (int)(0x310102103210ull 
 
 __host__ __device__ __forceinline__ int blocks_of(int len) { return len / TB + (len % TB != 0); }
 
+// Whether there is a state in front of a sequence's block (a gradient behind it), or nothing but zeros: then nothing is stored, loaded or multiplied.
+__device__ __forceinline__ bool state_in_front(const SsmArgs& a, int blk) { return blk > 0 || a.h0; }
+__device__ __forceinline__ bool gradient_behind(const SsmArgs& a, int blk, int blocks) { return blk + 1 < blocks || a.dhT; }
+
 // Workgroup -> (sequence and segment, head and column tile).  Workgroups go round the eight XCDs: the heads of one segment, which share B and C, are
 // given numbers of one XCD, so that its L2 holds what they share.
 __device__ __forceinline__ bool work_item(const SsmArgs& a, int& unit, int& h, int& p0) {
