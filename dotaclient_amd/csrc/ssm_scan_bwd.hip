@@ -34,7 +34,10 @@ struct BwdLds {
     union { struct { T x[TB * pitch<T>(PT)], y[TB * pitch<T>(PT)]; }; T c[TB * pitch<T>(NP)]; };
     T b[TB * pitch<T>(NP)], m[TB * pitch<T>(TB)];
     Steps st[2];
-    struct Sums { float R[4][TB], K[4][TB], RI[WN][TB], KI[WN][TB], diag[TB], dot[4 * WAVES], trace[4 * WAVES]; } sums[2];      // of one head
+    struct Sums { float R[4][TB], K[4][TB], RI[WN][TB], KI[WN][TB], diag[TB], dot[4 * WAVES], trace[4 * WAVES]; };      // of one head
+    // a head's, and the one's before, which are finished beside it - where two workgroups then still fit a CU's LDS (not f32 at N = 64)
+    static constexpr int KEEP = sizeof(T) == 4 && NP == 64 && WAVES == 4 ? 1 : 2;
+    Sums sums[KEEP];
 };
 
 // 64 x 16 of S or dS as an operand whose rows are its columns n and whose k is p: element 4 kk + e of lane (i, g) is [16 kk + 4 g + e][n0 + i].
@@ -145,10 +148,10 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ssm_bwd_kernel(SsmArgs a) {
         // sums that no tile writes
         for (int k = tid; k < 4 * TB; k += THREADS)
 #pragma unroll
-            for (int s = 0; s < 2; ++s) { (&L.sums[s].R[0][0])[k] = 0.f; (&L.sums[s].K[0][0])[k] = 0.f; }
+            for (int s = 0; s < Lds::KEEP; ++s) { (&L.sums[s].R[0][0])[k] = 0.f; (&L.sums[s].K[0][0])[k] = 0.f; }
         for (int k = tid; k < WN * TB; k += THREADS)
 #pragma unroll
-            for (int s = 0; s < 2; ++s) { (&L.sums[s].RI[0][0])[k] = 0.f; (&L.sums[s].KI[0][0])[k] = 0.f; }
+            for (int s = 0; s < Lds::KEEP; ++s) { (&L.sums[s].RI[0][0])[k] = 0.f; (&L.sums[s].KI[0][0])[k] = 0.f; }
         tb.store(L.b, LN, rows, N);
         tc.store(L.c, LN, rows, N);
         store_steps(h_first);
@@ -180,7 +183,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ssm_bwd_kernel(SsmArgs a) {
     // The gradients of a head's step sizes from its row L.  One wave, lane = row.
     auto finish = [&](int h) {
         const Steps& st = L.st[h & 1];
-        const typename Lds::Sums& s = L.sums[h & 1];
+        const typename Lds::Sums& s = L.sums[h & (Lds::KEEP - 1)];
         float R = (s.R[0][lane] + s.R[1][lane]) + (s.R[2][lane] + s.R[3][lane]), K = (s.K[0][lane] + s.K[1][lane]) + (s.K[2][lane] + s.K[3][lane]), KI = 0.f;
 #pragma unroll
         for (int k = 0; k < WN; ++k) { R += s.RI[k][lane]; KI += s.KI[k][lane]; }
@@ -211,7 +214,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ssm_bwd_kernel(SsmArgs a) {
         asm volatile("" : "+v"(i), "+v"(g));
         const int p0 = pt * PT, P = min(a.P - p0, PT);
         const Steps& st = L.st[h & 1];
-        typename Lds::Sums& sums = L.sums[h & 1];
+        typename Lds::Sums& sums = L.sums[h & (Lds::KEEP - 1)];
         // a head's row and column sums, over the lanes that share them
         auto put_tile = [&](int u) {
             if (wave + WAVES * u >= 10) return;
@@ -353,7 +356,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ssm_bwd_kernel(SsmArgs a) {
                 sums.trace[4 * wave + g] = strace;
             }
         }
-        if (wave == 3 && pt == 0 && h > h_first) finish(h - 1);
+        if (Lds::KEEP == 2 && wave == 3 && pt == 0 && h > h_first) finish(h - 1);
         __syncthreads();
         if (!tiles_left) store_steps(h + 1);                              // (the previous head's are finished with)
         // dx_s = dt_s (exp(a_T - a_s) dS B_s + sum_t G1 L dy_t) + D dy_s: lane i owns the row, four neighbouring columns p of it
@@ -406,11 +409,12 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ssm_bwd_kernel(SsmArgs a) {
                 }
             }
         }
+        if (Lds::KEEP == 1 && wave == 3 && !tiles_left) finish(h);
         __syncthreads();
         pt = tiles_left ? pt + 1 : 0;
         h = tiles_left ? h : h + 1;
     }
-    if (wave == 3) finish(h_last - 1);
+    if (Lds::KEEP == 2 && wave == 3) finish(h_last - 1);
     // dC_t += sum_s W[t,s] B_s, dB_s += sum_t W[t,s] C_t
 #pragma unroll
     for (int u = 0; u < GT; ++u) {
@@ -561,7 +565,7 @@ int launch_bwd(const SsmArgs& a, hipStream_t s) {
 // Four waves where two workgroups fit a CU's LDS - they fill each other's waits -, else eight.
 template <typename T, int V>
 int launch_bwd_n(const SsmArgs& a, hipStream_t s) {
-    constexpr int W64 = sizeof(T) == 4 ? 8 : 4;                          // f32 with four waves: 300 registers
+    constexpr int W64 = 4;
     return a.N <= 32 ? launch_bwd<T, 32, V, 4>(a, s) : a.N <= 64 ? launch_bwd<T, 64, V, W64>(a, s) : launch_bwd<T, 128, V, 8>(a, s);
 }
 

@@ -424,3 +424,368 @@ def test_ssm_scan_without_its_optional_inputs():
     _close(g.dx, ref['grads']['x'], ref['size']['x'], 1000, 'dx')
     _close(g.ddt, ref['grads']['raw'], ref['size']['raw'], 1000, 'ddt')
     _close(g.dA, ref['grads']['A'], ref['size']['A'], 1000, 'dA')
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('n,H,G', [(1100, 2, 1), (530, 4, 2)])
+def test_ssm_scan_many_short_sequences(n, H, G, dtype):
+    # more sequences than the slot table takes in one go, enough blocks for a workgroup to take all heads of a group; offsets not in order
+    from dotaclient_amd import ops
+    dev = _dev()
+    P, N = 16, 8
+    lens = [1 + (7 * k) % 3 for k in range(n)]
+    off_d, len_d, rows, off, d = _scan_inputs(n, lens, 0, H, P, G, N, dtype, 0)
+    order = torch.randperm(n, generator=torch.Generator().manual_seed(1))
+    off, lens = [off[k] for k in order], [lens[k] for k in order]
+    off_d, len_d = off_d[order.to(dev)].contiguous(), len_d[order.to(dev)].contiguous()
+    i64 = {k: v.cpu().double() for k, v in d.items()}
+    ref = _scan_reference(i64, off, lens, True)
+    kw = dict(D=d['D'], dt_bias=d['bias'], h0=d['h0'], softplus=True)
+    y, hT = ops.ssm_scan(d['x'], d['dt'], d['A'], d['B'], d['C'], off_d, len_d, 3, **kw)
+    r = ref['rows'].to(dev)
+    out = 300 + (2 ** 16 if dtype == torch.bfloat16 else 0)
+    _close(y[r], ref['y'], ref['ya'], out, 'y')
+    _close(hT, ref['hT'], ref['ha'], 300, 'hT')
+    g = ops.ssm_scan_backward(d['dy'], d['x'], d['dt'], d['A'], d['B'], d['C'], off_d, len_d, 3, dhT=d['dhT'], **kw)
+    G_, S_ = ref['grads'], ref['size']
+    for name, got, terms in (('x', g.dx, out), ('B', g.dB, 2 * out), ('C', g.dC, 2 * out), ('raw', g.ddt, 600)):
+        _close(got[r], G_[name][ref['rows']], S_[name][ref['rows']], terms, name)
+    for name, got in (('A', g.dA), ('D', g.dD), ('bias', g.ddt_bias), ('h0', g.dh0)):
+        _close(got, G_[name], S_[name], 600, name)
+
+
+def _outputs(ops, d, seqs, softplus=True):
+    kw = dict(D=d['D'], dt_bias=d['bias'], h0=d['h0'], softplus=softplus)
+    return list(ops.ssm_scan(d['x'], d['dt'], d['A'], d['B'], d['C'], *seqs, **kw)) + \
+        list(ops.ssm_scan_backward(d['dy'], d['x'], d['dt'], d['A'], d['B'], d['C'], *seqs, dhT=d['dhT'], **kw))
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_ssm_scan_reads_only_its_sequences_and_repeats_itself(dtype):
+    # what lies between the sequences may be anything; the same call gives the same bits
+    from dotaclient_amd import ops
+    lens = [70, 0, 1, 129, 5]
+    off_d, len_d, rows, off, d = _scan_inputs(11, lens, 3, 4, 64, 2, 64, dtype, 8)
+    seqs = (off_d, len_d, 200)                             # max_len may be more than the longest
+    first = _outputs(ops, d, seqs)
+    again = _outputs(ops, d, seqs)
+    gaps = torch.ones(rows, dtype=torch.bool, device=_dev())
+    for o, m in zip(off, lens):
+        gaps[o:o + m] = False
+    for k in ('x', 'B', 'C', 'dt', 'dy'):
+        d[k][gaps] = float('nan')
+    spoiled = _outputs(ops, d, seqs)
+    for k, (a, b, c) in enumerate(zip(first, again, spoiled)):
+        if a.shape[0] == rows:
+            a, b, c = a[~gaps], b[~gaps], c[~gaps]
+        assert torch.isfinite(a).all(), k
+        assert torch.equal(a, b) and torch.equal(a, c), k
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_ssm_scan_extreme_step_sizes(dtype):
+    # decays that underflow to nothing, and none at all
+    from dotaclient_amd import ops
+    off_d, len_d, rows, off, d = _scan_inputs(12, [150], 0, 2, 16, 1, 16, dtype, 0)
+    d['A'] = torch.tensor([-1.0, -16.0], device=_dev())
+    dt = torch.zeros(rows, 2)
+    dt[20:40] = 40.0                                       # exp(-640): everything before is forgotten
+    dt[60:90] = 0.05
+    dt[100] = 1e-30
+    d['dt'], d['bias'] = dt.to(dtype).to(_dev()), torch.zeros(2, device=_dev())
+    i64 = {k: v.cpu().double() for k, v in d.items()}
+    ref = _scan_reference(i64, off, [150], False)
+    y, hT, *_ = _outputs(ops, d, (off_d, len_d, 150), softplus=False)
+    out = 500 + (2 ** 16 if dtype == torch.bfloat16 else 0)
+    _close(y, ref['y'], ref['ya'], out, 'y')
+    _close(hT, ref['hT'], ref['ha'], 500, 'hT')
+    g = ops.ssm_scan_backward(d['dy'], d['x'], d['dt'], d['A'], d['B'], d['C'], off_d, len_d, 150, D=d['D'], dt_bias=d['bias'], h0=d['h0'], dhT=d['dhT'])
+    for name, got, terms in (('x', g.dx, out), ('B', g.dB, 2 * out), ('C', g.dC, 2 * out), ('raw', g.ddt, 1000), ('A', g.dA, 1000), ('h0', g.dh0, 500)):
+        assert torch.isfinite(got).all(), name
+        _close(got, ref['grads'][name], ref['size'][name], terms, name)
+
+
+def test_ssm_scan_gradients_against_differences():
+    # d(sum of y * dy + hT * dhT) along random directions, by central differences of the f32 forward pass evaluated in its own arithmetic: the
+    # difference quotient of step h is off by h^2 times the third derivative and by the forward's rounding over h; with h = 2^-7 and values
+    # of order one both stay below 2 % of the directional derivative's magnitude
+    from dotaclient_amd import ops
+    off_d, len_d, rows, off, d = _scan_inputs(13, [90, 40], 0, 2, 32, 1, 16, torch.float32, 0)
+    seqs = (off_d, len_d, 90)
+    def value(**change):
+        e = dict(d, **change)
+        y, hT = ops.ssm_scan(e['x'], e['dt'], e['A'], e['B'], e['C'], *seqs, D=e['D'], dt_bias=e['bias'], h0=e['h0'], softplus=True)
+        return float((y.double() * d['dy'].double()).sum() + (hT.double() * d['dhT'].double()).sum())
+    g = ops.ssm_scan_backward(d['dy'], d['x'], d['dt'], d['A'], d['B'], d['C'], *seqs, D=d['D'], dt_bias=d['bias'], h0=d['h0'], softplus=True, dhT=d['dhT'])
+    gen = torch.Generator().manual_seed(3)
+    for key, grad in (('x', g.dx), ('dt', g.ddt), ('A', g.dA), ('B', g.dB), ('C', g.dC), ('D', g.dD), ('bias', g.ddt_bias), ('h0', g.dh0)):
+        direction = torch.randn(d[key].shape, generator=gen).to(_dev())
+        h = 2.0 ** -7
+        slope = (value(**{key: (d[key] + h * direction).contiguous()}) - value(**{key: (d[key] - h * direction).contiguous()})) / (2 * h)
+        want = float((grad.double() * direction.double()).sum())
+        scale = float((grad.double().abs() * direction.double().abs()).sum())
+        assert abs(slope - want) <= 0.02 * scale, (key, slope, want, scale)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('H,P,G,N', [(8, 64, 1, 64), (3, 7, 3, 5), (4, 100, 2, 128)])
+def test_ssm_step_against_the_definition(H, P, G, N, dtype):
+    from dotaclient_amd import ops
+    dev = _dev()
+    n = 5
+    _, _, rows, off, d = _scan_inputs(14, [1] * n, 0, H, P, G, N, dtype, 3)
+    i64 = {k: v.cpu().double() for k, v in d.items()}
+    ref = _scan_reference(i64, list(range(n)), [1] * n, True)
+    kw = dict(D=d['D'], dt_bias=d['bias'], softplus=True)
+    y, hT = ops.ssm_step(d['x'], d['dt'], d['A'], d['B'], d['C'], h0=d['h0'], **kw)
+    # N products in lanes of at most 4 and a tree of sixteen, exp and softplus a few steps each
+    _close(y, ref['y'], ref['ya'], N + 32, 'y')
+    _close(hT, ref['hT'], ref['ha'], 32, 'hT')
+    h = d['h0'].clone()
+    y2, h2 = ops.ssm_step(d['x'], d['dt'], d['A'], d['B'], d['C'], h0=h, hT=h, **kw)
+    assert h2.data_ptr() == h.data_ptr() and torch.equal(h2, hT) and torch.equal(y2, y)
+    y3, h3 = ops.ssm_step(d['x'], d['dt'], d['A'], d['B'], d['C'], **kw)
+    zero = torch.zeros_like(d['h0'])
+    y4, h4 = ops.ssm_step(d['x'], d['dt'], d['A'], d['B'], d['C'], h0=zero, **kw)
+    assert torch.equal(y3, y4) and torch.equal(h3, h4)
+
+
+def test_nothing_to_do_is_done():
+    from dotaclient_amd import ops
+    dev = _dev()
+    f = lambda *s: torch.zeros(*s, device=dev)                                         # noqa: E731
+    none = torch.zeros(0, dtype=torch.int64, device=dev), torch.zeros(0, dtype=torch.int32, device=dev), 0
+    empty = torch.zeros(2, dtype=torch.int64, device=dev), torch.zeros(2, dtype=torch.int32, device=dev), 0
+    h0, st = torch.randn(2, 2, 8, 4, device=dev), torch.randn(2, 2, 16, device=dev)
+    for seqs, n in ((none, 0), (empty, 2)):
+        for rows in (0, 3):
+            y, hT = ops.ssm_scan(f(rows, 2, 8), f(rows, 2), f(2), f(rows, 1, 4), f(rows, 1, 4), *seqs, h0=h0[:n].contiguous())
+            assert y.shape == (rows, 2, 8) and torch.equal(hT, h0[:n])
+            g = ops.ssm_scan_backward(f(rows, 2, 8), f(rows, 2, 8), f(rows, 2), f(2), f(rows, 1, 4), f(rows, 1, 4), *seqs, D=f(2), h0=h0[:n].contiguous(),
+                                      dhT=h0[:n].contiguous())
+            assert torch.equal(g.dh0, h0[:n]) and not g.dA.any() and not g.dD.any()
+            y, so = ops.causal_conv(f(rows, 16), f(16, 3), f(16), *seqs, state=st[:n].contiguous())
+            assert torch.equal(so, st[:n])
+            _, dw, db, ds = ops.causal_conv_backward(f(rows, 16), f(rows, 16), f(16, 3), f(16), *seqs, state=st[:n].contiguous(), dstate_out=st[:n].contiguous())
+            assert torch.equal(ds, st[:n]) and not dw.any() and not db.any()
+    r, x = ops.block_norm(f(0, 8), f(0, 8), f(8), w_pre=f(8))
+    assert r.shape == (0, 8) and x.shape == (0, 8)
+    out = ops.block_norm_backward(f(0, 8), f(0, 8), f(0, 8), f(0, 8), f(8), w_pre=f(8))
+    assert not out[2].any() and not out[5].any()
+    y, h = ops.ssm_step(f(0, 2, 8), f(0, 2), f(2), f(0, 1, 4), f(0, 1, 4))
+    assert h.shape == (0, 2, 8, 4)
+
+
+# ------------------------------------------------------------------------------------------------------------- a block of them
+
+
+def _block_weights(seed, D, inner, H, N, K):
+    g = torch.Generator().manual_seed(seed)
+    w = dict(w_in=_rand(g, D, 2 * inner + 2 * N + H) * D ** -0.5, w_conv=_rand(g, inner + 2 * N, K) * 0.5, b_conv=0.1 * _rand(g, inner + 2 * N),
+             A=-(1 + 3 * torch.rand(H, generator=g, dtype=torch.float64)), Dk=_rand(g, H), dt_bias=-2 + _rand(g, H), w_out=_rand(g, inner, D) * inner ** -0.5,
+             w_post=1 + 0.1 * _rand(g, D), scale=0.5 + 0.1 * _rand(g, D), w_pre=1 + 0.1 * _rand(g, D))
+    return w
+
+
+def _block_forward(ops, w, x, r, seqs, H, N, state=None, h0=None):
+    """x (normed input), r (residual) [rows, D] -> (r', x'), the carried states and what the backward pass needs."""
+    inner = w['w_out'].shape[0]
+    z_xbc = x @ w['w_in']
+    gate, xbc_in, dt = z_xbc[:, :inner], z_xbc[:, inner:2 * inner + 2 * N], z_xbc[:, 2 * inner + 2 * N:]
+    if seqs is None:
+        xbc, state = ops.causal_conv_step(xbc_in, state, w['w_conv'], w['b_conv'])
+    else:
+        xbc, state = ops.causal_conv(xbc_in, w['w_conv'], w['b_conv'], *seqs, state=state)
+    v = (xbc[:, :inner].unflatten(1, (H, -1)), dt, w['A'], xbc[:, inner:inner + N].unflatten(1, (1, N)), xbc[:, inner + N:].unflatten(1, (1, N)))
+    kw = dict(D=w['Dk'], dt_bias=w['dt_bias'], h0=h0, softplus=True)
+    y, h = ops.ssm_step(*v, **kw) if seqs is None else ops.ssm_scan(*v, *seqs, **kw)
+    y = y.flatten(1)
+    gated = y * torch.nn.functional.silu(gate)
+    out = gated @ w['w_out']
+    r2, x2 = ops.block_norm(out, r, w['w_post'], scale=w['scale'], w_pre=w['w_pre'])
+    return r2, x2, state, h, dict(x=x, gate=gate, xbc_in=xbc_in, v=v, y=y, gated=gated, out=out, r=r, kw=kw)
+
+
+def _block64(w, x, r, lens, H, N, dr, dx):
+    """The same block in f64 with autograd: outputs and the gradients of every weight."""
+    leaves = {k: v.clone().requires_grad_(True) for k, v in w.items()}
+    inner, K = w['w_out'].shape[0], w['w_conv'].shape[1]
+    zx = x @ leaves['w_in']
+    gate, xbc, dt = zx[:, :inner], zx[:, inner:2 * inner + 2 * N], zx[:, 2 * inner + 2 * N:]
+    ys, o = [], 0
+    for m in lens:
+        ext = torch.cat([xbc.new_zeros(K - 1, xbc.shape[1]), xbc[o:o + m]])
+        c = torch.nn.functional.silu(sum(leaves['w_conv'][:, k] * ext[k:k + m] for k in range(K)) + leaves['b_conv'])
+        d = torch.nn.functional.softplus(dt[o:o + m] + leaves['dt_bias'])
+        y, _ = _scan64(c[:, :inner].unflatten(1, (H, -1)), d, d * leaves['A'], c[:, inner:inner + N][:, None], c[:, inner + N:][:, None], leaves['Dk'],
+                       xbc.new_zeros(1, H, inner // H, N), [0], [m])
+        ys.append(y.flatten(1))
+        o += m
+    out = (torch.cat(ys) * torch.nn.functional.silu(gate)) @ leaves['w_out']
+    r2, x2 = _norm64(out, r, leaves['w_post'], None, leaves['scale'], leaves['w_pre'], 1e-5)
+    keys = list(leaves)
+    grads = torch.autograd.grad((r2 * dr).sum() + (x2 * dx).sum(), [leaves[k] for k in keys])
+    return r2.detach(), x2.detach(), dict(zip(keys, grads))
+
+
+def test_a_block_of_them_trains_and_steps():
+    # norm -> projection -> convolution -> scan -> gate -> projection -> norm, scale, residual -> norm: its outputs, its weights' gradients and their
+    # clipping against f64, and the same rows one at a time with the states carried.  Relative to each tensor's norm: the longest way through the
+    # block has some 2^7 roundings of f32 one after the other or summed up, and no cancellation beyond the sums' own: 2^9 * 2^-24 = 3e-5.
+    from dotaclient_amd import ops
+    dev = _dev()
+    D, H, P, N, K, lens = 32, 4, 16, 16, 4, [37, 70, 5]
+    inner, rows = H * P, sum(lens)
+    w64 = _block_weights(21, D, inner, H, N, K)
+    w = {k: v.float().to(dev) for k, v in w64.items()}
+    g = torch.Generator().manual_seed(22)
+    x64, r64, dr64, dx64 = (_rand(g, rows, D).float().double() for _ in range(4))
+    off_d, len_d, _, off = _packed(lens)
+    seqs = (off_d, len_d, max(lens))
+    r2, x2, state, h, s = _block_forward(ops, w, x64.float().to(dev), r64.float().to(dev), seqs, H, N)
+    w32 = {k: v.cpu().double() for k, v in w.items()}
+    rw, xw, gw = _block64(w32, x64, r64, lens, H, N, dr64, dx64)
+    near = lambda a, b, what, tol=3e-5: (float((a.cpu().double() - b).norm()) <= tol * float(b.norm())) or pytest.fail(     # noqa: E731
+        '%s: %.2e' % (what, float((a.cpu().double() - b).norm() / b.norm())))
+    near(r2, rw, 'r'), near(x2, xw, 'x')
+    # backward, by the operators' own gradients
+    dout, dres, dw_post, _, dscale, dw_pre = ops.block_norm_backward(dr64.float().to(dev), dx64.float().to(dev), s['out'], s['r'], w['w_post'],
+                                                                     scale=w['scale'], w_pre=w['w_pre'])
+    dgated = dout @ w['w_out'].t()
+    sg = torch.sigmoid(s['gate'])
+    dy, dgate = dgated * s['gate'] * sg, dgated * s['y'] * sg * (1 + s['gate'] * (1 - sg))
+    # the gradients of x, B and C go to the columns of one tensor, as the convolution wants them
+    dxbc = torch.empty(rows, inner + 2 * N, device=dev)
+    sc = ops.ssm_scan_backward(dy.unflatten(1, (H, P)), *s['v'], *seqs, **s['kw'], dx=dxbc[:, :inner].unflatten(1, (H, P)),
+                               dB=dxbc[:, inner:inner + N].unflatten(1, (1, N)), dC=dxbc[:, inner + N:].unflatten(1, (1, N)))
+    dconv, dw_conv, db_conv, _ = ops.causal_conv_backward(dxbc, s['xbc_in'], w['w_conv'], w['b_conv'], *seqs)
+    dzx = torch.cat([dgate, dconv, sc.ddt], 1)
+    grads = dict(w_in=s['x'].t() @ dzx, w_conv=dw_conv, b_conv=db_conv, A=sc.dA, Dk=sc.dD, dt_bias=sc.ddt_bias, w_out=s['gated'].t() @ dout, w_post=dw_post,
+                 scale=dscale, w_pre=dw_pre)
+    for k in gw:
+        near(grads[k], gw[k], 'gradient of ' + k, 1e-4)
+    keys = list(gw)
+    clip = ops.GradNormClip([grads[k].contiguous() for k in keys])
+    total, norms = clip(0.5)
+    want = torch.stack([gw[k].norm() for k in keys])
+    near(norms, want, 'norms', 1e-4), near(total[None], want.norm()[None], 'total', 1e-4)
+    near(torch.cat([t.flatten() for t in clip._tensors[0]]), torch.cat([gw[k].flatten() for k in keys]) * (0.5 / float(want.norm())), 'clipped', 2e-4)
+    # one row at a time, every sequence its own hero
+    n = len(lens)
+    st, hs = torch.zeros(n, K - 1, inner + 2 * N, device=dev), torch.zeros(n, H, P, N, device=dev)
+    xd, rd = x64.float().to(dev), r64.float().to(dev)
+    for t in range(max(lens)):
+        at = torch.tensor([o + min(t, m - 1) for o, m in zip(off, lens)], device=dev)
+        live = torch.tensor([t < m for m in lens], device=dev)
+        rs, xs, st2, hs2, _ = _block_forward(ops, w, xd[at], rd[at], None, H, N, st, hs)
+        st, hs = torch.where(live[:, None, None], st2, st), torch.where(live[:, None, None, None], hs2, hs)
+        for k in range(n):
+            if bool(live[k]):
+                near(rs[k], rw[int(at[k])], 'step %d of sequence %d' % (t, k))
+    near(hs, h.cpu().double(), 'carried state'), near(st, state.cpu().double(), 'carried convolution state')
+    # a sequence in two pieces with the states carried between them
+    cut = [20, 33, 2]
+    first = torch.tensor(cut, dtype=torch.int32, device=dev)
+    ra, _, sa, ha, _ = _block_forward(ops, w, xd, rd, (off_d, first, max(cut)), H, N)
+    rb, _, sb, hb, _ = _block_forward(ops, w, xd, rd, (off_d + first, len_d - first, max(lens)), H, N, sa, ha)
+    for k, (o, m) in enumerate(zip(off, lens)):
+        near(torch.cat([ra[o:o + cut[k]], rb[o + cut[k]:o + m]]), rw[o:o + m], 'pieces of sequence %d' % k)
+    near(hb, h.cpu().double(), 'state behind the pieces'), near(sb, state.cpu().double(), 'convolution state behind the pieces')
+
+
+# ------------------------------------------------------------------------------------------------------- streams, graphs, addresses
+
+
+def _all_calls(ops, d, conv, norm, clip):
+    seqs = d['seqs']
+    out = _outputs(ops, d, seqs)
+    y, so = ops.causal_conv(conv['x'], conv['w'], conv['b'], *seqs, state=conv['state'])
+    out += [y, so] + list(ops.causal_conv_backward(conv['dy'], conv['x'], conv['w'], conv['b'], *seqs, state=conv['state']))
+    out += list(ops.block_norm(norm['y'], norm['r'], norm['wp'], gate=norm['z'], scale=norm['s'], w_pre=norm['wq']))
+    out += list(ops.block_norm_backward(norm['dr'], norm['dx'], norm['y'], norm['r'], norm['wp'], gate=norm['z'], scale=norm['s'], w_pre=norm['wq']))
+    total, norms = clip(0.5)
+    return [t for t in out if t is not None] + [total, norms] + clip._tensors[1]
+
+
+def _call_inputs(seed):
+    dev = _dev()
+    g = torch.Generator().manual_seed(seed)
+    lens = [200, 3, 77]
+    off_d, len_d, rows, off, d = _scan_inputs(seed, lens, 0, 4, 32, 2, 16, torch.bfloat16, 0)
+    d['seqs'] = (off_d, len_d, 200)
+    f = lambda *s: _rand(g, *s).float().to(dev)                                        # noqa: E731
+    conv = dict(x=f(rows, 40), dy=f(rows, 40), w=f(40, 4), b=f(40), state=f(3, 3, 40))
+    norm = dict(y=f(rows, 100), r=f(rows, 100), z=f(rows, 100), dr=f(rows, 100), dx=f(rows, 100), wp=f(100), s=f(100), wq=f(100))
+    grads = [f(1000), f(7), f(40000)]
+    return d, conv, norm, grads
+
+
+def test_calls_on_two_streams_and_in_two_graphs_share_nothing():
+    from dotaclient_amd import ops
+    inputs = [_call_inputs(s) for s in (31, 32)]
+    clips = [ops.GradNormClip(i[3], [torch.empty_like(t) for t in i[3]]) for i in inputs]
+    # two of them on the same gradients with outputs of their own
+    want = [[t.clone() for t in _all_calls(ops, *i[:3], c)] for i, c in zip(inputs, clips)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(3):
+        got = [None, None]
+        for k, s in enumerate(streams):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                got[k] = _all_calls(ops, *inputs[k][:3], clips[k])
+        torch.cuda.synchronize()
+        for a, b in zip(want, got):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
+    graphs, outs = [], []
+    for k, s in enumerate(streams):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            outs.append(_all_calls(ops, *inputs[k][:3], clips[k]))
+        graphs.append(g)
+    for turn in range(3):
+        # new values in the same buffers, eager work of the program's own in between
+        for k in range(2):
+            fresh = _call_inputs(40 + 2 * turn + k)
+            for old, new in zip(inputs[k][:3], fresh[:3]):
+                for key in old:
+                    if torch.is_tensor(old[key]):
+                        old[key].copy_(new[key])
+            for old, new in zip(inputs[k][3], fresh[3]):
+                old.copy_(new)
+        want = [[t.clone() for t in _all_calls(ops, *i[:3], c)] for i, c in zip(inputs, clips)]
+        torch.cuda.synchronize()
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(want, outs):
+            assert all(torch.equal(x, y) for x, y in zip(a, b)), turn
+
+
+def test_rows_far_apart():
+    # rows 2^22 elements from each other: offsets beyond 2^31 elements
+    from dotaclient_amd import ops
+    dev = _dev()
+    rows, ld = 600, 1 << 22
+    lens = [300, 299]
+    off_d, len_d, _, off, d = _scan_inputs(51, lens, 0, 2, 16, 1, 16, torch.bfloat16, 0)
+    wide = torch.empty(rows * ld, dtype=torch.bfloat16, device=dev).view(rows, ld)
+    xs = wide[:599, ld - 32:].unflatten(1, (2, 16))
+    xs.copy_(d['x'])
+    near = _outputs(ops, d, (off_d, len_d, 300))
+    far = _outputs(ops, dict(d, x=xs), (off_d, len_d, 300))
+    assert all(torch.equal(a, b) for a, b in zip(near, far))
+    ys = wide[:599, 64:96].unflatten(1, (2, 16))
+    ops.ssm_scan(d['x'], d['dt'], d['A'], d['B'], d['C'], off_d, len_d, 300, D=d['D'], dt_bias=d['bias'], h0=d['h0'], softplus=True, y=ys)
+    assert torch.equal(ys, near[0])
+    flat = xs.flatten(1)
+    w = torch.randn(32, 4, device=dev)
+    assert torch.equal(ops.causal_conv(flat, w, None, off_d, len_d, 300)[0], ops.causal_conv(d['x'].flatten(1), w, None, off_d, len_d, 300)[0])
+    wp = torch.randn(32, device=dev)
+    assert torch.equal(ops.block_norm(flat, flat, wp)[0], ops.block_norm(d['x'].flatten(1).contiguous(), d['x'].flatten(1).contiguous(), wp)[0])
+    # one row of step sizes for all of them, not copied (raw ones: heads whose sizes are negative grow beyond every number, NaN in both)
+    one = d['dt'][:1].expand(599, -1)
+    a = ops.ssm_scan(d['x'], one, d['A'], d['B'], d['C'], off_d, len_d, 300)[0]
+    b = ops.ssm_scan(d['x'], one.contiguous(), d['A'], d['B'], d['C'], off_d, len_d, 300)[0]
+    assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(0.0), b.nan_to_num(0.0))

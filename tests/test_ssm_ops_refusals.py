@@ -1,0 +1,201 @@
+"""CPU: what the state space block's operators refuse, in Python (ops.*) and at the C ABI (dc_*; every check stands before the first launch)."""
+import ctypes
+
+import pytest
+import torch
+
+from dotaclient_amd import _lib, ops
+
+
+def _z(*shape, dtype=torch.float32):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+OFF, LEN = _z(2, dtype=torch.int64), _z(2, dtype=torch.int32)
+BF = torch.bfloat16
+
+
+def _scan(**change):
+    a = dict(x=_z(6, 4, 8), dt=_z(6, 4), A=_z(4), B=_z(6, 2, 16), C=_z(6, 2, 16), seq_off=OFF, seq_len=LEN, max_len=3)
+    kw = {k: change.pop(k) for k in ('D', 'dt_bias', 'h0', 'y', 'hT') if k in change}
+    a.update(change)
+    return ops.ssm_scan(*a.values(), **kw)
+
+
+def _scan_bwd(**change):
+    a = dict(dy=_z(6, 4, 8), x=_z(6, 4, 8), dt=_z(6, 4), A=_z(4), B=_z(6, 2, 16), C=_z(6, 2, 16), seq_off=OFF, seq_len=LEN, max_len=3)
+    kw = {k: change.pop(k) for k in ('dhT', 'dx', 'ddt', 'dB', 'dC', 'h0') if k in change}
+    a.update(change)
+    return ops.ssm_scan_backward(*a.values(), **kw)
+
+
+def _conv(**change):
+    a = dict(x=_z(6, 8), weight=_z(8, 4), bias=_z(8), seq_off=OFF, seq_len=LEN, max_len=3)
+    kw = {k: change.pop(k) for k in ('state', 'y', 'state_out') if k in change}
+    a.update(change)
+    return ops.causal_conv(*a.values(), **kw)
+
+
+def _norm(**change):
+    a = dict(y=_z(6, 8), residual=_z(6, 8), w_post=_z(8))
+    kw = {k: change.pop(k) for k in ('gate', 'scale', 'w_pre', 'residual_out') if k in change}
+    a.update(change)
+    return ops.block_norm(*a.values(), **kw)
+
+
+@pytest.mark.parametrize('call,change,error,says', [
+    (_scan, dict(x=_z(6, 4, 8, dtype=torch.float16)), TypeError, 'float32 or torch.bfloat16'),
+    (_scan, dict(dt=_z(6, 4, dtype=BF)), TypeError, 'dt'),
+    (_scan, dict(A=_z(4, dtype=BF)), TypeError, 'A'),
+    (_scan, dict(A=_z(8)[::2]), ValueError, 'contiguous'),
+    (_scan, dict(A=_z(3)), ValueError, 'A: expected shape'),
+    (_scan, dict(B=_z(6, 3, 16), C=_z(6, 3, 16)), ValueError, 'divide'),
+    (_scan, dict(B=_z(6, 2, 129), C=_z(6, 2, 129)), ValueError, 'N <= 128'),
+    (_scan, dict(x=_z(6, 4, 257)), ValueError, 'P <= 256'),
+    (_scan, dict(x=_z(6, 4, 16)[:, :, ::2]), ValueError, 'inside a row'),
+    (_scan, dict(C=_z(6, 2, 8)), ValueError, 'C: expected shape'),
+    (_scan, dict(C=_z(5, 2, 16)), ValueError, 'C: expected shape'),
+    (_scan, dict(x=_z(6, 32)), ValueError, 'rows, H, P'),
+    (_scan, dict(seq_off=OFF.int()), TypeError, 'seq_off'),
+    (_scan, dict(seq_len=LEN[:1]), ValueError, 'seq_len'),
+    (_scan, dict(seq_len=LEN.long()), TypeError, 'seq_len'),
+    (_scan, dict(max_len=-1), ValueError, 'max_len'),
+    (_scan, dict(max_len=2 ** 31), ValueError, 'max_len'),
+    (_scan, dict(h0=_z(2, 4, 8, 8)), ValueError, 'h0'),
+    (_scan, dict(h0=_z(2, 4, 8, 16, dtype=BF)), TypeError, 'h0'),
+    (_scan, dict(y=_z(1, 4, 8).expand(6, 4, 8)), ValueError, 'overlap'),
+    (_scan, dict(D=_z(1)), ValueError, 'D: expected'),
+    (_scan, {}, _lib.DotaHipError, 'GPU'),
+    (_scan_bwd, dict(dy=_z(6, 4, 8, dtype=BF)), TypeError, 'dy'),
+    (_scan_bwd, dict(dhT=_z(2, 4, 8, 15)), ValueError, 'dhT'),
+    (_scan_bwd, dict(dB=_z(6, 2, 15)), ValueError, 'dB'),
+    (_scan_bwd, {}, _lib.DotaHipError, 'GPU'),
+    (_conv, dict(weight=_z(8, 9)), ValueError, 'K <= 8'),
+    (_conv, dict(weight=_z(8, 1)), ValueError, '2 <= K'),
+    (_conv, dict(weight=_z(7, 4)), ValueError, 'weight'),
+    (_conv, dict(weight=_z(8, 4, dtype=BF)), TypeError, 'weight'),
+    (_conv, dict(state=_z(2, 4, 8)), ValueError, 'state'),
+    (_conv, dict(state=_z(2, 3, 8, dtype=BF)), TypeError, 'state'),
+    (_conv, dict(x=_z(6, 16)[:, ::2]), ValueError, 'inside a row'),
+    (_conv, dict(y=_z(6, 9)), ValueError, 'y'),
+    (_conv, {}, _lib.DotaHipError, 'GPU'),
+    (_norm, dict(residual=_z(6, 8, dtype=BF)), TypeError, 'residual'),
+    (_norm, dict(y=_z(6, 8193), residual=_z(6, 8193), w_post=_z(8193)), ValueError, '8192'),
+    (_norm, dict(gate=_z(6, 8, dtype=BF)), TypeError, 'gate'),
+    (_norm, dict(scale=_z(1)), ValueError, 'scale'),
+    (_norm, dict(w_pre=_z(8, dtype=torch.float64)), TypeError, 'w_pre'),
+    (_norm, {}, _lib.DotaHipError, 'GPU'),
+])
+def test_python_refuses(call, change, error, says):
+    with pytest.raises(error, match=says):
+        call(**change)
+
+
+def test_outputs_must_not_be_inputs():
+    x = _z(6, 8)
+    with pytest.raises(ValueError, match='y must not be one of the inputs'):
+        _conv(x=x, y=x)
+    st = _z(2, 3, 8)
+    with pytest.raises(ValueError, match='state_out'):
+        _conv(state=st, state_out=st)
+    v = _z(6, 4, 8)
+    with pytest.raises(ValueError, match='y must not'):
+        _scan(x=v, y=v)
+    with pytest.raises(ValueError, match='dx must not'):
+        _scan_bwd(dy=v, dx=v)
+    y = _z(6, 8)
+    with pytest.raises(ValueError, match='residual_out'):
+        _norm(y=y, residual_out=y)
+
+
+def test_norm_gradients_go_with_their_inputs():
+    a = (_z(6, 8), _z(6, 8), _z(8))
+    with pytest.raises(ValueError, match='dx: expected exactly with w_pre'):
+        ops.block_norm_backward(_z(6, 8), None, *a, w_pre=_z(8))
+    with pytest.raises(ValueError, match='dx: expected exactly with w_pre'):
+        ops.block_norm_backward(_z(6, 8), _z(6, 8), *a)
+
+
+def test_clipping_refuses():
+    flat = _z(100)
+    for grads, out, error, says in (([], None, ValueError, 'one or more'), ([_z(3)], [], ValueError, 'as many'), ([_z(3, dtype=torch.float16)], None, TypeError, 'float32'),
+                                    ([_z(6)[::2]], None, ValueError, 'contiguous'), ([_z(3)], [_z(4)], ValueError, 'type and shape'),
+                                    ([_z(3)], [_z(3, dtype=BF)], ValueError, 'type and shape'), ([flat[:60], flat[50:]], None, ValueError, 'overlap'),
+                                    ([flat, flat], None, ValueError, 'overlap'), ([flat[:50]], [flat[25:75]], ValueError, 'overlap'),
+                                    ([_z(3)], None, _lib.DotaHipError, 'GPU')):
+        with pytest.raises(error, match=says):
+            ops.GradNormClip(grads, out)
+
+
+# ---------------------------------------------------------------------------------------------------------------------- the C ABI
+
+P = 0x1000                                              # an address that no refused call looks at
+
+
+def _error(rc, code, says):
+    assert rc == code, rc
+    assert says in _lib.load().dc_last_error().decode()
+
+
+def test_c_abi_refuses_scans():
+    lib = _lib.load()
+
+    def fwd(x=P, ldx=32, lddt=4, ldb=16, rows=6, n=2, H=4, Pd=8, G=1, N=16, ty=0, y=P, max_len=6, scratch=None, size=0):
+        return lib.dc_ssm_scan_fwd(x, ldx, P, lddt, P, P, ldb, P, ldb, None, None, None, P, P, rows, n, max_len, H, Pd, G, N, ty, 0, y, 32, P, scratch, size, None)
+
+    def bwd(dx=P, scratch=P, size=1 << 40, H=4, G=1, N=16, ty=0):
+        return lib.dc_ssm_scan_bwd(P, 32, P, 32, P, 4, P, P, 16, P, 16, None, None, None, None, P, P, 6, 2, 6, H, 8, G, N, ty, 0, dx, 32, P, 4, P, 16, P, 16, P, None,
+                                   None, None, scratch, size, None)
+    for kw, code in ((dict(ty=2), 1101), (dict(H=0), 1102), (dict(H=4, G=3), 1102), (dict(G=0), 1102), (dict(Pd=0), 1102), (dict(Pd=257), 1102), (dict(N=0), 1102),
+                     (dict(N=129), 1102), (dict(rows=-1), 1103), (dict(n=-1), 1103), (dict(max_len=-1), 1103), (dict(ldx=(1 << 22) + 1), 1103), (dict(ldb=-1), 1103),
+                     (dict(x=None), 1104), (dict(y=None), 1104), (dict(max_len=100000, rows=100000), 1105), (dict(max_len=100000, rows=100000, scratch=P, size=8), 1105)):
+        _error(fwd(**kw), code, 'dc_ssm_scan_fwd')
+    assert fwd(n=0) == 0
+    for kw, code in ((dict(ty=-1), 1101), (dict(H=3, G=2), 1102), (dict(N=200), 1102), (dict(dx=None), 1104), (dict(scratch=None), 1105), (dict(size=16), 1105),
+                     (dict(scratch=P + 4), 1105)):
+        _error(bwd(**kw), code, 'dc_ssm_scan_bwd')
+    step = lambda **k: lib.dc_ssm_step(P, 32, P, 4, P, P, 16, P, 16, None, None, None, k.get('n', 2), 4, 8, 1, k.get('N', 16), k.get('ty', 0), 0, k.get('y', P), 32,     # noqa: E731
+                                       k.get('hT', P), None)
+    for kw, code in ((dict(ty=3), 1101), (dict(N=129), 1102), (dict(n=-2), 1103), (dict(y=None), 1104), (dict(hT=None), 1104)):
+        _error(step(**kw), code, 'dc_ssm_step')
+    assert step(n=0) == 0
+
+
+def test_c_abi_scratch_sizes():
+    lib = _lib.load()
+    assert lib.dc_ssm_scan_scratch(256, 256, 8, 64, 64) == 0                           # enough workgroups without segments
+    assert lib.dc_ssm_scan_scratch(1, 128, 1, 64, 64) == 0                             # too short for them
+    one = lib.dc_ssm_scan_scratch(1, 32768, 8, 64, 64)
+    assert one > 0 and one % (8 * (64 * 64 + 1) * 4) == 0
+    a, b = lib.dc_ssm_scan_bwd_scratch(4096, 16, 256, 4, 64, 1, 64), lib.dc_ssm_scan_bwd_scratch(8192, 32, 256, 4, 64, 1, 64)
+    assert a >= 2 * 4 * (4096 // 64 + 16) * 4 * 64 * 64 and b > a
+    assert lib.dc_ssm_scan_bwd_scratch(-1, 1, 1, 1, 1, 1, 1) == 0
+    assert lib.dc_causal_conv_scratch(2, 0, 8, 4) > 0 and lib.dc_block_norm_scratch(0, 8) == 0
+    sizes = (ctypes.c_int64 * 3)(0, 5, 100000)
+    assert lib.dc_grad_norm_clip_scratch(sizes, 3) >= 8 * 3
+
+
+def test_c_abi_refuses_the_rest():
+    lib = _lib.load()
+    conv = lambda **k: lib.dc_causal_conv_fwd(k.get('x', P), 8, k.get('w', P), None, P, P, k.get('rows', 6), k.get('n', 2), 3, k.get('D', 8), k.get('K', 4),     # noqa: E731
+                                              k.get('ty', 0), 1, None, P, 8, None, None)
+    for kw, code in ((dict(ty=2), 1101), (dict(K=1), 1102), (dict(K=9), 1102), (dict(D=0), 1102), (dict(rows=-1), 1103), (dict(n=-1), 1103), (dict(x=None), 1104),
+                     (dict(w=None), 1104)):
+        _error(conv(**kw), code, 'dc_causal_conv_fwd')
+    _error(lib.dc_causal_conv_bwd(P, 8, P, 8, P, None, P, P, 6, 2, 3, 8, 4, 0, 1, None, None, P, 8, P, None, None, P, 16, None), 1105, 'scratch')
+    _error(lib.dc_causal_conv_bwd(P, 8, P, 8, P, None, P, P, 6, 2, 3, 8, 4, 0, 1, None, None, P, 8, None, None, None, P, 1 << 30, None), 1104, 'dc_causal_conv_bwd')
+    _error(lib.dc_causal_conv_step(P, 8, None, P, None, 2, 8, 4, 0, 1, P, 8, None, None), 1104, 'dc_causal_conv_step')
+    norm = lambda **k: lib.dc_block_norm_fwd(k.get('y', P), 8, None, 0, P, 8, P, None, k.get('wq'), k.get('rows', 6), k.get('D', 8), k.get('ty', 0), k.get('tr', 0),     # noqa: E731
+                                             1e-5, k.get('r', P), 8, None, 0, None)
+    for kw, code in ((dict(ty=2), 1101), (dict(tr=1), 1101), (dict(D=0), 1102), (dict(D=8193), 1102), (dict(rows=-1), 1103), (dict(rows=1 << 31), 1103), (dict(y=None), 1104),
+                     (dict(r=None), 1104), (dict(wq=P), 1104)):
+        _error(norm(**kw), code, 'dc_block_norm_fwd')
+    assert norm(rows=0) == 0
+    _error(lib.dc_block_norm_bwd(P, 8, None, 0, P, 8, None, 0, P, 8, P, None, None, 6, 8, 0, 0, 1e-5, P, None, P, P, None, None, P, 16, None), 1105, 'scratch')
+    i64, i32 = ctypes.c_int64, ctypes.c_int32
+
+    def clip(sizes=(3, 4), types=(0, 1), grads=(P, P + 64), n=2, max_norm=1.0, size=1 << 20, scratch=P):
+        return lib.dc_grad_norm_clip((i64 * 2)(*grads), (i64 * 2)(*grads), (i64 * 2)(*sizes), (i32 * 2)(*types), n, max_norm, P, P, scratch, size, None)
+    for kw, code in ((dict(n=0), 1104), (dict(max_norm=-1.0), 1103), (dict(max_norm=float('nan')), 1103), (dict(sizes=(-1, 2)), 1103), (dict(types=(0, 2)), 1101),
+                     (dict(grads=(0, P)), 1104), (dict(size=8), 1105), (dict(scratch=None), 1104)):
+        _error(clip(**kw), code, 'dc_grad_norm_clip')
