@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(256, V > 1 && NP <= 64 ? (ROWS == 32 ? 4 : siz
                 const f32x4 hs = *reinterpret_cast<const f32x4*>(st.hi + s), ls = *reinterpret_cast<const f32x4*>(st.lo + s),
                             ds = *reinterpret_cast<const f32x4*>(st.dt + s);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) m[u][r] = s + r <= t ? m[u][r] * (__expf((ht - hs[r]) + (lt - ls[r])) * ds[r]) : 0.f;
+                for (int r = 0; r < 4; ++r) m[u][r] = s + r <= t ? m[u][r] * (exp_f((ht - hs[r]) + (lt - ls[r])) * ds[r]) : 0.f;
             } else {
                 const float f = st.rf[t] * between(st, jt[u], js[u]);
                 const f32x4 cd = *reinterpret_cast<const f32x4*>(st.cd + s);
@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(256, V > 1 && NP <= 64 ? (ROWS == 32 ? 4 : siz
                     if (p + r < P) out[r] = o[r];
             }
         }
-        const float et = __expf(st.total);
+        const float et = st.decay;
 #pragma unroll
         for (int c = 0; c < NP / 16; ++c) S[c] *= et;
         state_update<T, NP, ROWS>(S, L.x, LX, L.b, LN, st.w, p0, rows, i, g);
@@ -278,7 +278,7 @@ __device__ __forceinline__ void states(const SsmArgs& a, StateLds<T, NP>& L) {
             store_state<NP, 4>(S, (REV ? a.dS : a.S) + (((int64_t)(slot + blk) * a.H + h) * a.PS + pbase) * a.NS, a.NS, p0, a.PS - pbase, a.NS, i, g);
         sum += (double)st.total;
         if (blk != unasked) {
-            const float et = __expf(st.total);
+            const float et = st.decay;
 #pragma unroll
             for (int c = 0; c < NP / 16; ++c) S[c] *= et;
             state_update<T, NP, TB>(S, L.x, LX, L.b, LN, st.w, p0, rows, i, g);
@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(256) ssm_join_kernel(SsmArgs a) {
             if (j0 + k >= a.nseg) break;
             const int seg = rev ? a.nseg - 1 - (j0 + k) : j0 + k;
             buf[seg * n] = S;
-            S = fmaf(__expf(d[k]), S, add[k]);
+            S = fmaf(exp_f(d[k]), S, add[k]);
         }
     }
 }
@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(256) ssm_step_kernel(SsmArgs a) {
     const int grp = h / (a.H / a.G);
     float d = (float)static_cast<const T*>(a.dt)[b * a.lddt + h] + (a.dt_bias ? a.dt_bias[h] : 0.f);
     if (a.softplus) d = softplus_f(d);
-    const float x = (float)static_cast<const T*>(a.x)[b * a.ldx + (int64_t)h * a.P + p], e = __expf(d * a.A[h]), dx = d * x;
+    const float x = (float)static_cast<const T*>(a.x)[b * a.ldx + (int64_t)h * a.P + p], e = exp_f(d * a.A[h]), dx = d * x;
     const T* B = static_cast<const T*>(a.B) + b * a.ldb + (int64_t)grp * a.N;
     const T* C = static_cast<const T*>(a.C) + b * a.ldc + (int64_t)grp * a.N;
     const int64_t at = (((int64_t)b * a.H + h) * a.P + p) * a.N;

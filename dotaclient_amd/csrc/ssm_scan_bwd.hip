@@ -4,10 +4,9 @@
 //   G1[t,s] = C_t . B_s,  G2[t,s] = dy_t . x_s,  L[t,s] = exp(a_t - a_s) for s <= t, else 0
 //   dx_s = dt_s (sum_t G1 L dy_t + e_s dS B_s) + D dy_s,                     e_s = exp(a_T - a_s)
 //   dB_s = sum_t W[t,s] C_t + dt_s e_s dS^T x_s,   dC_t = sum_s W[t,s] B_s + exp(a_t) S^T dy_t,     W = G2 L dt_s
-//   R_t = sum_{s<t} Q dt_s + C_t . exp(a_t) S^T dy_t,   K_s = sum_{t>=s} Q[t,s] + B_s . e_s dS^T x_s,   Q = G1 G2 L
-//   d(a step)_t = sum_{u>=t} (R_u - dt_u (K_u - Q[u,u])) + exp(a_T) <S, dS> + sum_s dt_s B_s . e_s dS^T x_s
-//   d(dt')_t = A d(a step)_t + K_t,   dA = sum_t dt_t d(a step)_t,   dD = sum_t G2[t,t]
-// (the diagonal cancels in R - dt K and is left out of both, so that strong decays do not lose the gradient of A in it).
+//   Q = G1 G2 L,   RI_t = C_t . exp(a_t) S^T dy_t,   KI_s = B_s . e_s dS^T x_s
+//   d(a step)_u = sum_{s<u<=t} Q[t,s] dt_s + sum_{t>=u} RI_t + sum_{s<u} dt_s KI_s + exp(a_T) <S, dS>
+//   d(dt')_s = A d(a step)_s + sum_{t>=s} Q[t,s] + KI_s,   dA = sum_t dt_t d(a step)_t,   dD = sum_t G2[t,t]
 //
 // A workgroup of four or eight waves owns one block and the heads of one group (or a share of them, where blocks and groups alone are too few): G1 stays in its
 // registers, W and the gradients of B and C are added up over the heads there, so dB and dC cost two products per block instead of two per head, and
@@ -184,17 +183,35 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ssm_bwd_kernel(SsmArgs a) {
     auto finish = [&](int h) {
         const Steps& st = L.st[h & 1];
         const typename Lds::Sums& s = L.sums[h & (Lds::KEEP - 1)];
-        float R = (s.R[0][lane] + s.R[1][lane]) + (s.R[2][lane] + s.R[3][lane]), K = (s.K[0][lane] + s.K[1][lane]) + (s.K[2][lane] + s.K[3][lane]), KI = 0.f;
-#pragma unroll
-        for (int k = 0; k < WN; ++k) { R += s.RI[k][lane]; KI += s.KI[k][lane]; }
-        K += KI;
-        const int k = lane & (4 * WAVES - 1);
+        const int J = lane >> 4, k = lane & (4 * WAVES - 1);              // row tile
         const float d = st.dt[lane], A = a.A[h], dot = lane == k ? s.dot[k] : 0.f, trace = lane == k ? s.trace[k] : 0.f;
-        // exp(a_T) <S, dS> + sum_s dt_s KI_s reach every row of the block: they stand behind its last one
-        const double behind = lane_sum(fma((double)st.ea[TB - 1], (double)dot, (double)(d * KI)));
-        const double da = (double)R - (double)(d * K);
-        const double pre = lane_prefix(da);
-        const float suffix = (float)(last_lane(pre) - pre + da + behind);
+        float RI = 0.f, KI = 0.f, K = 0.f, Rd = 0.f, Kd = 0.f;
+#pragma unroll
+        for (int w = 0; w < WN; ++w) { RI += s.RI[w][lane]; KI += s.KI[w][lane]; }
+        // d(a step)_u = what goes from a row in front of u (or the state in front of the block) to u or one behind it (or the state behind the block).
+        // Sums of row and column sums, not differences of them: those would keep the rounding of what cancels.  Row tile u is in:
+        double from = 0.0, to = 0.0;                                      // to this row from earlier tiles, from this row to later ones
+        double tot0, tot1;                                                // sums of tiles (jt, 0), (jt, 1), jt the lane's
+#pragma unroll
+        for (int js = 0; js < 4; ++js) {
+            const float r = s.R[js][lane], c = s.K[js][lane];
+            K += c;
+            if (js < J) to += (double)r;
+            if (js == J) { Rd = r; Kd = c; }
+            if (js > J) from += (double)d * (double)c;
+            if (js == 0) tot0 = dpp<ROW_NEWBCAST + 15>(row_prefix((double)r));
+            if (js == 1) tot1 = dpp<ROW_NEWBCAST + 15>(row_prefix((double)r));
+        }
+        const double in = to + ((double)Rd - (double)d * (double)Kd);     // inside its own tile a difference is all there is
+        const double in_sum = row_prefix(in), from_sum = row_prefix(from);
+        double da = dpp<ROW_NEWBCAST + 15>(in_sum) - in_sum + in + (from_sum - from);
+        const double t20 = of_lane<32>(tot0), t30 = of_lane<48>(tot0), t31 = of_lane<48>(tot1);
+        da += J == 1 ? t20 + t30 : J == 2 ? t30 + t31 : 0.0;              // past this row's tile altogether
+        const double ri = lane_prefix((double)RI), ki = lane_prefix((double)d * (double)KI);
+        da += last_lane(ri) - ri + (double)RI + (ki - (double)d * (double)KI);
+        da += (double)st.ea[TB - 1] * lane_sum((double)dot);
+        K += KI;
+        const float suffix = (float)da;
         float ddt = fmaf(A, suffix, K + s.diag[lane]);
         if (a.softplus) ddt *= -expm1f(-d);                               // sigmoid(v) = 1 - exp(-softplus(v))
         if (lane >= rows) ddt = 0.f;
@@ -267,7 +284,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ssm_bwd_kernel(SsmArgs a) {
                     for (int r = 0; r < 4; ++r) {
                         // a product that is not finite stays out of what it does not belong to
                         const bool in = s <= t + r, strict = s < t + r;
-                        const float l = in ? __expf((ht[r] - hs) + (lt[r] - ls)) : 0.f, gl = in ? G2[u][r] * l : 0.f, qv = in ? G1[u][r] * gl : 0.f;
+                        const float l = in ? exp_f((ht[r] - hs) + (lt[r] - ls)) : 0.f, gl = in ? G2[u][r] * l : 0.f, qv = in ? G1[u][r] * gl : 0.f;
                         m[r] = in ? G1[u][r] * l : 0.f;
                         W[u][r] = fmaf(gl, ds, W[u][r]);
                         K[u] += strict ? qv : 0.f;

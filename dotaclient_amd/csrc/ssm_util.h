@@ -204,23 +204,44 @@ __device__ __forceinline__ float sum_g(float v) {
     p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(p[0]) + __uint_as_float(p[1]);
 }
-// Inclusive sum over the lanes, and what the last lane holds.
-template <typename F> __device__ __forceinline__ F lane_prefix(F v) {
+// Inclusive sum over the lanes of a row, over all lanes, and what the last lane holds.
+template <typename F> __device__ __forceinline__ F row_prefix(F v) {
     v += dpp<ROW_SHR + 1>(v);
     v += dpp<ROW_SHR + 2>(v);
     v += dpp<ROW_SHR + 4>(v);
     v += dpp<ROW_SHR + 8>(v);
+    return v;
+}
+template <typename F> __device__ __forceinline__ F lane_prefix(F v) {
+    v = row_prefix(v);
     v += dpp<ROW_BCAST15, 0xa>(v);
     v += dpp<ROW_BCAST31, 0xc>(v);
     return v;
 }
-__device__ __forceinline__ float last_lane(float v) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63)); }
-__device__ __forceinline__ double last_lane(double v) {
-    return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), 63), __builtin_amdgcn_readlane(__double2loint(v), 63));
+template <int LANE> __device__ __forceinline__ float of_lane(float v) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), LANE)); }
+template <int LANE> __device__ __forceinline__ double of_lane(double v) {
+    return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), LANE), __builtin_amdgcn_readlane(__double2loint(v), LANE));
 }
+template <typename F> __device__ __forceinline__ F last_lane(F v) { return of_lane<63>(v); }
 template <typename F> __device__ __forceinline__ F lane_sum(F v) { return last_lane(lane_prefix(v)); }
 
 __device__ __forceinline__ float softplus_f(float v) { return v > 20.f ? v : log1pf(expf(v)); }
+
+// exp(x) within 1.5 ulp: v_exp_f32 is exact enough, x * log2(e) is not - its rounding is 2^-24 of a number that may be 10 or 100 - so the part that the
+// rounding drops goes in behind.  Decays are factors of everything that is summed over a sequence; with the plain product the gradient of A
+// came out three times as far from 64 bits.  Where that part is no number (x infinite, or the result) the plain value stands.
+__device__ __forceinline__ float exp_f(float x) {
+    constexpr float L = 1.4426950216293335f, LO = 1.9259629911266175e-8f, LN2 = 0.6931471805599453f;      // log2(e) = L + LO
+    const float p = x * L, e = fmaf(x, LO, fmaf(x, L, -p)), r = __builtin_amdgcn_exp2f(p);
+    const float c = fmaf(r * e, LN2, r);
+    return c == c ? c : r;
+}
+__device__ __forceinline__ float exp_f(double x) {
+    double p = x * 1.4426950408889634;
+    p = p > 2000.0 ? 2000.0 : p < -2000.0 ? -2000.0 : p;                  // a NaN stays one
+    const double n = rint(p);
+    return ldexpf(__builtin_amdgcn_exp2f((float)(p - n)), (int)n);
+}
 
 // The block's step sizes and running sums (one wave, lane = row).  a is kept as hi + lo, so that exp(a_t - a_s) of neighbouring rows does not lose
 // what a long sum costs: a is summed in f64, the difference is taken of both halves.
@@ -229,13 +250,13 @@ struct Steps {
     float ea[TB], es[TB];                         // exp(a_t), exp(a_T - a_t)
     float rf[TB], cf[TB];                         // exp(a_t - a of its tile of 16's first row), exp(a of its tile's last row - a_t)
     float w[TB], cd[TB];                          // see make_steps; dt_t cf_t
-    float total;                                  // a of the last row
+    float total, decay;                           // a of the last row, exp of it
 };
 constexpr int STEPS_KEPT = 7 * TB;                // what the backward kernel takes over from the forward states' pass: dt .. cf
 // exp(a of row tile jt's first row - a of row tile js's last one), js < jt: with rf and cf the decay from s to t in three factors, none above 1 where
 // the decays are not.
 __device__ __forceinline__ float between(const Steps& s, int jt, int js) {
-    return __expf((s.hi[16 * jt] - s.hi[16 * js + 15]) + (s.lo[16 * jt] - s.lo[16 * js + 15]));
+    return exp_f((s.hi[16 * jt] - s.hi[16 * js + 15]) + (s.lo[16 * jt] - s.lo[16 * js + 15]));
 }
 
 // w[t] = dt_t exp(a_T - a_t): the weights of the block's rows in the state behind it; REV: exp(a_t), those of the gradients in the one in front.
@@ -249,17 +270,20 @@ __device__ __forceinline__ void make_steps(Steps& s, const SsmArgs& a, float raw
     s.dt[lane] = d;
     s.hi[lane] = (float)sum;
     s.lo[lane] = (float)(sum - (double)(float)sum);
-    const float es = __expf((float)(last - sum));
-    s.w[lane] = REV ? __expf((float)sum) : d * es;
+    const float es = exp_f(last - sum);
+    s.w[lane] = REV ? exp_f(sum) : d * es;
     if (FACTORS) {
-        const float cf = __expf((float)(dpp<ROW_NEWBCAST + 15>(sum) - sum));
-        s.ea[lane] = __expf((float)sum);
+        const float cf = exp_f(dpp<ROW_NEWBCAST + 15>(sum) - sum);
+        s.ea[lane] = exp_f(sum);
         s.es[lane] = es;
-        s.rf[lane] = __expf((float)(sum - dpp<ROW_NEWBCAST>(sum)));
+        s.rf[lane] = exp_f(sum - dpp<ROW_NEWBCAST>(sum));
         s.cf[lane] = cf;
         s.cd[lane] = d * cf;
     }
-    if (lane == 63) s.total = (float)last;
+    if (lane == 63) {
+        s.total = (float)last;
+        s.decay = exp_f(last);
+    }
 }
 
 // v as three bf16 pieces: 24 bits, all of an f32's.
