@@ -256,7 +256,8 @@ __global__ void __launch_bounds__(1024) norm_reduce_kernel(const float* __restri
 int check_common(const char* what, const NormArgs& a, int type, int rtype) {
     if (type < 0 || type > 1 || rtype < 0 || rtype > type) { set_error(what, 1101); return 1101; }
     if (a.D < 1 || a.D > 8192) { set_error(what, 1102); return 1102; }
-    if (a.rows < 0 || a.rows > 0x7fffffff) { set_error(what, 1103); return 1103; }
+    // a wave per row, four or eight for wide ones
+    if (a.rows < 0 || a.rows > 0x7fffffff || !fits_grid(a.rows + 3, a.D <= 1024 ? 64 : a.D <= 4096 ? 256 : 512)) { set_error(what, 1103); return 1103; }
     if (!a.w_post || (a.rows && (!a.y || !a.r))) { set_error(what, 1104); return 1104; }
     return 0;
 }
@@ -294,7 +295,7 @@ int block_norm_bwd(const void* dr, int64_t lddr, const void* dx, int64_t lddx, c
     if (!dw_post || (rows && (!dr || !dy || !dres || (z && !dz) || (w_pre && !dx)))) { set_error("dc_block_norm_bwd", 1104); return 1104; }
     if (scratch_bytes < block_norm_scratch(rows, D) || (rows && !scratch)) { set_error("dc_block_norm_bwd: scratch", 1105); return 1105; }
     if (rows) {
-    #define NORM_BGRID(RPB) dim3((unsigned)a.n_blocks)
+#define NORM_BGRID(RPB) dim3((unsigned)a.n_blocks)
         NORM_DISPATCH(norm_bwd_kernel, NORM_BGRID);
         if (int rc = launch_check("dc_block_norm_bwd")) return rc;
     }

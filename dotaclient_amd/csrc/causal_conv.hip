@@ -321,7 +321,7 @@ int chunks_in(int max_len) { return max_len > 0 ? max_len / CROWS + (max_len % C
 int check_common(const char* what, const ConvArgs& a, int type) {
     if (type != 0 && type != 1) { set_error(what, 1101); return 1101; }
     if (a.K < 2 || a.K > 8 || a.D < 1 || a.D > 1 << 20) { set_error(what, 1102); return 1102; }
-    if (a.rows < 0 || a.n_seq < 0 || a.max_len < 0) { set_error(what, 1103); return 1103; }
+    if (a.rows < 0 || a.n_seq < 0 || a.max_len < 0 || a.max_len > MAX_LEN) { set_error(what, 1103); return 1103; }
     if (!a.w || (a.rows && !a.x)) { set_error(what, 1104); return 1104; }
     return 0;
 }
@@ -341,16 +341,16 @@ int causal_conv_fwd(const void* x, int64_t ldx, const float* w, const float* bia
     a.D = D; a.K = K; a.silu = silu; a.state = state; a.y = y; a.ldy = ldy; a.state_out = state_out;
     if (int rc = check_common("dc_causal_conv_fwd", a, type)) return rc;
     if (n_seq == 0) return 0;
-    a.chunks_per_seq = chunks_in(max_len);
+    a.chunks_per_seq = chunks_in((int)(max_len < rows ? max_len : rows));
     a.n_chunks = (int64_t)n_seq * a.chunks_per_seq;
     const int64_t gx = (a.n_chunks + CGROUPS - 1) / CGROUPS;
-    if (gx > 0x7fffffff) { set_error("dc_causal_conv_fwd", 1103); return 1103; }
+    if (!fits_grid(gx, 256)) { set_error("dc_causal_conv_fwd", 1103); return 1103; }
 #define CONV_GRID(V) dim3((unsigned)gx, (D + CLANES * V - 1) / (CLANES * V))
     CONV_DISPATCH(conv_fwd_kernel, CONV_GRID);
     return launch_check("dc_causal_conv_fwd");
 }
 
-int64_t causal_conv_scratch(int n_seq, int max_len, int D, int K) {      // bytes, for either vector width
+int64_t causal_conv_scratch(int n_seq, int max_len, int D, int K) {      // bytes
     const int64_t n_chunks = (int64_t)n_seq * chunks_in(max_len);
     return (int64_t)row_blocks(n_chunks, 1) * (K + 1) * D * (int64_t)sizeof(float);
 }
@@ -365,7 +365,7 @@ int causal_conv_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, co
     a.dy = dy; a.lddy = lddy; a.dstate_out = dstate_out; a.dx = dx; a.lddx = lddx; a.dstate = dstate; a.part = scratch;
     if (int rc = check_common("dc_causal_conv_bwd", a, type)) return rc;
     if (!dw) { set_error("dc_causal_conv_bwd", 1104); return 1104; }
-    a.chunks_per_seq = chunks_in(max_len);
+    a.chunks_per_seq = chunks_in((int)(max_len < rows ? max_len : rows));
     a.n_chunks = (int64_t)n_seq * a.chunks_per_seq;
     const int lanes = CLANES * CV, groups = (D + lanes - 1) / lanes;
     a.n_row_blocks = row_blocks(a.n_chunks, groups);
@@ -391,6 +391,7 @@ int causal_conv_step(const void* x, int64_t ldx, const void* state, const float*
     if (int rc = check_common("dc_causal_conv_step", a, type)) return rc;
     if (n_seq == 0) return 0;
     if (!y || !state_out) { set_error("dc_causal_conv_step", 1104); return 1104; }
+    if (!fits_grid((int64_t)n_seq * ((D + CV - 1) / CV) / 256 + 1, 256)) { set_error("dc_causal_conv_step", 1103); return 1103; }
 #define CONV_SGRID(V) dim3((unsigned)(((int64_t)n_seq * ((D + V - 1) / V) + 255) / 256))
     CONV_DISPATCH(conv_step_kernel, CONV_SGRID);
     return launch_check("dc_causal_conv_step");

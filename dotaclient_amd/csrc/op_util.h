@@ -70,4 +70,8 @@ __device__ __forceinline__ SeqRange seq_range(const int64_t* __restrict__ seq_of
     return r;
 }
 
+// What a launch takes: 2^32 threads along x.  Sequences' row numbers stay in an int, also a chunk or two behind the last row.
+inline bool fits_grid(int64_t groups, int threads) { return groups * threads <= 0xffffffffll; }
+constexpr int MAX_LEN = 0x7fffffff - 255;
+
 }  // namespace dc

@@ -415,8 +415,8 @@ int ssm_join_segments(const SsmArgs& a, bool both, hipStream_t s) {
 int ssm_check(const char* what, const SsmArgs& a, int type) {
     if (type != 0 && type != 1) { set_error(what, 1101); return 1101; }
     if (a.H < 1 || a.G < 1 || a.H % a.G || a.H > 4096 || a.P < 1 || a.P > 256 || a.N < 1 || a.N > 128) { set_error(what, 1102); return 1102; }
-    if (a.rows < 0 || a.n_seq < 0 || a.max_len < 0 || (int64_t)a.n_seq * a.H * ((a.P + 15) / 16) > 0x3fffffff) { set_error(what, 1103); return 1103; }
-    for (int64_t ld : {a.ldx, a.lddt, a.ldb, a.ldc, a.ldy, a.lddy, a.lddx, a.lddb, a.lddc})
+    if (a.rows < 0 || a.n_seq < 0 || a.max_len < 0 || a.max_len > MAX_LEN) { set_error(what, 1103); return 1103; }
+    for (int64_t ld : {a.ldx, a.lddt, a.ldb, a.ldc, a.ldy, a.lddy, a.lddx, a.ldddt, a.lddb, a.lddc})
         if (ld < 0 || ld > 1 << 22) { set_error(what, 1103); return 1103; }
     if (!a.A || (a.rows && (!a.x || !a.dt || !a.B || !a.C))) { set_error(what, 1104); return 1104; }
     return 0;
@@ -455,7 +455,7 @@ int ssm_scan_fwd(SsmArgs a, int type, void* scratch, int64_t scratch_bytes, hipS
     if (a.n_seq == 0) return 0;
     if (!a.y && a.rows) { set_error("dc_ssm_scan_fwd", 1104); return 1104; }
     ssm_segments(a, FWD_WORKGROUPS);
-    if (work_items(a) > 0x7fffffff) { set_error("dc_ssm_scan_fwd", 1103); return 1103; }
+    if (!fits_grid(work_items(a), 256)) { set_error("dc_ssm_scan_fwd", 1103); return 1103; }
     const bool vec = scan_vec(a, type);
     if (a.nseg > 1) {
         if (!scratch || scratch_bytes < ssm_scan_scratch(a.n_seq, a.max_len, a.H, a.P, a.N)) { set_error("dc_ssm_scan_fwd: scratch", 1105); return 1105; }
@@ -475,7 +475,9 @@ int ssm_step(SsmArgs a, int type, hipStream_t s) {
     if (!a.y || !a.hT) { set_error("dc_ssm_step", 1104); return 1104; }
     const uintptr_t p = reinterpret_cast<uintptr_t>(a.h0) | reinterpret_cast<uintptr_t>(a.hT), q = reinterpret_cast<uintptr_t>(a.B) | reinterpret_cast<uintptr_t>(a.C);
     const bool vec = a.N % 4 == 0 && a.ldb % 4 == 0 && a.ldc % 4 == 0 && (p & 15) == 0 && (q & (type ? 7 : 15)) == 0;
-    const dim3 grid((unsigned)((int64_t)a.n_seq * a.H * ((a.P + 15) / 16)));
+    const int64_t groups = (int64_t)a.n_seq * a.H * ((a.P + 15) / 16);
+    if (!fits_grid(groups, 256)) { set_error("dc_ssm_step", 1103); return 1103; }
+    const dim3 grid((unsigned)groups);
     if (type == 0) {
         if (vec) hipLaunchKernelGGL((ssm_step_kernel<float, 4>), grid, dim3(256), 0, s, a);
         else hipLaunchKernelGGL((ssm_step_kernel<float, 1>), grid, dim3(256), 0, s, a);

@@ -582,8 +582,7 @@ int launch_bwd(const SsmArgs& a, hipStream_t s) {
 // Four waves where two workgroups fit a CU's LDS - they fill each other's waits -, else eight.
 template <typename T, int V>
 int launch_bwd_n(const SsmArgs& a, hipStream_t s) {
-    constexpr int W64 = 4;
-    return a.N <= 32 ? launch_bwd<T, 32, V, 4>(a, s) : a.N <= 64 ? launch_bwd<T, 64, V, W64>(a, s) : launch_bwd<T, 128, V, 8>(a, s);
+    return a.N <= 32 ? launch_bwd<T, 32, V, 4>(a, s) : a.N <= 64 ? launch_bwd<T, 64, V, 4>(a, s) : launch_bwd<T, 128, V, 8>(a, s);
 }
 
 bool bwd_vec(const SsmArgs& a, int type) {
@@ -640,13 +639,13 @@ int64_t ssm_scan_bwd_scratch(int64_t rows, int n_seq, int max_len, int H, int P,
 
 int ssm_scan_bwd(SsmArgs a, int type, void* scratch, int64_t scratch_bytes, hipStream_t s) {
     if (int rc = ssm_check("dc_ssm_scan_bwd", a, type)) return rc;
-    if (a.rows / TB + a.n_seq > 0x7fffffff || a.G > 65535) { set_error("dc_ssm_scan_bwd", 1103); return 1103; }
+    if (!fits_grid(a.rows / TB + a.n_seq, 512)) { set_error("dc_ssm_scan_bwd", 1103); return 1103; }
     if (!a.dA || (a.rows && (!a.dy || !a.dx || !a.ddt || !a.dB || !a.dC))) { set_error("dc_ssm_scan_bwd", 1104); return 1104; }
     if (!scratch || (reinterpret_cast<uintptr_t>(scratch) & 15) || scratch_bytes < bwd_plan(a, static_cast<char*>(scratch))) {
         set_error("dc_ssm_scan_bwd: scratch", 1105);
         return 1105;
     }
-    if (work_items(a) > 0x7fffffff) { set_error("dc_ssm_scan_bwd", 1103); return 1103; }
+    if (!fits_grid(work_items(a), 256)) { set_error("dc_ssm_scan_bwd", 1103); return 1103; }
     const bool vec = bwd_vec(a, type);
     hipLaunchKernelGGL(ssm_slots_kernel, dim3(1), dim3(1024), 0, s, a);
     if (int rc = launch_check("dc_ssm_scan_bwd")) return rc;

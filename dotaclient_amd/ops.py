@@ -100,11 +100,15 @@ def gemm(A, B, C, M, N, K, lda, ldb, ldc, a_kmajor=False, b_kmajor=False, bias=N
 # ---------------------------------------------------------------------------------------------------------------------------------------
 # A state space core's operators over the same packed rows (csrc/causal_conv.hip, ssm_scan.hip, block_norm.hip, grad_clip.hip).
 # Row tensors ([rows, ...], f32 or bf16) may be column slices of wider ones: the distance between rows is free, everything inside a row is
-# contiguous.  Parameters and recurrent states are f32 and contiguous, as are their gradients.  Rows that belong to no sequence are neither
-# read nor written: in an output allocated here they hold whatever was there.  A call runs on its tensors' device, on the stream that is
-# current there; its scratch is allocated per call, so calls on several streams or in several graphs share nothing.
+# contiguous.  Parameters and recurrent states are f32 and contiguous, as are their gradients.  A row belongs to one sequence at most; rows
+# that belong to none are neither read nor written: in an output allocated here they hold whatever was there.  A sequence that points outside
+# the rows or is longer than max_len is cut.  Outputs given by the caller must not share memory with an input or another output (column slices
+# of one tensor, side by side, do not), but for the states of the single steps and block_norm's residual, which may be updated in place.
+# A call runs on its tensors' device, on the stream that is current there; its scratch is allocated per call, so calls on several streams or
+# in several graphs share nothing.
 # ---------------------------------------------------------------------------------------------------------------------------------------
 _TYPES = {torch.float32: 0, torch.bfloat16: 1}
+MAX_LEN = 2 ** 31 - 256
 
 
 def _rows(t, name, dtype, shape):
@@ -113,14 +117,15 @@ def _rows(t, name, dtype, shape):
         raise TypeError('%s: expected %s, got %s' % (name, dtype, t.dtype))
     if t.shape != shape:
         raise ValueError('%s: expected shape %s, got %s' % (name, tuple(shape), tuple(t.shape)))
-    if t.is_contiguous():
-        return t.stride(0)
-    width, st = 1, t.stride()
+    st = t.stride()
+    if shape[0] > 1 and t.is_contiguous():
+        return st[0]
+    width = 1
     for i in range(len(shape) - 1, 0, -1):
         if shape[i] != 1 and st[i] != width:
             raise ValueError('%s: everything inside a row must be contiguous' % name)
         width *= shape[i]
-    return st[0] if shape[0] > 1 else width
+    return st[0] if shape[0] > 1 else width                  # (a single row's distance may be anything)
 
 
 def _out_rows(t, name, dtype, shape, like):
@@ -154,16 +159,42 @@ def _sequences(seq_off, seq_len, max_len):
     n = seq_off.shape[0] if seq_off.dim() == 1 else -1
     _param(seq_off, 'seq_off', (n,), torch.int64)
     _param(seq_len, 'seq_len', (n,), torch.int32)
-    if not 0 <= max_len < 2 ** 31:
-        raise ValueError('max_len: expected 0 <= max_len < 2^31, got %d' % max_len)
+    if not 0 <= max_len <= MAX_LEN:
+        raise ValueError('max_len: expected 0 <= max_len <= 2^31 - 256, got %d' % max_len)
     return n
 
 
+def _span(t):
+    """The addresses that a tensor's elements lie between."""
+    p, size = t.data_ptr(), t.element_size()
+    if t.is_contiguous():
+        return p, p + t.numel() * size
+    return p, p + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * size
+
+
+def _beside(t, u):
+    """Whether two tensors with a span in common are column slices side by side: rows at the same distance, different columns."""
+    pitch = t.stride(0) * t.element_size()
+    if t.dim() < 2 or u.dim() < 2 or not pitch or u.stride(0) * u.element_size() != pitch or t.shape[0] < 2 or u.shape[0] < 2:
+        return False
+    behind = (u.data_ptr() - t.data_ptr()) % pitch
+    return behind >= t.numel() // t.shape[0] * t.element_size() and behind + u.numel() // u.shape[0] * u.element_size() <= pitch
+
+
 def _distinct(outs, ins):
-    """Refuses an output of the caller's that starts where an input does."""
-    for name, t in outs:
-        if t is not None and t.numel() and any(i is not None and i.data_ptr() == t.data_ptr() for i in ins):
-            raise ValueError('%s must not be one of the inputs' % name)
+    """Refuses an output of the caller's that shares memory with an input or another output.  outs: (name, tensor) or (name, tensor, the one
+    of the inputs that it may be)."""
+    given = [o for o in outs if o[1] is not None and o[1].numel()]
+    for k, (name, t, *itself) in enumerate(given):
+        lo, hi = _span(t)
+
+        def shares(u):
+            return u is not None and u.data_ptr() < hi and u.numel() and _span(u)[1] > lo and not _beside(t, u)
+        for u in ins:
+            if shares(u) and not (itself and u is itself[0] and u.data_ptr() == lo and u.stride() == t.stride() and u.dtype is t.dtype):
+                raise ValueError('%s must not be one of the inputs or share memory with one' % name)
+        if any(shares(o[1]) for o in given[:k]):
+            raise ValueError('%s must not share memory with another output' % name)
 
 
 def _run(name, tensors, *args):
@@ -247,8 +278,7 @@ def causal_conv_step(x, state, weight, bias, silu=True, y=None, state_out=None):
     ldx = _rows(x, 'x', x.dtype, (n, D))
     if state is not None:
         _param(state, 'state', (n, K - 1, D), x.dtype)
-    _distinct((('y', y),), (x, state))
-    _distinct((('state_out', state_out),), (x,))
+    _distinct((('y', y), ('state_out', state_out, state)), (x, state))
     y, ldy = _out_rows(y, 'y', x.dtype, (n, D), x)
     state_out = x.new_empty((n, K - 1, D)) if state_out is None else _param(state_out, 'state_out', (n, K - 1, D), x.dtype)
     _run('dc_causal_conv_step', (x, state, weight, bias, y, state_out), x.data_ptr(), ldx, _p(state), weight.data_ptr(), _p(bias), n, D, K, ty, int(silu),
@@ -315,7 +345,7 @@ def ssm_scan_backward(dy, x, dt, A, B, C, seq_off, seq_len, max_len, D=None, dt_
     for t, name in ((h0, 'h0'), (dhT, 'dhT')):
         if t is not None:
             _param(t, name, (n, H, P, N))
-    _distinct((('dx', dx), ('ddt', ddt), ('dB', dB), ('dC', dC)), (dy, x, dt, B, C))
+    _distinct((('dx', dx), ('ddt', ddt), ('dB', dB), ('dC', dC)), (dy, x, dt, B, C, h0, dhT))
     dx, lddx = _out_rows(dx, 'dx', x.dtype, (rows, H, P), x)
     ddt, ldddt = _out_rows(ddt, 'ddt', x.dtype, (rows, H), x)
     dB, lddb = _out_rows(dB, 'dB', x.dtype, (rows, G, N), x)
@@ -336,8 +366,7 @@ def ssm_step(x, dt, A, B, C, h0=None, D=None, dt_bias=None, softplus=False, y=No
     n, H, P, G, N, ty, (ldx, lddt, ldb, ldc) = _scan_operands(x, dt, A, B, C, D, dt_bias)
     if h0 is not None:
         _param(h0, 'h0', (n, H, P, N))
-    _distinct((('y', y),), (x, dt, B, C, h0))
-    _distinct((('hT', hT),), (x, dt, B, C))
+    _distinct((('y', y), ('hT', hT, h0)), (x, dt, B, C, h0))
     y, ldy = _out_rows(y, 'y', x.dtype, (n, H, P), x)
     hT = x.new_empty((n, H, P, N), dtype=torch.float32) if hT is None else _param(hT, 'hT', (n, H, P, N))
     _run('dc_ssm_step', (x, dt, A, B, C, D, dt_bias, h0, y, hT), x.data_ptr(), ldx, dt.data_ptr(), lddt, A.data_ptr(), B.data_ptr(), ldb, C.data_ptr(), ldc,
@@ -367,7 +396,7 @@ def block_norm(y, residual, w_post, gate=None, scale=None, w_pre=None, eps=1e-5,
     y, gate [rows, D]; residual [rows, D] in y's type or f32; w_post, scale, w_pre [D]; gate, scale, w_pre may be None.  D <= 8192.
     -> (r in residual's type, x in y's type; None without w_pre).  residual_out may be residual itself; x is taken from r before r is rounded."""
     rows, D, ty, tr, ldy, ldr, ldg = _norm_operands(y, residual, w_post, gate, scale, w_pre)
-    _distinct((('residual_out', residual_out),), (y, gate))
+    _distinct((('residual_out', residual_out, residual),), (y, gate, residual))
     r, ldro = _out_rows(residual_out, 'residual_out', residual.dtype, (rows, D), y)
     x = None if w_pre is None else y.new_empty((rows, D))
     _run('dc_block_norm_fwd', (y, residual, w_post, gate, scale, w_pre, r), y.data_ptr(), ldy, _p(gate), ldg, residual.data_ptr(), ldr, w_post.data_ptr(),
@@ -398,7 +427,7 @@ def block_norm_backward(dr, dx, y, residual, w_post, gate=None, scale=None, w_pr
 class GradNormClip:
     """The global norm of many gradients, and clipping (clip_grad_norm_ of optimizer.py:674-675 for tensors that are not one flat buffer):
     built once over a list of contiguous f32 / bf16 tensors and, with `out`, the tensors that the clipped gradients go to (default: in
-    place); each call reads what the tensors hold then.  No two of the tensors may overlap.
+    place); each call reads what the tensors hold then, also where one was given other memory since.  No two of the tensors may overlap.
     clip(max_norm) -> (total [] f32, norms [n] f32): out_i = grads_i * min(1, max_norm / (total + 1e-6)); a total that is not finite
     clips nothing."""
 
@@ -407,6 +436,13 @@ class GradNormClip:
         out = grads if out is None else list(out)
         if not grads or len(out) != len(grads):
             raise ValueError('GradNormClip: expected one or more gradients and as many outputs')
+        self._tensors, self._n = (grads, out), len(grads)
+        self._all = grads if all(o is g for o, g in zip(out, grads)) else grads + out
+        self._bind()
+
+    def _bind(self):
+        """Checks the tensors as they are now and lays out what the C entry takes."""
+        (grads, out), n = self._tensors, self._n
         spans = []
         for i, (g, o) in enumerate(zip(grads, out)):
             _float_type(g, 'grads[%d]' % i)
@@ -421,28 +457,26 @@ class GradNormClip:
         spans.sort()
         if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
             raise ValueError('GradNormClip: two of the tensors overlap')
-        n = len(grads)
-        self._tensors, self._n = (grads, out), n
-        self._grads = (ctypes.c_int64 * n)(*[t.data_ptr() for t in grads])
-        self._outs = (ctypes.c_int64 * n)(*[t.data_ptr() for t in out])
+        if any(not t.is_cuda for t in self._all):
+            raise _lib.DotaHipError('GradNormClip: its tensors must live on the GPU (there is no CPU path)')
+        if any(t.device != grads[0].device for t in self._all):
+            raise ValueError('GradNormClip: its tensors live on different devices')
+        self._at = list(map(torch.Tensor.data_ptr, self._all))
+        self._from, self._to = ((ctypes.c_int64 * n)(*part) for part in (self._at[:n], self._at[-n:]))
         self._sizes = (ctypes.c_int64 * n)(*[t.numel() for t in grads])
         self._types = (ctypes.c_int32 * n)(*[_TYPES[t.dtype] for t in grads])
-        self._check = tuple({id(t): t for t in grads + out}.values())
-        if any(not t.is_cuda for t in self._check):
-            raise _lib.DotaHipError('GradNormClip: its tensors must live on the GPU (there is no CPU path)')
-        if any(t.device != grads[0].device for t in self._check):
-            raise ValueError('GradNormClip: its tensors live on different devices')
         self._scratch_bytes = _lib.load().dc_grad_norm_clip_scratch(self._sizes, n)
 
     def __call__(self, max_norm):
         if not max_norm >= 0:
             raise ValueError('max_norm: expected a number >= 0, got %r' % (max_norm,))
-        first, n = self._tensors[0][0], self._n
-        norms = torch.empty(n + 1, dtype=torch.float32, device=first.device)
-        scratch = torch.empty(self._scratch_bytes, dtype=torch.uint8, device=first.device)
-        _run('dc_grad_norm_clip', (first,), self._grads, self._outs, self._sizes, self._types, n, max_norm, norms.data_ptr() + 4 * n, norms.data_ptr(),
-             scratch.data_ptr(), self._scratch_bytes)
-        return norms[n], norms[:n]
+        if list(map(torch.Tensor.data_ptr, self._all)) != self._at:                     # a tensor was given other memory
+            self._bind()
+        first, n, at = self._all[0], self._n, self._scratch_bytes // 4
+        buf = torch.empty(at + n + 1, dtype=torch.float32, device=first.device)         # scratch, norms, total
+        p = buf.data_ptr()
+        _run('dc_grad_norm_clip', (first,), self._from, self._to, self._sizes, self._types, n, max_norm, p + 4 * (at + n), p + 4 * at, p, self._scratch_bytes)
+        return buf[at + n], buf[at:at + n]
 
 
 def grad_norm_clip(grads, max_norm, out=None):

@@ -336,9 +336,9 @@ int dc_dp_average_grads(const int64_t* seg_off, const int32_t* seg_len, const in
 /* ------------------------------------------------------------------------------------------------
  * Operators of a state space core over the same packed rows (beside the GRU / LSTM of dc_policy_forward, policy.py:66,152-156: the same
  * seq_off / seq_len, the same state carried from chunk to chunk and, one row at a time, from env-step to env-step).  Element types:
- * 0 = f32, 1 = bf16; parameters, states and their gradients are f32 unless noted; `ld*` = distance of two rows in elements.  A sequence that
- * points outside [0, rows) or is longer than max_len is cut; rows of no sequence are neither read nor written.  Outputs must not overlap inputs
- * unless noted.  All scratch is the caller's, of the size that the matching dc_*_scratch gives (bytes; host only), and carries nothing from
+ * 0 = f32, 1 = bf16; parameters, states and their gradients are f32 unless noted; `ld*` = distance of two rows in elements (the scan's: 2^22 at
+ * most).  A sequence that points outside [0, rows) or is longer than max_len (2^31 - 256 at most) is cut; a row belongs to one sequence at most;
+ * rows of no sequence are neither read nor written.  Outputs must not overlap inputs or each other unless noted.  All scratch is the caller's, of the size that the matching dc_*_scratch gives (bytes; host only), and carries nothing from
  * call to call.  Errors: 1101 type, 1102 a width out of range, 1103 a size out of range, 1104 a NULL buffer, 1105 scratch too small.
  * ------------------------------------------------------------------------------------------------ */
 

@@ -292,6 +292,25 @@ def test_grad_norm_clip_of_a_norm_that_is_not_finite_changes_nothing(bad):
     assert abs(float(total) / (1e30 * 1000 ** 0.5) - 1) < 1e-6 and torch.isfinite(big[0]).all() and float(big[0].norm()) < 1.001
 
 
+def test_grad_norm_clip_follows_its_tensors():
+    """A gradient that is given other memory, of another size too, after the handle was built is clipped where it is then; the old memory stays as it was."""
+    from dotaclient_amd import ops
+    dev = _dev()
+    a, b = torch.full((1000,), 2.0, device=dev), torch.full((77,), 1.0, device=dev)
+    old = a.data
+    clip = ops.GradNormClip([a, b])
+    clip(1e9)
+    a.data = torch.full((5000,), 3.0, device=dev)
+    total, norms = clip(1.0)
+    want = (5000 * 9 + 77) ** 0.5
+    assert abs(float(total) - want) < 1e-6 * want and abs(float(norms[0]) - 45000 ** 0.5) < 1e-6 * want
+    assert torch.allclose(a, torch.full_like(a, 3 / want), rtol=1e-6) and torch.allclose(b, torch.full_like(b, 1 / want), rtol=1e-6)
+    assert torch.equal(old, torch.full_like(old, 2.0))
+    b.data = a.data[100:177]
+    with pytest.raises(ValueError, match='overlap'):
+        clip(1.0)
+
+
 # ----------------------------------------------------------------------------------------------------------- state space scan
 
 

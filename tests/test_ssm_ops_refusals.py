@@ -108,6 +108,61 @@ def test_outputs_must_not_be_inputs():
         _norm(y=y, residual_out=y)
 
 
+def test_outputs_share_no_memory_with_inputs_or_each_other():
+    """Column slices side by side do not share any; shifted ones, rows of another distance and the same tensor twice do."""
+    wide = _z(6, 40)
+    st = _z(2, 3, 8)
+    for x, y in ((wide[:, :8], wide[:, 4:12]), (wide[:, 4:12], wide[:, :8]), (wide[:, :8], wide.view(-1)[8:56].view(6, 8)), (wide[:4, :8], wide[2:, :8])):
+        n = x.shape[0]
+        with pytest.raises(ValueError, match='y must not be one of the inputs or share'):
+            _conv(x=x, y=y[:n])
+    with pytest.raises(ValueError, match='state_out must not share memory with another output'):
+        _conv(y=st.view(6, 8), state_out=st)
+    grads = _z(6, 64)
+    slices = dict(dx=grads[:, :32].unflatten(1, (4, 8)), ddt=grads[:, 32:36], dB=_z(6, 2, 16), dC=_z(6, 2, 16))
+    for change, name in ((dict(dC=slices['dB']), 'dC'), (dict(ddt=grads[:, 31:35]), 'ddt'), (dict(ddt=grads[:, 28:32]), 'ddt')):
+        with pytest.raises(ValueError, match='%s must not share memory with another output' % name):
+            _scan_bwd(**{**slices, **change})
+    with pytest.raises(_lib.DotaHipError, match='GPU'):                      # all of them side by side: refused for the missing GPU only
+        _scan_bwd(**slices)
+    with pytest.raises(_lib.DotaHipError, match='GPU'):
+        _conv(x=wide[:, :8], y=wide[:, 8:16])
+    # in place: the states of a step and the residual, as they are, not shifted
+    both = _z(3, 3, 8)
+    step = lambda s, o: ops.causal_conv_step(_z(2, 8), s, _z(8, 4), None, state_out=o)      # noqa: E731
+    with pytest.raises(_lib.DotaHipError, match='GPU'):
+        step(both[:2], both[:2])
+    with pytest.raises(ValueError, match='state_out must not'):
+        step(both[:2], both[1:])
+    r = _z(7, 8)
+    with pytest.raises(_lib.DotaHipError, match='GPU'):
+        ops.block_norm(_z(6, 8), r[:6], _z(8), residual_out=r[:6])
+    with pytest.raises(ValueError, match='residual_out must not'):
+        ops.block_norm(_z(6, 8), r[:6], _z(8), residual_out=r[1:])
+
+
+def test_a_single_row_may_lie_anywhere():
+    """The distance of one row to the next says nothing where there is no next one."""
+    x = _z(1, 2).expand(1, 2).as_strided((1, 2), (1 << 40, 1))
+    assert x.stride(0) == 1 << 40 and ops._rows(x, 'x', torch.float32, (1, 2)) == 2
+    assert ops._rows(_z(1, 4, 2).as_strided((1, 4, 2), (1 << 40, 2, 1)), 'x', torch.float32, (1, 4, 2)) == 8
+
+
+def test_sizes_past_the_launch_limits_are_refused():
+    """Before anything is launched: a launch takes 2^32 threads along x, row numbers of a sequence stay in an int."""
+    lib = _lib.load()
+    P = 4096
+    top = 2 ** 31 - 256
+    conv = lambda rows, n, m: lib.dc_causal_conv_fwd(P, 8, P, None, P, P, rows, n, m, 8, 4, 0, 1, None, P, 8, P, None)      # noqa: E731
+    assert conv(1 << 40, 1, top + 1) == 1103 and conv(1 << 40, 5, top) == 1103
+    assert lib.dc_causal_conv_step(P, 1 << 20, P, P, None, 1 << 24, 1 << 20, 4, 0, 1, P, 1 << 20, P, None) == 1103
+    assert lib.dc_block_norm_fwd(P, 8192, None, 0, P, 8192, P, None, None, 1 << 23, 8192, 0, 0, 1e-5, P, 8192, None, 0, None) == 1103
+    assert lib.dc_block_norm_fwd(P, 8, None, 0, P, 8, P, None, None, 1 << 26, 8, 0, 0, 1e-5, P, 8, None, 0, None) == 1103
+    assert lib.dc_ssm_step(P, 64, P, 1, P, P, 16, P, 16, None, None, None, 1 << 22, 1, 64, 1, 16, 0, 0, P, 64, P, None) == 1103
+    scan = lambda n, m: lib.dc_ssm_scan_fwd(P, 256, P, 4, P, P, 16, P, 16, None, None, None, P, P, 1 << 30, n, m, 4, 64, 1, 16, 0, 0, P, 256, P, None, 0, None)      # noqa: E731
+    assert scan(1 << 22, 1) == 1103 and scan(1, top + 1) == 1103
+
+
 def test_norm_gradients_go_with_their_inputs():
     a = (_z(6, 8), _z(6, 8), _z(8))
     with pytest.raises(ValueError, match='dx: expected exactly with w_pre'):
