@@ -18,9 +18,9 @@ struct FwdLds {
     Steps st[2];
 };
 
-// ROWS: rows of a block.
+// ROWS: rows of a block; 32 where no sequence is longer, so that there is one block.
 template <typename T, int NP, int V, int ROWS>
-__global__ void __launch_bounds__(256, V > 1 && NP <= 64 ? (ROWS == 32 ? 4 : sizeof(T) == 2 ? 3 : 2) : 1) ssm_fwd_kernel(SsmArgs a) {
+__global__ void __launch_bounds__(256, V > 1 ? (NP > 64 ? (sizeof(T) == 2 || ROWS == 32 ? 2 : 1) : ROWS == 32 ? 4 : sizeof(T) == 2 ? 3 : 2) : 1) ssm_fwd_kernel(SsmArgs a) {
     typedef Mat<T> M;
     typedef typename Four<T>::vec four_t;
     constexpr int LX = pitch<T>(PT), LN = pitch<T>(NP), LM = pitch<T>(ROWS), NK = NP / M::KS, NT = ROWS / 16;
@@ -61,10 +61,10 @@ __global__ void __launch_bounds__(256, V > 1 && NP <= 64 ? (ROWS == 32 ? 4 : siz
             tc.template load<false>(cp + t0 * a.ldc, a.ldc, rows);
         }
     };
-    // step sizes: wave 3 makes those of the next block from what it loaded one block before
+    // step sizes: wave 3 sums those of the next block up from what it loaded one block before
     auto fetch_dt = [&](int blk) { return dp[min((int64_t)blk * ROWS + lane, (int64_t)q.len - 1) * a.lddt]; };
-    auto steps = [&](int blk, T raw) {
-        make_steps<false, true>(L.st[blk & 1], a, (float)raw, lane < ROWS && (int64_t)blk * ROWS + lane < q.len, A, bias, lane);
+    auto sums = [&](int blk, T raw) {
+        make_sums(L.st[blk & 1], a, (float)raw, lane < ROWS && (int64_t)blk * ROWS + lane < q.len, A, bias, lane);
     };
     T raw = (T)0.f;
     if (first < last) {
@@ -73,19 +73,26 @@ __global__ void __launch_bounds__(256, V > 1 && NP <= 64 ? (ROWS == 32 ? 4 : siz
     }
     load_state<NP, V>(S, init, N, p0, P, N, i, g);
     if (first < last && wave == 3) {
-        steps(first, raw);
-        raw = fetch_dt(first + 1);
+        sums(first, raw);
+        if (ROWS == 32) {                                  // the only block: its factors without a barrier in between
+#pragma unroll
+            for (int w = 0; w < 4; ++w) make_factors<false, true>(L.st[first & 1], w, lane);
+        } else {
+            raw = fetch_dt(first + 1);
+        }
     }
+    if (ROWS == 64) __syncthreads();
     auto block = [&](int blk, auto full_t) {
         constexpr bool FULL = decltype(full_t)::value;
         const int64_t t0 = (int64_t)blk * ROWS;
         const int rows = FULL ? ROWS : q.len - (int)t0;
-        const Steps& st = L.st[blk & 1];
+        Steps& st = L.st[blk & 1];
+        if (ROWS == 64) make_factors<false, true>(st, wave, lane);
         tx.template store<FULL>(L.x, LX, rows, all_p);
         tb.template store<FULL>(L.b, LN, rows, all_n);
         tc.template store<FULL>(L.c, LN, rows, all_n);
         __syncthreads();
-        if (blk + 1 < last) fetch(blk + 1);
+        if (ROWS == 64 && blk + 1 < last) fetch(blk + 1);
         // M, as (C B^T)^T: lane i owns row t, four neighbouring s of it.  64 rows: a wave takes a diagonal tile, one below, and one below or a zero
         // one; 32 rows: 00, 11, 10 and the zero 01.
         constexpr int TILES = ROWS == 64 ? 3 : 1;
@@ -97,38 +104,78 @@ __global__ void __launch_bounds__(256, V > 1 && NP <= 64 ? (ROWS == 32 ? 4 : siz
             js[u] = ROWS == 64 ? tile_col(wave + 4 * u) : (0x1010 >> (4 * wave)) & 15;
             m[u] = f32x4{};
         }
+        // exp(a_t - a_s) dt_s; it needs none of the products, so it runs beside them
+        f32x4 l[TILES];
+        auto decays = [&]() {
+#pragma unroll
+            for (int u = 0; u < TILES; ++u) {
+                const int t = 16 * jt[u] + i, s = 16 * js[u] + 4 * g;
+                if (ROWS == 64 ? u == 0 : wave < 2) {
+                    const float ht = st.hi[t], lt = st.lo[t];
+                    const f32x4 hs = *reinterpret_cast<const f32x4*>(st.hi + s), ls = *reinterpret_cast<const f32x4*>(st.lo + s),
+                                ds = *reinterpret_cast<const f32x4*>(st.dt + s);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) l[u][r] = exp_f((ht - hs[r]) + (lt - ls[r])) * ds[r];
+                } else {
+                    l[u] = *reinterpret_cast<const f32x4*>(st.cd + s) * (st.rf[t] * between(st, jt[u], js[u]));
+                }
+            }
+        };
+        // The fragments of the next step are on their way while this one's products run, here and below: left to itself the compiler reads one
+        // fragment, waits for it and multiplies.
+        auto products = [&](auto u0, auto u1) {
+            constexpr int U0 = decltype(u0)::value, U1 = decltype(u1)::value;
+            typename M::frag fb[2][U1 - U0], fc[2][U1 - U0];
+            auto fragments = [&](int k) {
+#pragma unroll
+                for (int u = U0; u < U1; ++u) {
+                    fb[k & 1][u - U0] = M::row(L.b + 16 * js[u] * LN + k * M::KS, LN, i, g);
+                    fc[k & 1][u - U0] = M::row(L.c + 16 * jt[u] * LN + k * M::KS, LN, i, g);
+                }
+            };
+            fragments(0);
+            if (U0 == 0) decays();
+#pragma unroll
+            for (int k = 0; k < NK; ++k) {
+                if (k + 1 < NK) fragments(k + 1);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int u = U0; u < U1; ++u) m[u] = M::mma(fb[k & 1][u - U0], fc[k & 1][u - U0], m[u]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
         // (the zero tile's products are left out where they cost: f32)
-        const int real = sizeof(T) == 4 && TILES == 3 && wave >= 2 ? 2 : TILES;
-#pragma unroll
-        for (int k = 0; k < NK; ++k)
-#pragma unroll
-            for (int u = 0; u < TILES; ++u)
-                if (u < 2 || real == 3) m[u] = M::mma(M::row(L.b + 16 * js[u] * LN + k * M::KS, LN, i, g), M::row(L.c + 16 * jt[u] * LN + k * M::KS, LN, i, g), m[u]);
+        typedef std::integral_constant<int, 0> zero_t;
+        if constexpr (sizeof(T) == 4 && TILES == 3) {
+            products(zero_t{}, std::integral_constant<int, 2>{});
+            if (wave < 2) products(std::integral_constant<int, 2>{}, std::integral_constant<int, 3>{});
+        } else {
+            products(zero_t{}, std::integral_constant<int, TILES>{});
+        }
 #pragma unroll
         for (int u = 0; u < TILES; ++u) {
             const int t = 16 * jt[u] + i, s = 16 * js[u] + 4 * g;
-            if (ROWS == 64 ? u == 0 : wave < 2) {
-                const float ht = st.hi[t], lt = st.lo[t];
-                const f32x4 hs = *reinterpret_cast<const f32x4*>(st.hi + s), ls = *reinterpret_cast<const f32x4*>(st.lo + s),
-                            ds = *reinterpret_cast<const f32x4*>(st.dt + s);
+            const bool diagonal = ROWS == 64 ? u == 0 : wave < 2, below = js[u] < jt[u];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) m[u][r] = s + r <= t ? m[u][r] * (exp_f((ht - hs[r]) + (lt - ls[r])) * ds[r]) : 0.f;
-            } else {
-                const float f = st.rf[t] * between(st, jt[u], js[u]);
-                const f32x4 cd = *reinterpret_cast<const f32x4*>(st.cd + s);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) m[u][r] = js[u] < jt[u] ? m[u][r] * (f * cd[r]) : 0.f;
+            for (int r = 0; r < 4; ++r) {
+                const float v = m[u][r] * l[u][r];
+                m[u][r] = (diagonal ? s + r <= t : below) ? v : 0.f;
             }
             *reinterpret_cast<four_t*>(L.m + t * LM + s) = four<T>(m[u]);
         }
-        if (wave == 3 && blk + 1 < last) {
-            steps(blk + 1, raw);
+        if (ROWS == 64 && wave == 3 && blk + 1 < last) {
+            sums(blk + 1, raw);
             raw = fetch_dt(blk + 2);
         }
         __syncthreads();
         f32x4 y[NT];
-        const bool have = state_in_front(a, blk);
-        {
+        constexpr int MK = ROWS / M::KS;
+        typename M::frag xf[MK], fr[2][NT];
+#pragma unroll
+        for (int k = 0; k < MK; ++k) xf[k] = M::col(L.x + k * M::KS * LX + p0, LX, i, g);
+#pragma unroll
+        for (int jt = 0; jt < NT; ++jt) y[jt] = f32x4{};
+        if (state_in_front(a, blk)) {
             // S is rounded once to bf16 here, like M: both only end in y
             typename M::frag sf[NK];
 #pragma unroll
@@ -140,22 +187,40 @@ __global__ void __launch_bounds__(256, V > 1 && NP <= 64 ? (ROWS == 32 ? 4 : siz
                     for (int e = 0; e < 8; ++e) sf[k][e] = (T)S[2 * k + (e >> 2)][e & 3];
                 }
             }
+            auto fragments = [&](int k) {
 #pragma unroll
-            for (int jt = 0; jt < NT; ++jt) {
-                y[jt] = f32x4{};
-                if ((!FULL && 16 * jt >= rows) || !have) continue;
+                for (int jt = 0; jt < NT; ++jt) fr[k & 1][jt] = M::row(L.c + 16 * jt * LN + k * M::KS, LN, i, g);
+            };
+            fragments(0);
 #pragma unroll
-                for (int k = 0; k < NK; ++k) y[jt] = M::mma(sf[k], M::row(L.c + 16 * jt * LN + k * M::KS, LN, i, g), y[jt]);
-                y[jt] *= st.ea[16 * jt + i];
+            for (int k = 0; k < NK; ++k) {
+                if (k + 1 < NK) fragments(k + 1);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int jt = 0; jt < NT; ++jt)
+                    if (FULL || 16 * jt < rows) y[jt] = M::mma(sf[k], fr[k & 1][jt], y[jt]);
+                __builtin_amdgcn_sched_barrier(0);
             }
+#pragma unroll
+            for (int jt = 0; jt < NT; ++jt) y[jt] *= st.ea[16 * jt + i];
         }
+        {
+            auto fragments = [&](int k) {
 #pragma unroll
-        for (int k = 0; k < ROWS; k += M::KS) {
-            if (!FULL && k >= rows) continue;
-            const typename M::frag xf = M::col(L.x + k * LX + p0, LX, i, g);
+                for (int jt = 0; jt < NT; ++jt)
+                    if (16 * jt + 16 > k * M::KS) fr[k & 1][jt] = M::row(L.m + 16 * jt * LM + k * M::KS, LM, i, g);
+            };
+            fragments(0);
 #pragma unroll
-            for (int jt = k / 16; jt < NT; ++jt)
-                if (FULL || 16 * jt < rows) y[jt] = M::mma(xf, M::row(L.m + 16 * jt * LM + k, LM, i, g), y[jt]);
+            for (int k = 0; k < MK; ++k) {
+                if (!FULL && k * M::KS >= rows) break;
+                if (k + 1 < MK) fragments(k + 1);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int jt = 0; jt < NT; ++jt)
+                    if (16 * jt + 16 > k * M::KS && (FULL || 16 * jt < rows)) y[jt] = M::mma(xf[k], fr[k & 1][jt], y[jt]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
 #pragma unroll
         for (int jt = 0; jt < NT; ++jt) {
@@ -177,7 +242,7 @@ __global__ void __launch_bounds__(256, V > 1 && NP <= 64 ? (ROWS == 32 ? 4 : siz
         const float et = st.decay;
 #pragma unroll
         for (int c = 0; c < NP / 16; ++c) S[c] *= et;
-        state_update<T, NP, ROWS>(S, L.x, LX, L.b, LN, st.w, p0, rows, i, g);
+        state_update<T, NP, ROWS>(S, xf, L.b, LN, st.w, rows, i, g);
         __syncthreads();
     };
     const int whole = min(last, q.len / ROWS);
@@ -247,15 +312,17 @@ __device__ __forceinline__ void states(const SsmArgs& a, StateLds<T, NP>& L) {
         if (wave == 3) raw = fetch_dt(block(0));
         fetch(block(0));
         if (wave == 3) {
-            make_steps<REV, !REV && !FINAL>(L.st[0], a, (float)raw, block(0) * TB + lane < q.len, A, bias, lane);
+            make_sums(L.st[0], a, (float)raw, block(0) * TB + lane < q.len, A, bias, lane);
             raw = fetch_dt(block(1));
         }
     }
+    __syncthreads();
     for (int j = 0; j < last - first; ++j) {
         const int blk = block(j);
         const int rows = min(TB, q.len - blk * TB);
-        const Steps& st = L.st[j & 1];
+        Steps& st = L.st[j & 1];
         const bool more = j + 1 < last - first;
+        make_factors<REV, !REV && !FINAL>(st, wave, lane);
         if (blk == unasked) {
         } else if (rows == TB) {
             tx.template store<true>(L.x, LX, TB, all_p);
@@ -281,10 +348,13 @@ __device__ __forceinline__ void states(const SsmArgs& a, StateLds<T, NP>& L) {
             const float et = st.decay;
 #pragma unroll
             for (int c = 0; c < NP / 16; ++c) S[c] *= et;
-            state_update<T, NP, TB>(S, L.x, LX, L.b, LN, st.w, p0, rows, i, g);
+            typename Mat<T>::frag xf[TB / Mat<T>::KS];
+#pragma unroll
+            for (int k = 0; k < TB / Mat<T>::KS; ++k) xf[k] = Mat<T>::col(L.x + k * Mat<T>::KS * LX + p0, LX, i, g);
+            state_update<T, NP, TB>(S, xf, L.b, LN, st.w, rows, i, g);
         }
         if (wave == 3 && more) {
-            make_steps<REV, !REV && !FINAL>(L.st[(j + 1) & 1], a, (float)raw, block(j + 1) * TB + lane < q.len, A, bias, lane);
+            make_sums(L.st[(j + 1) & 1], a, (float)raw, block(j + 1) * TB + lane < q.len, A, bias, lane);
             raw = fetch_dt(block(j + 2));
         }
         __syncthreads();
@@ -298,7 +368,7 @@ __device__ __forceinline__ void states(const SsmArgs& a, StateLds<T, NP>& L) {
 }
 
 template <typename T, int NP, int V, bool FINAL>
-__global__ void __launch_bounds__(256) ssm_states_kernel(SsmArgs a) {
+__global__ void __launch_bounds__(256, V > 1 ? (NP > 64 ? 2 : sizeof(T) == 2 || NP == 32 ? 4 : 3) : 1) ssm_states_kernel(SsmArgs a) {
     __shared__ __attribute__((aligned(16))) StateLds<T, NP> L;
     if (blockIdx.y == 0) states<T, NP, V, false, FINAL>(a, L);
     else states<T, NP, V, true, FINAL>(a, L);

@@ -236,20 +236,13 @@ __device__ __forceinline__ float exp_f(float x) {
     const float c = fmaf(r * e, LN2, r);
     return c == c ? c : r;
 }
-__device__ __forceinline__ float exp_f(double x) {
-    double p = x * 1.4426950408889634;
-    p = p > 2000.0 ? 2000.0 : p < -2000.0 ? -2000.0 : p;                  // a NaN stays one
-    const double n = rint(p);
-    return ldexpf(__builtin_amdgcn_exp2f((float)(p - n)), (int)n);
-}
-
-// The block's step sizes and running sums (one wave, lane = row).  a is kept as hi + lo, so that exp(a_t - a_s) of neighbouring rows does not lose
+// The block's step sizes and running sums.  a is kept as hi + lo, so that exp(a_t - a_s) of neighbouring rows does not lose
 // what a long sum costs: a is summed in f64, the difference is taken of both halves.
 struct Steps {
     float dt[TB], hi[TB], lo[TB];
     float ea[TB], es[TB];                         // exp(a_t), exp(a_T - a_t)
     float rf[TB], cf[TB];                         // exp(a_t - a of its tile of 16's first row), exp(a of its tile's last row - a_t)
-    float w[TB], cd[TB];                          // see make_steps; dt_t cf_t
+    float w[TB], cd[TB];                          // see make_factors; dt_t cf_t
     float total, decay;                           // a of the last row, exp of it
 };
 constexpr int STEPS_KEPT = 7 * TB;                // what the backward kernel takes over from the forward states' pass: dt .. cf
@@ -259,30 +252,38 @@ __device__ __forceinline__ float between(const Steps& s, int jt, int js) {
     return exp_f((s.hi[16 * jt] - s.hi[16 * js + 15]) + (s.lo[16 * jt] - s.lo[16 * js + 15]));
 }
 
-// w[t] = dt_t exp(a_T - a_t): the weights of the block's rows in the state behind it; REV: exp(a_t), those of the gradients in the one in front.
-// FACTORS: ea, es, rf, cf, cd too.
-template <bool REV, bool FACTORS>
-__device__ __forceinline__ void make_steps(Steps& s, const SsmArgs& a, float raw, bool live, float A, float bias, int lane) {
+// What stands in a Steps is made in two parts, one a phase of the kernel before the other: the sums, by one wave, lane = row; and from them the
+// factors, shared out over the waves.  (One wave with all of it kept the others waiting for 1 700 of a block's 14 000 cycles.)
+__device__ __forceinline__ void make_sums(Steps& s, const SsmArgs& a, float raw, bool live, float A, float bias, int lane) {
     float d = raw + bias;
     if (a.softplus) d = softplus_f(d);
     if (!live) d = 0.f;
-    const double sum = lane_prefix((double)d * (double)A), last = last_lane(sum);
+    const double sum = lane_prefix((double)d * (double)A);
     s.dt[lane] = d;
     s.hi[lane] = (float)sum;
     s.lo[lane] = (float)(sum - (double)(float)sum);
-    const float es = exp_f(last - sum);
-    s.w[lane] = REV ? exp_f(sum) : d * es;
-    if (FACTORS) {
-        const float cf = exp_f(dpp<ROW_NEWBCAST + 15>(sum) - sum);
-        s.ea[lane] = exp_f(sum);
-        s.es[lane] = es;
-        s.rf[lane] = exp_f(sum - dpp<ROW_NEWBCAST>(sum));
-        s.cf[lane] = cf;
-        s.cd[lane] = d * cf;
+}
+// w[t] = dt_t exp(a_T - a_t): the weights of the block's rows in the state behind it; REV: exp(a_t), those of the gradients in the one in front.
+// FACTORS: ea, es, rf, cf, cd too.  Waves 0 .. 3.
+template <bool REV, bool FACTORS>
+__device__ __forceinline__ void make_factors(Steps& s, int wave, int lane) {
+    const float hi = s.hi[lane], lo = s.lo[lane];
+    if (wave == 0) {
+        const float hT = last_lane(hi), lT = last_lane(lo), es = exp_f((hT - hi) + (lT - lo)), ea = REV ? exp_f(hi + lo) : 0.f;
+        s.w[lane] = REV ? ea : s.dt[lane] * es;
+        if (FACTORS) s.es[lane] = es;
+        if (lane == 63) {
+            s.total = hi;
+            s.decay = exp_f(hi + lo);
+        }
     }
-    if (lane == 63) {
-        s.total = (float)last;
-        s.decay = exp_f(last);
+    if (!FACTORS) return;
+    if (wave == 1) s.ea[lane] = exp_f(hi + lo);
+    if (wave == 2) s.rf[lane] = exp_f((hi - dpp<ROW_NEWBCAST>(hi)) + (lo - dpp<ROW_NEWBCAST>(lo)));
+    if (wave == 3) {
+        const float cf = exp_f((dpp<ROW_NEWBCAST + 15>(hi) - hi) + (dpp<ROW_NEWBCAST + 15>(lo) - lo));
+        s.cf[lane] = cf;
+        s.cd[lane] = s.dt[lane] * cf;
     }
 }
 
@@ -301,33 +302,45 @@ __device__ __forceinline__ void split_bf16(float v, bf16_t (&p)[PIECES_F32]) {
 // they are at once the operand of the products over n, and a lane's four neighbouring n leave in one access.
 // The weights are f32: bf16 operands are scaled in f32 and used as three bf16 pieces, because the states they end in are f32 (with two pieces, 16 bits,
 // the gradients of A and dt_bias were off by 4e-6 .. 8e-6 of their norm, with three by what f32 sums are off by).
+// x: the wave's columns of X, as col() fragments of the block's row steps.
 template <typename T, int NP, int ROWS>
-__device__ __forceinline__ void state_update(f32x4 (&acc)[NP / 16], const T* X, int ldx, const T* Y, int ldy, const float* w, int p0, int rows, int i, int g) {
+__device__ __forceinline__ void state_update(f32x4 (&acc)[NP / 16], const typename Mat<T>::frag (&x)[ROWS / Mat<T>::KS], const T* Y, int ldy, const float* w, int rows, int i,
+                                             int g) {
     typedef Mat<T> M;
+    constexpr int NC = NP / 16, BATCH = NC < ROWS / 16 ? NC : ROWS / 16, PER_K = NC / BATCH, STEPS = ROWS / M::KS * PER_K;
+    typename M::frag y[2][BATCH];
+    auto fetch = [&](int s) {
 #pragma unroll
-    for (int k = 0; k < ROWS; k += M::KS) {
-        if (k >= rows) break;
-        typename M::frag x = M::col(X + k * ldx + p0, ldx, i, g);
+        for (int c = 0; c < BATCH; ++c) y[s & 1][c] = M::col(Y + s / PER_K * M::KS * ldy + 16 * (s % PER_K * BATCH + c), ldy, i, g);
+    };
+    fetch(0);
+#pragma unroll
+    for (int k = 0; k < ROWS / M::KS; ++k) {
+        if (k * M::KS >= rows) break;
+        constexpr int NPC = sizeof(T) == 4 ? 1 : PIECES_F32;
+        typename M::frag piece[NPC];
         if constexpr (sizeof(T) == 4) {
-            x *= *reinterpret_cast<const f32x4*>(w + k + 4 * g);
-#pragma unroll
-            for (int c = 0; c < NP / 16; ++c) acc[c] = M::mma(M::col(Y + k * ldy + 16 * c, ldy, i, g), x, acc[c]);
+            piece[0] = x[k] * *reinterpret_cast<const f32x4*>(w + k * M::KS + 4 * g);
         } else {
-            const f32x4 w0 = *reinterpret_cast<const f32x4*>(w + k + 4 * g), w1 = *reinterpret_cast<const f32x4*>(w + k + 16 + 4 * g);
-            typename M::frag piece[PIECES_F32];
+            const f32x4 w0 = *reinterpret_cast<const f32x4*>(w + k * M::KS + 4 * g), w1 = *reinterpret_cast<const f32x4*>(w + k * M::KS + 16 + 4 * g);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 bf16_t v[PIECES_F32];
-                split_bf16((float)x[e] * (e < 4 ? w0[e & 3] : w1[e & 3]), v);
+                split_bf16((float)x[k][e] * (e < 4 ? w0[e & 3] : w1[e & 3]), v);
 #pragma unroll
                 for (int pc = 0; pc < PIECES_F32; ++pc) piece[pc][e] = v[pc];
             }
+        }
 #pragma unroll
-            for (int c = 0; c < NP / 16; ++c) {
-                const typename M::frag y = M::col(Y + k * ldy + 16 * c, ldy, i, g);
+        for (int b = 0; b < PER_K; ++b) {
+            const int s = k * PER_K + b;
+            if (s + 1 < STEPS) fetch(s + 1);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int pc = PIECES_F32 - 1; pc >= 0; --pc) acc[c] = M::mma(y, piece[pc], acc[c]);
-            }
+            for (int pc = NPC - 1; pc >= 0; --pc)
+#pragma unroll
+                for (int c = 0; c < BATCH; ++c) acc[b * BATCH + c] = M::mma(y[s & 1][c], piece[pc], acc[b * BATCH + c]);
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
 }
