@@ -257,11 +257,27 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ssm_bwd_kernel(SsmArgs a) {
         for (int u = 0; u < GT; ++u) G2[u] = f32x4{};
         // (the products of a tile that is not there are left out where they cost: f32)
         const bool all_real = sizeof(T) == 2 || wave + WAVES * (GT - 1) < 10;
+        {
+            // here and below: the next step's fragments are on their way while this one's products run.  (dx's phase has no registers for it: 225 -> 234 us
+            // for 65 536 f32 rows with what that spills.)
+            typename M::frag fy[2][GT], fx[2][GT];
+            auto fragments = [&](int k) {
 #pragma unroll
-        for (int k = 0; k < PK; ++k) {
+                for (int u = 0; u < GT; ++u) {
+                    fy[k & 1][u] = M::row(L.y + 16 * jt_of[u] * LX + k * M::KS, LX, i, g);
+                    fx[k & 1][u] = M::row(L.x + 16 * js_of[u] * LX + k * M::KS, LX, i, g);
+                }
+            };
+            fragments(0);
 #pragma unroll
-            for (int u = 0; u < GT; ++u)
-                if (u + 1 < GT || all_real) G2[u] = M::mma(M::row(L.y + 16 * jt_of[u] * LX + k * M::KS, LX, i, g), M::row(L.x + 16 * js_of[u] * LX + k * M::KS, LX, i, g), G2[u]);
+            for (int k = 0; k < PK; ++k) {
+                if (k + 1 < PK) fragments(k + 1);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int u = 0; u < GT; ++u)
+                    if (u + 1 < GT || all_real) G2[u] = M::mma(fy[k & 1][u], fx[k & 1][u], G2[u]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
         if (!WIDE || pt == 0) {
 #pragma unroll
@@ -314,16 +330,22 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ssm_bwd_kernel(SsmArgs a) {
         }
         if (have_S) {
             const Pieces<T> f(S.v);
+            typename M::frag fy[2][PK];
+            auto fragments = [&](int j) {
+#pragma unroll
+                for (int k = 0; k < PK; ++k) fy[j & 1][k] = M::row(L.y + 16 * (jt0 + WT * j) * LX + k * M::KS, LX, i, g);
+            };
+            fragments(0);
 #pragma unroll
             for (int j = 0; j < JT; ++j) {
                 const int t = 16 * (jt0 + WT * j);
                 f32x4 acc = {};
+                if (j + 1 < JT) fragments(j + 1);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int k = 0; k < PK; ++k) {
-                    const typename M::frag y = M::row(L.y + t * LX + k * M::KS, LX, i, g);
+                for (int k = 0; k < PK; ++k)
 #pragma unroll
-                    for (int pc = Pieces<T>::N - 1; pc >= 0; --pc) acc = M::mma(f.f[pc][k], y, acc);
-                }
+                    for (int pc = Pieces<T>::N - 1; pc >= 0; --pc) acc = M::mma(f.f[pc][k], fy[j & 1][k], acc);
                 acc *= st.ea[t + i];
                 dC[j] += acc;
 #pragma unroll
@@ -335,16 +357,22 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ssm_bwd_kernel(SsmArgs a) {
         fetch_rows(h, pt);
         if (have_dS) {
             const Pieces<T> f(dS.v);
+            typename M::frag fx[2][PK];
+            auto fragments = [&](int j) {
+#pragma unroll
+                for (int k = 0; k < PK; ++k) fx[j & 1][k] = M::row(L.x + 16 * (jt0 + WT * j) * LX + k * M::KS, LX, i, g);
+            };
+            fragments(0);
 #pragma unroll
             for (int j = 0; j < JT; ++j) {
                 const int s = 16 * (jt0 + WT * j);
                 f32x4 acc = {};
+                if (j + 1 < JT) fragments(j + 1);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int k = 0; k < PK; ++k) {
-                    const typename M::frag x = M::row(L.x + s * LX + k * M::KS, LX, i, g);
+                for (int k = 0; k < PK; ++k)
 #pragma unroll
-                    for (int pc = Pieces<T>::N - 1; pc >= 0; --pc) acc = M::mma(f.f[pc][k], x, acc);
-                }
+                    for (int pc = Pieces<T>::N - 1; pc >= 0; --pc) acc = M::mma(f.f[pc][k], fx[j & 1][k], acc);
                 acc *= st.es[s + i];
                 const float ds = st.dt[s + i];
                 const four_t bv = *reinterpret_cast<const four_t*>(L.b + (s + i) * LN + n0 + 4 * g);
