@@ -403,7 +403,7 @@ def run_workload(cell, hidden, layers, B, S, E, steps, warmup, dev, rank, world,
     barrier()
     elapsed = time.perf_counter() - t0
     if world > 1:
-        t = torch.tensor([elapsed], dtype=torch.float64, device=dev)
+        t = torch.tensor([elapsed], dtype=torch.float64, device='cpu' if torch.distributed.get_backend() == 'gloo' else dev)
         torch.distributed.all_reduce(t, op=torch.distributed.ReduceOp.MAX)
         elapsed = float(t.item())
     res['elapsed'] = elapsed

@@ -20,6 +20,25 @@ def is_distributed():
     return dist.is_available() and dist.is_initialized() and dist.get_world_size() > 1
 
 
+def over_host(device, group=None):
+    """Whether collectives of `device`'s tensors go through host memory: gloo is given CPU tensors only.  (Its collectives on GPU tensors run on
+    streams of another priority, and have hung the GPU where several ranks share one.)"""
+    return device.type == 'cuda' and torch.distributed.is_initialized() and torch.distributed.get_backend(group) == 'gloo'
+
+
+class HostCollective:
+    """A collective of a GPU tensor on a copy of it in host memory: copied there synchronously, and back by wait()."""
+
+    def __init__(self, call, t, **how):
+        self.t, self.host = t, t.to('cpu', copy=True)
+        self.work = call(self.host, **how)
+
+    def wait(self):
+        if self.work is not None:
+            self.work.wait()
+        self.t.copy_(self.host)
+
+
 class FlatGradAllReducer:
     """overlap (default on; DC_DP_OVERLAP=0 or overlap=False for the single collective): the bucket is reduced in two
     collectives.  The gradients of every parameter from affine_pre_rnn on (82 % of the bucket, final once the first half of the
@@ -39,11 +58,15 @@ class FlatGradAllReducer:
         self.bucket = torch.zeros(engine.total + 8, dtype=torch.float32, device=dev)
         engine.grads = self.bucket[:engine.total]
         self.tail = self.bucket[engine.total:]
+        self.over_host = over_host(self.bucket.device, group)
 
     def sync_parameters(self):
         """distributed.py:71-74: every rank starts from rank 0's weights (one broadcast of the flat buffer)."""
         if self.world > 1:
-            dist.broadcast(self.engine.params, src=0, group=self.group)
+            if self.over_host:
+                HostCollective(dist.broadcast, self.engine.params, src=0, group=self.group).wait()
+            else:
+                dist.broadcast(self.engine.params, src=0, group=self.group)
             self.engine.params_changed()
 
     def _set_tail(self, engine):
@@ -55,13 +78,13 @@ class FlatGradAllReducer:
         if self.world <= 1:
             return
         self._set_tail(engine)
-        self._work = dist.all_reduce(self.bucket[engine.embed_floats:], op=dist.ReduceOp.SUM, group=self.group, async_op=True)
+        self._work = self._all_reduce(self.bucket[engine.embed_floats:], async_op=True)
 
     def finish(self, engine):
         """After the second half: reduce the embedding gradients, join the first collective, average."""
         if self.world <= 1:
             return
-        dist.all_reduce(self.bucket[:engine.embed_floats], op=dist.ReduceOp.SUM, group=self.group)
+        self._all_reduce(self.bucket[:engine.embed_floats])
         self._work.wait()
         self._work = None
         self._average(engine)
@@ -71,8 +94,14 @@ class FlatGradAllReducer:
         if self.world <= 1:
             return
         self._set_tail(engine)
-        dist.all_reduce(self.bucket, op=dist.ReduceOp.SUM, group=self.group)
+        self._all_reduce(self.bucket)
         self._average(engine)
+
+    def _all_reduce(self, t, async_op=False):
+        if not self.over_host:
+            return dist.all_reduce(t, op=dist.ReduceOp.SUM, group=self.group, async_op=async_op)
+        work = HostCollective(dist.all_reduce, t, op=dist.ReduceOp.SUM, group=self.group, async_op=async_op)
+        return work if async_op else work.wait()
 
     def _average(self, engine):
         _lib.check(engine.lib.dc_dp_average_grads(

@@ -464,7 +464,9 @@ class DotaOptimizer:
             # agreed on (the team kernels' fault record is rank-local)
             any_fault = None
             if self.grad_hook is not None and getattr(self.grad_hook, 'world', 1) > 1:
-                flag = torch.tensor([1.0 if self.engine.fault() is not None else 0.0], device=self.device)
+                from .distributed import over_host
+                flag = torch.tensor([1.0 if self.engine.fault() is not None else 0.0],
+                                    device='cpu' if over_host(self.device, self.grad_hook.group) else self.device)
                 torch.distributed.all_reduce(flag, op=torch.distributed.ReduceOp.MAX, group=self.grad_hook.group)
                 any_fault = bool(flag.item() > 0)
             was_fast = self.engine.products == 'f16x2'
