@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(256, V > 1 ? (NP > 64 ? (sizeof(T) == 2 || ROW
                     const f32x4 hs = *reinterpret_cast<const f32x4*>(st.hi + s), ls = *reinterpret_cast<const f32x4*>(st.lo + s),
                                 ds = *reinterpret_cast<const f32x4*>(st.dt + s);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) l[u][r] = exp_f((ht - hs[r]) + (lt - ls[r])) * ds[r];
+                    for (int r = 0; r < 4; ++r) l[u][r] = __expf((ht - hs[r]) + (lt - ls[r])) * ds[r];
                 } else {
                     l[u] = *reinterpret_cast<const f32x4*>(st.cd + s) * (st.rf[t] * between(st, jt[u], js[u]));
                 }
@@ -399,7 +399,7 @@ __global__ void __launch_bounds__(256) ssm_join_kernel(SsmArgs a) {
             if (j0 + k >= a.nseg) break;
             const int seg = rev ? a.nseg - 1 - (j0 + k) : j0 + k;
             buf[seg * n] = S;
-            S = fmaf(exp_f(d[k]), S, add[k]);
+            S = fmaf(__expf(d[k]), S, add[k]);
         }
     }
 }
@@ -414,7 +414,7 @@ __global__ void __launch_bounds__(256) ssm_step_kernel(SsmArgs a) {
     const int grp = h / (a.H / a.G);
     float d = (float)static_cast<const T*>(a.dt)[b * a.lddt + h] + (a.dt_bias ? a.dt_bias[h] : 0.f);
     if (a.softplus) d = softplus_f(d);
-    const float x = (float)static_cast<const T*>(a.x)[b * a.ldx + (int64_t)h * a.P + p], e = exp_f(d * a.A[h]), dx = d * x;
+    const float x = (float)static_cast<const T*>(a.x)[b * a.ldx + (int64_t)h * a.P + p], e = __expf(d * a.A[h]), dx = d * x;
     const T* B = static_cast<const T*>(a.B) + b * a.ldb + (int64_t)grp * a.N;
     const T* C = static_cast<const T*>(a.C) + b * a.ldc + (int64_t)grp * a.N;
     const int64_t at = (((int64_t)b * a.H + h) * a.P + p) * a.N;

@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) ssm_bwd_kernel(SsmArgs a) {
                     for (int r = 0; r < 4; ++r) {
                         // a product that is not finite stays out of what it does not belong to
                         const bool in = s <= t + r, strict = s < t + r;
-                        float e = exp_f((ht[r] - hs) + (lt[r] - ls));
+                        float e = __expf((ht[r] - hs) + (lt[r] - ls));
                         asm volatile("" : "+v"(e));                       // by every lane: no branch around it
                         const float l = in ? e : 0.f, gl = in ? G2[u][r] * l : 0.f, qv = in ? G1[u][r] * gl : 0.f;
                         m[r] = in ? G1[u][r] * l : 0.f;

@@ -227,17 +227,9 @@ template <typename F> __device__ __forceinline__ F lane_sum(F v) { return last_l
 
 __device__ __forceinline__ float softplus_f(float v) { return v > 20.f ? v : log1pf(expf(v)); }
 
-// exp(x) within 1.5 ulp: v_exp_f32 is exact enough, x * log2(e) is not - its rounding is 2^-24 of a number that may be 10 or 100 - so the part that the
-// rounding drops goes in behind.  Decays are factors of everything that is summed over a sequence; with the plain product the gradient of A
-// came out three times as far from 64 bits.  Where that part is no number (x infinite, or the result) the plain value stands.
-__device__ __forceinline__ float exp_f(float x) {
-    constexpr float L = 1.4426950216293335f, LO = 1.9259629911266175e-8f, LN2 = 0.6931471805599453f;      // log2(e) = L + LO
-    const float p = x * L, e = fmaf(x, LO, fmaf(x, L, -p)), r = __builtin_amdgcn_exp2f(p);
-    const float c = fmaf(r * e, LN2, r);
-    return c == c ? c : r;
-}
 // The block's step sizes and running sums.  a is kept as hi + lo, so that exp(a_t - a_s) of neighbouring rows does not lose
-// what a long sum costs: a is summed in f64, the difference is taken of both halves.
+// what a long sum costs: a is summed in f64, the difference is taken of both halves.  (Exponentials that are exact but for their last rounding instead of
+// __expf leave every gradient as far from 64 bits as it is.)
 struct Steps {
     float dt[TB], hi[TB], lo[TB];
     float ea[TB], es[TB];                         // exp(a_t), exp(a_T - a_t)
@@ -249,7 +241,7 @@ constexpr int STEPS_KEPT = 7 * TB;                // what the backward kernel ta
 // exp(a of row tile jt's first row - a of row tile js's last one), js < jt: with rf and cf the decay from s to t in three factors, none above 1 where
 // the decays are not.
 __device__ __forceinline__ float between(const Steps& s, int jt, int js) {
-    return exp_f((s.hi[16 * jt] - s.hi[16 * js + 15]) + (s.lo[16 * jt] - s.lo[16 * js + 15]));
+    return __expf((s.hi[16 * jt] - s.hi[16 * js + 15]) + (s.lo[16 * jt] - s.lo[16 * js + 15]));
 }
 
 // What stands in a Steps is made in two parts, one a phase of the kernel before the other: the sums, by one wave, lane = row; and from them the
@@ -269,19 +261,19 @@ template <bool REV, bool FACTORS>
 __device__ __forceinline__ void make_factors(Steps& s, int wave, int lane) {
     const float hi = s.hi[lane], lo = s.lo[lane];
     if (wave == 0) {
-        const float hT = last_lane(hi), lT = last_lane(lo), es = exp_f((hT - hi) + (lT - lo)), ea = REV ? exp_f(hi + lo) : 0.f;
+        const float hT = last_lane(hi), lT = last_lane(lo), es = __expf((hT - hi) + (lT - lo)), ea = REV ? __expf(hi + lo) : 0.f;
         s.w[lane] = REV ? ea : s.dt[lane] * es;
         if (FACTORS) s.es[lane] = es;
         if (lane == 63) {
             s.total = hi;
-            s.decay = exp_f(hi + lo);
+            s.decay = __expf(hi + lo);
         }
     }
     if (!FACTORS) return;
-    if (wave == 1) s.ea[lane] = exp_f(hi + lo);
-    if (wave == 2) s.rf[lane] = exp_f((hi - dpp<ROW_NEWBCAST>(hi)) + (lo - dpp<ROW_NEWBCAST>(lo)));
+    if (wave == 1) s.ea[lane] = __expf(hi + lo);
+    if (wave == 2) s.rf[lane] = __expf((hi - dpp<ROW_NEWBCAST>(hi)) + (lo - dpp<ROW_NEWBCAST>(lo)));
     if (wave == 3) {
-        const float cf = exp_f((dpp<ROW_NEWBCAST + 15>(hi) - hi) + (dpp<ROW_NEWBCAST + 15>(lo) - lo));
+        const float cf = __expf((dpp<ROW_NEWBCAST + 15>(hi) - hi) + (dpp<ROW_NEWBCAST + 15>(lo) - lo));
         s.cf[lane] = cf;
         s.cd[lane] = s.dt[lane] * cf;
     }
