@@ -15,9 +15,15 @@
 //      that a wave owns, whose part of S and dS it alone reads - straight from memory into operands;
 //   2. dx for the columns p that a wave owns.
 // In the next head's phase 1 a wave that has fewer tiles of G2 runs along the rows for d(a step), ddt and the sums for dA, dD, ddt_bias.  What is made of
-// the step sizes comes from the forward states' pass, which needs it too.  The next head's x, dy, S, dS are loaded as soon as this one's are used.  Operands that are f32 by nature are used as three bf16 pieces where an f32
-// result depends on them (S and dS: R, K -> dA, ddt_bias); W and G1 L, which only end in bf16 outputs, are rounded once, and dS in dx takes its
-// first piece.
+// the step sizes comes from the forward states' pass, which needs it too.  The next head's x, dy, S, dS are loaded as soon as this one's are used.
+// Operands that are f32 by nature are used as three bf16 pieces where an f32 result depends on them (S and dS: RI, KI -> dA, ddt_bias); W and G1 L,
+// which only end in bf16 outputs, are rounded once, and dS in dx takes its first piece.
+//
+// Measured (heads of one group each):
+//   256 f32 sequences of 256 rows, H = 4, P = N = 64: 221 us, of which this kernel 160 (the f32 matrix cores busy for 37 %), the states 69 (4.0
+//     TB/s: x, B, dy, C read, S and dS written), the slot table and the parameters' sums 5 each.  Bound by the chain inside a block: 256 registers and
+//     80 KB of LDS leave two workgroups on a CU.
+//   97 ragged bf16 sequences, 24 907 rows, H = 6, G = 2, P = 48, N = 40, states carried: 102 us = 66 + 36 + 9; 880 workgroups of three heads are 1.7 rounds.
 #include "ssm_util.h"
 
 namespace dc {
@@ -609,7 +615,9 @@ int launch_bwd(const SsmArgs& a, hipStream_t s) {
         if (a.ptiles == 1) return launch_bwd_wide<T, NP, V, WAVES, false>(a, s);
     return launch_bwd_wide<T, NP, V, WAVES, true>(a, s);
 }
-// Four waves where two workgroups fit a CU's LDS - they fill each other's waits -, else eight.
+// Four waves where two workgroups fit a CU's LDS - they fill each other's waits -, else eight: 65 536 f32 rows, H = 4, N = 64 took 268 us with eight and
+// 231 with four, one a CU, 217 once two fitted.  (N = 128 has eight column tiles of dB and dC, and needs a wave for each.)  Rows that do not allow
+// for vector accesses always take the WIDE form, which also does for one column tile: fewer kernels for a case that is rare.
 template <typename T, int V>
 int launch_bwd_n(const SsmArgs& a, hipStream_t s) {
     return a.N <= 32 ? launch_bwd<T, 32, V, 4>(a, s) : a.N <= 64 ? launch_bwd<T, 64, V, 4>(a, s) : launch_bwd<T, 128, V, 8>(a, s);
