@@ -44,7 +44,7 @@ typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 // exchange between lanes.  row(): the operand's rows (A) or columns (B) are rows of the tile, k contiguous; col(): k runs down the tile's rows.
 template <typename T> struct Mat;
 template <> struct Mat<float> {           // v_mfma_f32_16x16x4_f32, four of them: the e-th takes k = 4 g + e
-    static constexpr int KS = 16, V = 4;
+    static constexpr int KS = 16;
     typedef f32x4 frag;
     static __device__ __forceinline__ frag row(const float* p, int ld, int i, int g) { return *reinterpret_cast<const f32x4*>(p + i * ld + 4 * g); }
     static __device__ __forceinline__ frag col(const float* p, int ld, int i, int g) {
@@ -58,7 +58,7 @@ template <> struct Mat<float> {           // v_mfma_f32_16x16x4_f32, four of the
     }
 };
 template <> struct Mat<bf16_t> {          // v_mfma_f32_16x16x32_bf16
-    static constexpr int KS = 32, V = 8;
+    static constexpr int KS = 32;
     typedef bf16x8 frag;
     static __device__ __forceinline__ frag row(const bf16_t* p, int ld, int i, int g) {
         const bf16_t* q = p + i * ld + 4 * g;
